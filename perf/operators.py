@@ -14,8 +14,13 @@ query heads over 4 key/value heads of width 128, vocabulary 131072) and odd ones
 
 import math
 import random
+import sys
+from pathlib import Path
 
 import torch
+
+# the package lies in a folder of its own below the repository's root
+sys.path.insert(0, str(Path(__file__).resolve().parent.parent / "ue5m3-fp4_b200"))
 
 own = False
 
