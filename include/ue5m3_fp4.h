@@ -360,6 +360,82 @@ int ue5m3_gemm_fp4_fallback_ws(const uint8_t *a_codes, const uint8_t *a_sf_raw, 
                                void *workspace, size_t workspace_bytes, int *status_dev,
                                void *stream);
 
+/* ---- token-by-token use of a frozen packed model; no reference counterparts ---------------- */
+
+/*
+ * out[t, n] = dec * sum over k of x[t, k] * p[n, k] * s[n, k / block]  (+ bias[n])
+ * for a few rows of activations (bf16 or fp32, not quantized) and a packed weight: codes
+ * [rows, ceil(cols/2)] and UE5M3 scale bytes [rows, ceil(cols/block)] (two_d == 0) or
+ * [ceil(rows/block), ceil(cols/block)], as ue5m3_quantize writes them.  dec is the tensor-scale
+ * decode factor (formats.py:408).  fp32 sums in an order fixed by the sizes; out is rounded once.
+ * ldx / ldo: row strides of x / out in elements.  Any sizes; code rows on 16-byte boundaries
+ * (ceil(cols/2) % 16 == 0) are read with wide loads.  The cost grows with tokens / 32.
+ */
+int ue5m3_packed_matvec(const void *x, int x_dtype, int64_t tokens, int64_t ldx,
+                        const uint8_t *codes, const uint8_t *scales, int64_t rows, int64_t cols,
+                        int block, int two_d, float dec, const void *bias, int bias_dtype,
+                        void *out, int out_dtype, int64_t ldo, void *stream);
+
+/*
+ * A paged key/value cache (host struct of device pointers): bf16 pages [pages][page_size][kv_heads]
+ * [head_dim] with strides in elements (multiples of 8; channels contiguous) and the table
+ * int32 [sequences][table_width] whose entry j is the page of a sequence's keys
+ * j * page_size ... .  page_size is 16, 32, 64, 128 or 256, head_dim 64 or 128.
+ */
+typedef struct ue5m3_paged_cache {
+    void *k_pages, *v_pages;
+    int64_t k_page_stride, k_slot_stride, k_head_stride;
+    int64_t v_page_stride, v_slot_stride, v_head_stride;
+    int64_t pages, page_size, kv_heads, head_dim;
+    const int *page_table;
+    int64_t sequences, table_width, table_stride;
+} ue5m3_paged_cache;
+
+/*
+ * Attention of new tokens over the cache.  q, out: bf16 [tokens, heads, head_dim] (out contiguous);
+ * sequence b's new tokens are rows query_starts[b] ... query_starts[b + 1] - 1 and its last keys:
+ * with L = kv_lengths[b] (new ones included) and n new tokens, token i sees keys
+ * 0 ... L - n + i.  A token that sees no key gets zeros.  new_k, new_v (both or neither): the new
+ * tokens' keys and values [tokens, kv_heads, head_dim], written into their pages first.  Rows
+ * behind the last sequence are left as they are, or zeroed when zero_tail != 0.
+ * query_starts and kv_lengths are read on the device; max_query and max_kv are bounds from which
+ * the launch is sized (larger actual values are right, only slower).  A page that the table does
+ * not name among the cache's is not touched: rows that need it come out as NaN (others that share
+ * their tile may, too); the same where kv_lengths exceeds the table.
+ * workspace: ue5m3_paged_attention_workspace_bytes bytes (16-byte aligned, contents free), in use
+ * until the call's work is done.
+ */
+size_t ue5m3_paged_attention_workspace_bytes(int64_t tokens, int64_t sequences, int64_t heads,
+                                             int64_t kv_heads, int64_t head_dim, int64_t max_query,
+                                             int64_t max_kv);
+int ue5m3_paged_attention(const void *q, int64_t q_token_stride, int64_t q_head_stride,
+                          int64_t tokens, int64_t heads, const ue5m3_paged_cache *cache,
+                          const int *kv_lengths, const int *query_starts, int64_t max_query,
+                          int64_t max_kv, float scale, const void *new_k,
+                          int64_t new_k_token_stride, int64_t new_k_head_stride, const void *new_v,
+                          int64_t new_v_token_stride, int64_t new_v_head_stride, void *out,
+                          int zero_tail, void *workspace, size_t workspace_bytes, int *status_dev,
+                          void *stream);
+
+/*
+ * One token per row of logits [rows, vocabulary] (bf16 or fp32, row stride ld) from the uniform
+ * number uniforms[row]: weights exp((l - max) / temperature); kept are the top_k largest (equal
+ * logits: lowest index first; top_k <= 0: all), of these the shortest prefix in descending order
+ * whose weight reaches top_p of theirs (top_p >= 1: all, at least one always), of these the tokens
+ * with weight >= min_p of the largest; the token is the first kept one, in vocabulary order, whose
+ * running weight exceeds uniform * (weight of all kept).  temperature <= 0: the largest logit.
+ * Minus infinity masks a token.  logprobs: log of the token's share of the kept weight.  A row with
+ * a NaN, or without a logit above minus infinity, gives token -1 and NaN.  Each setting is a value,
+ * or a device array with one value per row where its pointer is not NULL.  Exact sums of fp64
+ * weights rounded to multiples of 2^-44: the same inputs give the same token.
+ * vocabulary <= 2^18.
+ */
+int ue5m3_sample_tokens(const void *logits, int dtype, int64_t rows, int64_t vocabulary, int64_t ld,
+                        const float *uniforms, const float *temperature_dev, float temperature,
+                        const int *top_k_dev, int top_k, const float *top_p_dev, float top_p,
+                        const float *min_p_dev, float min_p, int64_t *tokens, float *logprobs,
+                        void *stream);
+
 /*
  * Test hook: compares the software E2M1 ties-to-even rounding with the sm_100a
  * cvt.rn.satfinite.e2m1x2.f32 instruction over `count` consecutive fp32 bit

@@ -1,0 +1,390 @@
+// A few rows of activations times a packed FP4 weight (the product of a decode step):
+//   out[t, n] = dec * sum_k x[t, k] * p[n, k] * s[n, k / B]  (+ bias[n])
+// with E2M1 payloads p and UE5M3 block scales s as the quantizer stores them (1 x B blocks or
+// B x B tiles) and the activations as they are: no activation is quantized here.
+//
+// Arithmetic.  p * s has at most six significant bits and lies between 2^-18 and 2^19, so
+// p * (s / 16) is EXACT in fp16 for every code and every scale byte.  x does not fit fp16 as it
+// is: 128 consecutive elements of a row share a power of two that brings their largest one to
+// [2^14, 2^15).  A bf16 element that is no smaller than 2^-32 of that largest one is then exact in
+// fp16; below that it is off by at most 2^-40 of the largest one.  An fp32 element is cut into
+// three fp16 parts (11 bits each), which take three columns of the product.  Tensor cores
+// (mma.m16n8k16, weights as the 16-row operand, activations as the 8 columns) sum 128 products in
+// fp32; the power of two is multiplied back when that sum joins the fp32 total.  The order of all
+// sums is fixed by the sizes: the same call gives the same bits.
+//
+// What bounds it: reading the codes, 0.5 byte per weight element, plus the scales.  Decoding costs
+// one cvt.rn.f16x2.e2m1x2 and one packed multiply per two weights.
+//
+// Work split.  Every CTA owns N / gridDim rows (not a multiple of 16: missing rows of the last
+// 16-row tile are not loaded, so that all SMs read the same number of bytes), every one of its
+// warps the 128-element chunks w, w + 16, ... of the reduction axis.  A warp keeps the activations
+// of its chunks in registers (as mma fragments) while it walks over the CTA's rows; the sums of
+// the 16 warps meet in shared memory once per block of rows.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "abi_common.cuh"
+
+namespace ue5m3 {
+namespace matvec {
+
+constexpr int kWarps = 16;
+constexpr int kThreads = kWarps * 32;
+constexpr int kChunk = 128;          // reduction elements of one warp step: 64 bytes of a row's codes
+constexpr int kPartialFloats = 24576;  // 96 KiB of partial sums per CTA
+
+struct Params {
+    const void* x;
+    int64_t ldx;
+    const uint8_t* codes;
+    const uint8_t* scales;
+    const void* bias;
+    void* out;
+    int64_t ldo;
+    int64_t code_stride;   // bytes per row of codes
+    int64_t scale_stride;  // bytes per row of scales
+    int tokens, rows, k;
+    int block_shift;       // 4 or 5
+    int row_shift;         // log2 of the rows that share a scale row: 0, 4 or 5
+    int rows_per_block;    // rows of one pass over shared memory, a multiple of 16
+    int vector_codes;      // code rows start on 16-byte boundaries
+    int vector_x;          // rows of x start on 16-byte boundaries and hold whole vectors
+    int bias_fp32, out_fp32;
+    float factor;          // 16 * dec
+};
+
+__device__ __forceinline__ uint32_t e2m1x2_to_half2(uint32_t byte) {
+    uint32_t d;
+    asm("{\n.reg .b8 b, c0, c1, c2;\nmov.b32 {b, c0, c1, c2}, %1;\ncvt.rn.f16x2.e2m1x2 %0, b;\n}" : "=r"(d) : "r"(byte));
+    return d;
+}
+
+__device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+
+// A scale byte E<<3|M as the fp16 pair (s/16, s/16): read as the top bits of an fp32 the byte is
+// s * 2^-112, subnormal bytes included, and s/16 is exact in fp16 for all 256 bytes.
+__device__ __forceinline__ uint32_t scale_half2(uint32_t byte) {
+    const float v = __uint_as_float(byte << 20) * 0x1p108f;
+    const __half2 h = __floats2half2_rn(v, v);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 32 consecutive activations (k0 ...) of one token as floats, zero behind the end
+template <bool kFp32>
+__device__ __forceinline__ void load_x(const Params& p, int token, int k0, float (&v)[32]) {
+    if constexpr (kFp32) {
+        const float* row = reinterpret_cast<const float*>(p.x) + (int64_t)token * p.ldx + k0;
+        if (p.vector_x && k0 + 32 <= p.k) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float4 f = __ldg(reinterpret_cast<const float4*>(row) + i);
+                v[4 * i] = f.x, v[4 * i + 1] = f.y, v[4 * i + 2] = f.z, v[4 * i + 3] = f.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = k0 + i < p.k ? __ldg(row + i) : 0.0f;
+        }
+    } else {
+        const uint16_t* row = reinterpret_cast<const uint16_t*>(p.x) + (int64_t)token * p.ldx + k0;
+        if (p.vector_x && k0 + 32 <= p.k) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint4 u = __ldg(reinterpret_cast<const uint4*>(row) + i);
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    v[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
+                    v[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = k0 + i < p.k ? __uint_as_float((uint32_t)__ldg(row + i) << 16) : 0.0f;
+        }
+    }
+}
+
+// One chunk's activations of column `column` as mma B fragments, and the factor that undoes the
+// chunk's power of two.  Lane (g, c) = (lane / 4, lane % 4) brings column g and elements
+// 32 c ... 32 c + 31; step j of the chunk's eight mma takes its elements 4 j ... 4 j + 3.
+template <bool kFp32>
+__device__ __forceinline__ void load_fragment(const Params& p, int column, int columns, int chunk, uint32_t (&b)[16],
+                                              float& undo) {
+    constexpr int kParts = kFp32 ? 3 : 1;
+    const int c = threadIdx.x & 3;
+    const bool present = column < columns && chunk * kChunk < p.k;
+    const int token = present ? column / kParts : 0, part = present ? column % kParts : 0;
+    float v[32];
+    if (present)
+        load_x<kFp32>(p, token, chunk * kChunk + 32 * c, v);
+    else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+    // 2^(14 - e) for a largest element in [2^e, 2^(e+1)), held to 2^126 so that its inverse is a
+    // normal number; an infinity or a NaN among the elements stays one in fp16
+    const int field = min(268 - (int)(top >> 23), 253);
+    const float scale = __uint_as_float((uint32_t)field << 23);
+    undo = __uint_as_float((uint32_t)(254 - field) << 23);
+    if (kFp32) undo *= part == 0 ? 1.0f : part == 1 ? 0x1p-11f : 0x1p-22f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        float lo = v[2 * i] * scale, hi = v[2 * i + 1] * scale;
+        if (kFp32) {
+#pragma unroll
+            for (int step = 1; step < kParts; ++step) {
+                if (part >= step) {
+                    const float l = __half2float(__float2half_rn(lo)), h = __half2float(__float2half_rn(hi));
+                    // what the parts before left over, exactly; nothing behind an infinity or a NaN
+                    lo = fabsf(l) <= 65504.0f ? (lo - l) * 2048.0f : 0.0f;
+                    hi = fabsf(h) <= 65504.0f ? (hi - h) * 2048.0f : 0.0f;
+                }
+            }
+        }
+        const __half2 h = __floats2half2_rn(lo, hi);
+        b[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+
+// The 16 bytes of codes (32 elements) and the scale bytes of one row that a lane decodes in one
+// chunk; everything behind the row's end is zero.
+struct Piece {
+    uint4 codes;
+    uint32_t scales;  // byte 0: elements 0..15 of the 32, byte 1: elements 16..31 (B = 32: the same)
+};
+
+__device__ __forceinline__ Piece load_piece(const Params& p, int64_t row, bool valid, int chunk) {
+    Piece piece;
+    piece.codes = make_uint4(0, 0, 0, 0);
+    piece.scales = 0;
+    const int c = threadIdx.x & 3;
+    const int64_t byte = (int64_t)chunk * (kChunk / 2) + 16 * c;
+    if (!valid || byte >= p.code_stride) return piece;
+    const uint8_t* source = p.codes + row * p.code_stride + byte;
+    if (p.vector_codes) {
+        piece.codes = __ldg(reinterpret_cast<const uint4*>(source));
+    } else {
+        const int left = (int)min((int64_t)16, p.code_stride - byte);
+        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (i < left) w[i / 4] |= (uint32_t)__ldg(source + i) << (8 * (i % 4));
+        piece.codes = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    const uint8_t* scale = p.scales + (row >> p.row_shift) * p.scale_stride;
+    const int64_t first = byte * 2 >> p.block_shift;
+    piece.scales = __ldg(scale + first);
+    if (p.block_shift == 5)
+        piece.scales |= piece.scales << 8;
+    else if (first + 1 < p.scale_stride)
+        piece.scales |= (uint32_t)__ldg(scale + first + 1) << 8;
+    return piece;
+}
+
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
+    return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+}
+
+// kTiles: 8-column tiles of the product that a CTA computes at a time; kDepth: chunks that a warp
+// keeps in registers.
+template <bool kFp32, int kTiles, int kDepth>
+__global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params p) {
+    extern __shared__ float partial[];  // [warp][column][row of the block]
+    constexpr int kParts = kFp32 ? 3 : 1;
+    constexpr int kColumns = kTiles * 8;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int chunks = (p.k + kChunk - 1) / kChunk;
+    const int first_row = (int)((int64_t)p.rows * blockIdx.x / gridDim.x);
+    const int last_row = (int)((int64_t)p.rows * (blockIdx.x + 1) / gridDim.x);
+    const int block_rows = p.rows_per_block;
+    // whole tokens per pass, so that the parts of a token meet in one pass
+    constexpr int kTokens = kColumns / kParts;
+    for (int token0 = blockIdx.y * kTokens; token0 < p.tokens; token0 += gridDim.y * kTokens) {
+        const int column0 = token0 * kParts;
+        const int tokens = min(kTokens, p.tokens - token0);
+        const int used = tokens * kParts;
+        for (int row0 = first_row; row0 < last_row; row0 += block_rows) {
+            const int row_count = min(block_rows, last_row - row0);
+            for (int base = warp, pass = 0; base < chunks || pass == 0; base += kWarps * kDepth, ++pass) {
+                uint32_t b[kDepth][kTiles][16];
+                float undo[kDepth][kTiles][2];
+#pragma unroll
+                for (int d = 0; d < kDepth; ++d)
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t) {
+                        float mine;
+                        load_fragment<kFp32>(p, column0 + 8 * t + g, column0 + used, base + d * kWarps, b[d][t], mine);
+                        undo[d][t][0] = __shfl_sync(0xFFFFFFFFu, mine, 8 * c);
+                        undo[d][t][1] = __shfl_sync(0xFFFFFFFFu, mine, 8 * c + 4);
+                    }
+                Piece next[kDepth][2];
+#pragma unroll
+                for (int d = 0; d < kDepth; ++d)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        next[d][h] = load_piece(p, row0 + g + 8 * h, g + 8 * h < row_count, base + d * kWarps);
+                for (int tile = 0; tile < row_count; tile += 16) {
+                    Piece now[kDepth][2];
+#pragma unroll
+                    for (int d = 0; d < kDepth; ++d)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            now[d][h] = next[d][h];
+                            const int r = tile + 16 + g + 8 * h;
+                            next[d][h] = load_piece(p, row0 + r, r < row_count, base + d * kWarps);
+                        }
+                    float total[kTiles][4];
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t) total[t][0] = total[t][1] = total[t][2] = total[t][3] = 0.0f;
+#pragma unroll
+                    for (int d = 0; d < kDepth; ++d) {
+                        float sum[kTiles][4];
+#pragma unroll
+                        for (int t = 0; t < kTiles; ++t) sum[t][0] = sum[t][1] = sum[t][2] = sum[t][3] = 0.0f;
+                        uint32_t scale[2][2];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            scale[h][0] = scale_half2(now[d][h].scales & 0xFFu);
+                            scale[h][1] = scale_half2(now[d][h].scales >> 8);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            uint32_t a[2][2];
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const uint32_t word = word_of(now[d][h].codes, j / 2) >> (16 * (j & 1));
+                                a[h][0] = mul_half2(e2m1x2_to_half2(word), scale[h][j / 4]);
+                                a[h][1] = mul_half2(e2m1x2_to_half2(word >> 8), scale[h][j / 4]);
+                            }
+#pragma unroll
+                            for (int t = 0; t < kTiles; ++t)
+                                mma_f16(sum[t], a[0][0], a[1][0], a[0][1], a[1][1], b[d][t][2 * j], b[d][t][2 * j + 1]);
+                        }
+#pragma unroll
+                        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) total[t][i] = __fmaf_rn(sum[t][i], undo[d][t][i & 1], total[t][i]);
+                    }
+#pragma unroll
+                    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int column = 8 * t + 2 * c + (i & 1), r = tile + g + 8 * (i >> 1);
+                            if (column < used) {
+                                float* slot = partial + ((size_t)warp * used + column) * block_rows + r;
+                                *slot = pass == 0 ? total[t][i] : *slot + total[t][i];
+                            }
+                        }
+                }
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < row_count * tokens; i += kThreads) {
+                const int token = i / row_count, r = i - token * row_count;
+                float value = 0.0f;
+#pragma unroll
+                for (int part = kParts - 1; part >= 0; --part)
+#pragma unroll
+                    for (int w = 0; w < kWarps; ++w)
+                        value += partial[((size_t)w * used + token * kParts + part) * block_rows + r];
+                value *= p.factor;
+                const int64_t n = row0 + r;
+                if (p.bias)
+                    value += p.bias_fp32 ? reinterpret_cast<const float*>(p.bias)[n]
+                                         : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.bias)[n]);
+                const int64_t at = (int64_t)(token0 + token) * p.ldo + n;
+                if (p.out_fp32)
+                    reinterpret_cast<float*>(p.out)[at] = value;
+                else
+                    reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(value);
+            }
+            __syncthreads();
+        }
+    }
+}
+
+template <bool kFp32, int kTiles, int kDepth>
+int launch(Params p, cudaStream_t stream) {
+    constexpr int kTokens = kTiles * 8 / (kFp32 ? 3 : 1);
+    const int used = (p.tokens < kTokens ? p.tokens : kTokens) * (kFp32 ? 3 : 1);
+    const int grid = p.rows < sm_count() ? p.rows : sm_count();
+    const int own = (p.rows + grid - 1) / grid;
+    int block = kPartialFloats / (kWarps * used) / 16 * 16;
+    const int need = (own + 15) / 16 * 16;
+    if (block > need) block = need;
+    p.rows_per_block = block;
+    const size_t bytes = (size_t)kWarps * used * block * sizeof(float);
+    auto* kernel = packed_matvec_kernel<kFp32, kTiles, kDepth>;
+    const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPartialFloats * 4);
+    if (error != cudaSuccess) return record_cuda_error(error);
+    kernel<<<grid, kThreads, bytes, stream>>>(p);
+    return check_launch();
+}
+
+}  // namespace matvec
+}  // namespace ue5m3
+
+extern "C" int ue5m3_packed_matvec(const void* x, int x_dtype, int64_t tokens, int64_t ldx, const uint8_t* codes,
+                                   const uint8_t* scales, int64_t rows, int64_t cols, int block, int two_d, float dec,
+                                   const void* bias, int bias_dtype, void* out, int out_dtype, int64_t ldo,
+                                   void* stream) {
+    using namespace ue5m3;
+    if (!x || !codes || !scales || !out || tokens <= 0 || rows <= 0 || cols <= 0 || ldx < cols || ldo < rows)
+        return UE5M3_ERR_INVALID_ARGUMENT;
+    if ((x_dtype | out_dtype | bias_dtype) & ~1) return UE5M3_ERR_INVALID_ARGUMENT;
+    if (block != 16 && block != 32) return UE5M3_ERR_BLOCK_SIZE;
+    if (tokens > (1 << 24) || rows > (1 << 30) || cols > (1 << 30)) return UE5M3_ERR_TOO_LARGE;
+    const bool fp32 = x_dtype == UE5M3_DTYPE_FP32;
+    const int element = fp32 ? 4 : 2;
+    if ((uintptr_t)x % element || (uintptr_t)out % (out_dtype == UE5M3_DTYPE_FP32 ? 4 : 2) ||
+        (bias && (uintptr_t)bias % (bias_dtype == UE5M3_DTYPE_FP32 ? 4 : 2)))
+        return UE5M3_ERR_ALIGNMENT;
+    matvec::Params p;
+    p.x = x;
+    p.ldx = ldx;
+    p.codes = codes;
+    p.scales = scales;
+    p.bias = bias;
+    p.out = out;
+    p.ldo = ldo;
+    p.code_stride = (cols + 1) / 2;
+    p.scale_stride = (cols + block - 1) / block;
+    p.tokens = (int)tokens;
+    p.rows = (int)rows;
+    p.k = (int)cols;
+    p.block_shift = block == 16 ? 4 : 5;
+    p.row_shift = two_d ? p.block_shift : 0;
+    p.vector_codes = p.code_stride % 16 == 0 && (uintptr_t)codes % 16 == 0;
+    p.vector_x = (uintptr_t)x % 16 == 0 && (ldx * element) % 16 == 0;
+    p.bias_fp32 = bias_dtype == UE5M3_DTYPE_FP32;
+    p.out_fp32 = out_dtype == UE5M3_DTYPE_FP32;
+    p.factor = 16.0f * dec;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (fp32) {
+        if (tokens <= 2) return matvec::launch<true, 1, 2>(p, s);
+        if (tokens <= 5) return matvec::launch<true, 2, 1>(p, s);
+        return matvec::launch<true, 4, 1>(p, s);
+    }
+    if (tokens <= 8) return matvec::launch<false, 1, 2>(p, s);
+    if (tokens <= 16) return matvec::launch<false, 2, 1>(p, s);
+    return matvec::launch<false, 4, 1>(p, s);
+}

@@ -1,0 +1,77 @@
+// Shared by the kernels of attention over a paged key/value cache: arguments, the row space, and
+// how a sequence's keys are split over CTAs.
+//
+// Sequence b has query_starts[b + 1] - query_starts[b] = n new tokens; its cache holds
+// kv_lengths[b] = L keys, the new ones included.  New token i stands at position L - n + i and sees
+// the keys up to it; with L < n the first ones see none and their output is zero.  The G = heads /
+// kv_heads query heads of one key/value head are rows of one matrix: row i * G + g is token i, head
+// h * G + g, so that a tile of keys is read once for all of them.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace ue5m3 {
+namespace paged {
+
+constexpr int kKeys = 64;  // keys per tile of the split, and of the small-rows kernel
+
+struct Params {
+    const __nv_bfloat16* q;
+    int64_t q_token, q_head;     // strides in elements
+    __nv_bfloat16* out;          // [tokens, heads, head_dim]
+    const int* page_table;       // [sequences, table_width]
+    int64_t table_stride;
+    const int* kv_lengths;
+    const int* query_starts;
+    float* partial;              // [tokens, heads, splits, head_dim], then [tokens, heads, splits, 2]
+    int* status;
+    int sequences, tokens, heads, kv_heads, group;
+    int table_width, pages, page_shift;
+    int chunk;                   // key tiles per split
+    int splits;                  // splits that the grid and the workspace have room for
+    int zero_tail;               // rows behind the last sequence are set to zero
+    float scale_log2;            // scale * log2(e)
+};
+
+struct Sequence {
+    int first;   // row of q of its first new token
+    int queries; // new tokens
+    int keys;    // keys in the cache, no more than the page table has room for
+    bool cut;    // kv_lengths says more than the table has room for
+};
+
+__device__ __forceinline__ Sequence sequence_of(const Params& p, int b) {
+    Sequence s;
+    const int start = min(max(p.query_starts[b], 0), p.tokens);
+    const int stop = min(max(p.query_starts[b + 1], start), p.tokens);
+    s.first = start;
+    s.queries = stop - start;
+    const int64_t room = (int64_t)p.table_width << p.page_shift;
+    const int length = max(p.kv_lengths[b], 0);
+    s.cut = length > room;
+    s.keys = s.cut ? (int)room : length;
+    return s;
+}
+
+// keys that the last of rows row0 ... row0 + count - 1 sees (the most that any of them sees)
+__device__ __forceinline__ int visible_keys(const Params& p, const Sequence& s, int row0, int count) {
+    const int last = min(s.queries - 1, (row0 + count - 1) / p.group);
+    return max(0, s.keys - s.queries + last + 1);
+}
+
+// key tiles per split for a row tile that sees `tiles` of them
+__device__ __forceinline__ int split_chunk(const Params& p, int tiles) {
+    return max(p.chunk, (tiles + p.splits - 1) / p.splits);
+}
+
+// The page of a key, or -1 where the table names none of the cache's.
+__device__ __forceinline__ int page_of(const Params& p, int b, int key) {
+    const int page = __ldg(p.page_table + (int64_t)b * p.table_stride + (key >> p.page_shift));
+    return page >= 0 && page < p.pages ? page : -1;
+}
+
+}  // namespace paged
+}  // namespace ue5m3

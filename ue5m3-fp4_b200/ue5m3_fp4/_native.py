@@ -35,6 +35,17 @@ _DEFAULT_LIB = Path(__file__).resolve().parent.parent / "lib" / "libue5m3_b200.s
 _lib: ctypes.CDLL | None = None
 
 
+class PagedCache(ctypes.Structure):
+    """``ue5m3_paged_cache`` of the C ABI."""
+
+    _fields_ = [("k_pages", ctypes.c_void_p), ("v_pages", ctypes.c_void_p),
+                *((name, ctypes.c_int64) for name in (
+                    "k_page_stride", "k_slot_stride", "k_head_stride", "v_page_stride", "v_slot_stride",
+                    "v_head_stride", "pages", "page_size", "kv_heads", "head_dim")),
+                ("page_table", ctypes.c_void_p),
+                *((name, ctypes.c_int64) for name in ("sequences", "table_width", "table_stride"))]
+
+
 class NativeLibraryError(RuntimeError):
     """The sm_100a library is missing or returned an error status."""
 
@@ -105,6 +116,15 @@ def load() -> ctypes.CDLL:
     lib.ue5m3_place_row_windows.argtypes = [p, p, p, i64, i32, p, p, p, i64, i32, i64, p]
     lib.ue5m3_test_e2m1_cvt.restype = i32
     lib.ue5m3_test_e2m1_cvt.argtypes = [ctypes.c_uint32, ctypes.c_uint64, p, p, p]
+    lib.ue5m3_packed_matvec.restype = i32
+    lib.ue5m3_packed_matvec.argtypes = [p, i32, i64, i64, p, p, i64, i64, i32, i32, f32, p, i32, p, i32, i64, p]
+    lib.ue5m3_paged_attention_workspace_bytes.restype = sz
+    lib.ue5m3_paged_attention_workspace_bytes.argtypes = [i64] * 7
+    lib.ue5m3_paged_attention.restype = i32
+    lib.ue5m3_paged_attention.argtypes = [p, i64, i64, i64, i64, ctypes.POINTER(PagedCache), p, p, i64, i64, f32,
+                                          p, i64, i64, p, i64, i64, p, i32, p, sz, p, p]
+    lib.ue5m3_sample_tokens.restype = i32
+    lib.ue5m3_sample_tokens.argtypes = [p, i32, i64, i64, i64, p, p, f32, p, i32, p, f32, p, f32, p, p, p]
     if hasattr(lib, "ue5m3_amax_static"):
         lib.ue5m3_amax_static.restype = i32
         lib.ue5m3_amax_static.argtypes = [p, i32, i64, p, p]

@@ -126,6 +126,16 @@ class PackedFP4Tensor:
                                       two_dimensional=self.blocking == "2d", tensor_amax=amax,
                                       scale_target=self.scale_target, out_dtype=out_dtype)
 
+    def matvec(self, x: Tensor, bias: Tensor | None = None, out_dtype: torch.dtype | None = None) -> Tensor:
+        """``x @ W.T + bias`` for a few rows of activations, which are not quantized
+        (``ue5m3_fp4.serving.packed_matvec``), on the tensors' CUDA device."""
+
+        from ue5m3_fp4.serving import packed_matvec
+
+        return packed_matvec(x, self.codes, self.scales, rows=self.rows, cols=self.cols, block_size=self.block_size,
+                             two_dimensional=self.blocking == "2d", tensor_amax=self.tensor_amax,
+                             scale_target=self.scale_target, bias=bias, out_dtype=out_dtype)
+
     def gemm_operand(self, *, shift_headroom: int = 0):
         """The K-major operand of the FP4 GEMM (codes as stored, scales re-laid for the tensor
         core); ``cols`` is the reduction axis and must be a multiple of 64."""
