@@ -18,7 +18,7 @@
 //
 // Work split.  Every CTA owns N / gridDim rows (not a multiple of 16: missing rows of the last
 // 16-row tile are not loaded, so that all SMs read the same number of bytes), every one of its
-// warps the 128-element chunks w, w + 16, ... of the reduction axis.  A warp keeps the activations
+// warps w the 128-element chunks w, w + 16, ... of the reduction axis.  A warp keeps the activations
 // of its chunks in registers (as mma fragments) while it walks over the CTA's rows; the sums of
 // the 16 warps meet in shared memory once per block of rows.
 #include <cuda_bf16.h>
@@ -50,7 +50,7 @@ struct Params {
     int block_shift;       // 4 or 5
     int row_shift;         // log2 of the rows that share a scale row: 0, 4 or 5
     int rows_per_block;    // rows of one pass over shared memory, a multiple of 16
-    int vector_codes;      // code rows start on 16-byte boundaries
+    int vector;            // code rows start on 16-byte boundaries, rows of 16-element scales on 2-byte ones
     int vector_x;          // rows of x start on 16-byte boundaries and hold whole vectors
     int bias_fp32, out_fp32;
     float factor;          // 16 * dec
@@ -167,37 +167,36 @@ __device__ __forceinline__ void load_fragment(const Params& p, int column, int c
 }
 
 // The 16 bytes of codes (32 elements) and the scale bytes of one row that a lane decodes in one
-// chunk; everything behind the row's end is zero.
+// chunk.  A chunk or row behind the end is read as the last one instead, so that no load hangs on
+// a branch: its activations are zero, or its sums are not stored.
 struct Piece {
     uint4 codes;
     uint32_t scales;  // byte 0: elements 0..15 of the 32, byte 1: elements 16..31 (B = 32: the same)
 };
 
-__device__ __forceinline__ Piece load_piece(const Params& p, int64_t row, bool valid, int chunk) {
+template <bool kVector>
+__device__ __forceinline__ Piece load_piece(const Params& p, int row, int chunk) {
     Piece piece;
-    piece.codes = make_uint4(0, 0, 0, 0);
-    piece.scales = 0;
     const int c = threadIdx.x & 3;
-    const int64_t byte = (int64_t)chunk * (kChunk / 2) + 16 * c;
-    if (!valid || byte >= p.code_stride) return piece;
-    const uint8_t* source = p.codes + row * p.code_stride + byte;
-    if (p.vector_codes) {
-        piece.codes = __ldg(reinterpret_cast<const uint4*>(source));
+    const uint8_t* codes = p.codes + row * p.code_stride;
+    const uint8_t* scales = p.scales + (row >> p.row_shift) * p.scale_stride;
+    int byte = chunk * (kChunk / 2) + 16 * c;
+    if constexpr (kVector) {
+        byte = min(byte, (int)p.code_stride - 16);
+        piece.codes = __ldg(reinterpret_cast<const uint4*>(codes + byte));
+        const int first = byte * 2 >> p.block_shift;
+        piece.scales = p.block_shift == 4 ? (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(scales + first))
+                                          : (uint32_t)__ldg(scales + first) * 0x101u;
     } else {
-        const int left = (int)min((int64_t)16, p.code_stride - byte);
+        const int last = (int)p.code_stride - 1;
         uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (i < left) w[i / 4] |= (uint32_t)__ldg(source + i) << (8 * (i % 4));
+        for (int i = 0; i < 16; ++i) w[i / 4] |= (uint32_t)__ldg(codes + min(byte + i, last)) << (8 * (i % 4));
         piece.codes = make_uint4(w[0], w[1], w[2], w[3]);
+        const int first = byte * 2 >> p.block_shift, last_scale = (int)p.scale_stride - 1;
+        piece.scales = __ldg(scales + min(first, last_scale));
+        piece.scales |= (uint32_t)__ldg(scales + min(first + (p.block_shift == 4), last_scale)) << 8;
     }
-    const uint8_t* scale = p.scales + (row >> p.row_shift) * p.scale_stride;
-    const int64_t first = byte * 2 >> p.block_shift;
-    piece.scales = __ldg(scale + first);
-    if (p.block_shift == 5)
-        piece.scales |= piece.scales << 8;
-    else if (first + 1 < p.scale_stride)
-        piece.scales |= (uint32_t)__ldg(scale + first + 1) << 8;
     return piece;
 }
 
@@ -206,26 +205,37 @@ __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
 }
 
 // kTiles: 8-column tiles of the product that a CTA computes at a time; kDepth: chunks that a warp
-// keeps in registers.
-template <bool kFp32, int kTiles, int kDepth>
+// keeps in registers; kVector: codes and scales are read with wide loads.
+template <bool kFp32, int kTiles, int kDepth, bool kVector>
 __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params p) {
     extern __shared__ float partial[];  // [warp][column][row of the block]
     constexpr int kParts = kFp32 ? 3 : 1;
     constexpr int kColumns = kTiles * 8;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int chunks = (p.k + kChunk - 1) / kChunk;
+    const int passes = (chunks + kWarps * kDepth - 1) / (kWarps * kDepth);
     const int first_row = (int)((int64_t)p.rows * blockIdx.x / gridDim.x);
     const int last_row = (int)((int64_t)p.rows * (blockIdx.x + 1) / gridDim.x);
     const int block_rows = p.rows_per_block;
     // whole tokens per pass, so that the parts of a token meet in one pass
     constexpr int kTokens = kColumns / kParts;
-    for (int token0 = blockIdx.y * kTokens; token0 < p.tokens; token0 += gridDim.y * kTokens) {
+    for (int token0 = 0; token0 < p.tokens; token0 += kTokens) {
         const int column0 = token0 * kParts;
         const int tokens = min(kTokens, p.tokens - token0);
         const int used = tokens * kParts;
         for (int row0 = first_row; row0 < last_row; row0 += block_rows) {
             const int row_count = min(block_rows, last_row - row0);
-            for (int base = warp, pass = 0; base < chunks || pass == 0; base += kWarps * kDepth, ++pass) {
+            Piece next[kDepth][2];
+            auto load = [&](int pass, int tile) {
+#pragma unroll
+                for (int d = 0; d < kDepth; ++d)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        next[d][h] = load_piece<kVector>(p, row0 + min(tile + g + 8 * h, row_count - 1),
+                                                         min((pass * kDepth + d) * kWarps + warp, chunks - 1));
+            };
+            load(0, 0);
+            for (int pass = 0; pass < passes; ++pass) {
                 uint32_t b[kDepth][kTiles][16];
                 float undo[kDepth][kTiles][2];
 #pragma unroll
@@ -233,26 +243,19 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
 #pragma unroll
                     for (int t = 0; t < kTiles; ++t) {
                         float mine;
-                        load_fragment<kFp32>(p, column0 + 8 * t + g, column0 + used, base + d * kWarps, b[d][t], mine);
+                        load_fragment<kFp32>(p, column0 + 8 * t + g, column0 + used, (pass * kDepth + d) * kWarps + warp,
+                                             b[d][t], mine);
                         undo[d][t][0] = __shfl_sync(0xFFFFFFFFu, mine, 8 * c);
                         undo[d][t][1] = __shfl_sync(0xFFFFFFFFu, mine, 8 * c + 4);
                     }
-                Piece next[kDepth][2];
-#pragma unroll
-                for (int d = 0; d < kDepth; ++d)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        next[d][h] = load_piece(p, row0 + g + 8 * h, g + 8 * h < row_count, base + d * kWarps);
                 for (int tile = 0; tile < row_count; tile += 16) {
                     Piece now[kDepth][2];
 #pragma unroll
-                    for (int d = 0; d < kDepth; ++d)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            now[d][h] = next[d][h];
-                            const int r = tile + 16 + g + 8 * h;
-                            next[d][h] = load_piece(p, row0 + r, r < row_count, base + d * kWarps);
-                        }
+                    for (int d = 0; d < kDepth; ++d) now[d][0] = next[d][0], now[d][1] = next[d][1];
+                    if (tile + 16 < row_count)
+                        load(pass, tile + 16);
+                    else if (pass + 1 < passes)
+                        load(pass + 1, 0);
                     float total[kTiles][4];
 #pragma unroll
                     for (int t = 0; t < kTiles; ++t) total[t][0] = total[t][1] = total[t][2] = total[t][3] = 0.0f;
@@ -291,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
                         for (int i = 0; i < 4; ++i) {
                             const int column = 8 * t + 2 * c + (i & 1), r = tile + g + 8 * (i >> 1);
                             if (column < used) {
-                                float* slot = partial + ((size_t)warp * used + column) * block_rows + r;
+                                float* slot = partial + (warp * used + column) * block_rows + r;
                                 *slot = pass == 0 ? total[t][i] : *slot + total[t][i];
                             }
                         }
@@ -322,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
     }
 }
 
-template <bool kFp32, int kTiles, int kDepth>
+template <bool kFp32, int kTiles, int kDepth, bool kVector>
 int launch(Params p, cudaStream_t stream) {
     constexpr int kTokens = kTiles * 8 / (kFp32 ? 3 : 1);
     const int used = (p.tokens < kTokens ? p.tokens : kTokens) * (kFp32 ? 3 : 1);
@@ -333,11 +336,23 @@ int launch(Params p, cudaStream_t stream) {
     if (block > need) block = need;
     p.rows_per_block = block;
     const size_t bytes = (size_t)kWarps * used * block * sizeof(float);
-    auto* kernel = packed_matvec_kernel<kFp32, kTiles, kDepth>;
+    auto* kernel = packed_matvec_kernel<kFp32, kTiles, kDepth, kVector>;
     const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPartialFloats * 4);
     if (error != cudaSuccess) return record_cuda_error(error);
     kernel<<<grid, kThreads, bytes, stream>>>(p);
     return check_launch();
+}
+
+template <bool kVector>
+int dispatch(const Params& p, bool fp32, cudaStream_t s) {
+    if (fp32) {
+        if (p.tokens <= 2) return launch<true, 1, 2, kVector>(p, s);
+        if (p.tokens <= 5) return launch<true, 2, 1, kVector>(p, s);
+        return launch<true, 4, 1, kVector>(p, s);
+    }
+    if (p.tokens <= 8) return launch<false, 1, 2, kVector>(p, s);
+    if (p.tokens <= 16) return launch<false, 2, 1, kVector>(p, s);
+    return launch<false, 4, 1, kVector>(p, s);
 }
 
 }  // namespace matvec
@@ -373,18 +388,12 @@ extern "C" int ue5m3_packed_matvec(const void* x, int x_dtype, int64_t tokens, i
     p.k = (int)cols;
     p.block_shift = block == 16 ? 4 : 5;
     p.row_shift = two_d ? p.block_shift : 0;
-    p.vector_codes = p.code_stride % 16 == 0 && (uintptr_t)codes % 16 == 0;
+    p.vector = p.code_stride % 16 == 0 && (uintptr_t)codes % 16 == 0 &&
+               (block == 32 || (p.scale_stride % 2 == 0 && (uintptr_t)scales % 2 == 0));
     p.vector_x = (uintptr_t)x % 16 == 0 && (ldx * element) % 16 == 0;
     p.bias_fp32 = bias_dtype == UE5M3_DTYPE_FP32;
     p.out_fp32 = out_dtype == UE5M3_DTYPE_FP32;
     p.factor = 16.0f * dec;
-    cudaStream_t s = (cudaStream_t)stream;
-    if (fp32) {
-        if (tokens <= 2) return matvec::launch<true, 1, 2>(p, s);
-        if (tokens <= 5) return matvec::launch<true, 2, 1>(p, s);
-        return matvec::launch<true, 4, 1>(p, s);
-    }
-    if (tokens <= 8) return matvec::launch<false, 1, 2>(p, s);
-    if (tokens <= 16) return matvec::launch<false, 2, 1>(p, s);
-    return matvec::launch<false, 4, 1>(p, s);
+    return p.vector ? matvec::dispatch<true>(p, fp32, (cudaStream_t)stream)
+                    : matvec::dispatch<false>(p, fp32, (cudaStream_t)stream);
 }

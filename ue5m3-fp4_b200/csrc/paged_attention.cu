@@ -342,36 +342,57 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
 }
 
 // The rows of a split sequence: sum of the splits' rows, each faded to the largest maximum.  One
-// warp per (token, head).
+// CTA per (token, head), a quarter of the splits per warp, four channels per lane (head_dim 64: two
+// splits side by side in a warp).
 template <int kDim>
 __global__ void __launch_bounds__(128) combine_kernel(const Params p, int rows_per_tile) {
+    constexpr int kLanes = kDim / 4, kSide = 128 / kLanes;  // lanes of a row, rows side by side in the CTA
+    __shared__ float values[kSide][kDim], sums[kSide], tops[4];
     const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int side = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
     const Sequence s = sequence_of(p, b);
-    const int64_t count = (int64_t)s.queries * p.heads;
-    for (int64_t i = blockIdx.x * 4 + warp; i < count; i += gridDim.x * 4) {
-        const int token = (int)(i / p.heads), head = (int)(i % p.heads);
+    for (int i = blockIdx.x; i < s.queries * p.heads; i += gridDim.x) {
+        const int token = i / p.heads, head = i % p.heads;
         const int row = token * p.group + head % p.group;
         const int all = (visible_keys(p, s, row / rows_per_tile * rows_per_tile, rows_per_tile) + kKeys - 1) / kKeys;
-        const int chunk = split_chunk(p, all), splits = (all + chunk - 1) / chunk;
+        const int chunk = split_chunk(p, all), splits = (all + chunk - 1) / max(chunk, 1);
         if (splits <= 1) continue;  // written by its only split
         const int64_t at = (int64_t)(s.first + token) * p.heads + head;
         const float* rows = p.partial + at * p.splits * kDim;
         const float* stats = p.partial + (int64_t)p.tokens * p.heads * p.splits * kDim + at * p.splits * 2;
         float most = -INFINITY;
-        for (int j = 0; j < splits; ++j) most = fmaxf(most, stats[2 * j]);
-        const float base = most == -INFINITY ? 0.0f : most;
-        float value[kDim / 32], total = 0.0f;
+        for (int j = threadIdx.x; j < splits; j += 128) most = fmaxf(most, stats[2 * j]);
 #pragma unroll
-        for (int d = 0; d < kDim / 32; ++d) value[d] = 0.0f;
-        for (int j = 0; j < splits; ++j) {
+        for (int m = 16; m; m >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, m));
+        if (lane == 0) tops[warp] = most;
+        __syncthreads();
+        most = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+        const float base = most == -INFINITY ? 0.0f : most;
+        float4 value = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float total = 0.0f;
+#pragma unroll 4
+        for (int j = side; j < splits; j += kSide) {
+            const float4 v = *reinterpret_cast<const float4*>(rows + (int64_t)j * kDim + d);
             const float weight = exp2_approx(stats[2 * j] - base);
             total = __fmaf_rn(stats[2 * j + 1], weight, total);
-#pragma unroll
-            for (int d = 0; d < kDim / 32; ++d) value[d] = __fmaf_rn(rows[j * kDim + d * 32 + lane], weight, value[d]);
+            value.x = __fmaf_rn(v.x, weight, value.x);
+            value.y = __fmaf_rn(v.y, weight, value.y);
+            value.z = __fmaf_rn(v.z, weight, value.z);
+            value.w = __fmaf_rn(v.w, weight, value.w);
         }
+        *reinterpret_cast<float4*>(&values[side][d]) = value;
+        if (d == 0) sums[side] = total;
+        __syncthreads();
+        if (threadIdx.x < kDim) {
+            float v = 0.0f, t = 0.0f;
 #pragma unroll
-        for (int d = 0; d < kDim / 32; ++d)
-            p.out[at * kDim + d * 32 + lane] = __float2bfloat16_rn(total == 0.0f ? 0.0f : value[d] / total);
+            for (int j = 0; j < kSide; ++j) {
+                v += values[j][threadIdx.x];
+                t += sums[j];
+            }
+            p.out[at * kDim + threadIdx.x] = __float2bfloat16_rn(t == 0.0f ? 0.0f : v / t);
+        }
+        __syncthreads();
     }
 }
 
@@ -457,7 +478,7 @@ int launch(const Params& p, const Plan& plan, const CUtensorMap& k_map, const CU
     attention_small_kernel<kDim><<<grid, kSmallThreads, SmallShared<kDim>::kBytes, stream>>>(p, k_map, v_map);
     int status = check_launch();
     if (status != UE5M3_OK || plan.splits == 1) return status;
-    int64_t blocks = (max_query * p.heads + 3) / 4;
+    int64_t blocks = max_query * p.heads;
     if (blocks > 65535) blocks = 65535;
     combine_kernel<kDim><<<dim3((unsigned)blocks, p.sequences), 128, 0, stream>>>(p, kRows);
     return check_launch();
