@@ -34,7 +34,8 @@ namespace matvec {
 constexpr int kWarps = 16;
 constexpr int kThreads = kWarps * 32;
 constexpr int kChunk = 128;          // reduction elements of one warp step: 64 bytes of a row's codes
-constexpr int kPartialFloats = 24576;  // 96 KiB of partial sums per CTA
+constexpr int kPartialFloats = 23552;  // 92 KiB of partial sums per CTA
+constexpr int kRing = 4;             // tiles of codes in shared memory, 32 KiB each at two chunks per warp
 
 struct Params {
     const void* x;
@@ -47,19 +48,19 @@ struct Params {
     int64_t code_stride;   // bytes per row of codes
     int64_t scale_stride;  // bytes per row of scales
     int tokens, rows, k;
-    int block_shift;       // 4 or 5
     int row_shift;         // log2 of the rows that share a scale row: 0, 4 or 5
     int rows_per_block;    // rows of one pass over shared memory, a multiple of 16
-    int vector;            // code rows start on 16-byte boundaries, rows of 16-element scales on 2-byte ones
     int vector_x;          // rows of x start on 16-byte boundaries and hold whole vectors
     int bias_fp32, out_fp32;
     float factor;          // 16 * dec
 };
 
-__device__ __forceinline__ uint32_t e2m1x2_to_half2(uint32_t byte) {
-    uint32_t d;
-    asm("{\n.reg .b8 b, c0, c1, c2;\nmov.b32 {b, c0, c1, c2}, %1;\ncvt.rn.f16x2.e2m1x2 %0, b;\n}" : "=r"(d) : "r"(byte));
-    return d;
+// eight codes -> four fp16 pairs, exactly
+__device__ __forceinline__ void e2m1x8_to_half2(uint32_t word, uint32_t (&d)[4]) {
+    asm("{\n.reg .b8 b0, b1, b2, b3;\nmov.b32 {b0, b1, b2, b3}, %4;\ncvt.rn.f16x2.e2m1x2 %0, b0;\n"
+        "cvt.rn.f16x2.e2m1x2 %1, b1;\ncvt.rn.f16x2.e2m1x2 %2, b2;\ncvt.rn.f16x2.e2m1x2 %3, b3;\n}"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(word));
 }
 
 __device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
@@ -171,33 +172,46 @@ __device__ __forceinline__ void load_fragment(const Params& p, int column, int c
 // a branch: its activations are zero, or its sums are not stored.
 struct Piece {
     uint4 codes;
-    uint32_t scales;  // byte 0: elements 0..15 of the 32, byte 1: elements 16..31 (B = 32: the same)
+    uint32_t scales;  // byte 0: elements 0..15 of the 32, byte 1: elements 16..31 (B = 32: byte 0 for all)
 };
 
-template <bool kVector>
-__device__ __forceinline__ Piece load_piece(const Params& p, int row, int chunk) {
+// Rows that do not start on 16-byte boundaries.
+enum class Loads {
+    kWords,  // any rows: aligned words, shifted into place; reads up to 19 bytes behind a row's end
+    kBytes   // byte by byte: the first row and the last ones of the weight
+};
+
+// The codes at `code` bytes and the scales at `scale` bytes (that of the lane's first element; the
+// row's last one is `last_scale`); `left`: the row's bytes from `code` on.
+template <Loads kLoads, int kBlock>
+__device__ __forceinline__ Piece load_piece(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                                            uint32_t code, uint32_t scale, uint32_t last_scale, int left) {
     Piece piece;
-    const int c = threadIdx.x & 3;
-    const uint8_t* codes = p.codes + row * p.code_stride;
-    const uint8_t* scales = p.scales + (row >> p.row_shift) * p.scale_stride;
-    int byte = chunk * (kChunk / 2) + 16 * c;
-    if constexpr (kVector) {
-        byte = min(byte, (int)p.code_stride - 16);
-        piece.codes = __ldg(reinterpret_cast<const uint4*>(codes + byte));
-        const int first = byte * 2 >> p.block_shift;
-        piece.scales = p.block_shift == 4 ? (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(scales + first))
-                                          : (uint32_t)__ldg(scales + first) * 0x101u;
-    } else {
-        const int last = (int)p.code_stride - 1;
-        uint32_t w[4] = {0, 0, 0, 0};
+    const uint8_t* source = codes + code;
+    uint32_t w[4];
+    if constexpr (kLoads == Loads::kWords) {
+        const uint32_t off = (uint32_t)((uintptr_t)source & 3);
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(source - off);
+        uint32_t v[5];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) w[i / 4] |= (uint32_t)__ldg(codes + min(byte + i, last)) << (8 * (i % 4));
-        piece.codes = make_uint4(w[0], w[1], w[2], w[3]);
-        const int first = byte * 2 >> p.block_shift, last_scale = (int)p.scale_stride - 1;
-        piece.scales = __ldg(scales + min(first, last_scale));
-        piece.scales |= (uint32_t)__ldg(scales + min(first + (p.block_shift == 4), last_scale)) << 8;
+        for (int i = 0; i < 5; ++i) v[i] = __ldg(words + i);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(v[i], v[i + 1], 8 * off);
+    } else {
+        w[0] = w[1] = w[2] = w[3] = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i / 4] |= (uint32_t)__ldg(source + min(i, left - 1)) << (8 * (i % 4));
     }
+    piece.codes = make_uint4(w[0], w[1], w[2], w[3]);
+    piece.scales = __ldg(scales + scale);
+    if (kBlock == 16) piece.scales |= (uint32_t)__ldg(scales + min(scale + 1, last_scale)) << 8;
     return piece;
+}
+
+__device__ __forceinline__ void copy_async(uint4* to, const uint8_t* from) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)),
+                 "l"(from)
+                 : "memory");
 }
 
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
@@ -205,18 +219,21 @@ __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
 }
 
 // kTiles: 8-column tiles of the product that a CTA computes at a time; kDepth: chunks that a warp
-// keeps in registers; kVector: codes and scales are read with wide loads.
-template <bool kFp32, int kTiles, int kDepth, bool kVector>
+// keeps in registers.
+template <bool kFp32, int kTiles, int kDepth, bool kVector, int kBlock>
 __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params p) {
-    extern __shared__ float partial[];  // [warp][column][row of the block]
+    extern __shared__ uint4 ring[];  // kVector: [slot][chunk][row half][thread]
+    float* partial = reinterpret_cast<float*>(ring + (kVector ? kRing * kDepth * 2 * kThreads : 0));  // [warp][column][row]
     constexpr int kParts = kFp32 ? 3 : 1;
     constexpr int kColumns = kTiles * 8;
+    constexpr int kBlockShift = kBlock == 16 ? 4 : 5;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int chunks = (p.k + kChunk - 1) / kChunk;
     const int passes = (chunks + kWarps * kDepth - 1) / (kWarps * kDepth);
     const int first_row = (int)((int64_t)p.rows * blockIdx.x / gridDim.x);
     const int last_row = (int)((int64_t)p.rows * (blockIdx.x + 1) / gridDim.x);
     const int block_rows = p.rows_per_block;
+    const int stride = (int)p.code_stride, scale_stride = (int)p.scale_stride;
     // whole tokens per pass, so that the parts of a token meet in one pass
     constexpr int kTokens = kColumns / kParts;
     for (int token0 = 0; token0 < p.tokens; token0 += kTokens) {
@@ -225,16 +242,87 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
         const int used = tokens * kParts;
         for (int row0 = first_row; row0 < last_row; row0 += block_rows) {
             const int row_count = min(block_rows, last_row - row0);
+            const uint8_t* codes = p.codes + row0 * p.code_stride;
+            const int scale_row0 = row0 >> p.row_shift;
+            const uint8_t* scales = p.scales + scale_row0 * p.scale_stride;
+            // rows from which 3 bytes back and 19 bytes further on are still inside the weight
+            const bool inner = row0 * p.code_stride >= 3 && (int64_t)(p.rows - row0 - row_count) * p.code_stride >= 20;
+            // Pieces of the tiles to come.  Wide rows: the codes wait in this lane's own slots of a ring
+            // in shared memory (asynchronous copies), kRing - 1 tiles ahead, the scales in registers, two
+            // tiles ahead.  Other rows: in registers, one tile ahead.
             Piece next[kDepth][2];
-            auto load = [&](int pass, int tile) {
+            uint32_t later[kDepth][2];
+            uint32_t code[2], scale[2], byte[kDepth], block[kDepth];
+            auto locate = [&](int pass, int tile) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int row = min(tile + g + 8 * h, row_count - 1);
+                    code[h] = row * stride;
+                    scale[h] = ((row0 + row >> p.row_shift) - scale_row0) * scale_stride;
+                }
+#pragma unroll
+                for (int d = 0; d < kDepth; ++d) {
+                    // a chunk behind the end is read as the row's last bytes
+                    byte[d] = min(((pass * kDepth + d) * kWarps + warp) * (kChunk / 2) + 16 * c, stride - (kVector ? 16 : 1));
+                    block[d] = byte[d] * 2 >> kBlockShift;
+                }
+            };
+            auto copy_codes = [&](int slot) {
 #pragma unroll
                 for (int d = 0; d < kDepth; ++d)
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
-                        next[d][h] = load_piece<kVector>(p, row0 + min(tile + g + 8 * h, row_count - 1),
-                                                         min((pass * kDepth + d) * kWarps + warp, chunks - 1));
+                        copy_async(ring + ((slot * kDepth + d) * 2 + h) * kThreads + threadIdx.x, codes + (code[h] + byte[d]));
             };
-            load(0, 0);
+            auto load_scales = [&](uint32_t(&to)[kDepth][2]) {
+#pragma unroll
+                for (int d = 0; d < kDepth; ++d)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        to[d][h] = kBlock == 16 ? (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(scales + (scale[h] + block[d])))
+                                                : (uint32_t)__ldg(scales + (scale[h] + block[d]));
+            };
+            auto load = [&](int pass, int tile) {
+                locate(pass, tile);
+#pragma unroll
+                for (int d = 0; d < kDepth; ++d)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t last = scale[h] + scale_stride - 1;
+                        if (inner)
+                            next[d][h] = load_piece<Loads::kWords, kBlock>(codes, scales, code[h] + byte[d], scale[h] + block[d],
+                                                                           last, 0);
+                        else
+                            next[d][h] = load_piece<Loads::kBytes, kBlock>(codes, scales, code[h] + byte[d], scale[h] + block[d],
+                                                                           last, stride - byte[d]);
+                    }
+            };
+            // the (pass, tile) that is copied next
+            int ahead_pass = 0, ahead_tile = 0;
+            auto copy_ahead = [&](int slot) {
+                if (ahead_pass < passes) {
+                    locate(ahead_pass, ahead_tile);
+                    copy_codes(slot);
+                    ahead_tile += 16;
+                    if (ahead_tile >= row_count) ahead_tile = 0, ++ahead_pass;
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+            int slot_now = 0;
+            uint32_t scales_now[kDepth][2];
+            if constexpr (kVector) {
+#pragma unroll
+                for (int i = 0; i < kRing - 1; ++i) copy_ahead(i);
+                locate(0, 0);
+                load_scales(scales_now);
+                if (row_count > 16)
+                    locate(0, 16);
+                else
+                    locate(min(1, passes - 1), 0);
+                load_scales(later);
+            } else {
+                load(0, 0);
+            }
             for (int pass = 0; pass < passes; ++pass) {
                 uint32_t b[kDepth][kTiles][16];
                 float undo[kDepth][kTiles][2];
@@ -248,17 +336,36 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
                         undo[d][t][0] = __shfl_sync(0xFFFFFFFFu, mine, 8 * c);
                         undo[d][t][1] = __shfl_sync(0xFFFFFFFFu, mine, 8 * c + 4);
                     }
-                for (int tile = 0; tile < row_count; tile += 16) {
+                float* slot = partial + (warp * used + 2 * c) * block_rows + g;
+#pragma unroll 2
+                for (int tile = 0; tile < row_count; tile += 16, slot += 16) {
                     Piece now[kDepth][2];
+                    if constexpr (kVector) {
+                        copy_ahead((slot_now + kRing - 1) % kRing);
+                        asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
 #pragma unroll
-                    for (int d = 0; d < kDepth; ++d) now[d][0] = next[d][0], now[d][1] = next[d][1];
-                    if (tile + 16 < row_count)
-                        load(pass, tile + 16);
-                    else if (pass + 1 < passes)
-                        load(pass + 1, 0);
+                        for (int d = 0; d < kDepth; ++d)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                now[d][h].codes = ring[((slot_now * kDepth + d) * 2 + h) * kThreads + threadIdx.x];
+                                now[d][h].scales = scales_now[d][h];
+                                scales_now[d][h] = later[d][h];
+                            }
+                        slot_now = (slot_now + 1) % kRing;
+                        // two tiles on
+                        int tile2 = tile + 32, pass2 = pass;
+                        while (tile2 >= row_count && pass2 + 1 < passes) tile2 = max(tile2 - (row_count + 15) / 16 * 16, 0), ++pass2;
+                        locate(pass2, tile2);
+                        load_scales(later);
+                    } else {
+#pragma unroll
+                        for (int d = 0; d < kDepth; ++d) now[d][0] = next[d][0], now[d][1] = next[d][1];
+                        if (tile + 16 < row_count)
+                            load(pass, tile + 16);
+                        else if (pass + 1 < passes)
+                            load(pass + 1, 0);
+                    }
                     float total[kTiles][4];
-#pragma unroll
-                    for (int t = 0; t < kTiles; ++t) total[t][0] = total[t][1] = total[t][2] = total[t][3] = 0.0f;
 #pragma unroll
                     for (int d = 0; d < kDepth; ++d) {
                         float sum[kTiles][4];
@@ -267,37 +374,44 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
                         uint32_t scale[2][2];
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            scale[h][0] = scale_half2(now[d][h].scales & 0xFFu);
-                            scale[h][1] = scale_half2(now[d][h].scales >> 8);
+                            scale[h][0] = scale_half2(kBlock == 16 ? now[d][h].scales & 0xFFu : now[d][h].scales);
+                            scale[h][1] = kBlock == 16 ? scale_half2(now[d][h].scales >> 8) : scale[h][0];
                         }
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            uint32_t a[2][2];
+                        for (int j = 0; j < 4; ++j) {
+                            uint32_t a[2][4];
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
-                                const uint32_t word = word_of(now[d][h].codes, j / 2) >> (16 * (j & 1));
-                                a[h][0] = mul_half2(e2m1x2_to_half2(word), scale[h][j / 4]);
-                                a[h][1] = mul_half2(e2m1x2_to_half2(word >> 8), scale[h][j / 4]);
+                                e2m1x8_to_half2(word_of(now[d][h].codes, j), a[h]);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) a[h][i] = mul_half2(a[h][i], scale[h][j / 2]);
                             }
 #pragma unroll
-                            for (int t = 0; t < kTiles; ++t)
-                                mma_f16(sum[t], a[0][0], a[1][0], a[0][1], a[1][1], b[d][t][2 * j], b[d][t][2 * j + 1]);
+                            for (int t = 0; t < kTiles; ++t) {
+                                mma_f16(sum[t], a[0][0], a[1][0], a[0][1], a[1][1], b[d][t][4 * j], b[d][t][4 * j + 1]);
+                                mma_f16(sum[t], a[0][2], a[1][2], a[0][3], a[1][3], b[d][t][4 * j + 2], b[d][t][4 * j + 3]);
+                            }
                         }
 #pragma unroll
                         for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) total[t][i] = __fmaf_rn(sum[t][i], undo[d][t][i & 1], total[t][i]);
+                            for (int i = 0; i < 4; ++i)
+                                total[t][i] = d == 0 ? sum[t][i] * undo[d][t][i & 1]
+                                                     : __fmaf_rn(sum[t][i], undo[d][t][i & 1], total[t][i]);
                     }
 #pragma unroll
                     for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int column = 8 * t + 2 * c + (i & 1), r = tile + g + 8 * (i >> 1);
-                            if (column < used) {
-                                float* slot = partial + (warp * used + column) * block_rows + r;
-                                *slot = pass == 0 ? total[t][i] : *slot + total[t][i];
+                        for (int i = 0; i < 2; ++i)
+                            if (8 * t + 2 * c + i < used) {
+                                float* at = slot + (8 * t + i) * block_rows;
+                                if (pass > 0) {
+                                    total[t][i] += at[0];
+                                    total[t][i + 2] += at[8];
+                                }
+                                at[0] = total[t][i];
+                                at[8] = total[t][i + 2];
                             }
-                        }
                 }
             }
             __syncthreads();
@@ -325,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
     }
 }
 
-template <bool kFp32, int kTiles, int kDepth, bool kVector>
+template <bool kFp32, int kTiles, int kDepth, bool kVector, int kBlock>
 int launch(Params p, cudaStream_t stream) {
     constexpr int kTokens = kTiles * 8 / (kFp32 ? 3 : 1);
     const int used = (p.tokens < kTokens ? p.tokens : kTokens) * (kFp32 ? 3 : 1);
@@ -335,24 +449,27 @@ int launch(Params p, cudaStream_t stream) {
     const int need = (own + 15) / 16 * 16;
     if (block > need) block = need;
     p.rows_per_block = block;
-    const size_t bytes = (size_t)kWarps * used * block * sizeof(float);
-    auto* kernel = packed_matvec_kernel<kFp32, kTiles, kDepth, kVector>;
-    const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPartialFloats * 4);
+    constexpr size_t kRingBytes = kVector ? kRing * kDepth * 2 * kThreads * sizeof(uint4) : 0;
+    const size_t bytes = kRingBytes + (size_t)kWarps * used * block * sizeof(float);
+    auto* kernel = packed_matvec_kernel<kFp32, kTiles, kDepth, kVector, kBlock>;
+    const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   (int)kRingBytes + kPartialFloats * 4);
     if (error != cudaSuccess) return record_cuda_error(error);
     kernel<<<grid, kThreads, bytes, stream>>>(p);
     return check_launch();
 }
 
-template <bool kVector>
+template <bool kVector, int kBlock>
 int dispatch(const Params& p, bool fp32, cudaStream_t s) {
+    constexpr int kDepth = kVector ? 2 : 1;
     if (fp32) {
-        if (p.tokens <= 2) return launch<true, 1, 2, kVector>(p, s);
-        if (p.tokens <= 5) return launch<true, 2, 1, kVector>(p, s);
-        return launch<true, 4, 1, kVector>(p, s);
+        if (p.tokens <= 2) return launch<true, 1, kDepth, kVector, kBlock>(p, s);
+        if (p.tokens <= 5) return launch<true, 2, 1, kVector, kBlock>(p, s);
+        return launch<true, 4, 1, kVector, kBlock>(p, s);
     }
-    if (p.tokens <= 8) return launch<false, 1, 2, kVector>(p, s);
-    if (p.tokens <= 16) return launch<false, 2, 1, kVector>(p, s);
-    return launch<false, 4, 1, kVector>(p, s);
+    if (p.tokens <= 8) return launch<false, 1, kDepth, kVector, kBlock>(p, s);
+    if (p.tokens <= 16) return launch<false, 2, 1, kVector, kBlock>(p, s);
+    return launch<false, 4, 1, kVector, kBlock>(p, s);
 }
 
 }  // namespace matvec
@@ -367,7 +484,10 @@ extern "C" int ue5m3_packed_matvec(const void* x, int x_dtype, int64_t tokens, i
         return UE5M3_ERR_INVALID_ARGUMENT;
     if ((x_dtype | out_dtype | bias_dtype) & ~1) return UE5M3_ERR_INVALID_ARGUMENT;
     if (block != 16 && block != 32) return UE5M3_ERR_BLOCK_SIZE;
-    if (tokens > (1 << 24) || rows > (1 << 30) || cols > (1 << 30)) return UE5M3_ERR_TOO_LARGE;
+    if (tokens > (1 << 24) || rows > (1 << 30) || cols > (1 << 22)) {
+        record_error_text("at most 2^24 tokens, 2^30 rows and 2^22 columns");
+        return UE5M3_ERR_TOO_LARGE;
+    }
     const bool fp32 = x_dtype == UE5M3_DTYPE_FP32;
     const int element = fp32 ? 4 : 2;
     if ((uintptr_t)x % element || (uintptr_t)out % (out_dtype == UE5M3_DTYPE_FP32 ? 4 : 2) ||
@@ -386,14 +506,14 @@ extern "C" int ue5m3_packed_matvec(const void* x, int x_dtype, int64_t tokens, i
     p.tokens = (int)tokens;
     p.rows = (int)rows;
     p.k = (int)cols;
-    p.block_shift = block == 16 ? 4 : 5;
-    p.row_shift = two_d ? p.block_shift : 0;
-    p.vector = p.code_stride % 16 == 0 && (uintptr_t)codes % 16 == 0 &&
+    p.row_shift = !two_d ? 0 : block == 16 ? 4 : 5;
+    const bool vector = p.code_stride % 16 == 0 && (uintptr_t)codes % 16 == 0 &&
                (block == 32 || (p.scale_stride % 2 == 0 && (uintptr_t)scales % 2 == 0));
     p.vector_x = (uintptr_t)x % 16 == 0 && (ldx * element) % 16 == 0;
     p.bias_fp32 = bias_dtype == UE5M3_DTYPE_FP32;
     p.out_fp32 = out_dtype == UE5M3_DTYPE_FP32;
     p.factor = 16.0f * dec;
-    return p.vector ? matvec::dispatch<true>(p, fp32, (cudaStream_t)stream)
-                    : matvec::dispatch<false>(p, fp32, (cudaStream_t)stream);
+    cudaStream_t s = (cudaStream_t)stream;
+    if (block == 16) return vector ? matvec::dispatch<true, 16>(p, fp32, s) : matvec::dispatch<false, 16>(p, fp32, s);
+    return vector ? matvec::dispatch<true, 32>(p, fp32, s) : matvec::dispatch<false, 32>(p, fp32, s);
 }
