@@ -15,7 +15,7 @@ from pathlib import Path
 HERE = Path(__file__).resolve().parent
 SOURCES = ["abi.cu", "amax.cu", "quantize.cu", "quantize_operand.cu", "gemm_sm100.cu", "gemm_fp4_sm100.cu",
            "gemm_fallback.cu", "fallback_workspace.cu", "window_place.cu", "packed_matvec.cu", "paged_attention.cu",
-           "sample.cu"]
+           "paged_attention_wide.cu", "sample.cu"]
 OUTPUT = HERE / "lib" / "libue5m3_b200.so"
 
 

@@ -30,14 +30,6 @@ constexpr int kConsumers = 4;
 constexpr int kSmallThreads = (kConsumers + 1) * 32;
 constexpr int kSiteFull = 0x50, kSiteEmpty = 0x51;
 
-__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, unsigned long long* bar, int x, int y,
-                                            int z, int w) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
-        ::"r"(ptx::smem_u32(dst)), "l"(map), "r"(ptx::smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
-        : "memory");
-}
-
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t address) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -57,25 +49,6 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// rows of q behind the last sequence
-__device__ __forceinline__ void zero_tail_rows(const Params& p, int64_t thread, int64_t threads, int head_dim) {
-    const int64_t width = (int64_t)p.heads * head_dim / 8;  // 16-byte pieces of a row
-    const int first = min(max(p.query_starts[p.sequences], 0), p.tokens);
-    uint4* out = reinterpret_cast<uint4*>(p.out);
-    for (int64_t i = first * width + thread; i < p.tokens * width; i += threads) out[i] = make_uint4(0, 0, 0, 0);
 }
 
 // ---- new keys and values into their pages -------------------------------------------------------
@@ -167,7 +140,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
             const int box = min(kKeys, 1 << p.page_shift), boxes = kKeys / box;
             for (int tile = first; tile < last; ++tile, ++issue) {
                 const int stage = issue % kStages;
-                if (issue >= kStages && !ptx::mbar_wait(&empty[stage], ((issue / kStages) & 1) ^ 1, abort_flag,
+                if (issue >= kStages && !warp_wait(&empty[stage], ((issue / kStages) & 1) ^ 1, abort_flag,
                                                         p.status, kSiteEmpty, issue))
                     break;
                 const int key = tile * kKeys + lane * box;
@@ -216,7 +189,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
             float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
             for (int tile = first; tile < last; ++tile, ++issue) {
                 const int stage = issue % kStages;
-                if (!ptx::mbar_wait(&full[stage], (issue / kStages) & 1, abort_flag, p.status, kSiteFull, issue)) break;
+                if (!warp_wait(&full[stage], (issue / kStages) & 1, abort_flag, p.status, kSiteFull, issue)) break;
                 unsigned char* k = tiles + stage * 2 * kTileBytes;
                 unsigned char* v = k + kTileBytes;
                 const int key0 = tile * kKeys + warp * 16;  // this warp's keys
@@ -436,27 +409,37 @@ static int encode_pages(CUtensorMap* map, const void* base, const ue5m3_paged_ca
 }
 
 struct Plan {
+    bool wide;
     int row_tiles;  // per sequence and key/value head, at most
     int chunk, splits;
     size_t workspace;
 };
 
-// Splits of the keys: enough CTAs for two on every SM, runs of at least 4 and at most 16 tiles.
+// Up to 32 rows per key/value head: the kernel for few rows, whose 16-row tiles read the keys once
+// each; more: the tensor-core kernel with its 256-row tiles.  Splits of the keys: few rows, enough
+// CTAs for two on every SM, runs of 4 to 16 tiles; many rows, only where there are fewer CTAs than
+// SMs, runs of at least 8 tiles.
 static Plan make_plan(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t head_dim,
                       int64_t max_query, int64_t max_kv) {
     Plan plan;
-    const int64_t rows = max_query * (heads / kv_heads);
-    int64_t tiles = (rows + kRows - 1) / kRows;
+    const int64_t rows = max_query * (heads / kv_heads), sms = sm_count();
+    plan.wide = rows > 2 * kRows;
+    const int64_t tile_rows = plan.wide ? kWideRows : kRows;
+    int64_t tiles = (rows + tile_rows - 1) / tile_rows;
     if (tiles * kv_heads > 65535) tiles = 65535 / kv_heads;
     plan.row_tiles = (int)tiles;
     const int64_t all = (max_kv + kKeys - 1) / kKeys, lists = sequences * kv_heads * tiles;
-    int64_t chunk = (all * lists + 2 * sm_count() - 1) / (2 * sm_count());
-    chunk = chunk < 4 ? 4 : chunk > 16 ? 16 : chunk;
-    int64_t splits = all > 0 ? (all + chunk - 1) / chunk : 1;
-    if (rows > 4 * kRows) splits = 1;  // enough row tiles; a workspace of `splits` outputs would be large
+    int64_t chunk;
+    if (plan.wide) {
+        chunk = lists >= sms ? all : (all * lists + sms - 1) / sms;
+        chunk = ((chunk < 8 ? 8 : chunk) + 1) / 2 * 2;  // whole 128-key tiles
+    } else {
+        chunk = (all * lists + 2 * sms - 1) / (2 * sms);
+        chunk = chunk < 4 ? 4 : chunk > 16 ? 16 : chunk;
+    }
     plan.chunk = (int)chunk;
-    plan.splits = (int)splits;
-    plan.workspace = splits > 1 ? (size_t)tokens * heads * splits * (head_dim + 2) * sizeof(float) : 0;
+    plan.splits = (int)((all + chunk - 1) / chunk);
+    plan.workspace = plan.splits > 1 ? (size_t)tokens * heads * plan.splits * (head_dim + 2) * sizeof(float) : 0;
     return plan;
 }
 
@@ -471,16 +454,21 @@ int launch(const Params& p, const Plan& plan, const CUtensorMap& k_map, const CU
         const int status = check_launch();
         if (status != UE5M3_OK) return status;
     }
-    const cudaError_t error = cudaFuncSetAttribute(attention_small_kernel<kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   SmallShared<kDim>::kBytes);
-    if (error != cudaSuccess) return record_cuda_error(error);
     const dim3 grid(plan.splits, p.kv_heads * plan.row_tiles, p.sequences);
-    attention_small_kernel<kDim><<<grid, kSmallThreads, SmallShared<kDim>::kBytes, stream>>>(p, k_map, v_map);
-    int status = check_launch();
+    int status;
+    if (plan.wide) {
+        status = launch_wide(p, kDim, grid, k_map, v_map, stream);
+    } else {
+        const cudaError_t error = cudaFuncSetAttribute(
+            attention_small_kernel<kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, SmallShared<kDim>::kBytes);
+        if (error != cudaSuccess) return record_cuda_error(error);
+        attention_small_kernel<kDim><<<grid, kSmallThreads, SmallShared<kDim>::kBytes, stream>>>(p, k_map, v_map);
+        status = check_launch();
+    }
     if (status != UE5M3_OK || plan.splits == 1) return status;
     int64_t blocks = max_query * p.heads;
     if (blocks > 65535) blocks = 65535;
-    combine_kernel<kDim><<<dim3((unsigned)blocks, p.sequences), 128, 0, stream>>>(p, kRows);
+    combine_kernel<kDim><<<dim3((unsigned)blocks, p.sequences), 128, 0, stream>>>(p, plan.wide ? kWideRows : kRows);
     return check_launch();
 }
 
@@ -510,7 +498,7 @@ extern "C" int ue5m3_paged_attention(const void* q, int64_t q_token_stride, int6
     using namespace ue5m3;
     using namespace ue5m3::paged;
     if (!q || !cache || !kv_lengths || !query_starts || !out || !cache->k_pages || !cache->v_pages ||
-        !cache->page_table || (new_k == nullptr) != (new_v == nullptr) || !(scale == scale))
+        !cache->page_table || (new_k == nullptr) != (new_v == nullptr) || !(scale > 0.0f) || scale > 3e38f)
         return UE5M3_ERR_INVALID_ARGUMENT;
     const int64_t dim = cache->head_dim;
     if (!paged_sizes_ok(tokens, cache->sequences, heads, cache->kv_heads, dim, max_query, max_kv) || cache->pages <= 0 ||

@@ -13,6 +13,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "tcgen05_ptx.cuh"
+
 namespace ue5m3 {
 namespace paged {
 
@@ -62,9 +64,10 @@ __device__ __forceinline__ int visible_keys(const Params& p, const Sequence& s, 
     return max(0, s.keys - s.queries + last + 1);
 }
 
-// key tiles per split for a row tile that sees `tiles` of them
+// key tiles per split for a row tile that sees `tiles` of them, an even number if the plan's is
 __device__ __forceinline__ int split_chunk(const Params& p, int tiles) {
-    return max(p.chunk, (tiles + p.splits - 1) / p.splits);
+    const int least = (tiles + p.splits - 1) / p.splits;
+    return max(p.chunk, p.chunk & 1 ? least : (least + 1) & ~1);
 }
 
 // The page of a key, or -1 where the table names none of the cache's.
@@ -72,6 +75,46 @@ __device__ __forceinline__ int page_of(const Params& p, int b, int key) {
     const int page = __ldg(p.page_table + (int64_t)b * p.table_stride + (key >> p.page_shift));
     return page >= 0 && page < p.pages ? page : -1;
 }
+
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, unsigned long long* bar, int x, int y,
+                                            int z, int w) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+        ::"r"(ptx::smem_u32(dst)), "l"(map), "r"(ptx::smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+        : "memory");
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// rows of q behind the last sequence
+__device__ __forceinline__ void zero_tail_rows(const Params& p, int64_t thread, int64_t threads, int head_dim) {
+    const int64_t width = (int64_t)p.heads * head_dim / 8;  // 16-byte pieces of a row
+    const int first = min(max(p.query_starts[p.sequences], 0), p.tokens);
+    uint4* out = reinterpret_cast<uint4*>(p.out);
+    for (int64_t i = first * width + thread; i < p.tokens * width; i += threads) out[i] = make_uint4(0, 0, 0, 0);
+}
+
+// mbar_wait with one answer for the whole (converged) warp
+__device__ __forceinline__ bool warp_wait(unsigned long long* bar, uint32_t parity, int* abort_flag, int* status, int where,
+                                          int iter) {
+    return __all_sync(0xFFFFFFFFu, ptx::mbar_wait(bar, parity, abort_flag, status, where, iter));
+}
+
+// ---- the kernel for many rows (paged_attention_wide.cu) ------------------------------------------
+
+constexpr int kWideRows = 256;  // rows of one CTA
+
+int launch_wide(const Params& p, int head_dim, dim3 grid, const CUtensorMap& k_map, const CUtensorMap& v_map,
+                cudaStream_t stream);
 
 }  // namespace paged
 }  // namespace ue5m3

@@ -1,0 +1,438 @@
+// Attention of a chunk of new tokens over a paged key/value cache: the kernel for many rows (prompt
+// chunks).
+//
+// What bounds it: the tensor cores (4 * head_dim flops per row and visible key) and, nearly as much,
+// the exponentials.  One CTA owns 256 rows of a key/value head (its query heads side by side, see
+// paged_attention.cuh) as two tiles of 128, so that one tile's softmax runs while the other's
+// products do.  Per 128 keys: S = Q K^T (tcgen05.mma, both operands in shared memory) into TMEM; a
+// warpgroup per tile, one thread per row, reads S, keeps the running maximum and sum in fp32 and
+// writes the probabilities as bf16 over S; O += P V with P read from TMEM and V [keys][channels]
+// as it lies in the cache (the N-major operand), O in fp32 in TMEM.
+//
+// TMEM: S/P of the two tiles 128 columns each, O head_dim columns each.  The output is rescaled
+// only when a row's maximum has grown by more than 2^8 since the last time (probabilities then stay
+// below 2^8, which bf16 and the fp32 sums hold as well as any), so that TMEM is hardly ever read
+// and written between products.
+//
+// Warps: 0 TMA (keys and values page by page into two stages of 128 keys each), 1 MMA issue and
+// TMEM, 4..7 and 8..11 the softmax of the two tiles (TMEM lanes by warp % 4); 2 and 3 idle.
+#include <math.h>
+
+#include "abi_common.cuh"
+#include "paged_attention.cuh"
+#include "tcgen05_ptx.cuh"
+
+namespace ue5m3 {
+namespace paged {
+
+constexpr int kWideKeys = 128;   // keys of a stage
+constexpr int kWideStages = 2;
+constexpr int kWideThreads = 384;
+constexpr float kRescale = 8.0f;  // log2 of the growth of a maximum that is left in the probabilities
+constexpr int kSiteWide = 0x60;
+
+template <int kDim>
+struct WideShared {
+    static constexpr int kSlabs = kDim / 64;
+    static constexpr int kTileBytes = 128 * kDim * 2;  // 128 rows or keys: kSlabs x [128][128 bytes], swizzled
+    static constexpr int kQ = 0;
+    static constexpr int kK = 2 * kTileBytes;
+    static constexpr int kV = kK + kWideStages * kTileBytes;
+    static constexpr int kBarriers = kV + kWideStages * kTileBytes;
+    static constexpr int kBytes = kBarriers + 256 + 1024;
+};
+
+struct WideBarriers {
+    unsigned long long k_full[kWideStages], k_empty[kWideStages], v_full[kWideStages], v_empty[kWideStages];
+    unsigned long long q_ready, s_full[2], p_ready[2], o_done[2], drained;
+    uint32_t tmem;
+    int abort_flag, bad;
+};
+
+// Instruction descriptor for kind::f16, D = F32, A = B = BF16; b_rows: B is [k][n] in memory
+__host__ __device__ constexpr uint32_t wide_idesc(int m, int n, bool b_rows) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((b_rows ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+           ((uint32_t)(m >> 4) << 24);
+}
+
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+
+// B operand [k][n], n contiguous: 64-channel slabs of [keys][128 bytes], 128-byte swizzle; slabs
+// are kWideKeys * 128 bytes apart, groups of eight keys 1024 bytes
+__device__ __forceinline__ uint64_t desc_rows(uint32_t address) {
+    uint64_t desc = 0;
+    desc |= (uint64_t)((address & 0x3FFFFu) >> 4);
+    desc |= (uint64_t)((kWideKeys * 128) >> 4) << 16;
+    desc |= (uint64_t)(1024 >> 4) << 32;
+    desc |= (uint64_t)1 << 46;
+    desc |= (uint64_t)2 << 61;
+    return desc;
+}
+
+__device__ __forceinline__ void tmem_store_16(uint32_t address, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16};" ::"r"(address),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_store_32(uint32_t address, const uint32_t (&r)[32]) {
+    uint32_t half[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) half[i] = r[i];
+    tmem_store_16(address, half);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) half[i] = r[16 + i];
+    tmem_store_16(address + 16, half);
+}
+
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <int kDim>
+__global__ void __launch_bounds__(kWideThreads, 1)
+    attention_wide_kernel(const Params p, const __grid_constant__ CUtensorMap k_map,
+                          const __grid_constant__ CUtensorMap v_map) {
+    using Shared = WideShared<kDim>;
+    constexpr int kSlabs = Shared::kSlabs, kTileBytes = Shared::kTileBytes;
+    extern __shared__ unsigned char raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    WideBarriers& bar = *reinterpret_cast<WideBarriers*>(smem + Shared::kBarriers);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int b = blockIdx.z;
+    const int row_tiles = gridDim.y / p.kv_heads;
+    const int head = blockIdx.y / row_tiles;
+    const Sequence s = sequence_of(p, b);
+    if (p.zero_tail)
+        zero_tail_rows(p, ((int64_t)(blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * kWideThreads + threadIdx.x,
+                       (int64_t)gridDim.x * gridDim.y * gridDim.z * kWideThreads, kDim);
+    const int rows = s.queries * p.group;
+    if (rows == 0) return;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kWideStages; ++i) {
+            ptx::mbar_init(&bar.k_full[i], 1);
+            ptx::mbar_init(&bar.k_empty[i], 1);
+            ptx::mbar_init(&bar.v_full[i], 1);
+            ptx::mbar_init(&bar.v_empty[i], 1);
+        }
+        ptx::mbar_init(&bar.q_ready, 256);
+        ptx::mbar_init(&bar.drained, 1);
+        for (int i = 0; i < 2; ++i) {
+            ptx::mbar_init(&bar.s_full[i], 1);
+            ptx::mbar_init(&bar.p_ready[i], 128);
+            ptx::mbar_init(&bar.o_done[i], 1);
+        }
+        bar.abort_flag = p.status && *((volatile int*)p.status) != 0;  // a recorded failure: no work, NaN
+        ptx::mbar_fence_init();
+    }
+    if (warp == 1) ptx::tmem_alloc(&bar.tmem, 512);
+    ptx::tcgen05_fence_before();
+    __syncthreads();
+    ptx::tcgen05_fence_after();
+    const uint32_t tmem = bar.tmem;
+    constexpr uint32_t kS = 0, kO = 256;  // columns: S of tile t at 128 t, O at 256 + kDim t
+    int stage_count = 0;   // key stages used so far (every role counts alike)
+    int list = 0;          // row tiles done so far
+    int wait_count = 0;    // phases of the per-tile barriers so far
+    // later row tiles see more keys: they start first
+    for (int at = blockIdx.y % row_tiles; at * kWideRows < rows; at += row_tiles) {
+        const int in_wave = (rows + kWideRows - 1) / kWideRows;
+        const int row0 = (in_wave - 1 - at) * kWideRows;
+        const int limit = visible_keys(p, s, row0, kWideRows);
+        const int all = (limit + kKeys - 1) / kKeys;  // in units of the split, 64 keys
+        const int chunk = split_chunk(p, all);
+        const int splits = (all + chunk - 1) / chunk;
+        const int first = blockIdx.x * chunk;
+        if (first >= all && blockIdx.x > 0) continue;
+        const int key_begin = first * kKeys, key_end = min(limit, (first + chunk) * kKeys);
+        const int tiles = (key_end - key_begin + kWideKeys - 1) / kWideKeys;
+        __syncthreads();
+        if (threadIdx.x == 0) bar.bad = s.cut;
+        __syncthreads();
+        const bool dead = *((volatile int*)&bar.abort_flag) != 0;
+        if (warp == 0) {
+            if (!dead) {
+                const int box = min(kKeys, 1 << p.page_shift), boxes = kWideKeys / box;
+                int j = 0;
+                for (; j < tiles; ++j) {
+                    const int n = stage_count + j, stage = n % kWideStages, parity = (n / kWideStages) & 1;
+                    const int key = key_begin + j * kWideKeys + lane * box;
+                    const bool wanted = lane < boxes && key < key_end;
+                    const int page = wanted ? page_of(p, b, key) : -1;
+                    if (wanted && page < 0) bar.bad = 1;
+                    const uint32_t bytes = __popc(__ballot_sync(0xFFFFFFFFu, page >= 0)) * box * kDim * 2;
+                    const int slot = key & ((1 << p.page_shift) - 1);
+                    unsigned char* to = smem + Shared::kK + stage * kTileBytes + lane * box * 128;
+                    if (n >= kWideStages &&
+                        !warp_wait(&bar.k_empty[stage], parity ^ 1, &bar.abort_flag, p.status, kSiteWide, n))
+                        break;
+                    if (lane == 0) ptx::mbar_arrive_expect_tx(&bar.k_full[stage], bytes);
+                    __syncwarp();
+                    if (page >= 0)
+                        for (int i = 0; i < kSlabs; ++i)
+                            tma_load_4d(to + i * kWideKeys * 128, &k_map, &bar.k_full[stage], i * 64, head, slot, page);
+                    if (n >= kWideStages &&
+                        !warp_wait(&bar.v_empty[stage], parity ^ 1, &bar.abort_flag, p.status, kSiteWide + 1, n)) {
+                        // the copy of K of this tile lands before its memory is given up
+                        for (int spin = 0; spin < 1000000 && !ptx::mbar_try_wait(&bar.k_full[stage], parity);) ++spin;
+                        break;
+                    }
+                    if (lane == 0) ptx::mbar_arrive_expect_tx(&bar.v_full[stage], bytes);
+                    __syncwarp();
+                    to += Shared::kV - Shared::kK;
+                    if (page >= 0)
+                        for (int i = 0; i < kSlabs; ++i)
+                            tma_load_4d(to + i * kWideKeys * 128, &v_map, &bar.v_full[stage], i * 64, head, slot, page);
+                }
+                if (*((volatile int*)&bar.abort_flag))
+                    for (int i = max(0, stage_count + j - kWideStages); i < stage_count + j; ++i)
+                        for (int spin = 0; spin < 1000000 && !(ptx::mbar_try_wait(&bar.k_full[i % kWideStages], (i / kWideStages) & 1) &&
+                                                               ptx::mbar_try_wait(&bar.v_full[i % kWideStages], (i / kWideStages) & 1));)
+                            ++spin;
+            }
+        } else if (warp == 1) {
+            constexpr uint32_t kIdescS = wide_idesc(128, kWideKeys, false), kIdescO = wide_idesc(128, kDim, true);
+            const uint32_t base = ptx::smem_u32(smem);
+            auto scores = [&](int t, int stage) {
+                if (ptx::elect_one()) {
+#pragma unroll
+                    for (int i = 0; i < kDim / 16; ++i) {
+                        const uint32_t off = (i / 4) * kWideKeys * 128 + (i % 4) * 32;
+                        umma_ss(tmem + kS + 128 * t, ptx::smem_desc_sw128(base + Shared::kQ + t * kTileBytes + off),
+                                ptx::smem_desc_sw128(base + Shared::kK + stage * kTileBytes + off), kIdescS, i > 0);
+                    }
+                    ptx::umma_commit(&bar.s_full[t]);
+                    if (t == 1) ptx::umma_commit(&bar.k_empty[stage]);
+                }
+                __syncwarp();
+            };
+            auto values = [&](int t, int stage, bool accumulate) {
+                if (ptx::elect_one()) {
+#pragma unroll
+                    for (int i = 0; i < kWideKeys / 16; ++i)
+                        umma_ts(tmem + kO + kDim * t, tmem + kS + 128 * t + 8 * i,
+                                desc_rows(base + Shared::kV + stage * kTileBytes + i * 2048), kIdescO, accumulate || i > 0);
+                    ptx::umma_commit(&bar.o_done[t]);
+                    if (t == 1) ptx::umma_commit(&bar.v_empty[stage]);
+                }
+                __syncwarp();
+            };
+            auto wait = [&](unsigned long long* which, uint32_t parity, int site) {
+                const bool ok = warp_wait(which, parity, &bar.abort_flag, p.status, kSiteWide + site, wait_count);
+                ptx::tcgen05_fence_after();
+                return ok;
+            };
+            bool ok = !dead && tiles > 0 && wait(&bar.q_ready, list & 1, 2);
+            ok = ok && wait(&bar.k_full[stage_count % kWideStages], (stage_count / kWideStages) & 1, 3);
+            if (ok) {
+                scores(0, stage_count % kWideStages);
+                scores(1, stage_count % kWideStages);
+            }
+            for (int j = 0; ok && j < tiles; ++j) {
+                const int n = stage_count + j, stage = n % kWideStages, next = (n + 1) % kWideStages;
+                for (int t = 0; ok && t < 2; ++t) {
+                    ok = wait(&bar.p_ready[t], (wait_count + j) & 1, 4);
+                    if (ok && t == 0) ok = wait(&bar.v_full[stage], (n / kWideStages) & 1, 5);
+                    if (!ok) break;
+                    values(t, stage, j > 0);
+                    if (j + 1 < tiles) {
+                        if (t == 0) ok = wait(&bar.k_full[next], ((n + 1) / kWideStages) & 1, 6);
+                        if (ok) scores(t, next);
+                    }
+                }
+            }
+        } else if (warp >= 4) {
+            const int t = (warp - 4) / 4, r = (warp % 4) * 32 + lane;  // tile, row in it
+            const uint32_t lanes = tmem + ((uint32_t)((warp % 4) * 32) << 16);
+            const int row = row0 + t * 128 + r;
+            const int token = row / p.group;
+            const bool present = row < rows;
+            const int last_key = present ? s.keys - s.queries + token : -1;
+            const int fewest = visible_keys(p, s, min(row0 + t * 128, rows - 1), 1);  // of the tile's rows
+            float top = -INFINITY, sum = 0.0f;
+            if (!dead) {
+                // this thread's row of Q into the swizzled tile
+                const uint4* source = reinterpret_cast<const uint4*>(
+                    p.q + (int64_t)(s.first + token) * p.q_token + (int64_t)(head * p.group + row % p.group) * p.q_head);
+                unsigned char* q = smem + Shared::kQ + t * kTileBytes + r * 128;
+#pragma unroll
+                for (int i = 0; i < kDim / 8; ++i)
+                    *reinterpret_cast<uint4*>(q + (i / 8) * 128 * 128 + (((i & 7) ^ (r & 7)) << 4)) =
+                        present ? source[i] : make_uint4(0, 0, 0, 0);
+                asm volatile("fence.proxy.async;" ::: "memory");
+                ptx::mbar_arrive(&bar.q_ready);
+            }
+            bool ok = !dead;
+            for (int j = 0; ok && j < tiles; ++j) {
+                const int key0 = key_begin + j * kWideKeys;
+                const uint32_t parity = (wait_count + j) & 1;
+                ok = warp_wait(&bar.s_full[t], parity, &bar.abort_flag, p.status, kSiteWide + 8, j);
+                if (!ok) break;
+                ptx::tcgen05_fence_after();
+                const bool masked = key0 + kWideKeys > fewest;
+                uint32_t x[32];
+                float now = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    ptx::tmem_load_32_async(lanes + kS + 128 * t + 32 * i, x);
+                    ptx::tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const float v = __uint_as_float(x[e]);
+                        now = fmaxf(now, masked && key0 + 32 * i + e > last_key ? -INFINITY : v);
+                    }
+                }
+                now *= p.scale_log2;
+                if (__any_sync(0xFFFFFFFFu, now > top + kRescale || (top == -INFINITY && now > top))) {
+                    // the maximum moves; what has been summed so far fades
+                    const float moved = fmaxf(top, now);
+                    const float fade = moved == -INFINITY ? 1.0f : exp2_approx(top - moved);
+                    sum *= fade;
+                    top = moved;
+                    if (j > 0) {
+                        ok = warp_wait(&bar.o_done[t], parity ^ 1, &bar.abort_flag, p.status, kSiteWide + 9, j);
+                        if (!ok) break;
+                        ptx::tcgen05_fence_after();
+#pragma unroll 1
+                        for (int i = 0; i < kDim / 32; ++i) {
+                            ptx::tmem_load_32_async(lanes + kO + kDim * t + 32 * i, x);
+                            ptx::tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * fade);
+                            tmem_store_32(lanes + kO + kDim * t + 32 * i, x);
+                        }
+                    }
+                }
+                const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    ptx::tmem_load_32_async(lanes + kS + 128 * t + 32 * i, x);
+                    ptx::tmem_wait_ld();
+                    uint32_t packed[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        float y[2];
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const float v = exp2_approx(__fmaf_rn(__uint_as_float(x[e + k]), p.scale_log2, -base));
+                            y[k] = masked && key0 + 32 * i + e + k > last_key ? 0.0f : v;
+                            sum += y[k];
+                        }
+                        packed[e / 2] = pack_bf16(y[0], y[1]);
+                    }
+                    tmem_store_16(lanes + kS + 128 * t + 16 * i, packed);
+                }
+                if (t == 0 && key0 + kWideKeys > key_end) {
+                    // rows of V behind the last key may hold anything: 0 * NaN is not 0
+                    const int n = stage_count + j, stage = n % kWideStages;
+                    ok = warp_wait(&bar.v_full[stage], (n / kWideStages) & 1, &bar.abort_flag, p.status, kSiteWide + 10, j);
+                    if (!ok) break;
+                    if (key0 + r >= key_end) {
+                        unsigned char* v = smem + Shared::kV + stage * kTileBytes + r * 128;
+#pragma unroll
+                        for (int i = 0; i < kDim / 8; ++i)
+                            *reinterpret_cast<uint4*>(v + (i / 8) * kWideKeys * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    asm volatile("fence.proxy.async;" ::: "memory");
+                }
+                tmem_wait_st();
+                ptx::tcgen05_fence_before();
+                ptx::mbar_arrive(&bar.p_ready[t]);
+            }
+            if (ok && tiles > 0)
+                ok = warp_wait(&bar.o_done[t], (wait_count + tiles - 1) & 1, &bar.abort_flag, p.status, kSiteWide + 11, 0);
+            ptx::tcgen05_fence_after();
+            __syncwarp();
+            const bool failed = !ok || *((volatile int*)&bar.abort_flag) || *((volatile int*)&bar.bad);
+            const int64_t out_at = (int64_t)(s.first + token) * p.heads + head * p.group + row % p.group;
+            const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll 1
+            for (int i = 0; i < kDim / 32; ++i) {
+                uint32_t x[32];
+                __syncwarp();
+                if (tiles > 0 && !dead) {
+                    ptx::tmem_load_32_async(lanes + kO + kDim * t + 32 * i, x);
+                    ptx::tmem_wait_ld();
+                }
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    float v = tiles > 0 && !dead ? __uint_as_float(x[e]) : 0.0f;
+                    if (sum == 0.0f) v = 0.0f;
+                    if (failed) v = __uint_as_float(0x7FC00000u);
+                    x[e] = __float_as_uint(v);
+                }
+                if (present && splits <= 1) {
+                    uint4* to = reinterpret_cast<uint4*>(p.out + out_at * kDim + 32 * i);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            w[k] = pack_bf16(__uint_as_float(x[8 * e + 2 * k]) * inverse,
+                                             __uint_as_float(x[8 * e + 2 * k + 1]) * inverse);
+                        to[e] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                } else if (present) {
+                    float4* to = reinterpret_cast<float4*>(p.partial + (out_at * p.splits + blockIdx.x) * kDim + 32 * i);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        to[e] = make_float4(__uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1]),
+                                            __uint_as_float(x[4 * e + 2]), __uint_as_float(x[4 * e + 3]));
+                }
+            }
+            if (splits > 1 && present) {
+                float* stats = p.partial + (int64_t)p.tokens * p.heads * p.splits * kDim + (out_at * p.splits + blockIdx.x) * 2;
+                stats[0] = failed ? 0.0f : top;
+                stats[1] = failed ? __uint_as_float(0x7FC00000u) : sum;
+            }
+            ptx::tcgen05_fence_before();
+        }
+        stage_count += tiles;
+        wait_count += tiles;
+        ++list;
+    }
+    __syncthreads();
+    if (warp == 1) {
+        if (*((volatile int*)&bar.abort_flag)) {
+            // products in flight end before their memory is given up
+            if (ptx::elect_one()) ptx::umma_commit(&bar.drained);
+            __syncwarp();
+            for (int spin = 0; spin < 1000000 && !ptx::mbar_try_wait(&bar.drained, 0);) ++spin;
+            __syncwarp();
+        }
+        ptx::tcgen05_fence_after();
+        ptx::tmem_dealloc(tmem, 512);
+    }
+}
+
+template <int kDim>
+static int launch_wide_dim(const Params& p, dim3 grid, const CUtensorMap& k_map, const CUtensorMap& v_map,
+                           cudaStream_t stream) {
+    const cudaError_t error = cudaFuncSetAttribute(attention_wide_kernel<kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   WideShared<kDim>::kBytes);
+    if (error != cudaSuccess) return record_cuda_error(error);
+    attention_wide_kernel<kDim><<<grid, kWideThreads, WideShared<kDim>::kBytes, stream>>>(p, k_map, v_map);
+    return check_launch();
+}
+
+int launch_wide(const Params& p, int head_dim, dim3 grid, const CUtensorMap& k_map, const CUtensorMap& v_map,
+                cudaStream_t stream) {
+    return head_dim == 64 ? launch_wide_dim<64>(p, grid, k_map, v_map, stream)
+                          : launch_wide_dim<128>(p, grid, k_map, v_map, stream);
+}
+
+}  // namespace paged
+}  // namespace ue5m3

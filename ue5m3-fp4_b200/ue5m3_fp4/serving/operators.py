@@ -196,6 +196,7 @@ def paged_attention(
     _require(max_query_length > 0, "max_query_length must be positive")
     if scale is None:
         scale = head_dim ** -0.5
+    _require(0 < scale < float("inf"), "scale must be positive and finite")
     if (new_k is None) != (new_v is None):
         raise ValueError("new_k and new_v come together")
     for name, tensor in (("new_k", new_k), ("new_v", new_v)):
