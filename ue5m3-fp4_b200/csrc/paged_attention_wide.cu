@@ -30,6 +30,8 @@ constexpr int kWideStages = 2;
 constexpr int kWideThreads = 384;
 constexpr float kRescale = 8.0f;  // log2 of the growth of a maximum that is left in the probabilities
 constexpr int kSiteWide = 0x60;
+constexpr int kProducerRegisters = 88, kSoftmaxRegisters = 208;  // 128 * 88 + 256 * 208 <= 384 * 168
+constexpr int kPolynomial = 3;  // of every eight pairs of exponentials, those computed on the fp32 pipe
 
 template <int kDim>
 struct WideShared {
@@ -90,17 +92,90 @@ __device__ __forceinline__ void tmem_store_16(uint32_t address, const uint32_t (
         : "memory");
 }
 
-__device__ __forceinline__ void tmem_store_32(uint32_t address, const uint32_t (&r)[32]) {
-    uint32_t half[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) half[i] = r[i];
-    tmem_store_16(address, half);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) half[i] = r[16 + i];
-    tmem_store_16(address + 16, half);
+__device__ __forceinline__ void tmem_load_16(uint32_t address, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+        "[%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(address)
+        : "memory");
+}
+
+template <int kValue>
+struct Number {
+    static constexpr int value = kValue;
+};
+
+// two fp32 operations in one instruction
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+    return d;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// 2^x of a pair on the fp32 pipe: x = n + f, n the nearest integer, 2^f by a polynomial of degree 3
+// fitted on [-1/2, 1/2] (relative error below 7.5e-5; the rounding of the result to bf16 is 2^-8),
+// n added to the exponent.  x below -126 counts as -126.
+__device__ __forceinline__ void exp2_pair(uint64_t x, float& lo, float& hi) {
+    float a, b;
+    unpack2(x, a, b);
+    x = pack2(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+    const uint64_t magic = pack2(12582912.0f, 12582912.0f);  // 1.5 * 2^23: the sum's low bits are n
+    const uint64_t n = add2(x, magic);
+    const uint64_t f = fma2(add2(n, pack2(-12582912.0f, -12582912.0f)), pack2(-1.0f, -1.0f), x);
+    uint64_t y = pack2(0.05517132207751274f, 0.05517132207751274f);
+    y = fma2(y, f, pack2(0.24261054396629333f, 0.24261054396629333f));
+    y = fma2(y, f, pack2(0.6932609677314758f, 0.6932609677314758f));
+    y = fma2(y, f, pack2(0.9999281167984009f, 0.9999281167984009f));
+    float n0, n1;
+    unpack2(n, n0, n1);
+    unpack2(y, lo, hi);
+    lo = __int_as_float(__float_as_int(lo) + (__float_as_int(n0) << 23));
+    hi = __int_as_float(__float_as_int(hi) + (__float_as_int(n1) << 23));
 }
 
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// one row tile's work
+struct Job {
+    int row0, limit, key_begin, key_end, tiles, splits;
+    bool mine;  // this CTA's split has keys of it, or it is the one that writes the zeros of rows without any
+};
+
+// later row tiles see more keys: they come first
+__device__ __forceinline__ Job job_of(const Params& p, const Sequence& s, int rows, int at) {
+    Job job;
+    job.row0 = ((rows + kWideRows - 1) / kWideRows - 1 - at) * kWideRows;
+    job.limit = visible_keys(p, s, job.row0, kWideRows);
+    const int all = (job.limit + kKeys - 1) / kKeys;  // in units of the split, 64 keys
+    const int chunk = split_chunk(p, all);
+    job.splits = (all + chunk - 1) / chunk;
+    const int first = blockIdx.x * chunk;
+    job.mine = first < all || blockIdx.x == 0;
+    job.key_begin = first * kKeys;
+    job.key_end = min(job.limit, (first + chunk) * kKeys);
+    job.tiles = (job.key_end - job.key_begin + kWideKeys - 1) / kWideKeys;
+    return job;
+}
 
 template <int kDim>
 __global__ void __launch_bounds__(kWideThreads, 1)
@@ -144,25 +219,23 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     ptx::tcgen05_fence_after();
     const uint32_t tmem = bar.tmem;
     constexpr uint32_t kS = 0, kO = 256;  // columns: S of tile t at 128 t, O at 256 + kDim t
-    int stage_count = 0;   // key stages used so far (every role counts alike)
+    int stage_count = 0;   // key stages used so far (every role counts alike); also the per-tile barriers' phases
     int list = 0;          // row tiles done so far
-    int wait_count = 0;    // phases of the per-tile barriers so far
-    // later row tiles see more keys: they start first
-    for (int at = blockIdx.y % row_tiles; at * kWideRows < rows; at += row_tiles) {
-        const int in_wave = (rows + kWideRows - 1) / kWideRows;
-        const int row0 = (in_wave - 1 - at) * kWideRows;
-        const int limit = visible_keys(p, s, row0, kWideRows);
-        const int all = (limit + kKeys - 1) / kKeys;  // in units of the split, 64 keys
-        const int chunk = split_chunk(p, all);
-        const int splits = (all + chunk - 1) / chunk;
-        const int first = blockIdx.x * chunk;
-        if (first >= all && blockIdx.x > 0) continue;
-        const int key_begin = first * kKeys, key_end = min(limit, (first + chunk) * kKeys);
-        const int tiles = (key_end - key_begin + kWideKeys - 1) / kWideKeys;
+    // between two row tiles; true when a wait gave up, here or in an earlier launch
+    auto begin = [&]() {
         __syncthreads();
         if (threadIdx.x == 0) bar.bad = s.cut;
         __syncthreads();
-        const bool dead = *((volatile int*)&bar.abort_flag) != 0;
+        return *((volatile int*)&bar.abort_flag) != 0;
+    };
+    if (warp < 4) {
+        // a row's 128 scores live in registers: what these roles do not need goes to the softmax
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegisters));
+    for (int at = blockIdx.y % row_tiles; at * kWideRows < rows; at += row_tiles) {
+        const Job job = job_of(p, s, rows, at);
+        if (!job.mine) continue;
+        const int key_begin = job.key_begin, key_end = job.key_end, tiles = job.tiles;
+        const bool dead = begin();
         if (warp == 0) {
             if (!dead) {
                 const int box = min(kKeys, 1 << p.page_shift), boxes = kWideKeys / box;
@@ -231,7 +304,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 __syncwarp();
             };
             auto wait = [&](unsigned long long* which, uint32_t parity, int site) {
-                const bool ok = warp_wait(which, parity, &bar.abort_flag, p.status, kSiteWide + site, wait_count);
+                const bool ok = warp_wait(which, parity, &bar.abort_flag, p.status, kSiteWide + site, stage_count);
                 ptx::tcgen05_fence_after();
                 return ok;
             };
@@ -244,7 +317,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             for (int j = 0; ok && j < tiles; ++j) {
                 const int n = stage_count + j, stage = n % kWideStages, next = (n + 1) % kWideStages;
                 for (int t = 0; ok && t < 2; ++t) {
-                    ok = wait(&bar.p_ready[t], (wait_count + j) & 1, 4);
+                    ok = wait(&bar.p_ready[t], (stage_count + j) & 1, 4);
                     if (ok && t == 0) ok = wait(&bar.v_full[stage], (n / kWideStages) & 1, 5);
                     if (!ok) break;
                     values(t, stage, j > 0);
@@ -254,7 +327,17 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                     }
                 }
             }
-        } else if (warp >= 4) {
+        }
+        stage_count += tiles;
+        ++list;
+    }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
+    for (int at = blockIdx.y % row_tiles; at * kWideRows < rows; at += row_tiles) {
+        const Job job = job_of(p, s, rows, at);
+        if (!job.mine) continue;
+        const int row0 = job.row0, key_begin = job.key_begin, key_end = job.key_end, tiles = job.tiles, splits = job.splits;
+        const bool dead = begin();
             const int t = (warp - 4) / 4, r = (warp % 4) * 32 + lane;  // tile, row in it
             const uint32_t lanes = tmem + ((uint32_t)((warp % 4) * 32) << 16);
             const int row = row0 + t * 128 + r;
@@ -278,24 +361,29 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             bool ok = !dead;
             for (int j = 0; ok && j < tiles; ++j) {
                 const int key0 = key_begin + j * kWideKeys;
-                const uint32_t parity = (wait_count + j) & 1;
+                const uint32_t parity = (stage_count + j) & 1;
                 ok = warp_wait(&bar.s_full[t], parity, &bar.abort_flag, p.status, kSiteWide + 8, j);
                 if (!ok) break;
                 ptx::tcgen05_fence_after();
                 const bool masked = key0 + kWideKeys > fewest;
-                uint32_t x[32];
-                float now = -INFINITY;
+                uint32_t x[4][32];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) ptx::tmem_load_32_async(lanes + kS + 128 * t + 32 * i, x[i]);
+                ptx::tmem_wait_ld();
+                if (masked) {
+#pragma unroll
+                    for (int e = 0; e < 128; ++e)
+                        if (key0 + e > last_key) x[e / 32][e % 32] = 0xFF800000u;
+                }
+                float most[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    ptx::tmem_load_32_async(lanes + kS + 128 * t + 32 * i, x);
-                    ptx::tmem_wait_ld();
+                    most[i] = fmaxf(__uint_as_float(x[i][0]), __uint_as_float(x[i][1]));
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const float v = __uint_as_float(x[e]);
-                        now = fmaxf(now, masked && key0 + 32 * i + e > last_key ? -INFINITY : v);
-                    }
+                    for (int e = 2; e < 32; e += 2)
+                        most[i] = max3(most[i], __uint_as_float(x[i][e]), __uint_as_float(x[i][e + 1]));
                 }
-                now *= p.scale_log2;
+                const float now = max3(fmaxf(most[0], most[1]), most[2], most[3]) * p.scale_log2;
                 if (__any_sync(0xFFFFFFFFu, now > top + kRescale || (top == -INFINITY && now > top))) {
                     // the maximum moves; what has been summed so far fades
                     const float moved = fmaxf(top, now);
@@ -307,34 +395,48 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                         if (!ok) break;
                         ptx::tcgen05_fence_after();
 #pragma unroll 1
-                        for (int i = 0; i < kDim / 32; ++i) {
-                            ptx::tmem_load_32_async(lanes + kO + kDim * t + 32 * i, x);
+                        for (int i = 0; i < kDim / 16; ++i) {
+                            uint32_t o[16];
+                            tmem_load_16(lanes + kO + kDim * t + 16 * i, o);
                             ptx::tmem_wait_ld();
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * fade);
-                            tmem_store_32(lanes + kO + kDim * t + 32 * i, x);
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
+                            tmem_store_16(lanes + kO + kDim * t + 16 * i, o);
                         }
                     }
                 }
                 const float base = top == -INFINITY ? 0.0f : top;
+                const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2), base2 = pack2(-base, -base);
+                uint64_t sums[4] = {0, 0, 0, 0};
+                // masked keys come out as exact zeros only from the special-function unit
+                auto probabilities = [&](auto polynomial) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    ptx::tmem_load_32_async(lanes + kS + 128 * t + 32 * i, x);
-                    ptx::tmem_wait_ld();
-                    uint32_t packed[16];
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t packed[16];
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        float y[2];
-#pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            const float v = exp2_approx(__fmaf_rn(__uint_as_float(x[e + k]), p.scale_log2, -base));
-                            y[k] = masked && key0 + 32 * i + e + k > last_key ? 0.0f : v;
-                            sum += y[k];
+                        for (int e = 0; e < 32; e += 2) {
+                            const uint64_t y = fma2(pack2(__uint_as_float(x[i][e]), __uint_as_float(x[i][e + 1])), scale2, base2);
+                            float lo, hi;
+                            if ((e / 2) % 8 < decltype(polynomial)::value) {
+                                exp2_pair(y, lo, hi);
+                            } else {
+                                unpack2(y, lo, hi);
+                                lo = exp2_approx(lo);
+                                hi = exp2_approx(hi);
+                            }
+                            sums[(e / 2) % 4] = add2(sums[(e / 2) % 4], pack2(lo, hi));
+                            packed[e / 2] = pack_bf16(lo, hi);
                         }
-                        packed[e / 2] = pack_bf16(y[0], y[1]);
+                        tmem_store_16(lanes + kS + 128 * t + 16 * i, packed);
                     }
-                    tmem_store_16(lanes + kS + 128 * t + 16 * i, packed);
-                }
+                };
+                if (masked)
+                    probabilities(Number<0>());
+                else
+                    probabilities(Number<kPolynomial>());
+                float lo, hi;
+                unpack2(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])), lo, hi);
+                sum += lo + hi;
                 if (t == 0 && key0 + kWideKeys > key_end) {
                     // rows of V behind the last key may hold anything: 0 * NaN is not 0
                     const int n = stage_count + j, stage = n % kWideStages;
@@ -353,7 +455,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 ptx::mbar_arrive(&bar.p_ready[t]);
             }
             if (ok && tiles > 0)
-                ok = warp_wait(&bar.o_done[t], (wait_count + tiles - 1) & 1, &bar.abort_flag, p.status, kSiteWide + 11, 0);
+                ok = warp_wait(&bar.o_done[t], (stage_count + tiles - 1) & 1, &bar.abort_flag, p.status, kSiteWide + 11, 0);
             ptx::tcgen05_fence_after();
             __syncwarp();
             const bool failed = !ok || *((volatile int*)&bar.abort_flag) || *((volatile int*)&bar.bad);
@@ -399,10 +501,8 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 stats[1] = failed ? __uint_as_float(0x7FC00000u) : sum;
             }
             ptx::tcgen05_fence_before();
-        }
         stage_count += tiles;
-        wait_count += tiles;
-        ++list;
+    }
     }
     __syncthreads();
     if (warp == 1) {
