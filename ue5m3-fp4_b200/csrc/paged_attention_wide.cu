@@ -31,7 +31,7 @@ constexpr int kWideThreads = 384;
 constexpr float kRescale = 8.0f;  // log2 of the growth of a maximum that is left in the probabilities
 constexpr int kSiteWide = 0x60;
 constexpr int kProducerRegisters = 88, kSoftmaxRegisters = 208;  // 128 * 88 + 256 * 208 <= 384 * 168
-constexpr int kPolynomial = 3;  // of every eight pairs of exponentials, those computed on the fp32 pipe
+constexpr int kPolynomial = 0;  // of every eight pairs of exponentials, those computed on the fp32 pipe
 
 template <int kDim>
 struct WideShared {
@@ -46,7 +46,7 @@ struct WideShared {
 
 struct WideBarriers {
     unsigned long long k_full[kWideStages], k_empty[kWideStages], v_full[kWideStages], v_empty[kWideStages];
-    unsigned long long q_ready, s_full[2], p_ready[2], o_done[2], drained;
+    unsigned long long q_ready, s_full[2], p_half[2], p_ready[2], o_done[2], drained;
     uint32_t tmem;
     int abort_flag, bad;
 };
@@ -207,7 +207,8 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         ptx::mbar_init(&bar.drained, 1);
         for (int i = 0; i < 2; ++i) {
             ptx::mbar_init(&bar.s_full[i], 1);
-            ptx::mbar_init(&bar.p_ready[i], 128);
+            ptx::mbar_init(&bar.p_half[i], 4);
+            ptx::mbar_init(&bar.p_ready[i], 4);
             ptx::mbar_init(&bar.o_done[i], 1);
         }
         bar.abort_flag = p.status && *((volatile int*)p.status) != 0;  // a recorded failure: no work, NaN
@@ -278,28 +279,35 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             }
         } else if (warp == 1) {
             constexpr uint32_t kIdescS = wide_idesc(128, kWideKeys, false), kIdescO = wide_idesc(128, kDim, true);
+            // descriptors differ by constants (in units of 16 bytes), so that an issue costs an addition
             const uint32_t base = ptx::smem_u32(smem);
+            const uint64_t q_desc = ptx::smem_desc_sw128(base + Shared::kQ), k_desc = ptx::smem_desc_sw128(base + Shared::kK),
+                           v_desc = desc_rows(base + Shared::kV);
             auto scores = [&](int t, int stage) {
+                const uint64_t q = q_desc + t * (kTileBytes / 16), k = k_desc + stage * (kTileBytes / 16);
                 if (ptx::elect_one()) {
 #pragma unroll
                     for (int i = 0; i < kDim / 16; ++i) {
-                        const uint32_t off = (i / 4) * kWideKeys * 128 + (i % 4) * 32;
-                        umma_ss(tmem + kS + 128 * t, ptx::smem_desc_sw128(base + Shared::kQ + t * kTileBytes + off),
-                                ptx::smem_desc_sw128(base + Shared::kK + stage * kTileBytes + off), kIdescS, i > 0);
+                        const int off = ((i / 4) * kWideKeys * 128 + (i % 4) * 32) / 16;
+                        umma_ss(tmem + kS + 128 * t, q + off, k + off, kIdescS, i > 0);
                     }
                     ptx::umma_commit(&bar.s_full[t]);
                     if (t == 1) ptx::umma_commit(&bar.k_empty[stage]);
                 }
                 __syncwarp();
             };
-            auto values = [&](int t, int stage, bool accumulate) {
+            auto values = [&](int t, int stage, int half, bool accumulate) {
+                const uint64_t v = v_desc + stage * (kTileBytes / 16) + half * (kTileBytes / 32 / kSlabs);
                 if (ptx::elect_one()) {
 #pragma unroll
-                    for (int i = 0; i < kWideKeys / 16; ++i)
-                        umma_ts(tmem + kO + kDim * t, tmem + kS + 128 * t + 8 * i,
-                                desc_rows(base + Shared::kV + stage * kTileBytes + i * 2048), kIdescO, accumulate || i > 0);
-                    ptx::umma_commit(&bar.o_done[t]);
-                    if (t == 1) ptx::umma_commit(&bar.v_empty[stage]);
+                    for (int k = 0; k < kWideKeys / 32; ++k) {
+                        umma_ts(tmem + kO + kDim * t, tmem + kS + 128 * t + 8 * (half * (kWideKeys / 32) + k), v + k * 128,
+                                kIdescO, accumulate || k > 0);
+                    }
+                    if (half == 1) {
+                        ptx::umma_commit(&bar.o_done[t]);
+                        if (t == 1) ptx::umma_commit(&bar.v_empty[stage]);
+                    }
                 }
                 __syncwarp();
             };
@@ -316,11 +324,16 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             }
             for (int j = 0; ok && j < tiles; ++j) {
                 const int n = stage_count + j, stage = n % kWideStages, next = (n + 1) % kWideStages;
-                for (int t = 0; ok && t < 2; ++t) {
-                    ok = wait(&bar.p_ready[t], (stage_count + j) & 1, 4);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (!ok) break;
+                    ok = wait(&bar.p_half[t], n & 1, 4);
                     if (ok && t == 0) ok = wait(&bar.v_full[stage], (n / kWideStages) & 1, 5);
                     if (!ok) break;
-                    values(t, stage, j > 0);
+                    values(t, stage, 0, j > 0);
+                    ok = wait(&bar.p_ready[t], n & 1, 7);
+                    if (!ok) break;
+                    values(t, stage, 1, true);
                     if (j + 1 < tiles) {
                         if (t == 0) ok = wait(&bar.k_full[next], ((n + 1) / kWideStages) & 1, 6);
                         if (ok) scores(t, next);
@@ -365,6 +378,19 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 ok = warp_wait(&bar.s_full[t], parity, &bar.abort_flag, p.status, kSiteWide + 8, j);
                 if (!ok) break;
                 ptx::tcgen05_fence_after();
+                if (t == 0 && key0 + kWideKeys > key_end) {
+                    // rows of V behind the last key may hold anything: 0 * NaN is not 0
+                    const int n = stage_count + j, stage = n % kWideStages;
+                    ok = warp_wait(&bar.v_full[stage], (n / kWideStages) & 1, &bar.abort_flag, p.status, kSiteWide + 10, j);
+                    if (!ok) break;
+                    if (key0 + r >= key_end) {
+                        unsigned char* v = smem + Shared::kV + stage * kTileBytes + r * 128;
+#pragma unroll
+                        for (int i = 0; i < kDim / 8; ++i)
+                            *reinterpret_cast<uint4*>(v + (i / 8) * kWideKeys * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    asm volatile("fence.proxy.async;" ::: "memory");
+                }
                 const bool masked = key0 + kWideKeys > fewest;
                 uint32_t x[4][32];
 #pragma unroll
@@ -428,6 +454,12 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                             packed[e / 2] = pack_bf16(lo, hi);
                         }
                         tmem_store_16(lanes + kS + 128 * t + 16 * i, packed);
+                        if (i & 1) {  // the product with the first 64 keys starts while the others are computed
+                            tmem_wait_st();
+                            ptx::tcgen05_fence_before();
+                            __syncwarp();
+                            if (lane == 0) ptx::mbar_arrive(i == 1 ? &bar.p_half[t] : &bar.p_ready[t]);
+                        }
                     }
                 };
                 if (masked)
@@ -437,22 +469,6 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 float lo, hi;
                 unpack2(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])), lo, hi);
                 sum += lo + hi;
-                if (t == 0 && key0 + kWideKeys > key_end) {
-                    // rows of V behind the last key may hold anything: 0 * NaN is not 0
-                    const int n = stage_count + j, stage = n % kWideStages;
-                    ok = warp_wait(&bar.v_full[stage], (n / kWideStages) & 1, &bar.abort_flag, p.status, kSiteWide + 10, j);
-                    if (!ok) break;
-                    if (key0 + r >= key_end) {
-                        unsigned char* v = smem + Shared::kV + stage * kTileBytes + r * 128;
-#pragma unroll
-                        for (int i = 0; i < kDim / 8; ++i)
-                            *reinterpret_cast<uint4*>(v + (i / 8) * kWideKeys * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    asm volatile("fence.proxy.async;" ::: "memory");
-                }
-                tmem_wait_st();
-                ptx::tcgen05_fence_before();
-                ptx::mbar_arrive(&bar.p_ready[t]);
             }
             if (ok && tiles > 0)
                 ok = warp_wait(&bar.o_done[t], (stage_count + tiles - 1) & 1, &bar.abort_flag, p.status, kSiteWide + 11, 0);
