@@ -92,6 +92,15 @@ __device__ __forceinline__ void tmem_store_16(uint32_t address, const uint32_t (
         : "memory");
 }
 
+// Waits for this thread's TMEM loads.  The registers pass through the statement, so that nothing
+// that reads them can be moved before the wait.
+template <int kCount>
+__device__ __forceinline__ void tmem_loaded(uint32_t (&r)[kCount]) {
+    ptx::tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) asm volatile("" : "+r"(r[i]));
+}
+
 __device__ __forceinline__ void tmem_load_16(uint32_t address, uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
@@ -189,7 +198,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int b = blockIdx.z;
     const int row_tiles = gridDim.y / p.kv_heads;
-    const int head = blockIdx.y / row_tiles;
+    const int head = blockIdx.y % p.kv_heads;  // the row tiles that see most keys start first, of all heads
     const Sequence s = sequence_of(p, b);
     if (p.zero_tail)
         zero_tail_rows(p, ((int64_t)(blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * kWideThreads + threadIdx.x,
@@ -232,7 +241,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     if (warp < 4) {
         // a row's 128 scores live in registers: what these roles do not need goes to the softmax
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegisters));
-    for (int at = blockIdx.y % row_tiles; at * kWideRows < rows; at += row_tiles) {
+    for (int at = blockIdx.y / p.kv_heads; at * kWideRows < rows; at += row_tiles) {
         const Job job = job_of(p, s, rows, at);
         if (!job.mine) continue;
         const int key_begin = job.key_begin, key_end = job.key_end, tiles = job.tiles;
@@ -346,7 +355,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
-    for (int at = blockIdx.y % row_tiles; at * kWideRows < rows; at += row_tiles) {
+    for (int at = blockIdx.y / p.kv_heads; at * kWideRows < rows; at += row_tiles) {
         const Job job = job_of(p, s, rows, at);
         if (!job.mine) continue;
         const int row0 = job.row0, key_begin = job.key_begin, key_end = job.key_end, tiles = job.tiles, splits = job.splits;
@@ -395,7 +404,8 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 uint32_t x[4][32];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) ptx::tmem_load_32_async(lanes + kS + 128 * t + 32 * i, x[i]);
-                ptx::tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tmem_loaded(x[i]);
                 if (masked) {
 #pragma unroll
                     for (int e = 0; e < 128; ++e)
@@ -424,7 +434,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                         for (int i = 0; i < kDim / 16; ++i) {
                             uint32_t o[16];
                             tmem_load_16(lanes + kO + kDim * t + 16 * i, o);
-                            ptx::tmem_wait_ld();
+                            tmem_loaded(o);
 #pragma unroll
                             for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fade);
                             tmem_store_16(lanes + kO + kDim * t + 16 * i, o);
@@ -483,7 +493,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 __syncwarp();
                 if (tiles > 0 && !dead) {
                     ptx::tmem_load_32_async(lanes + kO + kDim * t + 32 * i, x);
-                    ptx::tmem_wait_ld();
+                    tmem_loaded(x);
                 }
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
