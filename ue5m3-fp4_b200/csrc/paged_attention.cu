@@ -60,26 +60,34 @@ struct AppendParams {
     int64_t k_page, k_slot, k_page_head, v_page, v_slot, v_page_head;
 };
 
-// One thread per 16 bytes of a key and its value; the threads of a block run over (token, head,
-// piece) of one sequence.
+// One 16-byte piece of a new token's key and value.  Token `token` of the sequence, whose place is
+// key `position`; a page that is not one of the cache's is left out.
+__device__ __forceinline__ void append_piece(const Params& p, const AppendParams& a, const Sequence& s, int b, int token,
+                                             int position, int head, int piece) {
+    const int page = page_of(p, b, position);
+    if (page < 0) return;
+    const int slot = position & ((1 << p.page_shift) - 1);
+    const int64_t row = s.first + token;
+    const uint4 k = *reinterpret_cast<const uint4*>(a.k + row * a.k_token + head * a.k_head + piece * 8);
+    const uint4 v = *reinterpret_cast<const uint4*>(a.v + row * a.v_token + head * a.v_head + piece * 8);
+    *reinterpret_cast<uint4*>(a.k_pages + page * a.k_page + slot * a.k_slot + head * a.k_page_head + piece * 8) = k;
+    *reinterpret_cast<uint4*>(a.v_pages + page * a.v_page + slot * a.v_slot + head * a.v_page_head + piece * 8) = v;
+}
+
+// Before the kernel for many rows, whose CTAs read one another's new keys: one thread per piece, the
+// threads of a block run over (token, head, piece) of one sequence.
 template <int kDim>
 __global__ void __launch_bounds__(256) append_kernel(const Params p, const AppendParams a) {
     constexpr int kPieces = kDim / 8;
+    launch_dependents();
     const int b = blockIdx.y;
     const Sequence s = sequence_of(p, b);
+    if (s.cut) return;  // no place in the table
     const int64_t count = (int64_t)s.queries * p.kv_heads * kPieces;
     for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < count; i += gridDim.x * 256) {
         const int piece = (int)(i % kPieces), head = (int)(i / kPieces % p.kv_heads), token = (int)(i / kPieces / p.kv_heads);
         const int position = s.keys - s.queries + token;
-        if (position < 0 || s.cut) continue;  // before the sequence's first key, or no place in the table
-        const int page = page_of(p, b, position);
-        if (page < 0) continue;
-        const int slot = position & ((1 << p.page_shift) - 1);
-        const int64_t row = s.first + token;
-        const uint4 k = *reinterpret_cast<const uint4*>(a.k + row * a.k_token + head * a.k_head + piece * 8);
-        const uint4 v = *reinterpret_cast<const uint4*>(a.v + row * a.v_token + head * a.v_head + piece * 8);
-        *reinterpret_cast<uint4*>(a.k_pages + page * a.k_page + slot * a.k_slot + head * a.k_page_head + piece * 8) = k;
-        *reinterpret_cast<uint4*>(a.v_pages + page * a.v_page + slot * a.v_slot + head * a.v_page_head + piece * 8) = v;
+        if (position >= 0) append_piece(p, a, s, b, token, position, head, piece);
     }
 }
 
@@ -93,7 +101,7 @@ struct SmallShared {
 
 template <int kDim>
 __global__ void __launch_bounds__(kSmallThreads, 2)
-    attention_small_kernel(const Params p, const __grid_constant__ CUtensorMap k_map,
+    attention_small_kernel(const Params p, const AppendParams append, const __grid_constant__ CUtensorMap k_map,
                            const __grid_constant__ CUtensorMap v_map) {
     constexpr int kSlabs = kDim / 64, kSteps = kDim / 16;
     constexpr int kTileBytes = SmallShared<kDim>::kTileBytes;
@@ -114,6 +122,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
         zero_tail_rows(p, ((int64_t)(blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * kSmallThreads + threadIdx.x,
                        (int64_t)gridDim.x * gridDim.y * gridDim.z * kSmallThreads, kDim);
     const int rows = s.queries * p.group;
+    launch_dependents();
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) {
             ptx::mbar_init(&full[i], 1);
@@ -131,6 +140,15 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
         const int first = blockIdx.x * chunk, last = min(all, first + chunk);
         const int splits = (all + chunk - 1) / chunk;
         if (first >= all && blockIdx.x > 0) continue;
+        if (append.k && !s.cut) {
+            // The new tokens among this CTA's keys go to their pages; it alone reads them before the
+            // call ends, or, with a second row tile, next to one that writes the same.
+            constexpr int kPieces = kDim / 8;
+            const int start = max(s.keys - s.queries, first * kKeys), stop = min(limit, (first + chunk) * kKeys);
+            for (int i = threadIdx.x; i < (stop - start) * kPieces; i += kSmallThreads)
+                append_piece(p, append, s, b, start + i / kPieces - (s.keys - s.queries), start + i / kPieces, head, i % kPieces);
+            asm volatile("fence.proxy.async;" ::: "memory");
+        }
         if (threadIdx.x == 0) *bad = s.cut;
         __syncthreads();
         const bool dead = *((volatile int*)abort_flag) != 0;  // a wait gave up, here or in an earlier launch
@@ -319,6 +337,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
 // splits side by side in a warp).
 template <int kDim>
 __global__ void __launch_bounds__(128) combine_kernel(const Params p, int rows_per_tile) {
+    wait_for_launcher();
     constexpr int kLanes = kDim / 4, kSide = 128 / kLanes;  // lanes of a row, rows side by side in the CTA
     __shared__ float values[kSide][kDim], sums[kSide], tops[4];
     const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -444,32 +463,34 @@ static Plan make_plan(int64_t tokens, int64_t sequences, int64_t heads, int64_t 
 }
 
 template <int kDim>
-int launch(const Params& p, const Plan& plan, const CUtensorMap& k_map, const CUtensorMap& v_map, const AppendParams* append,
+int launch(const Params& p, const Plan& plan, const CUtensorMap& k_map, const CUtensorMap& v_map, const AppendParams& append,
            int64_t max_query, cudaStream_t stream) {
-    if (append) {
-        const int64_t pieces = max_query * p.kv_heads * (kDim / 8);
-        int64_t blocks = (pieces + 255) / 256;
-        if (blocks > 1024) blocks = 1024;
-        append_kernel<kDim><<<dim3((unsigned)blocks, p.sequences), 256, 0, stream>>>(p, *append);
-        const int status = check_launch();
-        if (status != UE5M3_OK) return status;
-    }
     const dim3 grid(plan.splits, p.kv_heads * plan.row_tiles, p.sequences);
-    int status;
+    cudaError_t error;
     if (plan.wide) {
-        status = launch_wide(p, kDim, grid, k_map, v_map, stream);
+        if (append.k) {
+            const int64_t pieces = max_query * p.kv_heads * (kDim / 8);
+            int64_t blocks = (pieces + 255) / 256;
+            if (blocks > 1024) blocks = 1024;
+            append_kernel<kDim><<<dim3((unsigned)blocks, p.sequences), 256, 0, stream>>>(p, append);
+            const int status = check_launch();
+            if (status != UE5M3_OK) return status;
+        }
+        const int status = launch_wide(p, kDim, grid, k_map, v_map, append.k != nullptr, stream);
+        if (status != UE5M3_OK) return status;
     } else {
-        const cudaError_t error = cudaFuncSetAttribute(
-            attention_small_kernel<kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, SmallShared<kDim>::kBytes);
+        error = allow_shared<attention_small_kernel<kDim>>(SmallShared<kDim>::kBytes);
+        if (error == cudaSuccess)
+            error = launch_after(attention_small_kernel<kDim>, grid, kSmallThreads, SmallShared<kDim>::kBytes, stream, false, p,
+                                 append, k_map, v_map);
         if (error != cudaSuccess) return record_cuda_error(error);
-        attention_small_kernel<kDim><<<grid, kSmallThreads, SmallShared<kDim>::kBytes, stream>>>(p, k_map, v_map);
-        status = check_launch();
     }
-    if (status != UE5M3_OK || plan.splits == 1) return status;
+    if (plan.splits == 1) return UE5M3_OK;
     int64_t blocks = max_query * p.heads;
     if (blocks > 65535) blocks = 65535;
-    combine_kernel<kDim><<<dim3((unsigned)blocks, p.sequences), 128, 0, stream>>>(p, plan.wide ? kWideRows : kRows);
-    return check_launch();
+    error = launch_after(combine_kernel<kDim>, dim3((unsigned)blocks, p.sequences), 128, 0, stream, true, p,
+                         plan.wide ? kWideRows : kRows);
+    return record_cuda_error(error);
 }
 
 }  // namespace paged
@@ -559,7 +580,7 @@ extern "C" int ue5m3_paged_attention(const void* q, int64_t q_token_stride, int6
         status = encode_pages(&v_map, cache->v_pages, *cache, cache->v_page_stride, cache->v_slot_stride,
                               cache->v_head_stride, (int)dim, box);
     if (status != UE5M3_OK) return status;
-    AppendParams a;
+    AppendParams a = {};
     if (new_k) {
         a.k = reinterpret_cast<const __nv_bfloat16*>(new_k);
         a.v = reinterpret_cast<const __nv_bfloat16*>(new_v);
@@ -577,6 +598,6 @@ extern "C" int ue5m3_paged_attention(const void* q, int64_t q_token_stride, int6
         a.v_page_head = cache->v_head_stride;
     }
     cudaStream_t s = (cudaStream_t)stream;
-    return dim == 64 ? launch<64>(p, plan, k_map, v_map, new_k ? &a : nullptr, max_query, s)
-                     : launch<128>(p, plan, k_map, v_map, new_k ? &a : nullptr, max_query, s);
+    return dim == 64 ? launch<64>(p, plan, k_map, v_map, a, max_query, s)
+                     : launch<128>(p, plan, k_map, v_map, a, max_query, s);
 }

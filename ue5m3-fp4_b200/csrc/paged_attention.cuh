@@ -103,6 +103,39 @@ __device__ __forceinline__ void zero_tail_rows(const Params& p, int64_t thread, 
     for (int64_t i = first * width + thread; i < p.tokens * width; i += threads) out[i] = make_uint4(0, 0, 0, 0);
 }
 
+// Programmatic launches: the next kernel of a call starts while this one ends, and waits for it
+// where it first reads what this one writes.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_launcher() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... Arguments>
+cudaError_t launch_after(void (*kernel)(Arguments...), dim3 grid, unsigned threads, size_t shared, cudaStream_t stream,
+                         bool early, Arguments... arguments) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = shared;
+    config.stream = stream;
+    cudaLaunchAttribute attribute;
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attribute;
+    config.numAttrs = early ? 1 : 0;
+    return cudaLaunchKernelEx(&config, kernel, arguments...);
+}
+
+// Dynamic shared memory above 48 KiB has to be asked for once per kernel and device.
+template <auto kKernel>
+cudaError_t allow_shared(int bytes) {
+    static bool done[64] = {};
+    int device = 0;
+    cudaError_t error = cudaGetDevice(&device);
+    if (error != cudaSuccess || (device < 64 && done[device])) return error;
+    error = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (error == cudaSuccess && device < 64) done[device] = true;
+    return error;
+}
+
 // mbar_wait with one answer for the whole (converged) warp
 __device__ __forceinline__ bool warp_wait(unsigned long long* bar, uint32_t parity, int* abort_flag, int* status, int where,
                                           int iter) {
@@ -113,7 +146,8 @@ __device__ __forceinline__ bool warp_wait(unsigned long long* bar, uint32_t pari
 
 constexpr int kWideRows = 256;  // rows of one CTA
 
-int launch_wide(const Params& p, int head_dim, dim3 grid, const CUtensorMap& k_map, const CUtensorMap& v_map,
+// early: the kernel launched before it on the stream belongs to the same call
+int launch_wide(const Params& p, int head_dim, dim3 grid, const CUtensorMap& k_map, const CUtensorMap& v_map, bool early,
                 cudaStream_t stream);
 
 }  // namespace paged

@@ -31,7 +31,6 @@ constexpr int kWideThreads = 384;
 constexpr float kRescale = 8.0f;  // log2 of the growth of a maximum that is left in the probabilities
 constexpr int kSiteWide = 0x60;
 constexpr int kProducerRegisters = 88, kSoftmaxRegisters = 208;  // 128 * 88 + 256 * 208 <= 384 * 168
-constexpr int kPolynomial = 0;  // of every eight pairs of exponentials, those computed on the fp32 pipe
 
 template <int kDim>
 struct WideShared {
@@ -111,11 +110,6 @@ __device__ __forceinline__ void tmem_load_16(uint32_t address, uint32_t (&r)[16]
         : "memory");
 }
 
-template <int kValue>
-struct Number {
-    static constexpr int value = kValue;
-};
-
 // two fp32 operations in one instruction
 __device__ __forceinline__ uint64_t pack2(float lo, float hi) {
     uint64_t d;
@@ -139,27 +133,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
-}
-
-// 2^x of a pair on the fp32 pipe: x = n + f, n the nearest integer, 2^f by a polynomial of degree 3
-// fitted on [-1/2, 1/2] (relative error below 7.5e-5; the rounding of the result to bf16 is 2^-8),
-// n added to the exponent.  x below -126 counts as -126.
-__device__ __forceinline__ void exp2_pair(uint64_t x, float& lo, float& hi) {
-    float a, b;
-    unpack2(x, a, b);
-    x = pack2(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
-    const uint64_t magic = pack2(12582912.0f, 12582912.0f);  // 1.5 * 2^23: the sum's low bits are n
-    const uint64_t n = add2(x, magic);
-    const uint64_t f = fma2(add2(n, pack2(-12582912.0f, -12582912.0f)), pack2(-1.0f, -1.0f), x);
-    uint64_t y = pack2(0.05517132207751274f, 0.05517132207751274f);
-    y = fma2(y, f, pack2(0.24261054396629333f, 0.24261054396629333f));
-    y = fma2(y, f, pack2(0.6932609677314758f, 0.6932609677314758f));
-    y = fma2(y, f, pack2(0.9999281167984009f, 0.9999281167984009f));
-    float n0, n1;
-    unpack2(n, n0, n1);
-    unpack2(y, lo, hi);
-    lo = __int_as_float(__float_as_int(lo) + (__float_as_int(n0) << 23));
-    hi = __int_as_float(__float_as_int(hi) + (__float_as_int(n1) << 23));
 }
 
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -224,6 +197,9 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         ptx::mbar_fence_init();
     }
     if (warp == 1) ptx::tmem_alloc(&bar.tmem, 512);
+    launch_dependents();
+    wait_for_launcher();  // the new keys and values are in their pages ...
+    asm volatile("fence.proxy.async;" ::: "memory");  // ... and TMA sees them
     ptx::tcgen05_fence_before();
     __syncthreads();
     ptx::tcgen05_fence_after();
@@ -444,8 +420,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 const float base = top == -INFINITY ? 0.0f : top;
                 const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2), base2 = pack2(-base, -base);
                 uint64_t sums[4] = {0, 0, 0, 0};
-                // masked keys come out as exact zeros only from the special-function unit
-                auto probabilities = [&](auto polynomial) {
+                auto probabilities = [&]() {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         uint32_t packed[16];
@@ -453,13 +428,9 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                         for (int e = 0; e < 32; e += 2) {
                             const uint64_t y = fma2(pack2(__uint_as_float(x[i][e]), __uint_as_float(x[i][e + 1])), scale2, base2);
                             float lo, hi;
-                            if ((e / 2) % 8 < decltype(polynomial)::value) {
-                                exp2_pair(y, lo, hi);
-                            } else {
-                                unpack2(y, lo, hi);
-                                lo = exp2_approx(lo);
-                                hi = exp2_approx(hi);
-                            }
+                            unpack2(y, lo, hi);
+                            lo = exp2_approx(lo);
+                            hi = exp2_approx(hi);
                             sums[(e / 2) % 4] = add2(sums[(e / 2) % 4], pack2(lo, hi));
                             packed[e / 2] = pack_bf16(lo, hi);
                         }
@@ -472,10 +443,11 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                         }
                     }
                 };
+                // written twice: the compiler's schedule of the common case is better for it (232 against 260 us)
                 if (masked)
-                    probabilities(Number<0>());
+                    probabilities();
                 else
-                    probabilities(Number<kPolynomial>());
+                    probabilities();
                 float lo, hi;
                 unpack2(add2(add2(sums[0], sums[1]), add2(sums[2], sums[3])), lo, hi);
                 sum += lo + hi;
@@ -545,19 +517,19 @@ __global__ void __launch_bounds__(kWideThreads, 1)
 }
 
 template <int kDim>
-static int launch_wide_dim(const Params& p, dim3 grid, const CUtensorMap& k_map, const CUtensorMap& v_map,
+static int launch_wide_dim(const Params& p, dim3 grid, const CUtensorMap& k_map, const CUtensorMap& v_map, bool early,
                            cudaStream_t stream) {
-    const cudaError_t error = cudaFuncSetAttribute(attention_wide_kernel<kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   WideShared<kDim>::kBytes);
-    if (error != cudaSuccess) return record_cuda_error(error);
-    attention_wide_kernel<kDim><<<grid, kWideThreads, WideShared<kDim>::kBytes, stream>>>(p, k_map, v_map);
-    return check_launch();
+    cudaError_t error = allow_shared<attention_wide_kernel<kDim>>(WideShared<kDim>::kBytes);
+    if (error == cudaSuccess)
+        error = launch_after(attention_wide_kernel<kDim>, grid, kWideThreads, WideShared<kDim>::kBytes, stream, early, p, k_map,
+                             v_map);
+    return record_cuda_error(error);
 }
 
-int launch_wide(const Params& p, int head_dim, dim3 grid, const CUtensorMap& k_map, const CUtensorMap& v_map,
+int launch_wide(const Params& p, int head_dim, dim3 grid, const CUtensorMap& k_map, const CUtensorMap& v_map, bool early,
                 cudaStream_t stream) {
-    return head_dim == 64 ? launch_wide_dim<64>(p, grid, k_map, v_map, stream)
-                          : launch_wide_dim<128>(p, grid, k_map, v_map, stream);
+    return head_dim == 64 ? launch_wide_dim<64>(p, grid, k_map, v_map, early, stream)
+                          : launch_wide_dim<128>(p, grid, k_map, v_map, early, stream);
 }
 
 }  // namespace paged

@@ -172,6 +172,12 @@ def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+# The current stream's pointer of a device index without building a Stream object (a third of the
+# host time of a small call); torch's own generated code calls the same function.
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 _amax_scratch: dict[tuple[int, int], torch.Tensor] = {}
 
 

@@ -8,8 +8,8 @@ in the reference, which evaluates frozen models by whole forward passes.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import functools
 
 import torch
 from torch import Tensor
@@ -17,26 +17,33 @@ from torch import Tensor
 from ue5m3_fp4 import _native
 from ue5m3_fp4.backends import b200
 
-_HEAD_DIMS = (64, 128)
 _PAGE_SIZES = (16, 32, 64, 128, 256)
+_BF16 = torch.bfloat16
 
 
-def _on(device: torch.device):
-    """The device of the operands as the current one, at no cost where it is already."""
-
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
-
-
-def _require(condition: bool, message: str) -> None:
-    if not condition:
-        raise ValueError(message)
+def _require_cuda(tensor: Tensor, name: str) -> None:
+    if not isinstance(tensor, Tensor) or not tensor.is_cuda:
+        b200._require_cuda(tensor, name)
 
 
 def _no_gradient(*tensors: Tensor | None) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("serving operators have no gradients; call them under torch.no_grad() or on detached tensors")
+    if torch.is_grad_enabled():
+        for tensor in tensors:
+            if tensor is not None and tensor.requires_grad:
+                raise RuntimeError("serving operators have no gradients; call them under torch.no_grad() or on "
+                                   "detached tensors")
+
+
+def _call(function, name: str, launches: int, device: torch.device, *arguments) -> None:
+    """The library call on ``device``'s current stream, with that device current."""
+
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        status = function(*arguments, _native.raw_stream(index))
+    else:
+        with torch.cuda.device(device):
+            status = function(*arguments, _native.raw_stream(index))
+    _native.check(status, name, launches)
 
 
 def decode_factor(tensor_amax: float, scale_target: float) -> float:
@@ -53,21 +60,13 @@ def decode_factor(tensor_amax: float, scale_target: float) -> float:
         return 1.0 if encode == 0 else float(np.float32(1.0) / np.float32(encode))
 
 
-_factors: dict[tuple[float, float], float] = {}
-
-
-def _cached_factor(tensor_amax: float, scale_target: float) -> float:
-    key = (tensor_amax, scale_target)
-    factor = _factors.get(key)
-    if factor is None:
-        if not (tensor_amax >= 0 and tensor_amax != float("inf")):
-            raise ValueError("tensor_amax must be finite and not negative")
-        if not 0 < scale_target < float("inf"):
-            raise ValueError("scale_target must be positive and finite")
-        if len(_factors) > 4096:
-            _factors.clear()
-        factor = _factors[key] = decode_factor(tensor_amax, scale_target)
-    return factor
+@functools.lru_cache(maxsize=4096)
+def _checked_factor(tensor_amax: float, scale_target: float) -> float:
+    if not 0 <= tensor_amax < float("inf"):
+        raise ValueError("tensor_amax must be finite and not negative")
+    if not 0 < scale_target < float("inf"):
+        raise ValueError("scale_target must be positive and finite")
+    return decode_factor(tensor_amax, scale_target)
 
 
 def packed_matvec(
@@ -91,55 +90,67 @@ def packed_matvec(
     contiguous.  The cost grows with every 32 rows of bf16 ``x`` (8 rows are read at the cost of one):
     for whole prompts use the GEMM."""
 
-    b200._require_cuda(x, "x")
+    _require_cuda(x, "x")
     _no_gradient(x, bias)
     device = x.device
-    _require(block_size in (16, 32), "block_size must be 16 or 32")
-    _require(x.ndim >= 1 and x.shape[-1] == cols, f"x must have {cols} columns")
+    if block_size != 16 and block_size != 32:
+        raise ValueError("block_size must be 16 or 32")
+    if x.ndim == 0 or x.shape[-1] != cols or cols <= 0:
+        raise ValueError(f"x must have {cols} columns, at least one")
     scale_rows = (rows + block_size - 1) // block_size if two_dimensional else rows
-    _require(codes.dtype is torch.uint8 and tuple(codes.shape) == (rows, (cols + 1) // 2) and codes.is_contiguous()
-             and codes.device == device, "codes must be contiguous uint8 [rows, ceil(cols/2)] on the operand's device")
-    _require(scales.dtype is torch.uint8 and tuple(scales.shape) == (scale_rows, (cols + block_size - 1) // block_size)
-             and scales.is_contiguous() and scales.device == device,
-             "scales must be contiguous uint8 with one byte per block, on the operand's device")
+    if (codes.dtype is not torch.uint8 or codes.shape != (rows, (cols + 1) // 2) or not codes.is_contiguous()
+            or codes.device != device):
+        raise ValueError("codes must be contiguous uint8 [rows, ceil(cols/2)] on the operand's device")
+    if (scales.dtype is not torch.uint8 or scales.shape != (scale_rows, (cols + block_size - 1) // block_size)
+            or not scales.is_contiguous() or scales.device != device):
+        raise ValueError("scales must be contiguous uint8 with one byte per block, on the operand's device")
     x_code = _native.dtype_code(x.dtype)
-    out_dtype = out_dtype or x.dtype
-    out_code = _native.dtype_code(out_dtype)
-    bias_code = 0
+    if out_dtype is None:
+        out_dtype, out_code = x.dtype, x_code
+    else:
+        out_code = _native.dtype_code(out_dtype)
+    bias_code, bias_pointer = 0, None
     if bias is not None:
-        bias_code = _native.dtype_code(bias.dtype)
-        _require(tuple(bias.shape) == (rows,) and bias.is_contiguous() and bias.device == device,
-                 "bias must be contiguous [rows] on the operand's device")
-    factor = _cached_factor(float(tensor_amax), float(scale_target))
-    shape = x.shape[:-1]
+        if bias.shape != (rows,) or not bias.is_contiguous() or bias.device != device:
+            raise ValueError("bias must be contiguous [rows] on the operand's device")
+        bias_code, bias_pointer = _native.dtype_code(bias.dtype), bias.data_ptr()
+    factor = _checked_factor(float(tensor_amax), float(scale_target))
     flat = x if x.ndim == 2 else x.reshape(-1, cols)
     tokens = flat.shape[0]
     out = torch.empty((tokens, rows), dtype=out_dtype, device=device)
-    if tokens == 0 or rows == 0:
-        return out.view(*shape, rows)
-    _require(cols > 0, "cols must be positive")
-    ldx = flat.stride(0) if tokens > 1 else cols
-    if (cols > 1 and flat.stride(1) != 1) or ldx < cols:
-        raise ValueError("the last axis of x must be contiguous and its rows must not overlap")
-    with _on(device):
-        status = _native.load().ue5m3_packed_matvec(
-            flat.data_ptr(), x_code, tokens, ldx, codes.data_ptr(), scales.data_ptr(), rows, cols, block_size,
-            int(two_dimensional), factor, None if bias is None else bias.data_ptr(), bias_code, out.data_ptr(),
-            out_code, rows, _native.stream_ptr(device))
-    _native.check(status, "ue5m3_packed_matvec")
-    return out if x.ndim == 2 else out.view(*shape, rows)
+    if tokens and rows:
+        ldx, step = flat.stride()
+        if tokens == 1:
+            ldx = cols
+        if (step != 1 and cols > 1) or ldx < cols:
+            raise ValueError("the last axis of x must be contiguous and its rows must not overlap")
+        _call(_native.load().ue5m3_packed_matvec, "ue5m3_packed_matvec", 1, device, flat.data_ptr(), x_code, tokens, ldx,
+              codes.data_ptr(), scales.data_ptr(), rows, cols, block_size, two_dimensional, factor, bias_pointer,
+              bias_code, out.data_ptr(), out_code, rows)
+    return out if x.ndim == 2 else out.view(*x.shape[:-1], rows)
 
 
-def _page_strides(pages: Tensor) -> tuple[int, int, int]:
-    """Strides of page, slot and head; that of an axis with one element is immaterial."""
+def _strides(name: str, tensor: Tensor) -> tuple[int, ...]:
+    """Strides of all axes but the channels', for the library: that of an axis with one element is immaterial."""
 
-    contiguous = (pages.shape[1] * pages.shape[2] * pages.shape[3], pages.shape[2] * pages.shape[3], pages.shape[3])
-    return tuple(pages.stride(i) if pages.shape[i] > 1 else contiguous[i] for i in range(3))
+    strides = tensor.stride()
+    if strides[-1] != 1:
+        raise ValueError(f"{name} must have contiguous channels")
+    if 1 in tensor.shape[:-1]:
+        strides = tuple(0 if size == 1 else stride for size, stride in zip(tensor.shape, strides))
+        if tensor.ndim == 4:  # the tensor map of the pages takes no zero strides
+            shape = tensor.shape
+            dense = (shape[1] * shape[2] * shape[3], shape[2] * shape[3], shape[3])
+            strides = tuple(stride or full for stride, full in zip(strides, dense))
+    for stride in strides[:tensor.ndim - 1]:
+        if stride % 8 or stride < 0:
+            raise ValueError(f"the strides of {name} must be multiples of 8 elements")
+    return strides[:tensor.ndim - 1]
 
 
-def _check_lengths(name: str, tensor: Tensor, count: int, device: torch.device) -> None:
-    _require(tensor.dtype is torch.int32 and tensor.device == device and tuple(tensor.shape) == (count,)
-             and tensor.is_contiguous(), f"{name} must be contiguous int32 [{count}] on the operand's device")
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(*sizes: int) -> int:
+    return _native.load().ue5m3_paged_attention_workspace_bytes(*sizes)
 
 
 def paged_attention(
@@ -174,85 +185,86 @@ def paged_attention(
     ``out`` was.  A page outside the cache is not touched; rows that need it are NaN.
     head_dim is 64 or 128, page_size 16, 32, 64, 128 or 256; heads is a multiple of kv_heads."""
 
-    b200._require_cuda(q, "q")
+    _require_cuda(q, "q")
     _no_gradient(q, new_k, new_v, k_pages, v_pages)
     device = q.device
-    _require(q.ndim == 3 and k_pages.ndim == 4 and v_pages.shape == k_pages.shape and page_table.ndim == 2,
-             "q must be [tokens, heads, head_dim], the pages [pages, page_size, kv_heads, head_dim], the table rank 2")
+    if q.ndim != 3 or k_pages.ndim != 4 or page_table.ndim != 2 or v_pages.shape != k_pages.shape:
+        raise ValueError("q must be [tokens, heads, head_dim], the pages [pages, page_size, kv_heads, head_dim], the "
+                         "table rank 2")
     tokens, heads, head_dim = q.shape
-    pages, page_size, kv_heads, _ = k_pages.shape
+    pages, page_size, kv_heads, width = k_pages.shape
+    if q.dtype is not _BF16 or k_pages.dtype is not _BF16 or v_pages.dtype is not _BF16:
+        raise ValueError("q, k_pages and v_pages must be bfloat16")
+    if k_pages.device != device or v_pages.device != device or page_table.device != device:
+        raise ValueError("the cache must be on the operand's device")
+    if head_dim != width or (head_dim != 64 and head_dim != 128):
+        raise ValueError("head_dim must be 64 or 128, and that of the pages")
+    if page_size not in _PAGE_SIZES:
+        raise ValueError("page_size must be 16, 32, 64, 128 or 256")
+    if kv_heads == 0 or heads == 0 or heads % kv_heads:
+        raise ValueError("heads must be a multiple of kv_heads")
     sequences, width = page_table.shape
-    for name, tensor in (("q", q), ("k_pages", k_pages), ("v_pages", v_pages)):
-        _require(tensor.dtype is torch.bfloat16, f"{name} must be bfloat16")
-        _require(tensor.device == device and tensor.shape[-1] == head_dim and tensor.stride(-1) == 1,
-                 f"{name} must be on the operand's device with contiguous channels of q's width")
-    _require(head_dim in _HEAD_DIMS, "head_dim must be 64 or 128")
-    _require(page_size in _PAGE_SIZES, "page_size must be 16, 32, 64, 128 or 256")
-    _require(kv_heads > 0 and heads % kv_heads == 0 and heads > 0, "heads must be a multiple of kv_heads")
-    _require(page_table.dtype is torch.int32 and page_table.device == device
-             and (width <= 1 or page_table.stride(1) == 1), "page_table must be int32 on the operand's device, rows contiguous")
-    _check_lengths("kv_lengths", kv_lengths, sequences, device)
-    _check_lengths("query_starts", query_starts, sequences + 1, device)
-    _require(max_query_length > 0, "max_query_length must be positive")
+    table_stride, step = page_table.stride()
+    if page_table.dtype is not torch.int32 or (step != 1 and width > 1) or (table_stride < width and sequences > 1):
+        raise ValueError("page_table must be int32 with contiguous rows")
+    if (kv_lengths.dtype is not torch.int32 or kv_lengths.shape != (sequences,) or kv_lengths.device != device
+            or not kv_lengths.is_contiguous()):
+        raise ValueError("kv_lengths must be contiguous int32 [sequences] on the operand's device")
+    if (query_starts.dtype is not torch.int32 or query_starts.shape != (sequences + 1,) or query_starts.device != device
+            or not query_starts.is_contiguous()):
+        raise ValueError("query_starts must be contiguous int32 [sequences + 1] on the operand's device")
+    if max_query_length <= 0 or (max_kv_length is not None and max_kv_length <= 0):
+        raise ValueError("max_query_length and max_kv_length must be positive")
     if scale is None:
         scale = head_dim ** -0.5
-    _require(0 < scale < float("inf"), "scale must be positive and finite")
-    if (new_k is None) != (new_v is None):
-        raise ValueError("new_k and new_v come together")
-    for name, tensor in (("new_k", new_k), ("new_v", new_v)):
-        if tensor is not None:
-            _require(tensor.dtype is torch.bfloat16 and tuple(tensor.shape) == (tokens, kv_heads, head_dim)
-                     and tensor.device == device and tensor.stride(2) == 1,
-                     f"{name} must be bfloat16 [tokens, kv_heads, head_dim] with contiguous channels")
+    elif not 0 < scale < float("inf"):
+        raise ValueError("scale must be positive and finite")
     zero_tail = out is None
-    if out is None:
-        out = torch.empty((tokens, heads, head_dim), dtype=torch.bfloat16, device=device)
-    else:
-        _require(out.dtype is torch.bfloat16 and out.shape == q.shape and out.is_contiguous() and out.device == device,
-                 "out must be contiguous bfloat16 of q's shape on its device")
+    if zero_tail:
+        out = torch.empty((tokens, heads, head_dim), dtype=_BF16, device=device)
+    elif out.dtype is not _BF16 or out.shape != q.shape or not out.is_contiguous() or out.device != device:
+        raise ValueError("out must be contiguous bfloat16 of q's shape on its device")
+    k_pointer = v_pointer = None
+    k_strides = v_strides = (0, 0)
+    if new_k is not None or new_v is not None:
+        if new_k is None or new_v is None:
+            raise ValueError("new_k and new_v come together")
+        for name, tensor in (("new_k", new_k), ("new_v", new_v)):
+            if tensor.dtype is not _BF16 or tensor.shape != (tokens, kv_heads, head_dim) or tensor.device != device:
+                raise ValueError(f"{name} must be bfloat16 [tokens, kv_heads, head_dim] on the operand's device")
+        k_pointer, v_pointer = new_k.data_ptr(), new_v.data_ptr()
+        k_strides, v_strides = _strides("new_k", new_k), _strides("new_v", new_v)
     if tokens == 0:
         return out
     if sequences == 0:
         return out.zero_() if zero_tail else out
-    _require(pages > 0 and width > 0, "the cache has no pages, or its table no columns")
-    if max_kv_length is None:
-        max_kv_length = width * page_size
-    _require(max_kv_length > 0, "max_kv_length must be positive")
-    k_strides, v_strides = _page_strides(k_pages), _page_strides(v_pages)
-    for stride in (*k_strides, *v_strides, *(t.stride(i) for t in (q, new_k, new_v) if t is not None
-                                             for i in range(2) if t.shape[i] > 1)):
-        _require(stride % 8 == 0, "strides must be multiples of 8 elements")
-    cache = _native.PagedCache(
-        k_pages.data_ptr(), v_pages.data_ptr(), *k_strides, *v_strides, pages, page_size, kv_heads, head_dim,
-        page_table.data_ptr(), sequences, width, page_table.stride(0) if sequences > 1 else width)
-    lib = _native.load()
+    if pages == 0 or width == 0:
+        raise ValueError("the cache has no pages, or its table no columns")
+    room = width * page_size
+    max_kv_length = room if max_kv_length is None else min(int(max_kv_length), room)
     max_query_length = min(int(max_query_length), tokens)
-    max_kv_length = min(int(max_kv_length), width * page_size)
-    with _on(device):
-        need = lib.ue5m3_paged_attention_workspace_bytes(tokens, sequences, heads, kv_heads, head_dim, max_query_length,
-                                                         max_kv_length)
-        # from the current stream's pool, for this call alone: calls and captured graphs share nothing
-        workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        strides = [(t.stride(0) if tokens > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0) if t is not None else (0, 0)
-                   for t in (q, new_k, new_v)]
-        status = lib.ue5m3_paged_attention(
-            q.data_ptr(), *strides[0], tokens, heads, ctypes.byref(cache), kv_lengths.data_ptr(),
-            query_starts.data_ptr(), max_query_length, max_kv_length, float(scale),
-            None if new_k is None else new_k.data_ptr(), *strides[1], None if new_v is None else new_v.data_ptr(),
-            *strides[2], out.data_ptr(), int(zero_tail), None if workspace is None else workspace.data_ptr(), need,
-            b200.gemm_status(device).data_ptr(), _native.stream_ptr(device))
-    _native.check(status, "ue5m3_paged_attention")
+    cache = _native.PagedCache(
+        k_pages.data_ptr(), v_pages.data_ptr(), *_strides("k_pages", k_pages), *_strides("v_pages", v_pages), pages,
+        page_size, kv_heads, head_dim, page_table.data_ptr(), sequences, width,
+        table_stride if sequences > 1 else width)
+    need = _workspace_bytes(tokens, sequences, heads, kv_heads, head_dim, max_query_length, max_kv_length)
+    # from the current stream's pool, for this call alone: calls and captured graphs share nothing
+    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _call(_native.load().ue5m3_paged_attention, "ue5m3_paged_attention", 2 if need else 1, device, q.data_ptr(),
+          *_strides("q", q), tokens, heads, ctypes.byref(cache), kv_lengths.data_ptr(), query_starts.data_ptr(),
+          max_query_length, max_kv_length, scale, k_pointer, *k_strides, v_pointer, *v_strides, out.data_ptr(),
+          zero_tail, None if workspace is None else workspace.data_ptr(), need, b200.gemm_status(device).data_ptr())
     return out
 
 
 def _setting(name: str, value, rows: int, dtype: torch.dtype, device: torch.device):
     """(device pointer or None, value) of a setting given as a number or as one number per row."""
 
-    if isinstance(value, Tensor):
-        _require(value.dtype is dtype and tuple(value.shape) == (rows,) and value.is_contiguous()
-                 and value.device == device, f"{name} must be a number or a contiguous {dtype} tensor [rows]")
-        return value.data_ptr(), 0
-    return None, value
+    if not isinstance(value, Tensor):
+        return None, value
+    if value.dtype is not dtype or value.shape != (rows,) or not value.is_contiguous() or value.device != device:
+        raise ValueError(f"{name} must be a number or a contiguous {dtype} tensor [rows] on the operand's device")
+    return value.data_ptr(), 0
 
 
 def sample_tokens(
@@ -277,39 +289,42 @@ def sample_tokens(
     token; a row with a NaN, or with every token masked, gives token -1 and NaN.  Sums are exact: the
     same inputs give the same tokens, whatever the launch."""
 
-    b200._require_cuda(logits, "logits")
+    _require_cuda(logits, "logits")
     _no_gradient(logits)
     device = logits.device
-    _require(logits.ndim == 2, "logits must be [rows, vocabulary]")
+    if logits.ndim != 2:
+        raise ValueError("logits must be [rows, vocabulary]")
     rows, vocabulary = logits.shape
     code = _native.dtype_code(logits.dtype)
-    _require(uniforms.dtype is torch.float32 and tuple(uniforms.shape) == (rows,) and uniforms.is_contiguous()
-             and uniforms.device == device, "uniforms must be contiguous float32 [rows] on the operand's device")
-    _require(0 < vocabulary <= 1 << 18, "the vocabulary must have between 1 and 2^18 tokens")
-    _require(vocabulary == 1 or logits.stride(1) == 1, "the rows of logits must be contiguous")
-    ld = logits.stride(0) if rows > 1 else vocabulary
-    _require(ld >= vocabulary, "the rows of logits must not overlap")
-    if not isinstance(temperature, Tensor):
-        _require(temperature >= 0, "temperature must not be negative")
-    if not isinstance(top_k, Tensor):
-        _require(top_k >= 0, "top_k must not be negative")
-        top_k = min(int(top_k), vocabulary)
-    if not isinstance(top_p, Tensor):
-        _require(0 < top_p <= 1, "top_p must be in (0, 1]")
-    if not isinstance(min_p, Tensor):
-        _require(0 <= min_p <= 1, "min_p must be in [0, 1]")
+    if (uniforms.dtype is not torch.float32 or uniforms.shape != (rows,) or not uniforms.is_contiguous()
+            or uniforms.device != device):
+        raise ValueError("uniforms must be contiguous float32 [rows] on the operand's device")
+    if not 0 < vocabulary <= 1 << 18:
+        raise ValueError("the vocabulary must have between 1 and 2^18 tokens")
+    ld, step = logits.stride()
+    if rows <= 1:
+        ld = vocabulary
+    if (step != 1 and vocabulary > 1) or ld < vocabulary:
+        raise ValueError("the rows of logits must be contiguous and must not overlap")
     heat = _setting("temperature", temperature, rows, torch.float32, device)
     k = _setting("top_k", top_k, rows, torch.int32, device)
     p = _setting("top_p", top_p, rows, torch.float32, device)
     least = _setting("min_p", min_p, rows, torch.float32, device)
+    if not heat[1] >= 0:
+        raise ValueError("temperature must not be negative")
+    if not k[1] >= 0:
+        raise ValueError("top_k must not be negative")
+    if p[0] is None and not 0 < p[1] <= 1:
+        raise ValueError("top_p must be in (0, 1]")
+    if not 0 <= least[1] <= 1:
+        raise ValueError("min_p must be in [0, 1]")
+    if k[1] > vocabulary:
+        k = (None, vocabulary)
     tokens = torch.empty(rows, dtype=torch.int64, device=device)
     logprobs = torch.empty(rows, dtype=torch.float32, device=device)
     if rows:
-        with _on(device):
-            status = _native.load().ue5m3_sample_tokens(
-                logits.data_ptr(), code, rows, vocabulary, ld, uniforms.data_ptr(), *heat, *k, *p, *least,
-                tokens.data_ptr(), logprobs.data_ptr(), _native.stream_ptr(device))
-        _native.check(status, "ue5m3_sample_tokens")
+        _call(_native.load().ue5m3_sample_tokens, "ue5m3_sample_tokens", 1, device, logits.data_ptr(), code, rows,
+              vocabulary, ld, uniforms.data_ptr(), *heat, *k, *p, *least, tokens.data_ptr(), logprobs.data_ptr())
     return tokens, logprobs
 
 
