@@ -451,11 +451,10 @@ int launch(Params p, cudaStream_t stream) {
     p.rows_per_block = block;
     constexpr size_t kRingBytes = kVector ? kRing * kDepth * 2 * kThreads * sizeof(uint4) : 0;
     const size_t bytes = kRingBytes + (size_t)kWarps * used * block * sizeof(float);
-    auto* kernel = packed_matvec_kernel<kFp32, kTiles, kDepth, kVector, kBlock>;
-    const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   (int)kRingBytes + kPartialFloats * 4);
+    const cudaError_t error = allow_shared<packed_matvec_kernel<kFp32, kTiles, kDepth, kVector, kBlock>>(
+        (int)kRingBytes + kPartialFloats * 4);
     if (error != cudaSuccess) return record_cuda_error(error);
-    kernel<<<grid, kThreads, bytes, stream>>>(p);
+    packed_matvec_kernel<kFp32, kTiles, kDepth, kVector, kBlock><<<grid, kThreads, bytes, stream>>>(p);
     return check_launch();
 }
 

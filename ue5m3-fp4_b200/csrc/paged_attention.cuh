@@ -13,6 +13,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "abi_common.cuh"
 #include "tcgen05_ptx.cuh"
 
 namespace ue5m3 {
@@ -122,18 +123,6 @@ cudaError_t launch_after(void (*kernel)(Arguments...), dim3 grid, unsigned threa
     config.attrs = &attribute;
     config.numAttrs = early ? 1 : 0;
     return cudaLaunchKernelEx(&config, kernel, arguments...);
-}
-
-// Dynamic shared memory above 48 KiB has to be asked for once per kernel and device.
-template <auto kKernel>
-cudaError_t allow_shared(int bytes) {
-    static bool done[64] = {};
-    int device = 0;
-    cudaError_t error = cudaGetDevice(&device);
-    if (error != cudaSuccess || (device < 64 && done[device])) return error;
-    error = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (error == cudaSuccess && device < 64) done[device] = true;
-    return error;
 }
 
 // mbar_wait with one answer for the whole (converged) warp

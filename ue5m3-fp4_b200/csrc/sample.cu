@@ -10,15 +10,17 @@
 // integer (logit in integer order, complement of its index), which no two elements share; top-k
 // and top-p each end as one threshold on it.
 //
-// What bounds it: a batch of rows, reading the logits and one fp64 exponential per logit that a sum
-// needs; a single row, the latency of about ten steps.  A cluster of up to eight CTAs holds a row in
+// What bounds it: a batch of rows, one fp64 exponential per logit that a sum needs, then reading the
+// logits; a single row, the latency of its steps.  A cluster of up to eight CTAs holds a row in
 // shared memory, so that it is read from memory once however many steps follow.  A step of a
 // threshold search is a histogram of 512 bins over the row, summed over the cluster through
 // distributed shared memory by every CTA for itself (one cluster barrier per step).  The first
 // step's bins are linear in (max - l) / T, which spreads real logits (bins of the integer order
-// would put a fifth of a row into one of them); the elements of the bin that holds the threshold
-// are then few enough to be ranked against one another, or the search goes on inside it with bins
-// of the 64-bit rank (many equal logits).
+// would put a fifth of a row into one of them); what lies in the last, open bin is counted in
+// registers.  Where the first step leaves at most 1024 elements that can be kept (top-k of a few
+// hundred, a peaked nucleus), these are gathered and the rest happens among them in one CTA.
+// Otherwise the elements of the bin that holds the threshold are ranked against one another, or the
+// search goes on inside it with bins of the 64-bit rank (many equal logits).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -69,7 +71,8 @@ struct alignas(16) Shared {
     uint64_t found, found_before;
     uint64_t low, high;          // bounds of the ranks in a bin (this CTA's)
     uint32_t top_key, top_index, bad, count;
-    uint32_t found_bin, found_count;
+    uint32_t found_bin, found_count, found_through;
+    uint32_t warp_number[kWarps];
 };
 
 // logits in integer order: a larger logit has a larger key
@@ -149,192 +152,340 @@ __device__ __forceinline__ uint32_t first_bin(const Row& row, float v) {
     return bin < (float)(kBins - 1) ? (uint32_t)bin : kBins - 1;
 }
 
-// A threshold search over the elements with rank >= floor: by number (kWeighted false, the
-// need-th largest) or by weight (the first one, in descending order, with which the running weight
-// reaches `need`; for top-p, need is a share of the weight of all of them).  Every CTA of the
-// cluster runs it with the same arguments and gets the same answer.  0 = everything is kept.
+// f(logit, place in the slice) for the elements of a slice that are not masked; the slice is filled
+// up to whole quadruples with minus infinity
+template <typename Function>
+__device__ __forceinline__ void for_each(const float* data, int count, Function f) {
+#pragma unroll 2
+    for (int i = 4 * threadIdx.x; i < count; i += 4 * kThreads) {
+        const float4 v = *reinterpret_cast<const float4*>(data + i);
+        if (v.x != -INFINITY) f(v.x, i);
+        if (v.y != -INFINITY) f(v.y, i + 1);
+        if (v.z != -INFINITY) f(v.z, i + 2);
+        if (v.w != -INFINITY) f(v.w, i + 3);
+    }
+}
+
+__device__ __forceinline__ uint64_t warp_total(uint64_t v) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
+    return v;
+}
+
+__device__ __forceinline__ uint64_t warp_running(uint64_t v) {
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const uint64_t from = __shfl_up_sync(0xFFFFFFFFu, v, d);
+        if ((int)(threadIdx.x & 31) >= d) v += from;
+    }
+    return v;
+}
+
+__device__ __forceinline__ void add_weight(uint32_t (*hist)[kBins], uint32_t bin, uint64_t w) {
+    atomicAdd(&hist[1][bin], (uint32_t)(w & 0x7FFF));
+    atomicAdd(&hist[2][bin], (uint32_t)(w >> 15 & 0x7FFF));
+    atomicAdd(&hist[3][bin], (uint32_t)(w >> 30));
+}
+
+// Where a histogram's running mass reaches `need`.
+struct Found {
+    uint64_t total;    // mass of all bins
+    uint64_t before;   // mass of the bins above the one found
+    uint32_t bin;
+    uint32_t inside;   // elements in that bin
+    uint32_t through;  // elements in it and the bins above
+};
+
+// The bins of all CTAs of the cluster, summed by each for itself (thread = bin), and the bin with
+// which the running mass (number, or weight) reaches `need`; share > 0: need is that share of the
+// total, rounded up.  Nothing is found where the total is below `need`.
 template <bool kWeighted>
-__device__ uint64_t find_threshold(cg::cluster_group& cluster, Shared& s, const float* data, int count, uint32_t base,
-                                   const Row& row, uint64_t floor, uint64_t need, float share, int& buffer) {
+__device__ Found scan_bins(cg::cluster_group& cluster, Shared& s, int& buffer, uint64_t& need, float share) {
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const int ctas = cluster.num_blocks();
-    uint64_t low = floor, high = ~0ull;  // ranks under consideration
-    uint64_t above = 0;                  // mass of the ranks above `high`
-    int shift = 0;
-    uint32_t bin1 = 0;
-    for (int level = 0;; ++level) {
-        uint32_t(*hist)[kBins] = s.hist[buffer];
-        for (int i = 0; i < 4; ++i) hist[i][t] = 0;
-        __syncthreads();
-        for (int i = t; i < count; i += kThreads) {
-            const float v = data[i];
-            if (v == -INFINITY) continue;
-            const uint64_t rank = rank_of(key_of(v), base + i);
-            if (rank < low || rank > high) continue;
-            const uint32_t bin = level == 0 ? first_bin(row, v) : (uint32_t)((high - rank) >> shift);
-            uint64_t w = 1;
-            if (kWeighted) {
-                w = weight_of(row, v);
-                if (w == 0) continue;
-                atomicAdd(&hist[1][bin], (uint32_t)(w & 0x7FFF));
-                atomicAdd(&hist[2][bin], (uint32_t)(w >> 15 & 0x7FFF));
-                atomicAdd(&hist[3][bin], (uint32_t)(w >> 30));
-            }
-            atomicAdd(&hist[0][bin], 1u);
-        }
-        cluster.sync();
-        // every CTA sums the bins of all; thread = bin
-        uint64_t mass = 0;
-        uint32_t number = 0;
-        for (int r = 0; r < ctas; ++r) {
-            const Shared* other = cluster.map_shared_rank(&s, r);
-            const uint32_t n = other->hist[buffer][0][t];
-            number += n;
-            if (kWeighted)
-                mass += (uint64_t)other->hist[buffer][1][t] + ((uint64_t)other->hist[buffer][2][t] << 15) +
-                        ((uint64_t)other->hist[buffer][3][t] << 30);
-            else
-                mass += n;
-        }
-        buffer ^= 1;
-        uint64_t running = mass;
+    cluster.sync();
+    uint64_t mass = 0;
+    uint32_t number = 0;
+    for (int r = 0; r < (int)cluster.num_blocks(); ++r) {
+        const Shared* other = cluster.map_shared_rank(&s, r);
+        number += other->hist[buffer][0][t];
+        if (kWeighted)
+            mass += (uint64_t)other->hist[buffer][1][t] + ((uint64_t)other->hist[buffer][2][t] << 15) +
+                    ((uint64_t)other->hist[buffer][3][t] << 30);
+    }
+    buffer ^= 1;  // the next step writes the other one, which nobody reads any more
+    if (!kWeighted) mass = number;
+    uint64_t running = warp_running(mass), numbers = kWeighted ? warp_running(number) : 0;
+    if (lane == 31) {
+        s.warp_sum[warp] = running;
+        s.warp_number[warp] = (uint32_t)numbers;
+    }
+    __syncthreads();
+    Found found;
+    found.total = 0;
+    uint64_t before = 0;
+    uint32_t numbers_before = 0;
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const uint64_t from = __shfl_up_sync(0xFFFFFFFFu, running, d);
-            if (lane >= d) running += from;
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before += s.warp_sum[w], numbers_before += s.warp_number[w];
+        found.total += s.warp_sum[w];
+    }
+    running += before;
+    if (share > 0.0f) need = share_of(share, found.total, true);
+    if (running >= need && running - mass < need) {
+        s.found_bin = t;
+        s.found_before = running - mass;
+        s.found_count = number;
+        s.found_through = kWeighted ? numbers_before + (uint32_t)numbers : (uint32_t)running;
+    }
+    __syncthreads();
+    found.bin = s.found_bin;
+    found.before = s.found_before;
+    found.inside = s.found_count;
+    found.through = s.found_through;
+    __syncthreads();
+    return found;
+}
+
+__device__ __forceinline__ void clear_bins(Shared& s, int buffer) {
+    for (int i = 0; i < 4; ++i) s.hist[buffer][i][threadIdx.x] = 0;
+    __syncthreads();
+}
+
+// The first step of a search among the elements with rank >= floor.
+template <bool kWeighted>
+__device__ Found first_step(cg::cluster_group& cluster, Shared& s, const float* data, int count, uint32_t base, const Row& row,
+                            uint64_t floor, uint64_t& need, float share, int& buffer) {
+    clear_bins(s, buffer);
+    uint32_t(*hist)[kBins] = s.hist[buffer];
+    uint64_t last_number = 0, last_weight = 0;
+    for_each(data, count, [&](float v, int i) {
+        if (floor != 0 && rank_of(key_of(v), base + i) < floor) return;
+        const uint32_t bin = first_bin(row, v);
+        const uint64_t w = kWeighted ? weight_of(row, v) : 1;
+        if (w == 0) return;
+        if (bin == kBins - 1) {
+            ++last_number;
+            last_weight += w;
+            return;
         }
-        if (lane == 31) s.warp_sum[warp] = running;
-        if (t == 0) s.found_bin = kBins;
-        __syncthreads();
-        uint64_t before = above, total = above;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            if (w < warp) before += s.warp_sum[w];
-            total += s.warp_sum[w];
+        atomicAdd(&hist[0][bin], 1u);
+        if (kWeighted) add_weight(hist, bin, w);
+    });
+    last_number = warp_total(last_number);
+    if (kWeighted) last_weight = warp_total(last_weight);
+    if ((threadIdx.x & 31) == 0 && last_number) {
+        atomicAdd(&hist[0][kBins - 1], (uint32_t)last_number);
+        if (kWeighted) add_weight(hist, kBins - 1, last_weight);
+    }
+    return scan_bins<kWeighted>(cluster, s, buffer, need, share);
+}
+
+// This CTA's elements that `take` names, into its list of candidates; the list's last writes are
+// seen after the next cluster barrier.
+template <typename Take>
+__device__ void gather(Shared& s, const float* data, int count, uint32_t base, Take take) {
+    if (threadIdx.x == 0) s.count = 0;
+    __syncthreads();
+    for_each(data, count, [&](float v, int i) {
+        const uint64_t rank = rank_of(key_of(v), base + i);
+        if (take(v, rank)) s.mine[atomicAdd(&s.count, 1u)] = rank;
+    });
+}
+
+// The candidates of all CTAs and their weights, in this one's memory.
+template <bool kWeighted>
+__device__ int collect(cg::cluster_group& cluster, Shared& s, const Row& row) {
+    int candidates = 0;
+    for (int r = 0; r < (int)cluster.num_blocks(); ++r) {
+        const Shared* other = cluster.map_shared_rank(&s, r);
+        const int n = (int)other->count;
+        for (int i = threadIdx.x; i < n; i += kThreads) {
+            const uint64_t rank = other->mine[i];
+            s.all[candidates + i] = rank;
+            s.weight[candidates + i] = kWeighted ? weight_of(row, value_of((uint32_t)(rank >> 32))) : 1;
         }
-        running += before;
-        if (level == 0 && kWeighted) {
-            // the running weight before the last kept element is below share * total
-            need = share > 0.0f ? share_of(share, total, true) : 1;
-        }
-        if (total <= need && level == 0 && !kWeighted) {
-            __syncthreads();
-            return floor;  // no more than `need` elements
-        }
-        if (running >= need && running - mass < need) {
-            s.found_bin = t;
-            s.found_before = running - mass;
-            s.found_count = number;
-        }
-        __syncthreads();
-        const uint32_t bin = s.found_bin, inside = s.found_count;
-        above = s.found_before;
-        __syncthreads();
-        if (level == 0)
-            bin1 = bin;
-        else {
-            high -= (uint64_t)bin << shift;
-            const uint64_t width = ((uint64_t)1 << shift) - 1;
-            low = high - low > width ? high - width : low;
-        }
-        // the elements of the bin: ranked against one another when they are few
-        const bool few = inside <= kCandidates;
-        if (t == 0) {
-            s.count = 0;
+        candidates += n;
+    }
+    __syncthreads();
+    return candidates;
+}
+
+// A threshold search whose first step left too many elements: the rank of the last one that is kept.
+template <bool kWeighted>
+__device__ uint64_t search(cg::cluster_group& cluster, Shared& s, const float* data, int count, uint32_t base, const Row& row,
+                           uint64_t floor, uint64_t need, Found found, int& buffer) {
+    uint64_t above = found.before;  // mass of the ranks above `high`
+    uint64_t low = floor, high = ~0ull;
+    if (found.inside <= kCandidates) {
+        gather(s, data, count, base, [&](float v, uint64_t rank) {
+            return rank >= floor && first_bin(row, v) == found.bin && (!kWeighted || weight_of(row, v) != 0);
+        });
+    } else {
+        if (threadIdx.x == 0) {
             s.low = ~0ull;
             s.high = 0;
         }
         __syncthreads();
-        if (few || level == 0) {
-            uint64_t my_low = ~0ull, my_high = 0;
-            for (int i = t; i < count; i += kThreads) {
-                const float v = data[i];
-                if (v == -INFINITY) continue;
+        uint64_t my_low = ~0ull, my_high = 0;
+        for_each(data, count, [&](float v, int i) {
+            const uint64_t rank = rank_of(key_of(v), base + i);
+            if (rank < floor || first_bin(row, v) != found.bin || (kWeighted && weight_of(row, v) == 0)) return;
+            my_low = my_low < rank ? my_low : rank;
+            my_high = my_high > rank ? my_high : rank;
+        });
+        atomicMin((unsigned long long*)&s.low, (unsigned long long)my_low);
+        atomicMax((unsigned long long*)&s.high, (unsigned long long)my_high);
+        cluster.sync();
+        low = ~0ull;
+        high = 0;
+        for (int r = 0; r < (int)cluster.num_blocks(); ++r) {
+            const Shared* other = cluster.map_shared_rank(&s, r);
+            low = low < other->low ? low : other->low;
+            high = high > other->high ? high : other->high;
+        }
+        // bins of the rank inside [low, high]; a bin of a range below 512 holds one element
+        while (true) {
+            int shift = 0;
+            while ((high - low) >> shift >= kBins) ++shift;
+            clear_bins(s, buffer);
+            uint32_t(*hist)[kBins] = s.hist[buffer];
+            for_each(data, count, [&](float v, int i) {
                 const uint64_t rank = rank_of(key_of(v), base + i);
-                if (rank < low || rank > high || (level == 0 && first_bin(row, v) != bin1)) continue;
-                if (kWeighted && weight_of(row, v) == 0) continue;
-                if (few)
-                    s.mine[atomicAdd(&s.count, 1u)] = rank;
-                else {
-                    my_low = my_low < rank ? my_low : rank;
-                    my_high = my_high > rank ? my_high : rank;
-                }
-            }
-            if (!few) {
-                atomicMin((unsigned long long*)&s.low, (unsigned long long)my_low);
-                atomicMax((unsigned long long*)&s.high, (unsigned long long)my_high);
-            }
+                if (rank < low || rank > high) return;
+                const uint64_t w = kWeighted ? weight_of(row, v) : 1;
+                if (w == 0) return;
+                const uint32_t bin = (uint32_t)((high - rank) >> shift);
+                atomicAdd(&hist[0][bin], 1u);
+                if (kWeighted) add_weight(hist, bin, w);
+            });
+            uint64_t rest = need - above;
+            const Found next = scan_bins<kWeighted>(cluster, s, buffer, rest, 0.0f);
+            above += next.before;
+            high -= (uint64_t)next.bin << shift;
+            const uint64_t width = ((uint64_t)1 << shift) - 1;
+            low = high - low > width ? high - width : low;
+            if (next.inside <= kCandidates) break;
         }
-        if (few) break;
-        if (level == 0) {
-            cluster.sync();
-            low = ~0ull;
-            high = 0;
-            for (int r = 0; r < ctas; ++r) {
-                const Shared* other = cluster.map_shared_rank(&s, r);
-                low = low < other->low ? low : other->low;
-                high = high > other->high ? high : other->high;
-            }
-            cluster.sync();  // the bounds are rewritten by a later search
-        }
-        const uint64_t range = high - low;
-        shift = 0;
-        while (range >> shift >= kBins) ++shift;
+        gather(s, data, count, base, [&](float v, uint64_t rank) {
+            return rank >= low && rank <= high && (!kWeighted || weight_of(row, v) != 0);
+        });
     }
     cluster.sync();
-    int candidates = 0;
-    for (int r = 0; r < ctas; ++r) {
-        const Shared* other = cluster.map_shared_rank(&s, r);
-        const int n = (int)other->count;
-        for (int i = t; i < n; i += kThreads) s.all[candidates + i] = other->mine[i];
-        candidates += n;
-    }
-    __syncthreads();
-    for (int i = t; i < candidates; i += kThreads)
-        s.weight[i] = kWeighted ? weight_of(row, value_of((uint32_t)(s.all[i] >> 32))) : 1;
-    __syncthreads();
-    for (int i = t; i < candidates; i += kThreads) {
+    const int candidates = collect<kWeighted>(cluster, s, row);
+    for (int i = threadIdx.x; i < candidates; i += kThreads) {
         const uint64_t rank = s.all[i];
         uint64_t before = above;
         for (int j = 0; j < candidates; ++j)
             if (s.all[j] > rank) before += s.weight[j];
         if (before < need && before + s.weight[i] >= need) s.found = rank;
     }
-    cluster.sync();  // found, and nobody still reads this CTA's candidates
-    const uint64_t found = s.found;
+    cluster.sync();  // found is written, and nobody still reads this CTA's candidates
+    const uint64_t rank = s.found;
     __syncthreads();
-    return found;
+    return rank;
 }
 
-__device__ void load_slice(const Params& p, int64_t at, int count, float* data) {
-    const int t = threadIdx.x;
-    if (p.bf16) {
-        const __nv_bfloat16* source = reinterpret_cast<const __nv_bfloat16*>(p.logits) + at;
-        int i = 0;
-        if (p.vector) {
-            const uint4* wide = reinterpret_cast<const uint4*>(source);
-            for (i = t; i < count / 8; i += kThreads) {
-                const uint4 u = __ldg(wide + i);
-                float4* to = reinterpret_cast<float4*>(data + 8 * i);
-                to[0] = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u),
-                                    __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xFFFF0000u));
-                to[1] = make_float4(__uint_as_float(u.z << 16), __uint_as_float(u.z & 0xFFFF0000u),
-                                    __uint_as_float(u.w << 16), __uint_as_float(u.w & 0xFFFF0000u));
+__device__ __forceinline__ uint64_t border_of(float u, uint64_t total) {
+    // a sum exceeds u * total exactly if it exceeds the largest integer that is not above it
+    return u >= 1.0f ? total - 1 : u > 0.0f ? share_of(u, total, false) : 0;
+}
+
+__device__ __forceinline__ float logprob_of(const Row& row, float v, uint64_t total) {
+    return (float)(exponent_of(row, v) - log((double)total / kOne));
+}
+
+// The rest of a row whose candidates are few, in one CTA: ranked, cut by top-k, top-p (of row_total,
+// or, where that is 0, of what top-k keeps) and min-p, and summed in vocabulary order.  Quadratic in
+// the number of candidates, each thread with its own.
+__device__ void finish_few(cg::cluster_group& cluster, Shared& s, const Params& p, const Row& row, int row_index, int top_k,
+                           float top_p, double least, uint64_t row_total) {
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int candidates = collect<true>(cluster, s, row);
+    constexpr int kOwn = kCandidates / kThreads;
+    uint64_t rank[kOwn], weight[kOwn], before[kOwn];
+    auto total_of_kept = [&]() {
+        uint64_t sum = 0;
+#pragma unroll
+        for (int o = 0; o < kOwn; ++o) sum += weight[o];
+        sum = warp_total(sum);
+        __syncthreads();
+        if (lane == 0) s.warp_sum[warp] = sum;
+        __syncthreads();
+        sum = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) sum += s.warp_sum[w];
+        return sum;
+    };
+#pragma unroll
+    for (int o = 0; o < kOwn; ++o) {
+        const int i = t + o * kThreads;
+        rank[o] = weight[o] = before[o] = 0;
+        if (i >= candidates) continue;
+        rank[o] = s.all[i];
+        weight[o] = s.weight[i];
+        int place = 0;
+        for (int j = 0; j < candidates; ++j)
+            if (s.all[j] > rank[o]) {
+                ++place;
+                before[o] += s.weight[j];
             }
-            for (i = count / 8 * 8 + t; i < count; i += kThreads) data[i] = __bfloat162float(source[i]);
-        } else {
-            for (i = t; i < count; i += kThreads) data[i] = __bfloat162float(source[i]);
-        }
-    } else {
-        const float* source = reinterpret_cast<const float*>(p.logits) + at;
-        if (p.vector) {
-            const float4* wide = reinterpret_cast<const float4*>(source);
-            for (int i = t; i < count / 4; i += kThreads) reinterpret_cast<float4*>(data)[i] = __ldg(wide + i);
-            for (int i = count / 4 * 4 + t; i < count; i += kThreads) data[i] = source[i];
-        } else {
-            for (int i = t; i < count; i += kThreads) data[i] = source[i];
+        if (top_k > 0 && place >= top_k) weight[o] = 0;
+    }
+    if (top_p < 1.0f) {
+        const uint64_t total = row_total ? row_total : total_of_kept();
+        const uint64_t need = top_p > 0.0f ? share_of(top_p, total, true) : 1;
+#pragma unroll
+        for (int o = 0; o < kOwn; ++o)
+            if (before[o] >= need) weight[o] = 0;
+    }
+#pragma unroll
+    for (int o = 0; o < kOwn; ++o)
+        if ((double)weight[o] < least && value_of((uint32_t)(rank[o] >> 32)) != row.top) weight[o] = 0;
+    const uint64_t total = total_of_kept();  // between its barriers everyone has read s.weight
+    const uint64_t border = border_of(p.uniforms[row_index], total);
+#pragma unroll
+    for (int o = 0; o < kOwn; ++o)
+        if (t + o * kThreads < candidates) s.weight[t + o * kThreads] = weight[o];
+    __syncthreads();
+#pragma unroll
+    for (int o = 0; o < kOwn; ++o) {
+        if (weight[o] == 0) continue;
+        uint64_t running = 0;
+        for (int j = 0; j < candidates; ++j)
+            if ((uint32_t)s.all[j] > (uint32_t)rank[o]) running += s.weight[j];  // a lower index has the larger complement
+        if (running <= border && running + weight[o] > border) {
+            p.tokens[row_index] = (long long)(0xFFFFFFFFu - (uint32_t)rank[o]);
+            p.logprobs[row_index] = logprob_of(row, value_of((uint32_t)(rank[o] >> 32)), total);
         }
     }
+}
+
+// A row's slice into shared memory as fp32, filled up to whole quadruples with minus infinity.
+__device__ void load_slice(const Params& p, int64_t at, int count, float* data) {
+    const int t = threadIdx.x;
+    const int step = p.bf16 ? 8 : 4, whole = p.vector ? count / step * step : 0;
+    if (p.bf16) {
+        const __nv_bfloat16* source = reinterpret_cast<const __nv_bfloat16*>(p.logits) + at;
+#pragma unroll 4
+        for (int i = 8 * t; i < whole; i += 8 * kThreads) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(source + i));
+            float4* to = reinterpret_cast<float4*>(data + i);
+            to[0] = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16),
+                                __uint_as_float(u.y & 0xFFFF0000u));
+            to[1] = make_float4(__uint_as_float(u.z << 16), __uint_as_float(u.z & 0xFFFF0000u), __uint_as_float(u.w << 16),
+                                __uint_as_float(u.w & 0xFFFF0000u));
+        }
+#pragma unroll 4
+        for (int i = whole + t; i < count; i += kThreads) data[i] = __bfloat162float(source[i]);
+    } else {
+        const float* source = reinterpret_cast<const float*>(p.logits) + at;
+#pragma unroll 4
+        for (int i = 4 * t; i < whole; i += 4 * kThreads)
+            *reinterpret_cast<float4*>(data + i) = __ldg(reinterpret_cast<const float4*>(source + i));
+#pragma unroll 4
+        for (int i = whole + t; i < count; i += kThreads) data[i] = source[i];
+    }
+    if (t < 4 && count + t < (count + 3) / 4 * 4) data[count + t] = -INFINITY;
 }
 
 __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
@@ -358,12 +509,11 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
     // the largest logit, the lowest index that has it, and whether a NaN is among them
     uint64_t best = 0;
     bool bad = false;
-    for (int i = t; i < count; i += kThreads) {
-        const float v = data[i];
+    for_each(data, count, [&](float v, int i) {
         bad |= v != v;
         const uint64_t rank = rank_of(key_of(v), (uint32_t)(first + i));
         best = best > rank ? best : rank;
-    }
+    });
 #pragma unroll
     for (int d = 16; d; d >>= 1) {
         const uint64_t other = __shfl_xor_sync(0xFFFFFFFFu, best, d);
@@ -391,7 +541,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
     const int top_k = p.top_k_dev ? p.top_k_dev[row_index] : p.top_k;
     const float top_p = p.top_p_dev ? p.top_p_dev[row_index] : p.top_p;
     const float min_p = p.min_p_dev ? p.min_p_dev[row_index] : p.min_p;
-    if (any_bad || row.top == -INFINITY) {
+    if (any_bad || best == 0) {
         if (rank_in_cluster == 0 && t == 0) {
             p.tokens[row_index] = -1;
             p.logprobs[row_index] = __uint_as_float(0x7FC00000u);
@@ -408,27 +558,51 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
     row.inverse = 1.0 / (double)temperature;
     row.bin_scale = fminf(kBinsPerUnit / temperature, 1e30f);
 
+    const double least = (double)min_p * kOne;
     uint64_t threshold = 0;
     int buffer = 0;
-    if (top_k > 0 && top_k < p.vocabulary)
-        threshold = find_threshold<false>(cluster, s, data, count, first, row, threshold, (uint64_t)top_k, 0.0f, buffer);
-    if (top_p < 1.0f)
-        threshold = find_threshold<true>(cluster, s, data, count, first, row, threshold, 0, top_p, buffer);
+    bool few = false;
+    uint64_t row_total = 0;
+    Found found;
+    if (top_k > 0 && top_k < p.vocabulary) {
+        uint64_t need = top_k;
+        found = first_step<false>(cluster, s, data, count, first, row, 0, need, 0.0f, buffer);
+        if (found.total > need) {
+            few = found.through <= kCandidates;
+            if (!few) threshold = search<false>(cluster, s, data, count, first, row, 0, need, found, buffer);
+        }
+    }
+    if (!few && top_p < 1.0f) {
+        uint64_t need = 1;
+        found = first_step<true>(cluster, s, data, count, first, row, threshold, need, top_p, buffer);
+        few = threshold == 0 && found.through <= kCandidates;
+        if (few)
+            row_total = found.total;
+        else
+            threshold = search<true>(cluster, s, data, count, first, row, threshold, need, found, buffer);
+    }
+    if (few) {
+        gather(s, data, count, first, [&](float v, uint64_t) { return first_bin(row, v) <= found.bin; });
+        cluster.sync();
+        if (rank_in_cluster == 0)
+            finish_few(cluster, s, p, row, row_index, row_total ? 0 : top_k, top_p, least, row_total);
+        cluster.sync();  // nobody leaves while its candidates may still be read
+        return;
+    }
 
     // the kept weight of every warp's run of the slice
-    const double least = (double)min_p * kOne;
     auto kept_weight = [&](int i) -> uint64_t {
         const float v = data[i];
-        if (rank_of(key_of(v), (uint32_t)(first + i)) < threshold) return 0;
+        if (v == -INFINITY || rank_of(key_of(v), (uint32_t)(first + i)) < threshold) return 0;
         const uint64_t w = weight_of(row, v);
         return v != row.top && (double)w < least ? 0 : w;
     };
     const int run = (count + kThreads - 1) / kThreads * 32;
     const int from = min(warp * run, count), to = min(from + run, count);
     uint64_t sum = 0;
+#pragma unroll 4
     for (int i = from + lane; i < to; i += 32) sum += kept_weight(i);
-#pragma unroll
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+    sum = warp_total(sum);
     if (lane == 0) s.warp_sum[warp] = sum;
     __syncthreads();
     if (t == 0) {
@@ -443,24 +617,17 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
         if (r < rank_in_cluster) before += of;
         total += of;
     }
-    // a sum exceeds u * total exactly if it exceeds the largest integer that is not above it
-    const float u = p.uniforms[row_index];
-    const uint64_t border = u >= 1.0f ? total - 1 : u > 0.0f ? share_of(u, total, false) : 0;
+    const uint64_t border = border_of(p.uniforms[row_index], total);
     for (int w = 0; w < warp; ++w) before += s.warp_sum[w];
     if (before <= border && before + s.warp_sum[warp] > border) {
         // this warp's run holds the token
         for (int i0 = from; i0 < to; i0 += 32) {
             const int i = i0 + lane;
             const uint64_t w = i < to ? kept_weight(i) : 0;
-            uint64_t running = w;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const uint64_t other = __shfl_up_sync(0xFFFFFFFFu, running, d);
-                if (lane >= d) running += other;
-            }
+            const uint64_t running = warp_running(w);
             if (w != 0 && before + running > border && before + running - w <= border) {
                 p.tokens[row_index] = first + i;
-                p.logprobs[row_index] = (float)(exponent_of(row, data[i]) - log((double)total / kOne));
+                p.logprobs[row_index] = logprob_of(row, data[i], total);
             }
             before += __shfl_sync(0xFFFFFFFFu, running, 31);
             if (before > border) break;
@@ -474,8 +641,7 @@ int launch(Params p, int64_t rows, cudaStream_t stream) {
     while (ctas < kMaxCluster && p.vocabulary > 4096 * ctas) ctas *= 2;
     p.slice = (int)(((p.vocabulary + ctas - 1) / ctas + 7) / 8 * 8);
     const size_t bytes = sizeof(Shared) + (size_t)p.slice * sizeof(float);
-    cudaError_t error = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int)(sizeof(Shared) + kMaxVocabulary / kMaxCluster * sizeof(float)));
+    cudaError_t error = allow_shared<sample_kernel>((int)(sizeof(Shared) + kMaxVocabulary / kMaxCluster * sizeof(float)));
     if (error != cudaSuccess) return record_cuda_error(error);
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3((unsigned)(rows * ctas));

@@ -117,7 +117,7 @@ def packed_matvec(
     factor = _checked_factor(float(tensor_amax), float(scale_target))
     flat = x if x.ndim == 2 else x.reshape(-1, cols)
     tokens = flat.shape[0]
-    out = torch.empty((tokens, rows), dtype=out_dtype, device=device)
+    out = x.new_empty((tokens, rows), dtype=out_dtype)
     if tokens and rows:
         ldx, step = flat.stride()
         if tokens == 1:
@@ -221,7 +221,7 @@ def paged_attention(
         raise ValueError("scale must be positive and finite")
     zero_tail = out is None
     if zero_tail:
-        out = torch.empty((tokens, heads, head_dim), dtype=_BF16, device=device)
+        out = q.new_empty((tokens, heads, head_dim))
     elif out.dtype is not _BF16 or out.shape != q.shape or not out.is_contiguous() or out.device != device:
         raise ValueError("out must be contiguous bfloat16 of q's shape on its device")
     k_pointer = v_pointer = None
@@ -320,8 +320,8 @@ def sample_tokens(
         raise ValueError("min_p must be in [0, 1]")
     if k[1] > vocabulary:
         k = (None, vocabulary)
-    tokens = torch.empty(rows, dtype=torch.int64, device=device)
-    logprobs = torch.empty(rows, dtype=torch.float32, device=device)
+    tokens = uniforms.new_empty(rows, dtype=torch.int64)
+    logprobs = uniforms.new_empty(rows)
     if rows:
         _call(_native.load().ue5m3_sample_tokens, "ue5m3_sample_tokens", 1, device, logits.data_ptr(), code, rows,
               vocabulary, ld, uniforms.data_ptr(), *heat, *k, *p, *least, tokens.data_ptr(), logprobs.data_ptr())
