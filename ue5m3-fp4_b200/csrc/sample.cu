@@ -62,6 +62,7 @@ struct Params {
 };
 
 struct alignas(16) Shared {
+    double power[8];             // 2^(j / 8)
     uint32_t hist[2][4][kBins];  // [buffer][count, weight bits 0..14, 15..29, 30..44]
     uint64_t mine[kCandidates];  // this CTA's candidates
     uint64_t all[kCandidates];
@@ -70,7 +71,8 @@ struct alignas(16) Shared {
     uint64_t cta_sum;
     uint64_t found, found_before;
     uint64_t low, high;          // bounds of the ranks in a bin (this CTA's)
-    uint32_t top_key, top_index, bad, count;
+    float warp_top[kWarps], cta_top;
+    uint32_t first_top, count;
     uint32_t found_bin, found_count, found_through;
     uint32_t warp_number[kWarps];
 };
@@ -81,34 +83,18 @@ __device__ __forceinline__ uint32_t key_of(float v) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
 __device__ __forceinline__ float value_of(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
 }
 
 __device__ __forceinline__ uint64_t rank_of(uint32_t key, uint32_t index) {
     return (uint64_t)key << 32 | (0xFFFFFFFFu - index);
-}
-
-// 2^44 exp(z), z <= 0, to the nearest integer: Taylor's polynomial of degree 11 on
-// |r| <= ln(2) / 2, whose remainder is below 2^-47 of the value.
-__device__ __forceinline__ uint64_t weight_of(double z) {
-    if (!(z > -31.2)) return 0;  // below half a unit
-    const double n = rint(z * 1.4426950408889634);
-    const double r = fma(n, -0.6931471805599453, z);  // |n| <= 45: the constant's rounding costs 2^-49
-    double e = 1.0 / 39916800.0;
-    e = fma(e, r, 1.0 / 3628800.0);
-    e = fma(e, r, 1.0 / 362880.0);
-    e = fma(e, r, 1.0 / 40320.0);
-    e = fma(e, r, 1.0 / 5040.0);
-    e = fma(e, r, 1.0 / 720.0);
-    e = fma(e, r, 1.0 / 120.0);
-    e = fma(e, r, 1.0 / 24.0);
-    e = fma(e, r, 1.0 / 6.0);
-    e = fma(e, r, 0.5);
-    e = fma(e, r, 1.0);
-    e = fma(e, r, 1.0);
-    const double scaled = __hiloint2double(__double2hiint(e) + (((int)n + 44) << 20), __double2loint(e));
-    return (uint64_t)__double2ull_rn(scaled);
 }
 
 // share * total for 0 <= share < 1, rounded down or up to an integer, exactly
@@ -131,9 +117,10 @@ __device__ __forceinline__ uint64_t share_of(float share, uint64_t total, bool u
 }
 
 struct Row {
-    float top;         // the largest logit
-    double inverse;    // 1 / T
-    float bin_scale;   // kBinsPerUnit / T, finite
+    float top;            // the largest logit
+    double inverse;       // 1 / T
+    float bin_scale;      // kBinsPerUnit / T, finite
+    const double* power;  // 2^(j / 8) in shared memory
 };
 
 __device__ __forceinline__ double exponent_of(const Row& row, float v) {
@@ -141,9 +128,27 @@ __device__ __forceinline__ double exponent_of(const Row& row, float v) {
     return ((double)v - (double)row.top) * row.inverse;
 }
 
+// 2^44 exp(z), z <= 0, to the nearest integer.  z = k ln(2) / 8 + r: a power of two, a table of eight
+// and Taylor's polynomial of degree 7, whose remainder on |r| <= ln(2) / 16 is below 2^-51 of the
+// value (ln(2) / 8 is rounded, which k <= 361 makes less than 2^-48).  Adding 1.5 * 2^52 leaves the
+// nearest integer in the low bits.
 __device__ __forceinline__ uint64_t weight_of(const Row& row, float v) {
-    if (v == -INFINITY) return 0;
-    return weight_of(exponent_of(row, v));
+    const double z = exponent_of(row, v);
+    if (!(z > -31.2)) return 0;  // below half a unit
+    constexpr double kMagic = 6755399441055744.0;
+    const double shifted = fma(z, 8.0 * 1.4426950408889634, kMagic);
+    const int k = __double2loint(shifted);
+    const double r = fma(shifted - kMagic, -0.6931471805599453 / 8.0, z);
+    double e = 1.0 / 5040.0;
+    e = fma(e, r, 1.0 / 720.0);
+    e = fma(e, r, 1.0 / 120.0);
+    e = fma(e, r, 1.0 / 24.0);
+    e = fma(e, r, 1.0 / 6.0);
+    e = fma(e, r, 0.5);
+    e = fma(e, r, 1.0);
+    e = fma(e, r, 1.0) * row.power[k & 7];
+    e = __hiloint2double(__double2hiint(e) + (((k >> 3) + 44) << 20), __double2loint(e)) + kMagic;
+    return (uint64_t)__double_as_longlong(e) & (((uint64_t)1 << 51) - 1);
 }
 
 __device__ __forceinline__ uint32_t first_bin(const Row& row, float v) {
@@ -164,6 +169,13 @@ __device__ __forceinline__ void for_each(const float* data, int count, Function 
         if (v.z != -INFINITY) f(v.z, i + 2);
         if (v.w != -INFINITY) f(v.w, i + 3);
     }
+}
+
+// f(0) ... f(kMaxCluster - 1), unrolled: reads of other CTAs' memory are in flight together
+template <typename Function>
+__device__ __forceinline__ void for_each_cta(Function f) {
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) f(r);
 }
 
 __device__ __forceinline__ uint64_t warp_total(uint64_t v) {
@@ -203,15 +215,20 @@ template <bool kWeighted>
 __device__ Found scan_bins(cg::cluster_group& cluster, Shared& s, int& buffer, uint64_t& need, float share) {
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     cluster.sync();
+    const int ctas = cluster.num_blocks();
+    uint32_t parts[kMaxCluster][4];
+    for_each_cta([&](int r) {
+        const Shared* other = cluster.map_shared_rank(&s, r < ctas ? r : 0);
+#pragma unroll
+        for (int i = 0; i < (kWeighted ? 4 : 1); ++i) parts[r][i] = other->hist[buffer][i][t];
+    });
     uint64_t mass = 0;
     uint32_t number = 0;
-    for (int r = 0; r < (int)cluster.num_blocks(); ++r) {
-        const Shared* other = cluster.map_shared_rank(&s, r);
-        number += other->hist[buffer][0][t];
-        if (kWeighted)
-            mass += (uint64_t)other->hist[buffer][1][t] + ((uint64_t)other->hist[buffer][2][t] << 15) +
-                    ((uint64_t)other->hist[buffer][3][t] << 30);
-    }
+    for_each_cta([&](int r) {
+        if (r >= ctas) return;
+        number += parts[r][0];
+        if (kWeighted) mass += (uint64_t)parts[r][1] + ((uint64_t)parts[r][2] << 15) + ((uint64_t)parts[r][3] << 30);
+    });
     buffer ^= 1;  // the next step writes the other one, which nobody reads any more
     if (!kWeighted) mass = number;
     uint64_t running = warp_running(mass), numbers = kWeighted ? warp_running(number) : 0;
@@ -295,16 +312,20 @@ __device__ void gather(Shared& s, const float* data, int count, uint32_t base, T
 // The candidates of all CTAs and their weights, in this one's memory.
 template <bool kWeighted>
 __device__ int collect(cg::cluster_group& cluster, Shared& s, const Row& row) {
-    int candidates = 0;
-    for (int r = 0; r < (int)cluster.num_blocks(); ++r) {
-        const Shared* other = cluster.map_shared_rank(&s, r);
-        const int n = (int)other->count;
-        for (int i = threadIdx.x; i < n; i += kThreads) {
-            const uint64_t rank = other->mine[i];
-            s.all[candidates + i] = rank;
-            s.weight[candidates + i] = kWeighted ? weight_of(row, value_of((uint32_t)(rank >> 32))) : 1;
-        }
-        candidates += n;
+    const int ctas = cluster.num_blocks();
+    int starts[kMaxCluster + 1];
+    for_each_cta([&](int r) { starts[r + 1] = (int)cluster.map_shared_rank(&s, r < ctas ? r : 0)->count; });
+    starts[0] = 0;
+    for_each_cta([&](int r) { starts[r + 1] = starts[r] + (r < ctas ? starts[r + 1] : 0); });
+    const int candidates = starts[kMaxCluster];
+    for (int i = threadIdx.x; i < candidates; i += kThreads) {
+        int from = 0, start = 0;
+        for_each_cta([&](int r) {
+            if (i >= starts[r] && i < starts[r + 1]) from = r, start = starts[r];
+        });
+        const uint64_t rank = cluster.map_shared_rank(&s, from)->mine[i - start];
+        s.all[i] = rank;
+        s.weight[i] = kWeighted ? weight_of(row, value_of((uint32_t)(rank >> 32))) : 1;
     }
     __syncthreads();
     return candidates;
@@ -338,7 +359,7 @@ __device__ uint64_t search(cg::cluster_group& cluster, Shared& s, const float* d
         cluster.sync();
         low = ~0ull;
         high = 0;
-        for (int r = 0; r < (int)cluster.num_blocks(); ++r) {
+        for (int r = 0; r < (int)cluster.num_blocks(); ++r) {  // seldom: many equal logits
             const Shared* other = cluster.map_shared_rank(&s, r);
             low = low < other->low ? low : other->low;
             high = high > other->high ? high : other->high;
@@ -460,32 +481,41 @@ __device__ void finish_few(cg::cluster_group& cluster, Shared& s, const Params& 
     }
 }
 
-// A row's slice into shared memory as fp32, filled up to whole quadruples with minus infinity.
-__device__ void load_slice(const Params& p, int64_t at, int count, float* data) {
+// A row's slice into shared memory as fp32, filled up to whole quadruples with minus infinity; returns
+// the largest of the thread's elements, or NaN if one of them is.
+__device__ float load_slice(const Params& p, int64_t at, int count, float* data) {
     const int t = threadIdx.x;
+    float top = -INFINITY;
     const int step = p.bf16 ? 8 : 4, whole = p.vector ? count / step * step : 0;
     if (p.bf16) {
         const __nv_bfloat16* source = reinterpret_cast<const __nv_bfloat16*>(p.logits) + at;
 #pragma unroll 4
         for (int i = 8 * t; i < whole; i += 8 * kThreads) {
             const uint4 u = __ldg(reinterpret_cast<const uint4*>(source + i));
-            float4* to = reinterpret_cast<float4*>(data + i);
-            to[0] = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16),
-                                __uint_as_float(u.y & 0xFFFF0000u));
-            to[1] = make_float4(__uint_as_float(u.z << 16), __uint_as_float(u.z & 0xFFFF0000u), __uint_as_float(u.w << 16),
-                                __uint_as_float(u.w & 0xFFFF0000u));
+            const float4 lo = make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u),
+                                          __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xFFFF0000u));
+            const float4 hi = make_float4(__uint_as_float(u.z << 16), __uint_as_float(u.z & 0xFFFF0000u),
+                                          __uint_as_float(u.w << 16), __uint_as_float(u.w & 0xFFFF0000u));
+            reinterpret_cast<float4*>(data + i)[0] = lo;
+            reinterpret_cast<float4*>(data + i)[1] = hi;
+            top = max_nan(top, max_nan(max_nan(lo.x, lo.y), max_nan(lo.z, lo.w)));
+            top = max_nan(top, max_nan(max_nan(hi.x, hi.y), max_nan(hi.z, hi.w)));
         }
 #pragma unroll 4
-        for (int i = whole + t; i < count; i += kThreads) data[i] = __bfloat162float(source[i]);
+        for (int i = whole + t; i < count; i += kThreads) top = max_nan(top, data[i] = __bfloat162float(source[i]));
     } else {
         const float* source = reinterpret_cast<const float*>(p.logits) + at;
 #pragma unroll 4
-        for (int i = 4 * t; i < whole; i += 4 * kThreads)
-            *reinterpret_cast<float4*>(data + i) = __ldg(reinterpret_cast<const float4*>(source + i));
+        for (int i = 4 * t; i < whole; i += 4 * kThreads) {
+            const float4 v = __ldg(reinterpret_cast<const float4*>(source + i));
+            *reinterpret_cast<float4*>(data + i) = v;
+            top = max_nan(top, max_nan(max_nan(v.x, v.y), max_nan(v.z, v.w)));
+        }
 #pragma unroll 4
-        for (int i = whole + t; i < count; i += kThreads) data[i] = source[i];
+        for (int i = whole + t; i < count; i += kThreads) top = max_nan(top, data[i] = source[i]);
     }
     if (t < 4 && count + t < (count + 3) / 4 * 4) data[count + t] = -INFINITY;
+    return top;
 }
 
 __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
@@ -498,61 +528,52 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const int first = min(rank_in_cluster * p.slice, p.vocabulary);
     const int count = min(p.slice, p.vocabulary - first);
-    load_slice(p, (int64_t)row_index * p.ld + first, count, data);
-    if (t == 0) {
-        s.top_key = 0;
-        s.top_index = 0xFFFFFFFFu;
-        s.bad = 0;
-    }
-    __syncthreads();
-
-    // the largest logit, the lowest index that has it, and whether a NaN is among them
-    uint64_t best = 0;
-    bool bad = false;
-    for_each(data, count, [&](float v, int i) {
-        bad |= v != v;
-        const uint64_t rank = rank_of(key_of(v), (uint32_t)(first + i));
-        best = best > rank ? best : rank;
-    });
+    float top = load_slice(p, (int64_t)row_index * p.ld + first, count, data);
+    if (t == 0) s.first_top = 0xFFFFFFFFu;
+    if (t < 8) s.power[t] = exp2(0.125 * t);
 #pragma unroll
-    for (int d = 16; d; d >>= 1) {
-        const uint64_t other = __shfl_xor_sync(0xFFFFFFFFu, best, d);
-        best = best > other ? best : other;
-    }
-    if (bad) s.bad = 1;
-    if (lane == 0) s.warp_sum[warp] = best;
+    for (int d = 16; d; d >>= 1) top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+    if (lane == 0) s.warp_top[warp] = top;
     __syncthreads();
-    if (t == 0) {
-        for (int w = 1; w < kWarps; ++w) best = best > s.warp_sum[w] ? best : s.warp_sum[w];
-        s.cta_sum = best;
+    if (warp == 0) {
+        top = s.warp_top[lane % kWarps];
+#pragma unroll
+        for (int d = 8; d; d >>= 1) top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+        if (lane == 0) s.cta_top = top;
     }
     cluster.sync();
-    best = 0;
-    uint32_t any_bad = 0;
-    for (int r = 0; r < ctas; ++r) {
-        const Shared* other = cluster.map_shared_rank(&s, r);
-        best = best > other->cta_sum ? best : other->cta_sum;
-        any_bad |= other->bad;
-    }
-    cluster.sync();  // cta_sum and warp_sum are used again
+    float tops[kMaxCluster];
+    for_each_cta([&](int r) { tops[r] = cluster.map_shared_rank(&s, r < ctas ? r : 0)->cta_top; });
+    top = tops[0];
+    for_each_cta([&](int r) { top = max_nan(top, tops[r]); });
     Row row;
-    row.top = value_of((uint32_t)(best >> 32));
+    row.power = s.power;
+    row.top = top;
     const float temperature = p.temperature_dev ? p.temperature_dev[row_index] : p.temperature;
     const int top_k = p.top_k_dev ? p.top_k_dev[row_index] : p.top_k;
     const float top_p = p.top_p_dev ? p.top_p_dev[row_index] : p.top_p;
     const float min_p = p.min_p_dev ? p.min_p_dev[row_index] : p.min_p;
-    if (any_bad || best == 0) {
+    if (top != top || top == -INFINITY) {
         if (rank_in_cluster == 0 && t == 0) {
             p.tokens[row_index] = -1;
             p.logprobs[row_index] = __uint_as_float(0x7FC00000u);
         }
+        cluster.sync();  // nobody leaves while its maximum may still be read
         return;
     }
     if (!(temperature > 0.0f) || top_k == 1) {
+        // the first of the largest logits
+        for_each(data, count, [&](float v, int i) {
+            if (v == top) atomicMin(&s.first_top, (uint32_t)(first + i));
+        });
+        cluster.sync();
         if (rank_in_cluster == 0 && t == 0) {
-            p.tokens[row_index] = (long long)(0xFFFFFFFFu - (uint32_t)best);
+            uint32_t index = 0xFFFFFFFFu;
+            for (int r = 0; r < ctas; ++r) index = min(index, cluster.map_shared_rank(&s, r)->first_top);
+            p.tokens[row_index] = index;
             p.logprobs[row_index] = 0.0f;
         }
+        cluster.sync();
         return;
     }
     row.inverse = 1.0 / (double)temperature;
@@ -611,12 +632,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
         s.cta_sum = all;
     }
     cluster.sync();
-    uint64_t total = 0, before = 0;
-    for (int r = 0; r < ctas; ++r) {
-        const uint64_t of = cluster.map_shared_rank(&s, r)->cta_sum;
-        if (r < rank_in_cluster) before += of;
-        total += of;
-    }
+    uint64_t sums[kMaxCluster], total = 0, before = 0;
+    for_each_cta([&](int r) { sums[r] = cluster.map_shared_rank(&s, r < ctas ? r : 0)->cta_sum; });
+    for_each_cta([&](int r) {
+        if (r < ctas) total += sums[r];
+        if (r < rank_in_cluster) before += sums[r];
+    });
     const uint64_t border = border_of(p.uniforms[row_index], total);
     for (int w = 0; w < warp; ++w) before += s.warp_sum[w];
     if (before <= border && before + s.warp_sum[warp] > border) {
