@@ -441,6 +441,26 @@ def test_sample_settings_per_row_and_uniform_range():
                  top_p=torch.tensor([1.0, 0.9, 0.4, 1.0, 0.0, 0.3, 0.99]), min_p=torch.tensor([0.0, 0.1, 0.0, 0.5, 0.0, 0.0, 0.01]))
 
 
+@pytest.mark.parametrize("vocabulary", [3000, 131072])
+def test_sample_tails_without_weight(vocabulary):
+    """A few tokens carry all the weight, thousands none or next to none: the nucleus ends among them."""
+
+    g = torch.Generator().manual_seed(4)
+    logits = torch.full((6, vocabulary), -100.0)
+    logits[:, ::vocabulary // 900] = 0.0
+    logits[1] -= torch.arange(vocabulary) / vocabulary          # all of weight zero, all different
+    logits[2, ::7] = -20.0                                      # thousands of equal tiny weights
+    logits[3] = -31.0 * torch.rand(vocabulary, generator=g)     # weights down to the last unit
+    logits[4] = -16.0 - 16.0 * torch.rand(vocabulary, generator=g)
+    logits[4, 5] = 0.0
+    logits[5] = -29.0
+    logits[5, 11] = 0.0
+    uniforms = torch.tensor([0.3, 0.9, 0.99999, 0.5, 1.0 - 2.0 ** -24, 1.0 - 2.0 ** -24])
+    for settings in (dict(top_p=0.9999999), dict(top_p=0.999), dict(top_p=1.0 - 2.0 ** -24, min_p=1e-9), dict(top_k=1500, top_p=0.99999),
+                     dict(top_k=1000, top_p=0.9999), dict(temperature=0.5, top_p=0.9999999)):
+        check_sample(logits, uniforms, **settings)
+
+
 def test_sample_strided_rows():
     from ue5m3_fp4 import serving
 

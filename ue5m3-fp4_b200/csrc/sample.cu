@@ -124,8 +124,8 @@ struct Row {
 };
 
 __device__ __forceinline__ double exponent_of(const Row& row, float v) {
-    if (v == row.top) return 0.0;  // also where both are infinite
-    return ((double)v - (double)row.top) * row.inverse;
+    const double z = ((double)v - (double)row.top) * row.inverse;
+    return v == row.top ? 0.0 : z;  // also where both are infinite
 }
 
 // 2^44 exp(z), z <= 0, to the nearest integer.  z = k ln(2) / 8 + r: a power of two, a table of eight
@@ -134,7 +134,6 @@ __device__ __forceinline__ double exponent_of(const Row& row, float v) {
 // nearest integer in the low bits.
 __device__ __forceinline__ uint64_t weight_of(const Row& row, float v) {
     const double z = exponent_of(row, v);
-    if (!(z > -31.2)) return 0;  // below half a unit
     constexpr double kMagic = 6755399441055744.0;
     const double shifted = fma(z, 8.0 * 1.4426950408889634, kMagic);
     const int k = __double2loint(shifted);
@@ -148,17 +147,28 @@ __device__ __forceinline__ uint64_t weight_of(const Row& row, float v) {
     e = fma(e, r, 1.0);
     e = fma(e, r, 1.0) * row.power[k & 7];
     e = __hiloint2double(__double2hiint(e) + (((k >> 3) + 44) << 20), __double2loint(e)) + kMagic;
-    return (uint64_t)__double_as_longlong(e) & (((uint64_t)1 << 51) - 1);
+    const uint64_t w = (uint64_t)__double_as_longlong(e) & (((uint64_t)1 << 51) - 1);
+    return z > -31.2 ? w : 0;  // below half a unit, or masked
 }
 
 __device__ __forceinline__ uint32_t first_bin(const Row& row, float v) {
-    if (v == row.top) return 0;
     const float bin = (row.top - v) * row.bin_scale;  // monotone in v: each step rounds monotonely
-    return bin < (float)(kBins - 1) ? (uint32_t)bin : kBins - 1;
+    return v == row.top ? 0 : (uint32_t)fminf(bin, (float)(kBins - 1));
 }
 
-// f(logit, place in the slice) for the elements of a slice that are not masked; the slice is filled
-// up to whole quadruples with minus infinity
+// f(four neighbouring logits, place of the first in the slice); the slice is filled up to whole
+// quadruples with minus infinity.  What f does to the four is written without branches where it is
+// done to all of a row: their latencies would add up.
+template <typename Function>
+__device__ __forceinline__ void for_each_four(const float* data, int count, Function f) {
+    for (int i = 4 * threadIdx.x; i < count; i += 4 * kThreads) {
+        const float4 v = *reinterpret_cast<const float4*>(data + i);
+        const float four[4] = {v.x, v.y, v.z, v.w};
+        f(four, i);
+    }
+}
+
+// f(logit, place in the slice) for the elements of a slice that are not masked
 template <typename Function>
 __device__ __forceinline__ void for_each(const float* data, int count, Function f) {
 #pragma unroll 2
@@ -275,18 +285,22 @@ __device__ Found first_step(cg::cluster_group& cluster, Shared& s, const float* 
     clear_bins(s, buffer);
     uint32_t(*hist)[kBins] = s.hist[buffer];
     uint64_t last_number = 0, last_weight = 0;
-    for_each(data, count, [&](float v, int i) {
-        if (floor != 0 && rank_of(key_of(v), base + i) < floor) return;
-        const uint32_t bin = first_bin(row, v);
-        const uint64_t w = kWeighted ? weight_of(row, v) : 1;
-        if (w == 0) return;
-        if (bin == kBins - 1) {
-            ++last_number;
-            last_weight += w;
-            return;
+    for_each_four(data, count, [&](const float(&v)[4], int i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            bool in = v[e] != -INFINITY;
+            if (floor != 0) in = in && rank_of(key_of(v[e]), base + i + e) >= floor;
+            const uint32_t bin = first_bin(row, v[e]);
+            const uint64_t w = kWeighted ? weight_of(row, v[e]) : 1;
+            in = in && w != 0;
+            const bool last = bin == kBins - 1;
+            last_number += in && last;
+            last_weight += in && last ? w : 0;
+            if (in && !last) {
+                atomicAdd(&hist[0][bin], 1u);
+                if (kWeighted) add_weight(hist, bin, w);
+            }
         }
-        atomicAdd(&hist[0][bin], 1u);
-        if (kWeighted) add_weight(hist, bin, w);
     });
     last_number = warp_total(last_number);
     if (kWeighted) last_weight = warp_total(last_weight);
@@ -297,15 +311,29 @@ __device__ Found first_step(cg::cluster_group& cluster, Shared& s, const float* 
     return scan_bins<kWeighted>(cluster, s, buffer, need, share);
 }
 
-// This CTA's elements that `take` names, into its list of candidates; the list's last writes are
-// seen after the next cluster barrier.
+// In the first step's bins: weights of zero, which are not counted, lie in the last one only.
+template <bool kWeighted>
+__device__ __forceinline__ bool counted(const Row& row, float v, uint32_t bin) {
+    return !kWeighted || bin < kBins - 1 || weight_of(row, v) != 0;
+}
+
+// This CTA's elements that `take` names (the caller has counted them: kCandidates at most), into its
+// list of candidates; the list's last writes are seen after the next cluster barrier.
 template <typename Take>
 __device__ void gather(Shared& s, const float* data, int count, uint32_t base, Take take) {
     if (threadIdx.x == 0) s.count = 0;
     __syncthreads();
-    for_each(data, count, [&](float v, int i) {
-        const uint64_t rank = rank_of(key_of(v), base + i);
-        if (take(v, rank)) s.mine[atomicAdd(&s.count, 1u)] = rank;
+    for_each_four(data, count, [&](const float(&v)[4], int i) {
+        bool taken[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) taken[e] = v[e] != -INFINITY && take(v[e], rank_of(key_of(v[e]), base + i + e));
+        if (taken[0] || taken[1] || taken[2] || taken[3])
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (taken[e]) {
+                    const uint32_t at = atomicAdd(&s.count, 1u);
+                    if (at < kCandidates) s.mine[at] = rank_of(key_of(v[e]), base + i + e);
+                }
     });
 }
 
@@ -339,7 +367,7 @@ __device__ uint64_t search(cg::cluster_group& cluster, Shared& s, const float* d
     uint64_t low = floor, high = ~0ull;
     if (found.inside <= kCandidates) {
         gather(s, data, count, base, [&](float v, uint64_t rank) {
-            return rank >= floor && first_bin(row, v) == found.bin && (!kWeighted || weight_of(row, v) != 0);
+            return rank >= floor && first_bin(row, v) == found.bin && counted<kWeighted>(row, v, found.bin);
         });
     } else {
         if (threadIdx.x == 0) {
@@ -388,7 +416,7 @@ __device__ uint64_t search(cg::cluster_group& cluster, Shared& s, const float* d
             if (next.inside <= kCandidates) break;
         }
         gather(s, data, count, base, [&](float v, uint64_t rank) {
-            return rank >= low && rank <= high && (!kWeighted || weight_of(row, v) != 0);
+            return rank >= low && rank <= high;  // `low` is the rank of an element with weight: all above have some
         });
     }
     cluster.sync();
@@ -603,7 +631,10 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
             threshold = search<true>(cluster, s, data, count, first, row, threshold, need, found, buffer);
     }
     if (few) {
-        gather(s, data, count, first, [&](float v, uint64_t) { return first_bin(row, v) <= found.bin; });
+        gather(s, data, count, first, [&](float v, uint64_t) {
+            const uint32_t bin = first_bin(row, v);
+            return bin <= found.bin && (row_total ? counted<true>(row, v, bin) : true);
+        });
         cluster.sync();
         if (rank_in_cluster == 0)
             finish_few(cluster, s, p, row, row_index, row_total ? 0 : top_k, top_p, least, row_total);
@@ -614,9 +645,9 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
     // the kept weight of every warp's run of the slice
     auto kept_weight = [&](int i) -> uint64_t {
         const float v = data[i];
-        if (v == -INFINITY || rank_of(key_of(v), (uint32_t)(first + i)) < threshold) return 0;
+        const bool kept = v != -INFINITY && rank_of(key_of(v), (uint32_t)(first + i)) >= threshold;
         const uint64_t w = weight_of(row, v);
-        return v != row.top && (double)w < least ? 0 : w;
+        return kept && (v == row.top || (double)w >= least) ? w : 0;
     };
     const int run = (count + kThreads - 1) / kThreads * 32;
     const int from = min(warp * run, count), to = min(from + run, count);
