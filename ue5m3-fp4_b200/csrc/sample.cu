@@ -152,8 +152,9 @@ __device__ __forceinline__ uint64_t weight_of(const Row& row, float v) {
 }
 
 __device__ __forceinline__ uint32_t first_bin(const Row& row, float v) {
-    const float bin = (row.top - v) * row.bin_scale;  // monotone in v: each step rounds monotonely
-    return v == row.top ? 0 : (uint32_t)fminf(bin, (float)(kBins - 1));
+    // monotone in v, as each step rounds monotonely; 2^23 leaves the nearest integer in the low bits
+    const float bin = fminf((row.top - v) * row.bin_scale, (float)(kBins - 1)) + 8388608.0f;
+    return v == row.top ? 0 : __float_as_uint(bin) & (kBins - 1);
 }
 
 // f(four neighbouring logits, place of the first in the slice); the slice is filled up to whole
@@ -288,11 +289,10 @@ __device__ Found first_step(cg::cluster_group& cluster, Shared& s, const float* 
     for_each_four(data, count, [&](const float(&v)[4], int i) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            bool in = v[e] != -INFINITY;
-            if (floor != 0) in = in && rank_of(key_of(v[e]), base + i + e) >= floor;
             const uint32_t bin = first_bin(row, v[e]);
             const uint64_t w = kWeighted ? weight_of(row, v[e]) : 1;
-            in = in && w != 0;
+            bool in = kWeighted ? w != 0 : v[e] != -INFINITY;
+            if (floor != 0) in = in && rank_of(key_of(v[e]), base + i + e) >= floor;
             const bool last = bin == kBins - 1;
             last_number += in && last;
             last_weight += in && last ? w : 0;
@@ -317,23 +317,26 @@ __device__ __forceinline__ bool counted(const Row& row, float v, uint32_t bin) {
     return !kWeighted || bin < kBins - 1 || weight_of(row, v) != 0;
 }
 
-// This CTA's elements that `take` names (the caller has counted them: kCandidates at most), into its
-// list of candidates; the list's last writes are seen after the next cluster barrier.
-template <typename Take>
-__device__ void gather(Shared& s, const float* data, int count, uint32_t base, Take take) {
+// This CTA's elements that `look`, a glance at the logit, and `take` name (the caller has counted them:
+// kCandidates at most), into its list of candidates; the list's last writes are seen after the next
+// cluster barrier.
+template <typename Look, typename Take>
+__device__ void gather(Shared& s, const float* data, int count, uint32_t base, Look look, Take take) {
     if (threadIdx.x == 0) s.count = 0;
     __syncthreads();
     for_each_four(data, count, [&](const float(&v)[4], int i) {
         bool taken[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) taken[e] = v[e] != -INFINITY && take(v[e], rank_of(key_of(v[e]), base + i + e));
+        for (int e = 0; e < 4; ++e) taken[e] = look(v[e]) && v[e] != -INFINITY;
         if (taken[0] || taken[1] || taken[2] || taken[3])
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (taken[e]) {
+            for (int e = 0; e < 4; ++e) {
+                const uint64_t rank = rank_of(key_of(v[e]), base + i + e);
+                if (taken[e] && take(v[e], rank)) {
                     const uint32_t at = atomicAdd(&s.count, 1u);
-                    if (at < kCandidates) s.mine[at] = rank_of(key_of(v[e]), base + i + e);
+                    if (at < kCandidates) s.mine[at] = rank;
                 }
+            }
     });
 }
 
@@ -366,9 +369,8 @@ __device__ uint64_t search(cg::cluster_group& cluster, Shared& s, const float* d
     uint64_t above = found.before;  // mass of the ranks above `high`
     uint64_t low = floor, high = ~0ull;
     if (found.inside <= kCandidates) {
-        gather(s, data, count, base, [&](float v, uint64_t rank) {
-            return rank >= floor && first_bin(row, v) == found.bin && counted<kWeighted>(row, v, found.bin);
-        });
+        gather(s, data, count, base, [&](float v) { return first_bin(row, v) == found.bin; },
+               [&](float v, uint64_t rank) { return rank >= floor && counted<kWeighted>(row, v, found.bin); });
     } else {
         if (threadIdx.x == 0) {
             s.low = ~0ull;
@@ -415,9 +417,9 @@ __device__ uint64_t search(cg::cluster_group& cluster, Shared& s, const float* d
             low = high - low > width ? high - width : low;
             if (next.inside <= kCandidates) break;
         }
-        gather(s, data, count, base, [&](float v, uint64_t rank) {
-            return rank >= low && rank <= high;  // `low` is the rank of an element with weight: all above have some
-        });
+        // `low` is the rank of an element with weight: all above have some
+        gather(s, data, count, base, [&](float v) { return first_bin(row, v) == found.bin; },
+               [&](float, uint64_t rank) { return rank >= low && rank <= high; });
     }
     cluster.sync();
     const int candidates = collect<kWeighted>(cluster, s, row);
@@ -546,7 +548,7 @@ __device__ float load_slice(const Params& p, int64_t at, int count, float* data)
     return top;
 }
 
-__global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
     extern __shared__ __align__(16) unsigned char raw[];
     Shared& s = *reinterpret_cast<Shared*>(raw);
     float* data = reinterpret_cast<float*>(raw + sizeof(Shared));
@@ -610,7 +612,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
     const double least = (double)min_p * kOne;
     uint64_t threshold = 0;
     int buffer = 0;
-    bool few = false;
+    bool few = false, in_bins = false;
     uint64_t row_total = 0;
     Found found;
     if (top_k > 0 && top_k < p.vocabulary) {
@@ -627,14 +629,14 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
         few = threshold == 0 && found.through <= kCandidates;
         if (few)
             row_total = found.total;
-        else
+        else {
+            in_bins = found.inside <= kCandidates;  // the search adds no histogram to the first step's
             threshold = search<true>(cluster, s, data, count, first, row, threshold, need, found, buffer);
+        }
     }
     if (few) {
-        gather(s, data, count, first, [&](float v, uint64_t) {
-            const uint32_t bin = first_bin(row, v);
-            return bin <= found.bin && (row_total ? counted<true>(row, v, bin) : true);
-        });
+        gather(s, data, count, first, [&](float v) { return first_bin(row, v) <= found.bin; },
+               [&](float v, uint64_t) { return row_total == 0 || counted<true>(row, v, first_bin(row, v)); });
         cluster.sync();
         if (rank_in_cluster == 0)
             finish_few(cluster, s, p, row, row_index, row_total ? 0 : top_k, top_p, least, row_total);
@@ -651,10 +653,26 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
     };
     const int run = (count + kThreads - 1) / kThreads * 32;
     const int from = min(warp * run, count), to = min(from + run, count);
-    uint64_t sum = 0;
+    auto sum_runs = [&]() {
+        uint64_t sum = 0;
 #pragma unroll 4
-    for (int i = from + lane; i < to; i += 32) sum += kept_weight(i);
-    sum = warp_total(sum);
+        for (int i = from + lane; i < to; i += 32) sum += kept_weight(i);
+        return warp_total(sum);
+    };
+    // What this CTA keeps: the bins above the one with top-p's threshold and, of that one, the
+    // candidates down to it; where there is no such step, or min-p cuts too, the sum over its slice.
+    const bool from_bins = in_bins && !(least > 0.0);
+    uint64_t sum = 0;
+    if (from_bins) {
+        const uint32_t(*hist)[kBins] = s.hist[buffer ^ 1];
+        if (t < (int)found.bin) sum = (uint64_t)hist[1][t] + ((uint64_t)hist[2][t] << 15) + ((uint64_t)hist[3][t] << 30);
+        for (int i = t; i < (int)s.count; i += kThreads)
+            if (s.mine[i] >= threshold) sum += weight_of(row, value_of((uint32_t)(s.mine[i] >> 32)));
+        sum = warp_total(sum);
+    } else {
+        sum = sum_runs();
+    }
+    __syncthreads();
     if (lane == 0) s.warp_sum[warp] = sum;
     __syncthreads();
     if (t == 0) {
@@ -670,8 +688,15 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const Params p) {
         if (r < rank_in_cluster) before += sums[r];
     });
     const uint64_t border = border_of(p.uniforms[row_index], total);
+    if (from_bins && before <= border && before + s.cta_sum > border) {  // the token is in this CTA's slice
+        sum = sum_runs();
+        __syncthreads();
+        if (lane == 0) s.warp_sum[warp] = sum;
+        __syncthreads();
+    }
+    const bool here = before <= border && before + s.cta_sum > border;
     for (int w = 0; w < warp; ++w) before += s.warp_sum[w];
-    if (before <= border && before + s.warp_sum[warp] > border) {
+    if (here && before <= border && before + s.warp_sum[warp] > border) {
         // this warp's run holds the token
         for (int i0 = from; i0 < to; i0 += 32) {
             const int i = i0 + lane;
