@@ -472,3 +472,219 @@ def test_sample_strided_rows():
     assert torch.equal(got[0], expect[0]) and torch.equal(got[1], expect[1])
     tokens, logprobs = serving.sample_tokens(view[:0], uniforms[:0])
     assert tokens.shape == (0,) and logprobs.shape == (0,)
+
+
+# ---- arguments that are refused -----------------------------------------------------------------------
+
+
+def test_matvec_refusals():
+    from ue5m3_fp4 import serving
+
+    codes, scales = (t.cuda() for t in packed_weight(8, 64, 16, False, 0))
+    good = dict(rows=8, cols=64, block_size=16, two_dimensional=False, tensor_amax=1.0)
+    x = torch.randn(2, 64, device="cuda")
+    serving.packed_matvec(x, codes, scales, **good)
+    for bad in (dict(block_size=8), dict(rows=9), dict(cols=62), dict(two_dimensional=True), dict(tensor_amax=math.nan),
+                dict(tensor_amax=-1.0), dict(scale_target=0.0), dict(bias=torch.zeros(7, device="cuda")), dict(bias=torch.zeros(8))):
+        with pytest.raises(ValueError):
+            serving.packed_matvec(x, codes, scales, **{**good, **bad})
+    with pytest.raises(TypeError):
+        serving.packed_matvec(x.half(), codes, scales, **good)
+    with pytest.raises(TypeError):
+        serving.packed_matvec(x, codes, scales, out_dtype=torch.float16, **good)
+    with pytest.raises(ValueError, match="contiguous"):
+        serving.packed_matvec(torch.randn(64, 2, device="cuda").T, codes, scales, **good)
+    with pytest.raises(ValueError, match="overlap"):
+        serving.packed_matvec(x[:1].expand(2, 64), codes, scales, **good)
+    with pytest.raises(ValueError):
+        serving.packed_matvec(x, codes.cpu(), scales, **good)
+    with pytest.raises(RuntimeError, match="no gradients"):
+        serving.packed_matvec(x.clone().requires_grad_(True), codes, scales, **good)
+
+
+def test_attention_refusals():
+    from ue5m3_fp4 import serving
+
+    k, v, table = build_cache([20], 16, 2, 64, 0)
+    q = torch.randn(1, 4, 64, device="cuda").to(torch.bfloat16)
+    kv, starts = torch.tensor([20]).int().cuda(), torch.tensor([0, 1]).int().cuda()
+
+    def call(q=q, k=k, v=v, table=table, kv=kv, starts=starts, max_query_length=1, **kw):
+        return serving.paged_attention(q, k, v, table, kv, starts, max_query_length=max_query_length, **kw)
+
+    call()
+    new = torch.randn(1, 2, 64, device="cuda").to(torch.bfloat16)
+    for bad in (dict(q=q.float()), dict(k=k.float()), dict(q=q[:, :3]), dict(q=q[0]), dict(table=table.long()), dict(kv=kv.long()),
+                dict(starts=starts[:1]), dict(max_query_length=0), dict(max_kv_length=0), dict(scale=0.0), dict(scale=math.nan),
+                dict(new_k=new), dict(new_k=new, new_v=new[:, :1]), dict(new_k=new.float(), new_v=new), dict(out=q[:, :2]),
+                dict(out=q.float()), dict(k=k[:, :12], v=v[:, :12]), dict(v=v[:-1]), dict(q=q.cpu().cuda()[..., :32]),
+                dict(table=table.cpu()), dict(q=torch.zeros(1, 4, 66, device="cuda").to(torch.bfloat16)[..., :64])):
+        with pytest.raises(ValueError):
+            call(**bad)
+    with pytest.raises(RuntimeError, match="no gradients"):
+        call(q=q.clone().requires_grad_(True))
+    assert call(q=q[:0], starts=torch.zeros(2).int().cuda()).shape == (0, 4, 64)
+
+
+def test_sample_refusals():
+    from ue5m3_fp4 import serving
+
+    logits, u = torch.randn(2, 50, device="cuda"), torch.rand(2, device="cuda")
+    for bad in (dict(temperature=-1.0), dict(temperature=math.nan), dict(top_k=-1), dict(top_p=0.0), dict(top_p=1.5),
+                dict(min_p=-0.1), dict(min_p=2.0), dict(top_k=torch.ones(2, device="cuda")), dict(top_p=torch.ones(3, device="cuda")),
+                dict(min_p=torch.ones(2))):
+        with pytest.raises(ValueError):
+            serving.sample_tokens(logits, u, **bad)
+    for args in ((logits[0], u), (logits, u[:1]), (logits, u.double()), (logits.T, torch.rand(50, device="cuda")),
+                 (logits[:1].expand(2, 50), u), (torch.empty(2, 0, device="cuda"), u)):
+        with pytest.raises(ValueError):
+            serving.sample_tokens(*args)
+    with pytest.raises(TypeError):
+        serving.sample_tokens(logits.half(), u)
+
+
+# ---- the operators together ------------------------------------------------------------------------------
+
+
+def small_stack(seed=0, **over):
+    from ue5m3_fp4.integrations.torchtitan.shaped_stack import NemotronHShapedStack, ShapedConfig
+
+    torch.manual_seed(seed)
+    config = ShapedConfig(**{**dict(hidden_size=256, intermediate_size=512, mamba_inner=256, mamba_extra=64, attention_heads=8,
+                                    kv_heads=2, head_dim=64, vocab_size=1000, num_hidden_layers=6,
+                                    hybrid_override_pattern="M-*-M*"), **over})
+    model = NemotronHShapedStack(config, device="cuda").eval()
+    with torch.no_grad():
+        for p in model.parameters():
+            if p.ndim == 2:
+                p.mul_(3.0)
+    return model
+
+
+def test_stack_served_in_steps_equals_its_forward_pass():
+    """Prompts of different lengths in chunks and single tokens against whole forward passes: the same
+    sums in other orders, rounded to bf16 after every layer."""
+
+    model = small_stack()
+    g = torch.Generator().manual_seed(1)
+    ids = [torch.randint(0, 1000, (n,), generator=g).cuda() for n in (57, 20, 91)]
+    cache = model.make_cache(sequences=3, max_length=128, page_size=16)
+    at = [0, 0, 0]
+    seen = [None] * 3
+    for counts in ([40, 1, 0], [1, 1, 33], [1, 16, 50], [15, 2, 8]):
+        cache.begin_step(counts)
+        logits = model.serve(torch.cat([ids[b][at[b]:at[b] + n] for b, n in enumerate(counts)]), cache)
+        for b, n in enumerate(counts):
+            at[b] += n
+            if n:
+                seen[b] = logits[b]
+    for b in range(3):
+        assert at[b] == ids[b].numel()
+        with torch.no_grad():
+            expect = model(ids[b][None])[0, -1].double()
+        # six layers, each with a handful of bf16 roundings of 2^-8 that add up like independent errors
+        assert float((seen[b].double() - expect).norm() / expect.norm()) < 6 * 4 ** 0.5 * 2.0 ** -8
+
+
+def test_frozen_stack_generates_with_packed_linears():
+    """Post-load lifecycle -> packed linears -> token loop: the linears' outputs are those of the frozen
+    weights, and the loop's tokens those that its own logits and numbers imply."""
+
+    from ue5m3_fp4 import FP4InferenceScalingController
+    from ue5m3_fp4 import serving
+    from ue5m3_fp4.nn import PackedFP4Linear, UE5M3Linear, convert_linear_modules, exclude_lm_head, pack_frozen_linears
+
+    model = small_stack(seed=3)
+    convert_linear_modules(model, selector=exclude_lm_head)
+    model.eval()
+    controller = FP4InferenceScalingController(model, activation_mode="current_tensor", checkpoint_identity={"name": "none"})
+    controller.reset_after_checkpoint_load()
+    controller.calibrate_and_freeze_weights()
+    layer = model.layers[1].mixer.up_proj
+    x = torch.randn(3, 256, device="cuda").to(torch.bfloat16)
+    packed = layer.packed_weight()
+    expect = x.double() @ packed.dequantize().double().T
+    records = pack_frozen_linears(model)
+    assert len(records) == 2 * 2 + 2 * 2 + 2 * 4 and not any(isinstance(m, UE5M3Linear) for m in model.modules())
+    got = model.layers[1].mixer.up_proj(x)
+    assert isinstance(model.layers[1].mixer.up_proj, PackedFP4Linear)
+    assert bool(((got.double() - expect).abs() <= 2.0 ** -8 * expect.abs() + 1e-4).all())
+    prompts = [torch.arange(5, device="cuda"), torch.arange(30, 75, device="cuda")]
+    uniforms = torch.rand(6, 2, device="cuda")
+    settings = dict(temperature=0.8, top_k=20, top_p=0.9)
+    tokens = model.generate(prompts, 6, uniforms=uniforms, **settings)
+    assert tokens.shape == (2, 6) and bool(((tokens >= 0) & (tokens < 1000)).all())
+    # the same loop, step by step, with the sampling checked against the definition
+    cache = model.make_cache(sequences=2, max_length=51)
+    counts, ids = [5, 45], torch.cat(prompts)
+    for step in range(6):
+        cache.begin_step(counts)
+        logits = model.serve(ids, cache)
+        ids, _ = check_sample(logits, uniforms[step].cpu(), **settings)
+        assert torch.equal(ids, tokens[:, step])
+        counts = [1, 1]
+
+
+def test_captured_step_replays_with_new_lengths_and_beside_another_graph():
+    """A decode step captured once is replayed as the sequences grow; two graphs alive at a time share
+    no workspace."""
+
+    model = small_stack(seed=5)
+    prompts = [torch.arange(3, device="cuda"), torch.arange(100, 180, device="cuda")]
+    uniforms = torch.rand(8, 2, device="cuda")
+    expect = model.generate(prompts, 8, uniforms=uniforms, top_p=0.9)
+
+    from ue5m3_fp4 import serving
+
+    def capture(cache, ids, u):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):  # warm-up: libraries load and allocate outside the capture
+            serving.sample_tokens(model.serve(ids, cache), u, top_p=0.9)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            tokens, logprobs = serving.sample_tokens(model.serve(ids, cache), u, top_p=0.9)
+        return graph, tokens
+
+    runs = []
+    for _ in range(2):
+        cache = model.make_cache(sequences=2, max_length=128, page_size=16)
+        cache.begin_step([3, 80])
+        first, _ = serving.sample_tokens(model.serve(torch.cat(prompts), cache), uniforms[0], top_p=0.9)
+        ids, u = first.clone(), uniforms[1].clone()
+        cache.begin_step([1, 1])
+        cache.max_kv_length = 128  # the graph's launches are sized for the longest
+        graph, tokens = capture(cache, ids, u)
+        runs.append((cache, ids, u, graph, tokens, [first]))
+    for step in range(1, 8):
+        for cache, ids, u, graph, tokens, out in runs:
+            if step > 1:
+                cache.begin_step([1, 1])
+            ids.copy_(out[-1])
+            u.copy_(uniforms[step])
+        for cache, ids, u, graph, tokens, out in runs:
+            graph.replay()
+        for cache, ids, u, graph, tokens, out in runs:
+            out.append(tokens.clone())
+    for *_, out in runs:
+        assert torch.equal(torch.stack(out, 1), expect)
+
+
+def test_operators_on_another_stream():
+    from ue5m3_fp4 import serving
+
+    codes, scales = (t.cuda() for t in packed_weight(512, 1024, 16, True, 0))
+    x = torch.randn(4, 1024, device="cuda").to(torch.bfloat16)
+    logits, u = torch.randn(4, 30000, device="cuda"), torch.rand(4, device="cuda")
+    kw = dict(rows=512, cols=1024, block_size=16, two_dimensional=True, tensor_amax=1.0)
+    expect = serving.packed_matvec(x, codes, scales, **kw), serving.sample_tokens(logits, u, top_p=0.9)[0]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    results = []
+    for _ in range(5):
+        for stream in streams:
+            with torch.cuda.stream(stream):
+                results.append((serving.packed_matvec(x, codes, scales, **kw), serving.sample_tokens(logits, u, top_p=0.9)[0]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, expect[0]) and torch.equal(b, expect[1]) for a, b in results)

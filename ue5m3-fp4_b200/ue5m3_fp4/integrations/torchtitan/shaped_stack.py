@@ -14,7 +14,8 @@ and causal-conv kernels of Mamba2 are separate libraries that are not part of th
 The Mamba2 stand-in gates the two 8192-wide streams of ``in_proj`` (silu(z) * x) and adds the
 B, C and dt columns onto the first 2176 channels, so that every output column of ``in_proj``
 receives a gradient of the same order of magnitude; attention is torch's scaled-dot-product attention (causal, 32 query heads over 4
-key/value heads of width 128, the reported k/v width 512); the MLP is up_proj ->
+key/value heads of width 128, the reported k/v width 512), or, when the stack answers token by
+token (``serve``, ``generate``), this package's attention over a paged cache; the MLP is up_proj ->
 squared ReLU -> down_proj as in the model.  Outputs of this stack mean nothing; its cost profile
 (FLOPs in the 112 linears, bytes of weights and gradients, number of amax samples) is the
 model's.
@@ -30,6 +31,7 @@ from torch.nn import functional as F
 
 from ue5m3_fp4.integrations.torchtitan.selection import (REPORTED_NEMOTRON_H_8B_PATTERN,
                                                           REPORTED_NEMOTRON_H_LAYER_COUNT)
+from ue5m3_fp4.serving import PagedKVCache, sample_tokens
 
 
 @dataclass(frozen=True)
@@ -93,6 +95,14 @@ class _Attention(nn.Module):
         out = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=True)
         return self.o_proj(out.transpose(1, 2).reshape(batch, seq, self.heads * self.head_dim))
 
+    def serve(self, x: torch.Tensor, cache: PagedKVCache, layer: int) -> torch.Tensor:
+        """The step's tokens [tokens, hidden] of all sequences over what the cache holds of them."""
+
+        q = self.q_proj(x).view(-1, self.heads, self.head_dim)
+        k = self.k_proj(x).view(-1, self.kv_heads, self.head_dim)
+        v = self.v_proj(x).view(-1, self.kv_heads, self.head_dim)
+        return self.o_proj(cache.attend(layer, q, k, v).view(-1, self.heads * self.head_dim))
+
 
 class _MLP(nn.Module):
     def __init__(self, c: ShapedConfig, device=None, dtype=None) -> None:
@@ -140,6 +150,58 @@ class NemotronHShapedStack(nn.Module):
         for layer in self.layers:
             x = layer(x)
         return self.lm_head(self.norm_f(x))
+
+    def make_cache(self, *, sequences: int, max_length: int, page_size: int = 64, pages: int | None = None) -> PagedKVCache:
+        """A cache for this stack's attention layers (default: pages for every sequence at full length)."""
+
+        c = self.config
+        if pages is None:
+            pages = sequences * ((max_length + page_size - 1) // page_size)
+        return PagedKVCache(layers=c.hybrid_override_pattern.count("*"), pages=pages, page_size=page_size,
+                            kv_heads=c.kv_heads, head_dim=c.head_dim, sequences=sequences, max_length=max_length,
+                            device=self.embed_tokens.weight.device)
+
+    @torch.no_grad()
+    def serve(self, input_ids: torch.Tensor, cache: PagedKVCache) -> torch.Tensor:
+        """One step behind ``cache.begin_step``: the new tokens of all sequences, one behind the other, to
+        the logits [sequences, vocabulary] of each sequence's last one (those of a sequence without new
+        tokens mean nothing).  The linears may be float, ``UE5M3Linear`` in inference or
+        ``PackedFP4Linear``; may be captured into a CUDA graph and replayed after the next begin_step
+        with the same counts."""
+
+        x = self.embed_tokens(input_ids)
+        attention = 0
+        for layer in self.layers:
+            if isinstance(layer.mixer, _Attention):
+                x = x + layer.mixer.serve(layer.norm(x), cache, attention)
+                attention += 1
+            else:
+                x = layer(x)
+        return self.lm_head(self.norm_f(x.index_select(0, cache.last_rows)))
+
+    @torch.no_grad()
+    def generate(self, prompts: list[torch.Tensor], steps: int, *, uniforms: torch.Tensor, cache: PagedKVCache | None = None,
+                 **sampling) -> torch.Tensor:
+        """``steps`` further tokens [prompts, steps] of every prompt (1-d id tensors) from the given uniform
+        numbers [steps, prompts]; ``sampling``: temperature, top_k, top_p and min_p of
+        :func:`ue5m3_fp4.serving.sample_tokens`, -1 where a row of logits has a NaN.  The host never waits
+        for the device."""
+
+        if not prompts or steps <= 0 or any(prompt.ndim != 1 or prompt.numel() == 0 for prompt in prompts):
+            raise ValueError("generate needs 1-d prompts with at least one token and a positive number of steps")
+        if tuple(uniforms.shape) != (steps, len(prompts)):
+            raise ValueError("uniforms must be [steps, prompts]")
+        counts = [prompt.numel() for prompt in prompts]
+        if cache is None:
+            cache = self.make_cache(sequences=len(prompts), max_length=max(counts) + steps)
+        ids, tokens = torch.cat(prompts), []
+        for step in range(steps):
+            cache.begin_step(counts)
+            drawn, _ = sample_tokens(self.serve(ids, cache), uniforms[step], **sampling)
+            tokens.append(drawn)
+            ids = drawn.clamp(min=0)  # -1, from logits that are not numbers, is no index
+            counts = [1] * len(prompts)
+        return torch.stack(tokens, dim=1)
 
     def fp4_linear_flops_per_token(self) -> int:
         """Forward + backward multiply-add FLOPs of the 112 internal linears per token (6 per weight)."""

@@ -573,15 +573,20 @@ class UE5M3Linear(torch.nn.Module):
         weight, at 0.5625 byte per element.  Requires the post-load lifecycle to have frozen the
         weight scale."""
 
+        self.packed_weight().save(path)
+
+    def packed_weight(self):
+        """This layer's weight, quantized with its FROZEN amax, as a ``PackedFP4Tensor``."""
+
         from ue5m3_fp4.packed import PackedFP4Tensor
 
         frozen = self._inference["frozen_weights"].get("forward.w") if self._inference["active"] else None
         if frozen is None:
             raise RuntimeError("Weight amax has not been frozen after checkpoint load")
-        PackedFP4Tensor.quantize(
+        return PackedFP4Tensor.quantize(
             self.weight.detach(), block_size=self.recipe.block_size, two_dimensional=self.recipe.two_dimensional_weights,
             tensor_amax=float(frozen), scale_target=self.recipe.scale_target_for("weight", self.module_name),
-            name=self.module_name).save(path)
+            name=self.module_name)
 
     def load_packed_weight(self, path) -> None:
         """Install a packed weight written by ``export_packed_weight`` as this layer's forward
