@@ -35,7 +35,11 @@ constexpr int kWarps = 16;
 constexpr int kThreads = kWarps * 32;
 constexpr int kChunk = 128;          // reduction elements of one warp step: 64 bytes of a row's codes
 constexpr int kPartialFloats = 23552;  // 92 KiB of partial sums per CTA
-constexpr int kRing = 4;             // tiles of codes in shared memory, 32 KiB each at two chunks per warp
+constexpr int kRing = 3;             // tiles of codes and scales in shared memory, 36 KiB each at two chunks per warp
+
+// 16-byte pieces of a ring slot: the codes of 16 rows and `depth` chunks per warp, and their scales
+// (16 rows x 8 bytes, half of it used for blocks of 32)
+__host__ __device__ constexpr int slot_pieces(int depth) { return depth * 2 * kThreads + kWarps * depth * 8; }
 
 struct Params {
     const void* x;
@@ -208,10 +212,13 @@ __device__ __forceinline__ Piece load_piece(const uint8_t* __restrict__ codes, c
     return piece;
 }
 
-__device__ __forceinline__ void copy_async(uint4* to, const uint8_t* from) {
-    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)),
-                 "l"(from)
-                 : "memory");
+template <int kBytes>
+__device__ __forceinline__ void copy_async(void* to, const uint8_t* from) {
+    const uint32_t address = (uint32_t)__cvta_generic_to_shared(to);
+    if constexpr (kBytes == 16)
+        asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(address), "l"(from) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(address), "l"(from), "n"(kBytes) : "memory");
 }
 
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
@@ -222,8 +229,9 @@ __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
 // keeps in registers.
 template <bool kFp32, int kTiles, int kDepth, bool kVector, int kBlock>
 __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params p) {
-    extern __shared__ uint4 ring[];  // kVector: [slot][chunk][row half][thread]
-    float* partial = reinterpret_cast<float*>(ring + (kVector ? kRing * kDepth * 2 * kThreads : 0));  // [warp][column][row]
+    extern __shared__ uint4 ring[];  // kVector: [slot]{codes [chunk][row half][thread], scales [warp][chunk][row]}
+    constexpr int kSlot = slot_pieces(kDepth);
+    float* partial = reinterpret_cast<float*>(ring + (kVector ? kRing * kSlot : 0));  // [warp][column][row of the block]
     constexpr int kParts = kFp32 ? 3 : 1;
     constexpr int kColumns = kTiles * 8;
     constexpr int kBlockShift = kBlock == 16 ? 4 : 5;
@@ -247,79 +255,69 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
             const uint8_t* scales = p.scales + scale_row0 * p.scale_stride;
             // rows from which 3 bytes back and 19 bytes further on are still inside the weight
             const bool inner = row0 * p.code_stride >= 3 && (int64_t)(p.rows - row0 - row_count) * p.code_stride >= 20;
-            // Pieces of the tiles to come.  Wide rows: the codes wait in this lane's own slots of a ring
-            // in shared memory (asynchronous copies), kRing - 1 tiles ahead, the scales in registers, two
-            // tiles ahead.  Other rows: in registers, one tile ahead.
+            // Pieces of the tiles to come.  Wide rows: codes and scales wait in a ring in shared memory,
+            // kRing - 1 tiles ahead: the codes in the slots of the lane that decodes them, the scale bytes
+            // of a row's chunk side by side.  A row or chunk behind the end is not copied: what its slot
+            // holds is finite, and meets zeros or is not stored.  Other rows: in registers, one tile ahead.
             Piece next[kDepth][2];
-            uint32_t later[kDepth][2];
-            uint32_t code[2], scale[2], byte[kDepth], block[kDepth];
-            auto locate = [&](int pass, int tile) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int row = min(tile + g + 8 * h, row_count - 1);
-                    code[h] = row * stride;
-                    scale[h] = ((row0 + row >> p.row_shift) - scale_row0) * scale_stride;
-                }
+            auto load = [&](int pass, int tile) {
 #pragma unroll
                 for (int d = 0; d < kDepth; ++d) {
                     // a chunk behind the end is read as the row's last bytes
-                    byte[d] = min(((pass * kDepth + d) * kWarps + warp) * (kChunk / 2) + 16 * c, stride - (kVector ? 16 : 1));
-                    block[d] = byte[d] * 2 >> kBlockShift;
-                }
-            };
-            auto copy_codes = [&](int slot) {
-#pragma unroll
-                for (int d = 0; d < kDepth; ++d)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        copy_async(ring + ((slot * kDepth + d) * 2 + h) * kThreads + threadIdx.x, codes + (code[h] + byte[d]));
-            };
-            auto load_scales = [&](uint32_t(&to)[kDepth][2]) {
-#pragma unroll
-                for (int d = 0; d < kDepth; ++d)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        to[d][h] = kBlock == 16 ? (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(scales + (scale[h] + block[d])))
-                                                : (uint32_t)__ldg(scales + (scale[h] + block[d]));
-            };
-            auto load = [&](int pass, int tile) {
-                locate(pass, tile);
-#pragma unroll
-                for (int d = 0; d < kDepth; ++d)
+                    const int byte = min(((pass * kDepth + d) * kWarps + warp) * (kChunk / 2) + 16 * c, stride - 1);
+                    const int block = byte * 2 >> kBlockShift;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const uint32_t last = scale[h] + scale_stride - 1;
+                        const int row = min(tile + g + 8 * h, row_count - 1);
+                        const uint32_t code = row * stride + byte;
+                        const uint32_t scale = ((row0 + row >> p.row_shift) - scale_row0) * scale_stride;
+                        const uint32_t last = scale + scale_stride - 1;
                         if (inner)
-                            next[d][h] = load_piece<Loads::kWords, kBlock>(codes, scales, code[h] + byte[d], scale[h] + block[d],
-                                                                           last, 0);
+                            next[d][h] = load_piece<Loads::kWords, kBlock>(codes, scales, code, scale + block, last, 0);
                         else
-                            next[d][h] = load_piece<Loads::kBytes, kBlock>(codes, scales, code[h] + byte[d], scale[h] + block[d],
-                                                                           last, stride - byte[d]);
+                            next[d][h] = load_piece<Loads::kBytes, kBlock>(codes, scales, code, scale + block, last, stride - byte);
                     }
+                }
             };
-            // the (pass, tile) that is copied next
+            // the (pass, tile) that is copied next, and where this lane's first row of it lies
             int ahead_pass = 0, ahead_tile = 0;
+            const uint8_t *ahead_codes = nullptr, *ahead_scales = nullptr;
+            auto locate = [&]() {
+                const int chunk = ahead_pass * kDepth * kWarps + warp;
+                ahead_codes = codes + (int64_t)(ahead_tile + g) * stride + chunk * (kChunk / 2) + 16 * c;
+                ahead_scales = scales + chunk * (kChunk / kBlock);
+            };
             auto copy_ahead = [&](int slot) {
                 if (ahead_pass < passes) {
-                    locate(ahead_pass, ahead_tile);
-                    copy_codes(slot);
+                    uint4* to = ring + slot * kSlot + threadIdx.x;
+                    uint8_t* scales_to = reinterpret_cast<uint8_t*>(ring + slot * kSlot + kDepth * 2 * kThreads) + warp * kDepth * 128;
+                    const int row = ahead_tile + g + 8 * c;  // lanes 0 and 1 of a row bring the scales of it and the one 8 on
+                    const int scale_row = (row0 + row >> p.row_shift) - scale_row0;
+#pragma unroll
+                    for (int d = 0; d < kDepth; ++d) {
+                        if ((ahead_pass * kDepth + d) * kWarps + warp >= chunks) continue;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            if (ahead_tile + g + 8 * h < row_count)
+                                copy_async<16>(to + (d * 2 + h) * kThreads, ahead_codes + h * 8 * stride + d * kWarps * (kChunk / 2));
+                        if (c < 2 && row < row_count)
+                            copy_async<kChunk / kBlock>(scales_to + d * 128 + (g + 8 * c) * (kChunk / kBlock),
+                                                        ahead_scales + scale_row * scale_stride + d * kWarps * (kChunk / kBlock));
+                    }
                     ahead_tile += 16;
-                    if (ahead_tile >= row_count) ahead_tile = 0, ++ahead_pass;
+                    ahead_codes += 16 * stride;
+                    if (ahead_tile >= row_count) {
+                        ahead_tile = 0, ++ahead_pass;
+                        locate();
+                    }
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
             };
             int slot_now = 0;
-            uint32_t scales_now[kDepth][2];
             if constexpr (kVector) {
+                locate();
 #pragma unroll
                 for (int i = 0; i < kRing - 1; ++i) copy_ahead(i);
-                locate(0, 0);
-                load_scales(scales_now);
-                if (row_count > 16)
-                    locate(0, 16);
-                else
-                    locate(min(1, passes - 1), 0);
-                load_scales(later);
             } else {
                 load(0, 0);
             }
@@ -341,22 +339,22 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
                 for (int tile = 0; tile < row_count; tile += 16, slot += 16) {
                     Piece now[kDepth][2];
                     if constexpr (kVector) {
-                        copy_ahead((slot_now + kRing - 1) % kRing);
+                        __syncwarp();  // the slot that is filled now has been read
+                        copy_ahead(slot_now == 0 ? kRing - 1 : slot_now - 1);
                         asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
+                        __syncwarp();  // scales come from other lanes
+                        const uint4* from = ring + slot_now * kSlot + threadIdx.x;
+                        const uint8_t* scales_from =
+                            reinterpret_cast<const uint8_t*>(ring + slot_now * kSlot + kDepth * 2 * kThreads) + warp * kDepth * 128;
 #pragma unroll
                         for (int d = 0; d < kDepth; ++d)
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
-                                now[d][h].codes = ring[((slot_now * kDepth + d) * 2 + h) * kThreads + threadIdx.x];
-                                now[d][h].scales = scales_now[d][h];
-                                scales_now[d][h] = later[d][h];
+                                now[d][h].codes = from[(d * 2 + h) * kThreads];
+                                const uint8_t* at = scales_from + d * 128 + (g + 8 * h) * (kChunk / kBlock) + c * (32 / kBlock);
+                                now[d][h].scales = kBlock == 16 ? *reinterpret_cast<const uint16_t*>(at) : *at;
                             }
-                        slot_now = (slot_now + 1) % kRing;
-                        // two tiles on
-                        int tile2 = tile + 32, pass2 = pass;
-                        while (tile2 >= row_count && pass2 + 1 < passes) tile2 = max(tile2 - (row_count + 15) / 16 * 16, 0), ++pass2;
-                        locate(pass2, tile2);
-                        load_scales(later);
+                        slot_now = slot_now == kRing - 1 ? 0 : slot_now + 1;
                     } else {
 #pragma unroll
                         for (int d = 0; d < kDepth; ++d) now[d][0] = next[d][0], now[d][1] = next[d][1];
@@ -449,7 +447,7 @@ int launch(Params p, cudaStream_t stream) {
     const int need = (own + 15) / 16 * 16;
     if (block > need) block = need;
     p.rows_per_block = block;
-    constexpr size_t kRingBytes = kVector ? kRing * kDepth * 2 * kThreads * sizeof(uint4) : 0;
+    constexpr size_t kRingBytes = kVector ? kRing * slot_pieces(kDepth) * sizeof(uint4) : 0;
     const size_t bytes = kRingBytes + (size_t)kWarps * used * block * sizeof(float);
     const cudaError_t error = allow_shared<packed_matvec_kernel<kFp32, kTiles, kDepth, kVector, kBlock>>(
         (int)kRingBytes + kPartialFloats * 4);
@@ -506,8 +504,8 @@ extern "C" int ue5m3_packed_matvec(const void* x, int x_dtype, int64_t tokens, i
     p.rows = (int)rows;
     p.k = (int)cols;
     p.row_shift = !two_d ? 0 : block == 16 ? 4 : 5;
-    const bool vector = p.code_stride % 16 == 0 && (uintptr_t)codes % 16 == 0 &&
-               (block == 32 || (p.scale_stride % 2 == 0 && (uintptr_t)scales % 2 == 0));
+    // whole chunks of codes and scales, copied asynchronously
+    const bool vector = cols % matvec::kChunk == 0 && (uintptr_t)codes % 16 == 0 && (uintptr_t)scales % 8 == 0;
     p.vector_x = (uintptr_t)x % 16 == 0 && (ldx * element) % 16 == 0;
     p.bias_fp32 = bias_dtype == UE5M3_DTYPE_FP32;
     p.out_fp32 = out_dtype == UE5M3_DTYPE_FP32;
