@@ -111,16 +111,14 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
     unsigned long long* empty = full + kStages;
     int* abort_flag = reinterpret_cast<int*>(empty + kStages);
     int* bad = abort_flag + 1;
-    float* merge = reinterpret_cast<float*>(tiles);  // after the last stage: [warp][16 rows][kDim + 2]
+    constexpr int kMergeRow = kDim + 4;  // a row's channels, its maximum and sum, on a 16-byte boundary
+    float* merge = reinterpret_cast<float*>(tiles);  // after the last stage: [warp][16 rows][kMergeRow]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int b = blockIdx.z;
     const int row_tiles = gridDim.y / p.kv_heads;
     const int head = blockIdx.y / row_tiles;
     const Sequence s = sequence_of(p, b);
-    if (p.zero_tail)
-        zero_tail_rows(p, ((int64_t)(blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * kSmallThreads + threadIdx.x,
-                       (int64_t)gridDim.x * gridDim.y * gridDim.z * kSmallThreads, kDim);
     const int rows = s.queries * p.group;
     launch_dependents();
     if (threadIdx.x == 0) {
@@ -282,12 +280,10 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
             for (int h = 0; h < 2; ++h) {
                 sum[h] += __shfl_xor_sync(0xFFFFFFFFu, sum[h], 1);
                 sum[h] += __shfl_xor_sync(0xFFFFFFFFu, sum[h], 2);
-                float* to = merge + (warp * kRows + g + 8 * h) * (kDim + 2);
+                float* to = merge + (warp * kRows + g + 8 * h) * kMergeRow;
 #pragma unroll
-                for (int i = 0; i < kDim / 8; ++i) {
-                    to[i * 8 + 2 * c] = o[i][2 * h];
-                    to[i * 8 + 2 * c + 1] = o[i][2 * h + 1];
-                }
+                for (int i = 0; i < kDim / 8; ++i)
+                    *reinterpret_cast<float2*>(to + i * 8 + 2 * c) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
                 if (c == 0) {
                     to[kDim] = top[h];
                     to[kDim + 1] = sum[h];
@@ -296,40 +292,51 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
         }
         __syncthreads();
         const bool failed = *((volatile int*)abort_flag) || *((volatile int*)bad);
-        for (int i = threadIdx.x; i < kRows * kDim; i += kSmallThreads) {
-            const int r = i / kDim, d = i % kDim;
+        for (int i = threadIdx.x; i < kRows * (kDim / 4); i += kSmallThreads) {
+            const int r = i / (kDim / 4), d = i % (kDim / 4) * 4;
             if (row0 + r >= rows) continue;
-            float most = -INFINITY, value = 0.0f, total = 0.0f;
+            float most = -INFINITY, total = 0.0f;
+            float4 value = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (failed) {
                 most = 0.0f;
-                value = total = __uint_as_float(0x7FC00000u);
+                value.x = value.y = value.z = value.w = total = __uint_as_float(0x7FC00000u);
             } else {
+                const float* from = merge + r * kMergeRow;
 #pragma unroll
-                for (int w = 0; w < kConsumers; ++w) most = fmaxf(most, merge[(w * kRows + r) * (kDim + 2) + kDim]);
+                for (int w = 0; w < kConsumers; ++w) most = fmaxf(most, from[w * kRows * kMergeRow + kDim]);
                 const float base = most == -INFINITY ? 0.0f : most;
 #pragma unroll
                 for (int w = 0; w < kConsumers; ++w) {
-                    const float* from = merge + (w * kRows + r) * (kDim + 2);
-                    const float weight = exp2_approx(from[kDim] - base);
-                    value = __fmaf_rn(from[d], weight, value);
-                    total = __fmaf_rn(from[kDim + 1], weight, total);
+                    const float4 v = *reinterpret_cast<const float4*>(from + w * kRows * kMergeRow + d);
+                    const float weight = exp2_approx(from[w * kRows * kMergeRow + kDim] - base);
+                    total = __fmaf_rn(from[w * kRows * kMergeRow + kDim + 1], weight, total);
+                    value.x = __fmaf_rn(v.x, weight, value.x);
+                    value.y = __fmaf_rn(v.y, weight, value.y);
+                    value.z = __fmaf_rn(v.z, weight, value.z);
+                    value.w = __fmaf_rn(v.w, weight, value.w);
                 }
             }
-            const int64_t row = s.first + (row0 + r) / p.group;
-            const int64_t at = row * p.heads + head * p.group + (row0 + r) % p.group;
+            const int token = (row0 + r) / p.group;
+            const int64_t at = (int64_t)(s.first + token) * p.heads + head * p.group + (row0 + r - token * p.group);
             if (splits <= 1) {
-                p.out[at * kDim + d] = __float2bfloat16_rn(total == 0.0f ? 0.0f : value / total);
+                const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+                *reinterpret_cast<uint2*>(p.out + at * kDim + d) =
+                    make_uint2(pack_bf16(value.x * inverse, value.y * inverse), pack_bf16(value.z * inverse, value.w * inverse));
             } else {
-                p.partial[(at * p.splits + blockIdx.x) * kDim + d] = value;
-                if (d < 2)
-                    p.partial[(int64_t)p.tokens * p.heads * p.splits * kDim + (at * p.splits + blockIdx.x) * 2 + d] =
-                        d == 0 ? most : total;
+                const int64_t slot = at * p.splits + blockIdx.x;
+                *reinterpret_cast<float4*>(p.partial + slot * kDim + d) = value;
+                if (d == 0)
+                    *reinterpret_cast<float2*>(p.partial + (int64_t)p.tokens * p.heads * p.splits * kDim + slot * 2) =
+                        make_float2(most, total);
             }
         }
         // the merge memory is the next row tile's first stages
         asm volatile("fence.proxy.async;" ::: "memory");
         __syncthreads();
     }
+    if (p.zero_tail)
+        zero_tail_rows(p, ((int64_t)(blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * kSmallThreads + threadIdx.x,
+                       (int64_t)gridDim.x * gridDim.y * gridDim.z * kSmallThreads, kDim);
 }
 
 // The rows of a split sequence: sum of the splits' rows, each faded to the largest maximum.  One

@@ -34,14 +34,13 @@ def _no_gradient(*tensors: Tensor | None) -> None:
                                    "detached tensors")
 
 
-def _call(function, name: str, launches: int, device: torch.device, *arguments) -> None:
-    """The library call on ``device``'s current stream, with that device current."""
+def _call(function, name: str, launches: int, index: int, *arguments) -> None:
+    """The library call on the current stream of the device ``index``, with that device current."""
 
-    index = device.index
     if index == torch._C._cuda_getDevice():
         status = function(*arguments, _native.raw_stream(index))
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             status = function(*arguments, _native.raw_stream(index))
     _native.check(status, name, launches)
 
@@ -92,17 +91,17 @@ def packed_matvec(
 
     _require_cuda(x, "x")
     _no_gradient(x, bias)
-    device = x.device
+    index = x.get_device()  # the operands' devices are compared by number: device objects cost host time
     if block_size != 16 and block_size != 32:
         raise ValueError("block_size must be 16 or 32")
     if x.ndim == 0 or x.shape[-1] != cols or cols <= 0:
         raise ValueError(f"x must have {cols} columns, at least one")
     scale_rows = (rows + block_size - 1) // block_size if two_dimensional else rows
     if (codes.dtype is not torch.uint8 or codes.shape != (rows, (cols + 1) // 2) or not codes.is_contiguous()
-            or codes.device != device):
+            or codes.get_device() != index):
         raise ValueError("codes must be contiguous uint8 [rows, ceil(cols/2)] on the operand's device")
     if (scales.dtype is not torch.uint8 or scales.shape != (scale_rows, (cols + block_size - 1) // block_size)
-            or not scales.is_contiguous() or scales.device != device):
+            or not scales.is_contiguous() or scales.get_device() != index):
         raise ValueError("scales must be contiguous uint8 with one byte per block, on the operand's device")
     x_code = _native.dtype_code(x.dtype)
     if out_dtype is None:
@@ -111,7 +110,7 @@ def packed_matvec(
         out_code = _native.dtype_code(out_dtype)
     bias_code, bias_pointer = 0, None
     if bias is not None:
-        if bias.shape != (rows,) or not bias.is_contiguous() or bias.device != device:
+        if bias.shape != (rows,) or not bias.is_contiguous() or bias.get_device() != index:
             raise ValueError("bias must be contiguous [rows] on the operand's device")
         bias_code, bias_pointer = _native.dtype_code(bias.dtype), bias.data_ptr()
     factor = _checked_factor(float(tensor_amax), float(scale_target))
@@ -124,7 +123,7 @@ def packed_matvec(
             ldx = cols
         if (step != 1 and cols > 1) or ldx < cols:
             raise ValueError("the last axis of x must be contiguous and its rows must not overlap")
-        _call(_native.load().ue5m3_packed_matvec, "ue5m3_packed_matvec", 1, device, flat.data_ptr(), x_code, tokens, ldx,
+        _call(_native.load().ue5m3_packed_matvec, "ue5m3_packed_matvec", 1, index, flat.data_ptr(), x_code, tokens, ldx,
               codes.data_ptr(), scales.data_ptr(), rows, cols, block_size, two_dimensional, factor, bias_pointer,
               bias_code, out.data_ptr(), out_code, rows)
     return out if x.ndim == 2 else out.view(*x.shape[:-1], rows)
@@ -133,6 +132,10 @@ def packed_matvec(
 def _strides(name: str, tensor: Tensor) -> tuple[int, ...]:
     """Strides of all axes but the channels', for the library: that of an axis with one element is immaterial."""
 
+    if tensor.is_contiguous():  # channels are 64 or 128: every stride is a multiple of 8
+        shape = tensor.shape
+        row = shape[-2] * shape[-1]
+        return (row, shape[-1]) if len(shape) == 3 else (shape[1] * row, row, shape[-1])
     strides = tensor.stride()
     if strides[-1] != 1:
         raise ValueError(f"{name} must have contiguous channels")
@@ -187,7 +190,7 @@ def paged_attention(
 
     _require_cuda(q, "q")
     _no_gradient(q, new_k, new_v, k_pages, v_pages)
-    device = q.device
+    index = q.get_device()
     if q.ndim != 3 or k_pages.ndim != 4 or page_table.ndim != 2 or v_pages.shape != k_pages.shape:
         raise ValueError("q must be [tokens, heads, head_dim], the pages [pages, page_size, kv_heads, head_dim], the "
                          "table rank 2")
@@ -195,7 +198,7 @@ def paged_attention(
     pages, page_size, kv_heads, width = k_pages.shape
     if q.dtype is not _BF16 or k_pages.dtype is not _BF16 or v_pages.dtype is not _BF16:
         raise ValueError("q, k_pages and v_pages must be bfloat16")
-    if k_pages.device != device or v_pages.device != device or page_table.device != device:
+    if k_pages.get_device() != index or v_pages.get_device() != index or page_table.get_device() != index:
         raise ValueError("the cache must be on the operand's device")
     if head_dim != width or (head_dim != 64 and head_dim != 128):
         raise ValueError("head_dim must be 64 or 128, and that of the pages")
@@ -207,10 +210,10 @@ def paged_attention(
     table_stride, step = page_table.stride()
     if page_table.dtype is not torch.int32 or (step != 1 and width > 1) or (table_stride < width and sequences > 1):
         raise ValueError("page_table must be int32 with contiguous rows")
-    if (kv_lengths.dtype is not torch.int32 or kv_lengths.shape != (sequences,) or kv_lengths.device != device
+    if (kv_lengths.dtype is not torch.int32 or kv_lengths.shape != (sequences,) or kv_lengths.get_device() != index
             or not kv_lengths.is_contiguous()):
         raise ValueError("kv_lengths must be contiguous int32 [sequences] on the operand's device")
-    if (query_starts.dtype is not torch.int32 or query_starts.shape != (sequences + 1,) or query_starts.device != device
+    if (query_starts.dtype is not torch.int32 or query_starts.shape != (sequences + 1,) or query_starts.get_device() != index
             or not query_starts.is_contiguous()):
         raise ValueError("query_starts must be contiguous int32 [sequences + 1] on the operand's device")
     if max_query_length <= 0 or (max_kv_length is not None and max_kv_length <= 0):
@@ -222,7 +225,7 @@ def paged_attention(
     zero_tail = out is None
     if zero_tail:
         out = q.new_empty((tokens, heads, head_dim))
-    elif out.dtype is not _BF16 or out.shape != q.shape or not out.is_contiguous() or out.device != device:
+    elif out.dtype is not _BF16 or out.shape != q.shape or not out.is_contiguous() or out.get_device() != index:
         raise ValueError("out must be contiguous bfloat16 of q's shape on its device")
     k_pointer = v_pointer = None
     k_strides = v_strides = (0, 0)
@@ -230,7 +233,7 @@ def paged_attention(
         if new_k is None or new_v is None:
             raise ValueError("new_k and new_v come together")
         for name, tensor in (("new_k", new_k), ("new_v", new_v)):
-            if tensor.dtype is not _BF16 or tensor.shape != (tokens, kv_heads, head_dim) or tensor.device != device:
+            if tensor.dtype is not _BF16 or tensor.shape != (tokens, kv_heads, head_dim) or tensor.get_device() != index:
                 raise ValueError(f"{name} must be bfloat16 [tokens, kv_heads, head_dim] on the operand's device")
         k_pointer, v_pointer = new_k.data_ptr(), new_v.data_ptr()
         k_strides, v_strides = _strides("new_k", new_k), _strides("new_v", new_v)
@@ -249,20 +252,20 @@ def paged_attention(
         table_stride if sequences > 1 else width)
     need = _workspace_bytes(tokens, sequences, heads, kv_heads, head_dim, max_query_length, max_kv_length)
     # from the current stream's pool, for this call alone: calls and captured graphs share nothing
-    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    _call(_native.load().ue5m3_paged_attention, "ue5m3_paged_attention", 2 if need else 1, device, q.data_ptr(),
+    workspace = q.new_empty(need // 2) if need else None
+    _call(_native.load().ue5m3_paged_attention, "ue5m3_paged_attention", 2 if need else 1, index, q.data_ptr(),
           *_strides("q", q), tokens, heads, ctypes.byref(cache), kv_lengths.data_ptr(), query_starts.data_ptr(),
           max_query_length, max_kv_length, scale, k_pointer, *k_strides, v_pointer, *v_strides, out.data_ptr(),
-          zero_tail, None if workspace is None else workspace.data_ptr(), need, b200.gemm_status(device).data_ptr())
+          zero_tail, None if workspace is None else workspace.data_ptr(), need, b200.gemm_status(q.device).data_ptr())
     return out
 
 
-def _setting(name: str, value, rows: int, dtype: torch.dtype, device: torch.device):
+def _setting(name: str, value, rows: int, dtype: torch.dtype, index: int):
     """(device pointer or None, value) of a setting given as a number or as one number per row."""
 
     if not isinstance(value, Tensor):
         return None, value
-    if value.dtype is not dtype or value.shape != (rows,) or not value.is_contiguous() or value.device != device:
+    if value.dtype is not dtype or value.shape != (rows,) or not value.is_contiguous() or value.get_device() != index:
         raise ValueError(f"{name} must be a number or a contiguous {dtype} tensor [rows] on the operand's device")
     return value.data_ptr(), 0
 
@@ -291,13 +294,13 @@ def sample_tokens(
 
     _require_cuda(logits, "logits")
     _no_gradient(logits)
-    device = logits.device
+    index = logits.get_device()
     if logits.ndim != 2:
         raise ValueError("logits must be [rows, vocabulary]")
     rows, vocabulary = logits.shape
     code = _native.dtype_code(logits.dtype)
     if (uniforms.dtype is not torch.float32 or uniforms.shape != (rows,) or not uniforms.is_contiguous()
-            or uniforms.device != device):
+            or uniforms.get_device() != index):
         raise ValueError("uniforms must be contiguous float32 [rows] on the operand's device")
     if not 0 < vocabulary <= 1 << 18:
         raise ValueError("the vocabulary must have between 1 and 2^18 tokens")
@@ -306,10 +309,10 @@ def sample_tokens(
         ld = vocabulary
     if (step != 1 and vocabulary > 1) or ld < vocabulary:
         raise ValueError("the rows of logits must be contiguous and must not overlap")
-    heat = _setting("temperature", temperature, rows, torch.float32, device)
-    k = _setting("top_k", top_k, rows, torch.int32, device)
-    p = _setting("top_p", top_p, rows, torch.float32, device)
-    least = _setting("min_p", min_p, rows, torch.float32, device)
+    heat = _setting("temperature", temperature, rows, torch.float32, index)
+    k = _setting("top_k", top_k, rows, torch.int32, index)
+    p = _setting("top_p", top_p, rows, torch.float32, index)
+    least = _setting("min_p", min_p, rows, torch.float32, index)
     if not heat[1] >= 0:
         raise ValueError("temperature must not be negative")
     if not k[1] >= 0:
@@ -323,7 +326,7 @@ def sample_tokens(
     tokens = uniforms.new_empty(rows, dtype=torch.int64)
     logprobs = uniforms.new_empty(rows)
     if rows:
-        _call(_native.load().ue5m3_sample_tokens, "ue5m3_sample_tokens", 1, device, logits.data_ptr(), code, rows,
+        _call(_native.load().ue5m3_sample_tokens, "ue5m3_sample_tokens", 1, index, logits.data_ptr(), code, rows,
               vocabulary, ld, uniforms.data_ptr(), *heat, *k, *p, *least, tokens.data_ptr(), logprobs.data_ptr())
     return tokens, logprobs
 
