@@ -323,6 +323,47 @@ def test_attention_pages_outside_the_cache(lengths, queries):
     assert bool(got[:queries[0]].isnan().all()) and torch.equal(got[queries[0]:], good[queries[0]:])
 
 
+@pytest.mark.parametrize("queries,kv_heads,group,page", [(3, 2, 4, 16), (8, 1, 4, 32), (60, 2, 4, 16), (300, 1, 1, 64), (150, 2, 5, 32)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_values_that_are_not_numbers_stay_with_the_rows_that_see_them(queries, kv_heads, group, page, dim):
+    """NaN and infinities in the keys and values of late tokens of a chunk, and of one that all rows see."""
+
+    from ue5m3_fp4 import serving
+
+    old = 70
+    length = old + queries
+    k_pages, v_pages, table = build_cache([length], page, kv_heads, dim, 1)
+    g = torch.Generator().manual_seed(2)
+    q = torch.randn(queries, kv_heads * group, dim, generator=g).to(torch.bfloat16).cuda()
+    new_k = torch.randn(queries, kv_heads, dim, generator=g).to(torch.bfloat16).cuda()
+    new_v = torch.randn(queries, kv_heads, dim, generator=g).to(torch.bfloat16).cuda()
+    late = [queries - 1, queries // 2]
+    new_v[late[0], 0, 3] = math.nan
+    new_v[late[1], 0, 5] = math.inf
+    new_v[late[1], kv_heads - 1, dim - 1] = -math.inf
+    starts, kv = torch.tensor([0, queries]).int().cuda(), torch.tensor([length]).int().cuda()
+
+    def run():
+        return serving.paged_attention(q, k_pages, v_pages, table, kv, starts, max_query_length=queries, new_k=new_k, new_v=new_v)
+
+    got = run().cpu().double()
+    expect, _ = reference_attention(q, k_pages, v_pages, table, [length], [queries], dim ** -0.5)
+    assert torch.equal(got.isnan(), expect.isnan())
+    assert torch.equal(got.isinf(), expect.isinf()) and torch.equal(got[got.isinf()].sign(), expect[expect.isinf()].sign())
+    finite = expect.isfinite()
+    assert float((got[finite] - expect[finite]).abs().max()) < 0.05
+    # a key that is not a number: the rows that see it, all channels of its heads
+    new_k[late[1], 0, 0] = math.nan
+    got = run().cpu()
+    assert bool(got[late[1]:, :group].isnan().all()) and bool(got[:late[1], :, 0].isfinite().all())
+    # a value that every row sees
+    new_k[late[1], 0, 0] = 0.0
+    at = int(table[0, 0])
+    v_pages[at, 1, 0, 2] = math.nan
+    got = run().cpu()
+    assert bool(got[:, :group, 2].isnan().all()) and bool(got[:late[1], :group, 1].isfinite().all())
+
+
 def test_attention_large_scores_and_scale():
     """Scores of a few hundred (one key takes all), and a scale of its own."""
 

@@ -203,6 +203,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
 #pragma unroll
             for (int i = 0; i < kDim / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
             float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+            const int fewest = visible_keys(p, s, row0, 1);  // keys that every row sees
             for (int tile = first; tile < last; ++tile, ++issue) {
                 const int stage = issue % kStages;
                 if (!warp_wait(&full[stage], (issue / kStages) & 1, abort_flag, p.status, kSiteFull, issue)) break;
@@ -262,14 +263,43 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
                         o[i][2 * h + 1] *= fade;
                     }
                 }
+                // keys that some rows do not see: are their values finite?
+                bool odd = false;
+                if (key0 + 16 > fewest && fewest < limit)
+                    for (int i = lane; i < 16 * kSlabs * 8; i += 32) {
+                        const int key = i / (kSlabs * 8), piece = i % (kSlabs * 8);
+                        odd |= key0 + key >= fewest &&
+                               odd_piece(*reinterpret_cast<const uint4*>(v + (piece / 8) * kKeys * 128 + (warp * 16 + key) * 128 +
+                                                                         ((piece & 7) << 4)));
+                    }
+                if (__any_sync(0xFFFFFFFFu, odd)) {
+                    // seldom: one key after the other, for the rows that see it
+                    for (int key = 0; key < 16; ++key) {
 #pragma unroll
-                for (int i = 0; i < kDim / 16; ++i) {
-                    uint32_t vb[4];
-                    const int key = warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), piece = i * 2 + (lane >> 4);
-                    ldmatrix_x4_trans(vb, ptx::smem_u32(v) + (piece / 8) * kKeys * 128 + key * 128 +
-                                              (((piece & 7) ^ (key & 7)) << 4));
-                    mma_bf16(o[2 * i], pr, vb[0], vb[1]);
-                    mma_bf16(o[2 * i + 1], pr, vb[2], vb[3]);
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t pair = __shfl_sync(0xFFFFFFFFu, pr[h + (key & 8 ? 2 : 0)], (lane & 28) + (key & 7) / 2);
+                            const float weight = __uint_as_float(key & 1 ? pair & 0xFFFF0000u : pair << 16);
+                            if (key0 + key > last_key[h]) continue;
+#pragma unroll
+                            for (int i = 0; i < kDim / 8; ++i) {
+                                const uint32_t word = *reinterpret_cast<const uint32_t*>(
+                                    v + (i / 8) * kKeys * 128 + (warp * 16 + key) * 128 + (((i & 7) ^ (key & 7)) << 4) + 4 * c);
+                                o[i][2 * h] = __fmaf_rn(weight, __uint_as_float(word << 16), o[i][2 * h]);
+                                o[i][2 * h + 1] = __fmaf_rn(weight, __uint_as_float(word & 0xFFFF0000u), o[i][2 * h + 1]);
+                            }
+                        }
+                        __syncwarp();
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kDim / 16; ++i) {
+                        uint32_t vb[4];
+                        const int key = warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), piece = i * 2 + (lane >> 4);
+                        ldmatrix_x4_trans(vb, ptx::smem_u32(v) + (piece / 8) * kKeys * 128 + key * 128 +
+                                                  (((piece & 7) ^ (key & 7)) << 4));
+                        mma_bf16(o[2 * i], pr, vb[0], vb[1]);
+                        mma_bf16(o[2 * i + 1], pr, vb[2], vb[3]);
+                    }
                 }
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(&empty[stage]);
@@ -563,6 +593,10 @@ extern "C" int ue5m3_paged_attention(const void* q, int64_t q_token_stride, int6
     p.table_stride = cache->table_stride;
     p.kv_lengths = kv_lengths;
     p.query_starts = query_starts;
+    p.v_pages = reinterpret_cast<const __nv_bfloat16*>(cache->v_pages);
+    p.v_page = cache->v_page_stride;
+    p.v_slot = cache->v_slot_stride;
+    p.v_head = cache->v_head_stride;
     p.partial = reinterpret_cast<float*>(workspace);
     p.status = status_dev;
     p.sequences = (int)cache->sequences;

@@ -29,6 +29,8 @@ struct Params {
     int64_t table_stride;
     const int* kv_lengths;
     const int* query_starts;
+    const __nv_bfloat16* v_pages;
+    int64_t v_page, v_slot, v_head;
     float* partial;              // [tokens, heads, splits, head_dim], then [tokens, heads, splits, 2]
     int* status;
     int sequences, tokens, heads, kv_heads, group;
@@ -102,6 +104,15 @@ __device__ __forceinline__ void zero_tail_rows(const Params& p, int64_t thread, 
     const int first = min(max(p.query_starts[p.sequences], 0), p.tokens);
     uint4* out = reinterpret_cast<uint4*>(p.out);
     for (int64_t i = first * width + thread; i < p.tokens * width; i += threads) out[i] = make_uint4(0, 0, 0, 0);
+}
+
+// Values that not every row of a tile sees may be infinite or NaN: a product with the others' zeros
+// would spread them.  Whether one of two bf16 in a word is not finite:
+__device__ __forceinline__ bool odd_pair(uint32_t w) {
+    return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
+}
+__device__ __forceinline__ bool odd_piece(const uint4& v) {
+    return odd_pair(v.x) || odd_pair(v.y) || odd_pair(v.z) || odd_pair(v.w);
 }
 
 // Programmatic launches: the next kernel of a call starts while this one ends, and waits for it

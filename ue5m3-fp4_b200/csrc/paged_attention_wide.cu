@@ -40,14 +40,17 @@ struct WideShared {
     static constexpr int kK = 2 * kTileBytes;
     static constexpr int kV = kK + kWideStages * kTileBytes;
     static constexpr int kBarriers = kV + kWideStages * kTileBytes;
-    static constexpr int kBytes = kBarriers + 256 + 1024;
+    static constexpr int kBytes = kBarriers + 2048 + 1024;
 };
 
 struct WideBarriers {
     unsigned long long k_full[kWideStages], k_empty[kWideStages], v_full[kWideStages], v_empty[kWideStages];
     unsigned long long q_ready, s_full[2], p_half[2], p_ready[2], o_done[2], drained;
+    unsigned long long v_there[kWideStages], v_settled[kWideStages];  // per stage: its next use waits for this one's
     uint32_t tmem;
     int abort_flag, bad;
+    int odd_count;             // keys with values that are not finite and that not every row sees
+    int odd_keys[kWideRows];
 };
 
 // Instruction descriptor for kind::f16, D = F32, A = B = BF16; b_rows: B is [k][n] in memory
@@ -137,6 +140,29 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// A row of V in its tile whose key not every row sees: behind the last key it is cleared; otherwise
+// values that are not finite become zero, and the key is noted.
+template <int kDim>
+__device__ void settle_values(unsigned char* v, int key, int key_end, WideBarriers& bar) {
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < kDim / 8; ++i) {
+        uint4* piece = reinterpret_cast<uint4*>(v + (i / 8) * kWideKeys * 128 + (i & 7) * 16);
+        if (key >= key_end) {
+            *piece = make_uint4(0, 0, 0, 0);
+        } else if (odd_piece(*piece)) {
+            odd = true;
+            uint32_t* w = reinterpret_cast<uint32_t*>(piece);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if ((w[e] & 0x7F80u) == 0x7F80u) w[e] &= 0xFFFF0000u;
+                if ((w[e] & 0x7F800000u) == 0x7F800000u) w[e] &= 0xFFFFu;
+            }
+        }
+    }
+    if (odd) bar.odd_keys[atomicAdd(&bar.odd_count, 1) % kWideRows] = key;
+}
+
 // one row tile's work
 struct Job {
     int row0, limit, key_begin, key_end, tiles, splits;
@@ -184,6 +210,8 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             ptx::mbar_init(&bar.k_empty[i], 1);
             ptx::mbar_init(&bar.v_full[i], 1);
             ptx::mbar_init(&bar.v_empty[i], 1);
+            ptx::mbar_init(&bar.v_there[i], 1);
+            ptx::mbar_init(&bar.v_settled[i], 2);
         }
         ptx::mbar_init(&bar.q_ready, 256);
         ptx::mbar_init(&bar.drained, 1);
@@ -193,6 +221,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
             ptx::mbar_init(&bar.p_ready[i], 4);
             ptx::mbar_init(&bar.o_done[i], 1);
         }
+        bar.odd_count = 0;
         bar.abort_flag = p.status && *((volatile int*)p.status) != 0;  // a recorded failure: no work, NaN
         ptx::mbar_fence_init();
     }
@@ -207,6 +236,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     constexpr uint32_t kS = 0, kO = 256;  // columns: S of tile t at 128 t, O at 256 + kDim t
     int stage_count = 0;   // key stages used so far (every role counts alike); also the per-tile barriers' phases
     int list = 0;          // row tiles done so far
+    uint32_t settled = 0;  // per stage, the parity of the tiles of V that needed settling
     // between two row tiles; true when a wait gave up, here or in an earlier launch
     auto begin = [&]() {
         __syncthreads();
@@ -214,128 +244,184 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         __syncthreads();
         return *((volatile int*)&bar.abort_flag) != 0;
     };
+    // Seldom: the noted keys' values that are not finite, added to the finished rows that see them (their
+    // weights are positive): to the output, or, where the keys are split, to the partial rows.  Warp 2.
+    auto add_odd_values = [&](const Job& job) {
+        const int count = min(*((volatile int*)&bar.odd_count), kWideRows);
+        for (int i = lane; i < count * min(kWideRows, rows - job.row0); i += 32) {
+            const int key = bar.odd_keys[i % count], row = job.row0 + i / count, token = row / p.group;
+            const int page = key <= s.keys - s.queries + token ? page_of(p, b, key) : -1;
+            if (page < 0) continue;
+            const __nv_bfloat16* v = p.v_pages + page * p.v_page + (key & ((1 << p.page_shift) - 1)) * p.v_slot + head * p.v_head;
+            const int64_t at = (int64_t)(s.first + token) * p.heads + head * p.group + row % p.group;
+            for (int d = 0; d < kDim; ++d) {
+                const float value = __bfloat162float(v[d]);
+                if (fabsf(value) <= 3.4e38f) continue;
+                if (job.splits <= 1)
+                    atomicAdd(p.out + at * kDim + d, v[d]);  // finite + inf, inf + inf, inf - inf: the same in any order
+                else
+                    atomicAdd(p.partial + (at * p.splits + blockIdx.x) * kDim + d, value);
+            }
+        }
+        __syncwarp();
+        if (lane == 0) bar.odd_count = 0;
+    };
     if (warp < 4) {
         // a row's 128 scores live in registers: what these roles do not need goes to the softmax
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegisters));
-    for (int at = blockIdx.y / p.kv_heads; at * kWideRows < rows; at += row_tiles) {
-        const Job job = job_of(p, s, rows, at);
-        if (!job.mine) continue;
-        const int key_begin = job.key_begin, key_end = job.key_end, tiles = job.tiles;
-        const bool dead = begin();
-        if (warp == 0) {
-            if (!dead) {
-                const int box = min(kKeys, 1 << p.page_shift), boxes = kWideKeys / box;
-                int j = 0;
-                for (; j < tiles; ++j) {
-                    const int n = stage_count + j, stage = n % kWideStages, parity = (n / kWideStages) & 1;
-                    const int key = key_begin + j * kWideKeys + lane * box;
-                    const bool wanted = lane < boxes && key < key_end;
-                    const int page = wanted ? page_of(p, b, key) : -1;
-                    if (wanted && page < 0) bar.bad = 1;
-                    const uint32_t bytes = __popc(__ballot_sync(0xFFFFFFFFu, page >= 0)) * box * kDim * 2;
-                    const int slot = key & ((1 << p.page_shift) - 1);
-                    unsigned char* to = smem + Shared::kK + stage * kTileBytes + lane * box * 128;
-                    if (n >= kWideStages &&
-                        !warp_wait(&bar.k_empty[stage], parity ^ 1, &bar.abort_flag, p.status, kSiteWide, n))
-                        break;
-                    if (lane == 0) ptx::mbar_arrive_expect_tx(&bar.k_full[stage], bytes);
+        for (int at = blockIdx.y / p.kv_heads; at * kWideRows < rows; at += row_tiles) {
+            const Job job = job_of(p, s, rows, at);
+            if (!job.mine) continue;
+            const int key_begin = job.key_begin, key_end = job.key_end, tiles = job.tiles;
+            const int all_see = visible_keys(p, s, job.row0, 1);  // keys that every row sees
+            const int settle_from = min(all_see, key_end);        // tiles with keys from here on are settled
+            const bool dead = begin();
+            if (warp == 0) {
+                if (!dead) {
+                    const int box = min(kKeys, 1 << p.page_shift), boxes = kWideKeys / box;
+                    int j = 0;
+                    for (; j < tiles; ++j) {
+                        const int n = stage_count + j, stage = n % kWideStages, parity = (n / kWideStages) & 1;
+                        const int key = key_begin + j * kWideKeys + lane * box;
+                        const bool wanted = lane < boxes && key < key_end;
+                        const int page = wanted ? page_of(p, b, key) : -1;
+                        if (wanted && page < 0) bar.bad = 1;
+                        const uint32_t bytes = __popc(__ballot_sync(0xFFFFFFFFu, page >= 0)) * box * kDim * 2;
+                        const int slot = key & ((1 << p.page_shift) - 1);
+                        unsigned char* to = smem + Shared::kK + stage * kTileBytes + lane * box * 128;
+                        if (n >= kWideStages &&
+                            !warp_wait(&bar.k_empty[stage], parity ^ 1, &bar.abort_flag, p.status, kSiteWide, n))
+                            break;
+                        if (lane == 0) ptx::mbar_arrive_expect_tx(&bar.k_full[stage], bytes);
+                        __syncwarp();
+                        if (page >= 0)
+                            for (int i = 0; i < kSlabs; ++i)
+                                tma_load_4d(to + i * kWideKeys * 128, &k_map, &bar.k_full[stage], i * 64, head, slot, page);
+                        if (n >= kWideStages &&
+                            !warp_wait(&bar.v_empty[stage], parity ^ 1, &bar.abort_flag, p.status, kSiteWide + 1, n)) {
+                            // the copy of K of this tile lands before its memory is given up
+                            for (int spin = 0; spin < 1000000 && !ptx::mbar_try_wait(&bar.k_full[stage], parity);) ++spin;
+                            break;
+                        }
+                        if (lane == 0) ptx::mbar_arrive_expect_tx(&bar.v_full[stage], bytes);
+                        __syncwarp();
+                        to += Shared::kV - Shared::kK;
+                        if (page >= 0)
+                            for (int i = 0; i < kSlabs; ++i)
+                                tma_load_4d(to + i * kWideKeys * 128, &v_map, &bar.v_full[stage], i * 64, head, slot, page);
+                        if (key_begin + (j + 1) * kWideKeys > settle_from) {
+                            // warps 2 and 3 follow no other tiles and could not tell one phase of v_full from the next
+                            if (!warp_wait(&bar.v_full[stage], parity, &bar.abort_flag, p.status, kSiteWide + 12, n)) {
+                                ++j;
+                                break;
+                            }
+                            if (lane == 0) ptx::mbar_arrive(&bar.v_there[stage]);
+                        }
+                    }
+                    if (*((volatile int*)&bar.abort_flag))
+                        for (int i = max(0, stage_count + j - kWideStages); i < stage_count + j; ++i)
+                            for (int spin = 0; spin < 1000000 && !(ptx::mbar_try_wait(&bar.k_full[i % kWideStages], (i / kWideStages) & 1) &&
+                                                                   ptx::mbar_try_wait(&bar.v_full[i % kWideStages], (i / kWideStages) & 1));)
+                                ++spin;
+                }
+            } else if (warp == 1) {
+                constexpr uint32_t kIdescS = wide_idesc(128, kWideKeys, false), kIdescO = wide_idesc(128, kDim, true);
+                // descriptors differ by constants (in units of 16 bytes), so that an issue costs an addition
+                const uint32_t base = ptx::smem_u32(smem);
+                const uint64_t q_desc = ptx::smem_desc_sw128(base + Shared::kQ), k_desc = ptx::smem_desc_sw128(base + Shared::kK),
+                               v_desc = desc_rows(base + Shared::kV);
+                auto scores = [&](int t, int stage) {
+                    const uint64_t q = q_desc + t * (kTileBytes / 16), k = k_desc + stage * (kTileBytes / 16);
+                    if (ptx::elect_one()) {
+#pragma unroll
+                        for (int i = 0; i < kDim / 16; ++i) {
+                            const int off = ((i / 4) * kWideKeys * 128 + (i % 4) * 32) / 16;
+                            umma_ss(tmem + kS + 128 * t, q + off, k + off, kIdescS, i > 0);
+                        }
+                        ptx::umma_commit(&bar.s_full[t]);
+                        if (t == 1) ptx::umma_commit(&bar.k_empty[stage]);
+                    }
                     __syncwarp();
-                    if (page >= 0)
-                        for (int i = 0; i < kSlabs; ++i)
-                            tma_load_4d(to + i * kWideKeys * 128, &k_map, &bar.k_full[stage], i * 64, head, slot, page);
-                    if (n >= kWideStages &&
-                        !warp_wait(&bar.v_empty[stage], parity ^ 1, &bar.abort_flag, p.status, kSiteWide + 1, n)) {
-                        // the copy of K of this tile lands before its memory is given up
-                        for (int spin = 0; spin < 1000000 && !ptx::mbar_try_wait(&bar.k_full[stage], parity);) ++spin;
-                        break;
+                };
+                auto values = [&](int t, int stage, int half, bool accumulate) {
+                    const uint64_t v = v_desc + stage * (kTileBytes / 16) + half * (kTileBytes / 32 / kSlabs);
+                    if (ptx::elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < kWideKeys / 32; ++k) {
+                            umma_ts(tmem + kO + kDim * t, tmem + kS + 128 * t + 8 * (half * (kWideKeys / 32) + k), v + k * 128,
+                                    kIdescO, accumulate || k > 0);
+                        }
+                        if (half == 1) {
+                            ptx::umma_commit(&bar.o_done[t]);
+                            if (t == 1) ptx::umma_commit(&bar.v_empty[stage]);
+                        }
                     }
-                    if (lane == 0) ptx::mbar_arrive_expect_tx(&bar.v_full[stage], bytes);
                     __syncwarp();
-                    to += Shared::kV - Shared::kK;
-                    if (page >= 0)
-                        for (int i = 0; i < kSlabs; ++i)
-                            tma_load_4d(to + i * kWideKeys * 128, &v_map, &bar.v_full[stage], i * 64, head, slot, page);
+                };
+                auto wait = [&](unsigned long long* which, uint32_t parity, int site) {
+                    const bool ok = warp_wait(which, parity, &bar.abort_flag, p.status, kSiteWide + site, stage_count);
+                    ptx::tcgen05_fence_after();
+                    return ok;
+                };
+                bool ok = !dead && tiles > 0 && wait(&bar.q_ready, list & 1, 2);
+                ok = ok && wait(&bar.k_full[stage_count % kWideStages], (stage_count / kWideStages) & 1, 3);
+                if (ok) {
+                    scores(0, stage_count % kWideStages);
+                    scores(1, stage_count % kWideStages);
                 }
-                if (*((volatile int*)&bar.abort_flag))
-                    for (int i = max(0, stage_count + j - kWideStages); i < stage_count + j; ++i)
-                        for (int spin = 0; spin < 1000000 && !(ptx::mbar_try_wait(&bar.k_full[i % kWideStages], (i / kWideStages) & 1) &&
-                                                               ptx::mbar_try_wait(&bar.v_full[i % kWideStages], (i / kWideStages) & 1));)
-                            ++spin;
-            }
-        } else if (warp == 1) {
-            constexpr uint32_t kIdescS = wide_idesc(128, kWideKeys, false), kIdescO = wide_idesc(128, kDim, true);
-            // descriptors differ by constants (in units of 16 bytes), so that an issue costs an addition
-            const uint32_t base = ptx::smem_u32(smem);
-            const uint64_t q_desc = ptx::smem_desc_sw128(base + Shared::kQ), k_desc = ptx::smem_desc_sw128(base + Shared::kK),
-                           v_desc = desc_rows(base + Shared::kV);
-            auto scores = [&](int t, int stage) {
-                const uint64_t q = q_desc + t * (kTileBytes / 16), k = k_desc + stage * (kTileBytes / 16);
-                if (ptx::elect_one()) {
+                for (int j = 0; ok && j < tiles; ++j) {
+                    const int n = stage_count + j, stage = n % kWideStages, next = (n + 1) % kWideStages;
 #pragma unroll
-                    for (int i = 0; i < kDim / 16; ++i) {
-                        const int off = ((i / 4) * kWideKeys * 128 + (i % 4) * 32) / 16;
-                        umma_ss(tmem + kS + 128 * t, q + off, k + off, kIdescS, i > 0);
-                    }
-                    ptx::umma_commit(&bar.s_full[t]);
-                    if (t == 1) ptx::umma_commit(&bar.k_empty[stage]);
-                }
-                __syncwarp();
-            };
-            auto values = [&](int t, int stage, int half, bool accumulate) {
-                const uint64_t v = v_desc + stage * (kTileBytes / 16) + half * (kTileBytes / 32 / kSlabs);
-                if (ptx::elect_one()) {
-#pragma unroll
-                    for (int k = 0; k < kWideKeys / 32; ++k) {
-                        umma_ts(tmem + kO + kDim * t, tmem + kS + 128 * t + 8 * (half * (kWideKeys / 32) + k), v + k * 128,
-                                kIdescO, accumulate || k > 0);
-                    }
-                    if (half == 1) {
-                        ptx::umma_commit(&bar.o_done[t]);
-                        if (t == 1) ptx::umma_commit(&bar.v_empty[stage]);
+                    for (int t = 0; t < 2; ++t) {
+                        if (!ok) break;
+                        ok = wait(&bar.p_half[t], n & 1, 4);
+                        if (ok && t == 0) {
+                            ok = wait(&bar.v_full[stage], (n / kWideStages) & 1, 5);
+                            if (ok && key_begin + (j + 1) * kWideKeys > settle_from) {
+                                ok = wait(&bar.v_settled[stage], settled >> stage & 1, 9);
+                                settled ^= 1u << stage;
+                            }
+                        }
+                        if (!ok) break;
+                        values(t, stage, 0, j > 0);
+                        ok = wait(&bar.p_ready[t], n & 1, 7);
+                        if (!ok) break;
+                        values(t, stage, 1, true);
+                        if (j + 1 < tiles) {
+                            if (t == 0) ok = wait(&bar.k_full[next], ((n + 1) / kWideStages) & 1, 6);
+                            if (ok) scores(t, next);
+                        }
                     }
                 }
-                __syncwarp();
-            };
-            auto wait = [&](unsigned long long* which, uint32_t parity, int site) {
-                const bool ok = warp_wait(which, parity, &bar.abort_flag, p.status, kSiteWide + site, stage_count);
-                ptx::tcgen05_fence_after();
-                return ok;
-            };
-            bool ok = !dead && tiles > 0 && wait(&bar.q_ready, list & 1, 2);
-            ok = ok && wait(&bar.k_full[stage_count % kWideStages], (stage_count / kWideStages) & 1, 3);
-            if (ok) {
-                scores(0, stage_count % kWideStages);
-                scores(1, stage_count % kWideStages);
-            }
-            for (int j = 0; ok && j < tiles; ++j) {
-                const int n = stage_count + j, stage = n % kWideStages, next = (n + 1) % kWideStages;
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    if (!ok) break;
-                    ok = wait(&bar.p_half[t], n & 1, 4);
-                    if (ok && t == 0) ok = wait(&bar.v_full[stage], (n / kWideStages) & 1, 5);
-                    if (!ok) break;
-                    values(t, stage, 0, j > 0);
-                    ok = wait(&bar.p_ready[t], n & 1, 7);
-                    if (!ok) break;
-                    values(t, stage, 1, true);
-                    if (j + 1 < tiles) {
-                        if (t == 0) ok = wait(&bar.k_full[next], ((n + 1) / kWideStages) & 1, 6);
-                        if (ok) scores(t, next);
-                    }
+            } else if (!dead) {
+                // Warps 2 and 3: values of keys that no row sees, or not every one, must not meet the others' zero
+                // probabilities where they are not finite.  The former are cleared; of the latter those that
+                // are not finite, which the rows that see the key get in the end.
+                for (int j = 0; j < tiles; ++j) {
+                    const int key0 = key_begin + j * kWideKeys, stage = (stage_count + j) % kWideStages;
+                    if (key0 + kWideKeys <= settle_from) continue;
+                    if (!warp_wait(&bar.v_there[stage], settled >> stage & 1, &bar.abort_flag, p.status, kSiteWide + 10, j)) break;
+                    settled ^= 1u << stage;
+                    for (int r = (warp - 2) * 32 + lane; r < kWideKeys; r += 64)
+                        if (key0 + r >= all_see || key0 + r >= key_end)
+                            settle_values<kDim>(smem + Shared::kV + stage * kTileBytes + r * 128, key0 + r, key_end, bar);
+                    asm volatile("fence.proxy.async;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(&bar.v_settled[stage]);
                 }
             }
+            stage_count += tiles;
+            ++list;
+            __syncthreads();  // the rows are written
+            if (warp == 2 && *((volatile int*)&bar.odd_count) != 0) add_odd_values(job);
         }
-        stage_count += tiles;
-        ++list;
-    }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters));
-    for (int at = blockIdx.y / p.kv_heads; at * kWideRows < rows; at += row_tiles) {
-        const Job job = job_of(p, s, rows, at);
-        if (!job.mine) continue;
-        const int row0 = job.row0, key_begin = job.key_begin, key_end = job.key_end, tiles = job.tiles, splits = job.splits;
-        const bool dead = begin();
+        for (int at = blockIdx.y / p.kv_heads; at * kWideRows < rows; at += row_tiles) {
+            const Job job = job_of(p, s, rows, at);
+            if (!job.mine) continue;
+            const int row0 = job.row0, key_begin = job.key_begin, tiles = job.tiles, splits = job.splits;
+            const bool dead = begin();
             const int t = (warp - 4) / 4, r = (warp % 4) * 32 + lane;  // tile, row in it
             const uint32_t lanes = tmem + ((uint32_t)((warp % 4) * 32) << 16);
             const int row = row0 + t * 128 + r;
@@ -363,19 +449,6 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 ok = warp_wait(&bar.s_full[t], parity, &bar.abort_flag, p.status, kSiteWide + 8, j);
                 if (!ok) break;
                 ptx::tcgen05_fence_after();
-                if (t == 0 && key0 + kWideKeys > key_end) {
-                    // rows of V behind the last key may hold anything: 0 * NaN is not 0
-                    const int n = stage_count + j, stage = n % kWideStages;
-                    ok = warp_wait(&bar.v_full[stage], (n / kWideStages) & 1, &bar.abort_flag, p.status, kSiteWide + 10, j);
-                    if (!ok) break;
-                    if (key0 + r >= key_end) {
-                        unsigned char* v = smem + Shared::kV + stage * kTileBytes + r * 128;
-#pragma unroll
-                        for (int i = 0; i < kDim / 8; ++i)
-                            *reinterpret_cast<uint4*>(v + (i / 8) * kWideKeys * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    asm volatile("fence.proxy.async;" ::: "memory");
-                }
                 const bool masked = key0 + kWideKeys > fewest;
                 uint32_t x[4][32];
 #pragma unroll
@@ -499,8 +572,9 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 stats[1] = failed ? __uint_as_float(0x7FC00000u) : sum;
             }
             ptx::tcgen05_fence_before();
-        stage_count += tiles;
-    }
+            stage_count += tiles;
+            __syncthreads();
+        }
     }
     __syncthreads();
     if (warp == 1) {
