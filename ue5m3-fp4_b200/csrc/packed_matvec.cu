@@ -89,61 +89,56 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// 32 consecutive activations (k0 ...) of one token as floats, zero behind the end
+// What a lane brings of a chunk's activations, as they are in memory: 32 consecutive elements of one
+// column's token, zero behind the end.
 template <bool kFp32>
-__device__ __forceinline__ void load_x(const Params& p, int token, int k0, float (&v)[32]) {
-    if constexpr (kFp32) {
-        const float* row = reinterpret_cast<const float*>(p.x) + (int64_t)token * p.ldx + k0;
-        if (p.vector_x && k0 + 32 <= p.k) {
+struct Raw {
+    uint32_t words[kFp32 ? 32 : 16];
+};
+
+template <bool kFp32>
+__device__ __forceinline__ Raw<kFp32> load_raw(const Params& p, int column, int columns, int chunk) {
+    constexpr int kParts = kFp32 ? 3 : 1, kWords = kFp32 ? 32 : 16, kSize = kFp32 ? 4 : 2;
+    const int k0 = chunk * kChunk + 32 * (threadIdx.x & 3);
+    const bool present = column < columns && k0 < p.k;
+    const int token = present ? column / kParts : 0;
+    const uint8_t* row = reinterpret_cast<const uint8_t*>(p.x) + ((int64_t)token * p.ldx + k0) * kSize;
+    Raw<kFp32> raw;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float4 f = __ldg(reinterpret_cast<const float4*>(row) + i);
-                v[4 * i] = f.x, v[4 * i + 1] = f.y, v[4 * i + 2] = f.z, v[4 * i + 3] = f.w;
-            }
-        } else {
+    for (int i = 0; i < kWords; ++i) raw.words[i] = 0;
+    if (!present) return raw;
+    if (p.vector_x && k0 + 32 <= p.k) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = k0 + i < p.k ? __ldg(row + i) : 0.0f;
-        }
+        for (int i = 0; i < kWords / 4; ++i)
+            *reinterpret_cast<uint4*>(raw.words + 4 * i) = __ldg(reinterpret_cast<const uint4*>(row) + i);
     } else {
-        const uint16_t* row = reinterpret_cast<const uint16_t*>(p.x) + (int64_t)token * p.ldx + k0;
-        if (p.vector_x && k0 + 32 <= p.k) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint4 u = __ldg(reinterpret_cast<const uint4*>(row) + i);
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    v[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
-                    v[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = k0 + i < p.k ? __uint_as_float((uint32_t)__ldg(row + i) << 16) : 0.0f;
+        for (int i = 0; i < 32; ++i) {
+            const bool in = k0 + i < p.k;
+            if constexpr (kFp32)
+                raw.words[i] = in ? __ldg(reinterpret_cast<const uint32_t*>(row) + i) : 0;
+            else
+                raw.words[i / 2] |= (in ? (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(row) + i) : 0u) << (16 * (i & 1));
         }
     }
+    return raw;
 }
 
-// One chunk's activations of column `column` as mma B fragments, and the factor that undoes the
-// chunk's power of two.  Lane (g, c) = (lane / 4, lane % 4) brings column g and elements
-// 32 c ... 32 c + 31; step j of the chunk's eight mma takes its elements 4 j ... 4 j + 3.
+// One chunk's activations as mma B fragments, and the factor that undoes the chunk's power of two.
+// Lane (g, c) = (lane / 4, lane % 4) brings column g and elements 32 c ... 32 c + 31; step j of the
+// chunk's eight mma takes its elements 4 j ... 4 j + 3.  part: which of an fp32 element's three parts.
 template <bool kFp32>
-__device__ __forceinline__ void load_fragment(const Params& p, int column, int columns, int chunk, uint32_t (&b)[16],
-                                              float& undo) {
-    constexpr int kParts = kFp32 ? 3 : 1;
-    const int c = threadIdx.x & 3;
-    const bool present = column < columns && chunk * kChunk < p.k;
-    const int token = present ? column / kParts : 0, part = present ? column % kParts : 0;
-    float v[32];
-    if (present)
-        load_x<kFp32>(p, token, chunk * kChunk + 32 * c, v);
-    else {
+__device__ __forceinline__ void make_fragment(const Raw<kFp32>& raw, int part, uint32_t (&b)[16], float& undo) {
+    uint32_t top = 0;  // the largest magnitude's bits, as those of an fp32; a NaN's are larger than all numbers'
+    if constexpr (kFp32) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+        for (int i = 0; i < 32; ++i) top = max(top, raw.words[i] & 0x7FFFFFFFu);
+    } else {
+        uint32_t two = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(two) : "r"(raw.words[i] & 0x7FFF7FFFu));
+        top = max(two << 16, two & 0xFFFF0000u);
     }
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
     top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
     top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
     // 2^(14 - e) for a largest element in [2^e, 2^(e+1)), held to 2^126 so that its inverse is a
@@ -151,23 +146,31 @@ __device__ __forceinline__ void load_fragment(const Params& p, int column, int c
     const int field = min(268 - (int)(top >> 23), 253);
     const float scale = __uint_as_float((uint32_t)field << 23);
     undo = __uint_as_float((uint32_t)(254 - field) << 23);
-    if (kFp32) undo *= part == 0 ? 1.0f : part == 1 ? 0x1p-11f : 0x1p-22f;
+    if constexpr (kFp32) {
+        undo *= part == 0 ? 1.0f : part == 1 ? 0x1p-11f : 0x1p-22f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        float lo = v[2 * i] * scale, hi = v[2 * i + 1] * scale;
-        if (kFp32) {
+        for (int i = 0; i < 16; ++i) {
+            float lo = __uint_as_float(raw.words[2 * i]) * scale, hi = __uint_as_float(raw.words[2 * i + 1]) * scale;
 #pragma unroll
-            for (int step = 1; step < kParts; ++step) {
+            for (int step = 1; step < 3; ++step)
                 if (part >= step) {
                     const float l = __half2float(__float2half_rn(lo)), h = __half2float(__float2half_rn(hi));
                     // what the parts before left over, exactly; nothing behind an infinity or a NaN
                     lo = fabsf(l) <= 65504.0f ? (lo - l) * 2048.0f : 0.0f;
                     hi = fabsf(h) <= 65504.0f ? (hi - h) * 2048.0f : 0.0f;
                 }
-            }
+            const __half2 h = __floats2half2_rn(lo, hi);
+            b[i] = *reinterpret_cast<const uint32_t*>(&h);
         }
-        const __half2 h = __floats2half2_rn(lo, hi);
-        b[i] = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const uint32_t scale2 = (uint32_t)field << 7 | (uint32_t)field << 23;  // the power of two as a bf16 pair
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            uint32_t w;
+            asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(w) : "r"(raw.words[i]), "r"(scale2));
+            const __half2 h = __floats2half2_rn(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+            b[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
     }
 }
 
@@ -328,9 +331,10 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
                 for (int d = 0; d < kDepth; ++d)
 #pragma unroll
                     for (int t = 0; t < kTiles; ++t) {
+                        const int column = 8 * t + g, chunk = (pass * kDepth + d) * kWarps + warp;
+                        const Raw<kFp32> raw = load_raw<kFp32>(p, column0 + column, column0 + used, chunk);
                         float mine;
-                        load_fragment<kFp32>(p, column0 + 8 * t + g, column0 + used, (pass * kDepth + d) * kWarps + warp,
-                                             b[d][t], mine);
+                        make_fragment<kFp32>(raw, kFp32 ? (column0 + column) % 3 : 0, b[d][t], mine);
                         undo[d][t][0] = __shfl_sync(0xFFFFFFFFu, mine, 8 * c);
                         undo[d][t][1] = __shfl_sync(0xFFFFFFFFu, mine, 8 * c + 4);
                     }
