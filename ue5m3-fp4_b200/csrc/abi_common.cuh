@@ -29,4 +29,33 @@ cudaError_t allow_shared(int bytes) {
     return error;
 }
 
+// Clusters of `size` CTAs that the current device holds at a time (0: none, or an error), asked for
+// once per kernel, device and size.
+template <auto kKernel>
+int resident_clusters(int size, int threads, int shared) {
+    static int known[64][5] = {};
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device >= 64 || size > 4) return 0;
+    if (known[device][size] == 0) {
+        cudaLaunchConfig_t config = {};
+        config.gridDim = dim3(size);
+        config.blockDim = dim3(threads);
+        config.dynamicSmemBytes = shared;
+        cudaLaunchAttribute attribute;
+        attribute.id = cudaLaunchAttributeClusterDimension;
+        attribute.val.clusterDim.x = size;
+        attribute.val.clusterDim.y = 1;
+        attribute.val.clusterDim.z = 1;
+        config.attrs = &attribute;
+        config.numAttrs = 1;
+        int count = 0;
+        if (cudaOccupancyMaxActiveClusters(&count, kKernel, &config) != cudaSuccess) {
+            cudaGetLastError();
+            count = 0;
+        }
+        known[device][size] = count > 0 ? count : -1;
+    }
+    return known[device][size] > 0 ? known[device][size] : 0;
+}
+
 }  // namespace ue5m3

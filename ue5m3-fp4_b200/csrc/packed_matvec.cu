@@ -21,6 +21,7 @@
 // warps w the 128-element chunks w, w + 16, ... of the reduction axis.  A warp keeps the activations
 // of its chunks in registers (as mma fragments) while it walks over the CTA's rows; the sums of
 // the 16 warps meet in shared memory once per block of rows.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -53,6 +54,7 @@ struct Params {
     int64_t scale_stride;  // bytes per row of scales
     int tokens, rows, k;
     int row_shift;         // log2 of the rows that share a scale row: 0, 4 or 5
+    int split;             // CTAs of a cluster that share the reduction axis
     int rows_per_block;    // rows of one pass over shared memory, a multiple of 16
     int vector_x;          // rows of x start on 16-byte boundaries and hold whole vectors
     int bias_fp32, out_fp32;
@@ -239,10 +241,12 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
     constexpr int kColumns = kTiles * 8;
     constexpr int kBlockShift = kBlock == 16 ? 4 : 5;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int chunks = (p.k + kChunk - 1) / kChunk;
-    const int passes = (chunks + kWarps * kDepth - 1) / (kWarps * kDepth);
-    const int first_row = (int)((int64_t)p.rows * blockIdx.x / gridDim.x);
-    const int last_row = (int)((int64_t)p.rows * (blockIdx.x + 1) / gridDim.x);
+    const int share = blockIdx.x % p.split, group = blockIdx.x / p.split, groups = gridDim.x / p.split;
+    const int all_chunks = (p.k + kChunk - 1) / kChunk;
+    const int first_chunk = all_chunks * share / p.split, chunks = all_chunks * (share + 1) / p.split;  // first and behind the last
+    const int passes = max(1, (chunks - first_chunk + kWarps * kDepth - 1) / (kWarps * kDepth));
+    const int first_row = (int)((int64_t)p.rows * group / groups);
+    const int last_row = (int)((int64_t)p.rows * (group + 1) / groups);
     const int block_rows = p.rows_per_block;
     const int stride = (int)p.code_stride, scale_stride = (int)p.scale_stride;
     // whole tokens per pass, so that the parts of a token meet in one pass
@@ -267,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
 #pragma unroll
                 for (int d = 0; d < kDepth; ++d) {
                     // a chunk behind the end is read as the row's last bytes
-                    const int byte = min(((pass * kDepth + d) * kWarps + warp) * (kChunk / 2) + 16 * c, stride - 1);
+                    const int byte = min((first_chunk + (pass * kDepth + d) * kWarps + warp) * (kChunk / 2) + 16 * c, stride - 1);
                     const int block = byte * 2 >> kBlockShift;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
@@ -286,7 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
             int ahead_pass = 0, ahead_tile = 0;
             const uint8_t *ahead_codes = nullptr, *ahead_scales = nullptr;
             auto locate = [&]() {
-                const int chunk = ahead_pass * kDepth * kWarps + warp;
+                const int chunk = first_chunk + ahead_pass * kDepth * kWarps + warp;
                 ahead_codes = codes + (int64_t)(ahead_tile + g) * stride + chunk * (kChunk / 2) + 16 * c;
                 ahead_scales = scales + chunk * (kChunk / kBlock);
             };
@@ -298,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
                     const int scale_row = (row0 + row >> p.row_shift) - scale_row0;
 #pragma unroll
                     for (int d = 0; d < kDepth; ++d) {
-                        if ((ahead_pass * kDepth + d) * kWarps + warp >= chunks) continue;
+                        if (first_chunk + (ahead_pass * kDepth + d) * kWarps + warp >= chunks) continue;
 #pragma unroll
                         for (int h = 0; h < 2; ++h)
                             if (ahead_tile + g + 8 * h < row_count)
@@ -331,8 +335,8 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
                 for (int d = 0; d < kDepth; ++d)
 #pragma unroll
                     for (int t = 0; t < kTiles; ++t) {
-                        const int column = 8 * t + g, chunk = (pass * kDepth + d) * kWarps + warp;
-                        const Raw<kFp32> raw = load_raw<kFp32>(p, column0 + column, column0 + used, chunk);
+                        const int column = 8 * t + g, chunk = first_chunk + (pass * kDepth + d) * kWarps + warp;
+                        const Raw<kFp32> raw = load_raw<kFp32>(p, column0 + column, chunk < chunks ? column0 + used : 0, chunk);
                         float mine;
                         make_fragment<kFp32>(raw, kFp32 ? (column0 + column) % 3 : 0, b[d][t], mine);
                         undo[d][t][0] = __shfl_sync(0xFFFFFFFFu, mine, 8 * c);
@@ -417,14 +421,31 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
                 }
             }
             __syncthreads();
-            for (int i = threadIdx.x; i < row_count * tokens; i += kThreads) {
+            if (p.split > 1) {
+                // the sums of this CTA's warps, in the place of its first warp's; then those of the cluster
+                for (int i = threadIdx.x; i < row_count * used; i += kThreads) {
+                    const int column = i / row_count, r = i - column * row_count;
+                    float value = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < kWarps; ++w) value += partial[(w * used + column) * block_rows + r];
+                    partial[column * block_rows + r] = value;
+                }
+                cooperative_groups::this_cluster().sync();
+            }
+            for (int i = share * kThreads + threadIdx.x; i < row_count * tokens; i += p.split * kThreads) {
                 const int token = i / row_count, r = i - token * row_count;
                 float value = 0.0f;
+                if (p.split > 1) {
 #pragma unroll
-                for (int part = kParts - 1; part >= 0; --part)
+                    for (int part = kParts - 1; part >= 0; --part)
+                        for (int q = 0; q < p.split; ++q)
+                            value += cooperative_groups::this_cluster().map_shared_rank(partial, q)[(token * kParts + part) * block_rows + r];
+                } else {
 #pragma unroll
-                    for (int w = 0; w < kWarps; ++w)
-                        value += partial[((size_t)w * used + token * kParts + part) * block_rows + r];
+                    for (int part = kParts - 1; part >= 0; --part)
+#pragma unroll
+                        for (int w = 0; w < kWarps; ++w) value += partial[(w * used + token * kParts + part) * block_rows + r];
+                }
                 value *= p.factor;
                 const int64_t n = row0 + r;
                 if (p.bias)
@@ -436,7 +457,10 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
                 else
                     reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(value);
             }
-            __syncthreads();
+            if (p.split > 1)
+                cooperative_groups::this_cluster().sync();  // the others have read this CTA's sums
+            else
+                __syncthreads();
         }
     }
 }
@@ -445,19 +469,40 @@ template <bool kFp32, int kTiles, int kDepth, bool kVector, int kBlock>
 int launch(Params p, cudaStream_t stream) {
     constexpr int kTokens = kTiles * 8 / (kFp32 ? 3 : 1);
     const int used = (p.tokens < kTokens ? p.tokens : kTokens) * (kFp32 ? 3 : 1);
-    const int grid = p.rows < sm_count() ? p.rows : sm_count();
+    constexpr size_t kRingBytes = kVector ? kRing * slot_pieces(kDepth) * sizeof(uint4) : 0;
+    constexpr auto kKernel = packed_matvec_kernel<kFp32, kTiles, kDepth, kVector, kBlock>;
+    cudaError_t error = allow_shared<kKernel>((int)kRingBytes + kPartialFloats * 4);
+    if (error != cudaSuccess) return record_cuda_error(error);
+    // Few rows and a long reduction axis: with the rows spread over all SMs, every one of them would convert
+    // all activations, for a few row tiles each time.  Pairs of CTAs share the axis and own twice the rows
+    // (8 x 4096 x 21504: 23.2 -> 20.1 us; four CTAs 22.0, since only 33 such clusters fit on the SMs).
+    const int passes = (p.k + kChunk * kWarps * kDepth - 1) / (kChunk * kWarps * kDepth);
+    p.split = passes > 1 && p.rows <= 64 * sm_count() ? 2 : 1;
+    int grid = sm_count();
+    if (p.split > 1) {
+        grid = resident_clusters<kKernel>(p.split, kThreads, (int)kRingBytes + kPartialFloats * 4);
+        if (grid <= 0) grid = sm_count(), p.split = 1;
+    }
+    if (grid > p.rows) grid = p.rows;
     const int own = (p.rows + grid - 1) / grid;
     int block = kPartialFloats / (kWarps * used) / 16 * 16;
     const int need = (own + 15) / 16 * 16;
     if (block > need) block = need;
     p.rows_per_block = block;
-    constexpr size_t kRingBytes = kVector ? kRing * slot_pieces(kDepth) * sizeof(uint4) : 0;
     const size_t bytes = kRingBytes + (size_t)kWarps * used * block * sizeof(float);
-    const cudaError_t error = allow_shared<packed_matvec_kernel<kFp32, kTiles, kDepth, kVector, kBlock>>(
-        (int)kRingBytes + kPartialFloats * 4);
-    if (error != cudaSuccess) return record_cuda_error(error);
-    packed_matvec_kernel<kFp32, kTiles, kDepth, kVector, kBlock><<<grid, kThreads, bytes, stream>>>(p);
-    return check_launch();
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(grid * p.split);
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = bytes;
+    config.stream = stream;
+    cudaLaunchAttribute attribute;
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = p.split;
+    attribute.val.clusterDim.y = 1;
+    attribute.val.clusterDim.z = 1;
+    config.attrs = &attribute;
+    config.numAttrs = p.split > 1 ? 1 : 0;
+    return record_cuda_error(cudaLaunchKernelEx(&config, kKernel, p));
 }
 
 template <bool kVector, int kBlock>
