@@ -44,7 +44,7 @@ struct WideShared {
 };
 
 struct WideBarriers {
-    unsigned long long k_full[kWideStages], k_empty[kWideStages], v_full[kWideStages], v_empty[kWideStages];
+    unsigned long long k_full[kWideStages], k_empty[kWideStages], v_full[kWideStages];
     unsigned long long q_ready, s_full[2], p_half[2], p_ready[2], o_done[2], drained;
     unsigned long long v_there[kWideStages], v_settled[kWideStages];  // per stage: its next use waits for this one's
     uint32_t tmem;
@@ -207,9 +207,8 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     if (threadIdx.x == 0) {
         for (int i = 0; i < kWideStages; ++i) {
             ptx::mbar_init(&bar.k_full[i], 1);
-            ptx::mbar_init(&bar.k_empty[i], 1);
+            ptx::mbar_init(&bar.k_empty[i], 4);
             ptx::mbar_init(&bar.v_full[i], 1);
-            ptx::mbar_init(&bar.v_empty[i], 1);
             ptx::mbar_init(&bar.v_there[i], 1);
             ptx::mbar_init(&bar.v_settled[i], 2);
         }
@@ -236,6 +235,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     constexpr uint32_t kS = 0, kO = 256;  // columns: S of tile t at 128 t, O at 256 + kDim t
     int stage_count = 0;   // key stages used so far (every role counts alike); also the per-tile barriers' phases
     int list = 0;          // row tiles done so far
+    int finished = 0;      // row tiles with keys done so far
     uint32_t settled = 0;  // per stage, the parity of the tiles of V that needed settling
     // between two row tiles; true when a wait gave up, here or in an earlier launch
     auto begin = [&]() {
@@ -297,8 +297,9 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                         if (page >= 0)
                             for (int i = 0; i < kSlabs; ++i)
                                 tma_load_4d(to + i * kWideKeys * 128, &k_map, &bar.k_full[stage], i * 64, head, slot, page);
-                        if (n >= kWideStages &&
-                            !warp_wait(&bar.v_empty[stage], parity ^ 1, &bar.abort_flag, p.status, kSiteWide + 1, n)) {
+                        // the scores of tile n - 1 are issued behind the products with the values of tile n - 2
+                        if (n >= kWideStages && !warp_wait(&bar.k_empty[(n - 1) % kWideStages], ((n - 1) / kWideStages) & 1,
+                                                           &bar.abort_flag, p.status, kSiteWide + 1, n)) {
                             // the copy of K of this tile lands before its memory is given up
                             for (int spin = 0; spin < 1000000 && !ptx::mbar_try_wait(&bar.k_full[stage], parity);) ++spin;
                             break;
@@ -339,11 +340,10 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                             umma_ss(tmem + kS + 128 * t, q + off, k + off, kIdescS, i > 0);
                         }
                         ptx::umma_commit(&bar.s_full[t]);
-                        if (t == 1) ptx::umma_commit(&bar.k_empty[stage]);
                     }
                     __syncwarp();
                 };
-                auto values = [&](int t, int stage, int half, bool accumulate) {
+                auto values = [&](int t, int stage, int half, bool accumulate, bool last) {
                     const uint64_t v = v_desc + stage * (kTileBytes / 16) + half * (kTileBytes / 32 / kSlabs);
                     if (ptx::elect_one()) {
 #pragma unroll
@@ -351,10 +351,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                             umma_ts(tmem + kO + kDim * t, tmem + kS + 128 * t + 8 * (half * (kWideKeys / 32) + k), v + k * 128,
                                     kIdescO, accumulate || k > 0);
                         }
-                        if (half == 1) {
-                            ptx::umma_commit(&bar.o_done[t]);
-                            if (t == 1) ptx::umma_commit(&bar.v_empty[stage]);
-                        }
+                        if (last && half == 1) ptx::umma_commit(&bar.o_done[t]);
                     }
                     __syncwarp();
                 };
@@ -383,10 +380,10 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                             }
                         }
                         if (!ok) break;
-                        values(t, stage, 0, j > 0);
+                        values(t, stage, 0, j > 0, false);
                         ok = wait(&bar.p_ready[t], n & 1, 7);
                         if (!ok) break;
-                        values(t, stage, 1, true);
+                        values(t, stage, 1, true, j == tiles - 1);
                         if (j + 1 < tiles) {
                             if (t == 0) ok = wait(&bar.k_full[next], ((n + 1) / kWideStages) & 1, 6);
                             if (ok) scores(t, next);
@@ -449,6 +446,8 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 ok = warp_wait(&bar.s_full[t], parity, &bar.abort_flag, p.status, kSiteWide + 8, j);
                 if (!ok) break;
                 ptx::tcgen05_fence_after();
+                // the keys' stage is free when both tiles' scores are; a commit for it would cost the issuing warp
+                if (t == 1 && lane == 0) ptx::mbar_arrive(&bar.k_empty[(stage_count + j) % kWideStages]);
                 const bool masked = key0 + kWideKeys > fewest;
                 uint32_t x[4][32];
 #pragma unroll
@@ -475,10 +474,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                     const float fade = moved == -INFINITY ? 1.0f : exp2_approx(top - moved);
                     sum *= fade;
                     top = moved;
-                    if (j > 0) {
-                        ok = warp_wait(&bar.o_done[t], parity ^ 1, &bar.abort_flag, p.status, kSiteWide + 9, j);
-                        if (!ok) break;
-                        ptx::tcgen05_fence_after();
+                    if (j > 0) {  // the scores' arrival tells that the products before them are done
 #pragma unroll 1
                         for (int i = 0; i < kDim / 16; ++i) {
                             uint32_t o[16];
@@ -526,7 +522,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                 sum += lo + hi;
             }
             if (ok && tiles > 0)
-                ok = warp_wait(&bar.o_done[t], (stage_count + tiles - 1) & 1, &bar.abort_flag, p.status, kSiteWide + 11, 0);
+                ok = warp_wait(&bar.o_done[t], finished++ & 1, &bar.abort_flag, p.status, kSiteWide + 11, 0);
             ptx::tcgen05_fence_after();
             __syncwarp();
             const bool failed = !ok || *((volatile int*)&bar.abort_flag) || *((volatile int*)&bar.bad);
