@@ -8,7 +8,7 @@
 // is: 128 consecutive elements of a row share a power of two that brings their largest one to
 // [2^14, 2^15).  A bf16 element that is no smaller than 2^-32 of that largest one is then exact in
 // fp16; below that it is off by at most 2^-40 of the largest one.  An fp32 element is cut into
-// three fp16 parts (11 bits each), which take three columns of the product.  Tensor cores
+// three fp16 parts (11 bits each) with a product of its own each.  Tensor cores
 // (mma.m16n8k16, weights as the 16-row operand, activations as the 8 columns) sum 128 products in
 // fp32; the power of two is multiplied back when that sum joins the fp32 total.  The order of all
 // sums is fixed by the sizes: the same call gives the same bits.
@@ -37,6 +37,10 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kChunk = 128;          // reduction elements of one warp step: 64 bytes of a row's codes
 constexpr int kPartialFloats = 23552;  // 92 KiB of partial sums per CTA
 constexpr int kRing = 3;             // tiles of codes and scales in shared memory, 36 KiB each at two chunks per warp
+
+// one chunk of eight tokens, 36 words for every 32 elements: the lanes' reads meet no bank twice
+constexpr int kStageWords = 8 * 4 * 36;
+constexpr int kStagePieces = kWarps * kStageWords / 4;
 
 // 16-byte pieces of a ring slot: the codes of 16 rows and `depth` chunks per warp, and their scales
 // (16 rows x 8 bytes, half of it used for blocks of 32)
@@ -92,19 +96,18 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
 }
 
 // What a lane brings of a chunk's activations, as they are in memory: 32 consecutive elements of one
-// column's token, zero behind the end.
+// token, zero behind the end.
 template <bool kFp32>
 struct Raw {
     uint32_t words[kFp32 ? 32 : 16];
 };
 
 template <bool kFp32>
-__device__ __forceinline__ Raw<kFp32> load_raw(const Params& p, int column, int columns, int chunk) {
-    constexpr int kParts = kFp32 ? 3 : 1, kWords = kFp32 ? 32 : 16, kSize = kFp32 ? 4 : 2;
+__device__ __forceinline__ Raw<kFp32> load_raw(const Params& p, int token, bool wanted, int chunk) {
+    constexpr int kWords = kFp32 ? 32 : 16, kSize = kFp32 ? 4 : 2;
     const int k0 = chunk * kChunk + 32 * (threadIdx.x & 3);
-    const bool present = column < columns && k0 < p.k;
-    const int token = present ? column / kParts : 0;
-    const uint8_t* row = reinterpret_cast<const uint8_t*>(p.x) + ((int64_t)token * p.ldx + k0) * kSize;
+    const bool present = wanted && k0 < p.k;
+    const uint8_t* row = reinterpret_cast<const uint8_t*>(p.x) + (present ? (int64_t)token * p.ldx + k0 : 0) * kSize;
     Raw<kFp32> raw;
 #pragma unroll
     for (int i = 0; i < kWords; ++i) raw.words[i] = 0;
@@ -126,11 +129,12 @@ __device__ __forceinline__ Raw<kFp32> load_raw(const Params& p, int column, int 
     return raw;
 }
 
-// One chunk's activations as mma B fragments, and the factor that undoes the chunk's power of two.
-// Lane (g, c) = (lane / 4, lane % 4) brings column g and elements 32 c ... 32 c + 31; step j of the
-// chunk's eight mma takes its elements 4 j ... 4 j + 3.  part: which of an fp32 element's three parts.
+// One chunk's activations as mma B fragments (fp32: three, of 11 bits each, the second to be multiplied
+// by 2^-11, the third by 2^-22), and the factor that undoes the chunk's power of two.  Lane (g, c) =
+// (lane / 4, lane % 4) brings column g and elements 32 c ... 32 c + 31; step j of the chunk's eight mma
+// takes its elements 4 j ... 4 j + 3.
 template <bool kFp32>
-__device__ __forceinline__ void make_fragment(const Raw<kFp32>& raw, int part, uint32_t (&b)[16], float& undo) {
+__device__ __forceinline__ void make_fragments(const Raw<kFp32>& raw, uint32_t (&b)[kFp32 ? 3 : 1][16], float& undo) {
     uint32_t top = 0;  // the largest magnitude's bits, as those of an fp32; a NaN's are larger than all numbers'
     if constexpr (kFp32) {
 #pragma unroll
@@ -149,20 +153,18 @@ __device__ __forceinline__ void make_fragment(const Raw<kFp32>& raw, int part, u
     const float scale = __uint_as_float((uint32_t)field << 23);
     undo = __uint_as_float((uint32_t)(254 - field) << 23);
     if constexpr (kFp32) {
-        undo *= part == 0 ? 1.0f : part == 1 ? 0x1p-11f : 0x1p-22f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             float lo = __uint_as_float(raw.words[2 * i]) * scale, hi = __uint_as_float(raw.words[2 * i + 1]) * scale;
 #pragma unroll
-            for (int step = 1; step < 3; ++step)
-                if (part >= step) {
-                    const float l = __half2float(__float2half_rn(lo)), h = __half2float(__float2half_rn(hi));
-                    // what the parts before left over, exactly; nothing behind an infinity or a NaN
-                    lo = fabsf(l) <= 65504.0f ? (lo - l) * 2048.0f : 0.0f;
-                    hi = fabsf(h) <= 65504.0f ? (hi - h) * 2048.0f : 0.0f;
-                }
-            const __half2 h = __floats2half2_rn(lo, hi);
-            b[i] = *reinterpret_cast<const uint32_t*>(&h);
+            for (int part = 0; part < 3; ++part) {
+                const __half2 h = __floats2half2_rn(lo, hi);
+                b[part][i] = *reinterpret_cast<const uint32_t*>(&h);
+                // what this part leaves over, exactly; nothing behind an infinity or a NaN
+                const float2 f = __half22float2(h);
+                lo = fabsf(f.x) <= 65504.0f ? (lo - f.x) * 2048.0f : 0.0f;
+                hi = fabsf(f.y) <= 65504.0f ? (hi - f.y) * 2048.0f : 0.0f;
+            }
         }
     } else {
         const uint32_t scale2 = (uint32_t)field << 7 | (uint32_t)field << 23;  // the power of two as a bf16 pair
@@ -171,7 +173,7 @@ __device__ __forceinline__ void make_fragment(const Raw<kFp32>& raw, int part, u
             uint32_t w;
             asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(w) : "r"(raw.words[i]), "r"(scale2));
             const __half2 h = __floats2half2_rn(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
-            b[i] = *reinterpret_cast<const uint32_t*>(&h);
+            b[0][i] = *reinterpret_cast<const uint32_t*>(&h);
         }
     }
 }
@@ -230,15 +232,14 @@ __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
     return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
 }
 
-// kTiles: 8-column tiles of the product that a CTA computes at a time; kDepth: chunks that a warp
-// keeps in registers.
+// kTiles: tiles of 8 tokens that a CTA computes at a time; kDepth: chunks that a warp keeps in registers.
 template <bool kFp32, int kTiles, int kDepth, bool kVector, int kBlock>
 __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params p) {
     extern __shared__ uint4 ring[];  // kVector: [slot]{codes [chunk][row half][thread], scales [warp][chunk][row]}
     constexpr int kSlot = slot_pieces(kDepth);
-    float* partial = reinterpret_cast<float*>(ring + (kVector ? kRing * kSlot : 0));  // [warp][column][row of the block]
+    // kVector: the ring; otherwise one chunk of eight tokens' activations per warp, on its way to the lanes
+    float* partial = reinterpret_cast<float*>(ring + (kVector ? kRing * kSlot : kStagePieces));  // [warp][token][row of the block]
     constexpr int kParts = kFp32 ? 3 : 1;
-    constexpr int kColumns = kTiles * 8;
     constexpr int kBlockShift = kBlock == 16 ? 4 : 5;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int share = blockIdx.x % p.split, group = blockIdx.x / p.split, groups = gridDim.x / p.split;
@@ -249,12 +250,9 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
     const int last_row = (int)((int64_t)p.rows * (group + 1) / groups);
     const int block_rows = p.rows_per_block;
     const int stride = (int)p.code_stride, scale_stride = (int)p.scale_stride;
-    // whole tokens per pass, so that the parts of a token meet in one pass
-    constexpr int kTokens = kColumns / kParts;
+    constexpr int kTokens = kTiles * 8;
     for (int token0 = 0; token0 < p.tokens; token0 += kTokens) {
-        const int column0 = token0 * kParts;
         const int tokens = min(kTokens, p.tokens - token0);
-        const int used = tokens * kParts;
         for (int row0 = first_row; row0 < last_row; row0 += block_rows) {
             const int row_count = min(block_rows, last_row - row0);
             const uint8_t* codes = p.codes + row0 * p.code_stride;
@@ -320,6 +318,39 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
             };
+            // Activations whose rows do not start on 16-byte boundaries, as those of an odd width: read by the
+            // whole warp side by side, 32 elements of a token at a time, and taken from shared memory.
+            auto load_staged = [&](int t, int chunk) {
+                uint32_t* mine = reinterpret_cast<uint32_t*>(ring) + warp * kStageWords;
+                const int here = chunk < chunks ? min(8, tokens - 8 * t) : 0;
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (j < here)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const int k = chunk * kChunk + q * 32 + lane;
+                            const int64_t at = (int64_t)(token0 + 8 * t + j) * p.ldx + k;
+                            uint32_t word = 0;
+                            if (k < p.k)
+                                word = kFp32 ? __ldg(reinterpret_cast<const uint32_t*>(p.x) + at)
+                                             : (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(p.x) + at);
+                            mine[j * 144 + q * 36 + lane] = word;
+                        }
+                __syncwarp();
+                Raw<kFp32> raw;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint4 w = g < here ? *reinterpret_cast<const uint4*>(mine + g * 144 + c * 36 + 4 * i) : make_uint4(0, 0, 0, 0);
+                    if constexpr (kFp32) {
+                        raw.words[4 * i] = w.x, raw.words[4 * i + 1] = w.y, raw.words[4 * i + 2] = w.z, raw.words[4 * i + 3] = w.w;
+                    } else {
+                        raw.words[2 * i] = w.x | w.y << 16;
+                        raw.words[2 * i + 1] = w.z | w.w << 16;
+                    }
+                }
+                return raw;
+            };
             int slot_now = 0;
             if constexpr (kVector) {
                 locate();
@@ -329,20 +360,21 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
                 load(0, 0);
             }
             for (int pass = 0; pass < passes; ++pass) {
-                uint32_t b[kDepth][kTiles][16];
+                uint32_t b[kDepth][kTiles][kParts][16];
                 float undo[kDepth][kTiles][2];
 #pragma unroll
                 for (int d = 0; d < kDepth; ++d)
 #pragma unroll
                     for (int t = 0; t < kTiles; ++t) {
-                        const int column = 8 * t + g, chunk = first_chunk + (pass * kDepth + d) * kWarps + warp;
-                        const Raw<kFp32> raw = load_raw<kFp32>(p, column0 + column, chunk < chunks ? column0 + used : 0, chunk);
+                        const int token = 8 * t + g, chunk = first_chunk + (pass * kDepth + d) * kWarps + warp;
                         float mine;
-                        make_fragment<kFp32>(raw, kFp32 ? (column0 + column) % 3 : 0, b[d][t], mine);
+                        make_fragments<kFp32>(kVector ? load_raw<kFp32>(p, token0 + token, token < tokens && chunk < chunks, chunk)
+                                                      : load_staged(t, chunk),
+                                              b[d][t], mine);
                         undo[d][t][0] = __shfl_sync(0xFFFFFFFFu, mine, 8 * c);
                         undo[d][t][1] = __shfl_sync(0xFFFFFFFFu, mine, 8 * c + 4);
                     }
-                float* slot = partial + (warp * used + 2 * c) * block_rows + g;
+                float* slot = partial + (warp * tokens + 2 * c) * block_rows + g;
 #pragma unroll 2
                 for (int tile = 0; tile < row_count; tile += 16, slot += 16) {
                     Piece now[kDepth][2];
@@ -374,9 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
                     float total[kTiles][4];
 #pragma unroll
                     for (int d = 0; d < kDepth; ++d) {
-                        float sum[kTiles][4];
-#pragma unroll
-                        for (int t = 0; t < kTiles; ++t) sum[t][0] = sum[t][1] = sum[t][2] = sum[t][3] = 0.0f;
+                        float sum[kTiles][kParts][4] = {};
                         uint32_t scale[2][2];
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
@@ -393,23 +423,29 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
                                 for (int i = 0; i < 4; ++i) a[h][i] = mul_half2(a[h][i], scale[h][j / 2]);
                             }
 #pragma unroll
-                            for (int t = 0; t < kTiles; ++t) {
-                                mma_f16(sum[t], a[0][0], a[1][0], a[0][1], a[1][1], b[d][t][4 * j], b[d][t][4 * j + 1]);
-                                mma_f16(sum[t], a[0][2], a[1][2], a[0][3], a[1][3], b[d][t][4 * j + 2], b[d][t][4 * j + 3]);
-                            }
+                            for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                                for (int part = 0; part < kParts; ++part) {
+                                    const uint32_t(&x)[16] = b[d][t][part];
+                                    mma_f16(sum[t][part], a[0][0], a[1][0], a[0][1], a[1][1], x[4 * j], x[4 * j + 1]);
+                                    mma_f16(sum[t][part], a[0][2], a[1][2], a[0][3], a[1][3], x[4 * j + 2], x[4 * j + 3]);
+                                }
                         }
 #pragma unroll
                         for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                total[t][i] = d == 0 ? sum[t][i] * undo[d][t][i & 1]
-                                                     : __fmaf_rn(sum[t][i], undo[d][t][i & 1], total[t][i]);
+                            for (int i = 0; i < 4; ++i) {
+                                float whole = sum[t][0][i];
+                                if constexpr (kFp32)
+                                    whole = __fmaf_rn(sum[t][2][i], 0x1p-22f, __fmaf_rn(sum[t][1][i], 0x1p-11f, whole));
+                                total[t][i] = d == 0 ? whole * undo[d][t][i & 1] : __fmaf_rn(whole, undo[d][t][i & 1], total[t][i]);
+                            }
                     }
 #pragma unroll
                     for (int t = 0; t < kTiles; ++t)
 #pragma unroll
                         for (int i = 0; i < 2; ++i)
-                            if (8 * t + 2 * c + i < used) {
+                            if (8 * t + 2 * c + i < tokens) {
                                 float* at = slot + (8 * t + i) * block_rows;
                                 if (pass > 0) {
                                     total[t][i] += at[0];
@@ -423,12 +459,12 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
             __syncthreads();
             if (p.split > 1) {
                 // the sums of this CTA's warps, in the place of its first warp's; then those of the cluster
-                for (int i = threadIdx.x; i < row_count * used; i += kThreads) {
-                    const int column = i / row_count, r = i - column * row_count;
+                for (int i = threadIdx.x; i < row_count * tokens; i += kThreads) {
+                    const int token = i / row_count, r = i - token * row_count;
                     float value = 0.0f;
 #pragma unroll
-                    for (int w = 0; w < kWarps; ++w) value += partial[(w * used + column) * block_rows + r];
-                    partial[column * block_rows + r] = value;
+                    for (int w = 0; w < kWarps; ++w) value += partial[(w * tokens + token) * block_rows + r];
+                    partial[token * block_rows + r] = value;
                 }
                 cooperative_groups::this_cluster().sync();
             }
@@ -436,15 +472,11 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
                 const int token = i / row_count, r = i - token * row_count;
                 float value = 0.0f;
                 if (p.split > 1) {
-#pragma unroll
-                    for (int part = kParts - 1; part >= 0; --part)
-                        for (int q = 0; q < p.split; ++q)
-                            value += cooperative_groups::this_cluster().map_shared_rank(partial, q)[(token * kParts + part) * block_rows + r];
+                    for (int q = 0; q < p.split; ++q)
+                        value += cooperative_groups::this_cluster().map_shared_rank(partial, q)[token * block_rows + r];
                 } else {
 #pragma unroll
-                    for (int part = kParts - 1; part >= 0; --part)
-#pragma unroll
-                        for (int w = 0; w < kWarps; ++w) value += partial[(w * used + token * kParts + part) * block_rows + r];
+                    for (int w = 0; w < kWarps; ++w) value += partial[(w * tokens + token) * block_rows + r];
                 }
                 value *= p.factor;
                 const int64_t n = row0 + r;
@@ -467,9 +499,8 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
 
 template <bool kFp32, int kTiles, int kDepth, bool kVector, int kBlock>
 int launch(Params p, cudaStream_t stream) {
-    constexpr int kTokens = kTiles * 8 / (kFp32 ? 3 : 1);
-    const int used = (p.tokens < kTokens ? p.tokens : kTokens) * (kFp32 ? 3 : 1);
-    constexpr size_t kRingBytes = kVector ? kRing * slot_pieces(kDepth) * sizeof(uint4) : 0;
+    const int used = p.tokens < kTiles * 8 ? p.tokens : kTiles * 8;
+    constexpr size_t kRingBytes = (kVector ? kRing * slot_pieces(kDepth) : kStagePieces) * sizeof(uint4);
     constexpr auto kKernel = packed_matvec_kernel<kFp32, kTiles, kDepth, kVector, kBlock>;
     cudaError_t error = allow_shared<kKernel>((int)kRingBytes + kPartialFloats * 4);
     if (error != cudaSuccess) return record_cuda_error(error);
@@ -508,11 +539,7 @@ int launch(Params p, cudaStream_t stream) {
 template <bool kVector, int kBlock>
 int dispatch(const Params& p, bool fp32, cudaStream_t s) {
     constexpr int kDepth = kVector ? 2 : 1;
-    if (fp32) {
-        if (p.tokens <= 2) return launch<true, 1, kDepth, kVector, kBlock>(p, s);
-        if (p.tokens <= 5) return launch<true, 2, 1, kVector, kBlock>(p, s);
-        return launch<true, 4, 1, kVector, kBlock>(p, s);
-    }
+    if (fp32) return launch<true, 1, 1, kVector, kBlock>(p, s);
     if (p.tokens <= 8) return launch<false, 1, kDepth, kVector, kBlock>(p, s);
     if (p.tokens <= 16) return launch<false, 2, 1, kVector, kBlock>(p, s);
     return launch<false, 4, 1, kVector, kBlock>(p, s);
