@@ -369,9 +369,53 @@ __global__ void __launch_bounds__(kSmallThreads, 2)
                        (int64_t)gridDim.x * gridDim.y * gridDim.z * kSmallThreads, kDim);
 }
 
-// The rows of a split sequence: sum of the splits' rows, each faded to the largest maximum.  One
-// CTA per (token, head), a quarter of the splits per warp, four channels per lane (head_dim 64: two
-// splits side by side in a warp).
+// The rows of a split sequence: sum of the splits' rows, each faded to the largest maximum.  Few
+// splits: one warp per (token, head), kDim / 32 channels per lane.
+template <int kDim>
+__global__ void __launch_bounds__(256) combine_few_kernel(const Params p, int rows_per_tile) {
+    constexpr int kOwn = kDim / 32;
+    wait_for_launcher();
+    const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Sequence s = sequence_of(p, b);
+    for (int i = blockIdx.x * 8 + warp; i < s.queries * p.heads; i += gridDim.x * 8) {
+        const int token = i / p.heads, head = i - token * p.heads;
+        const int row = token * p.group + head % p.group;
+        const int all = (visible_keys(p, s, row / rows_per_tile * rows_per_tile, rows_per_tile) + kKeys - 1) / kKeys;
+        const int chunk = split_chunk(p, all), splits = (all + chunk - 1) / max(chunk, 1);
+        if (splits <= 1) continue;  // written by its only split
+        const int64_t at = (int64_t)(s.first + token) * p.heads + head;
+        const float* rows = p.partial + at * p.splits * kDim + lane * kOwn;
+        const float2* stats =
+            reinterpret_cast<const float2*>(p.partial + (int64_t)p.tokens * p.heads * p.splits * kDim + at * p.splits * 2);
+        const float2 mine = lane < splits ? stats[lane] : make_float2(-INFINITY, 0.0f);
+        float most = mine.x;
+#pragma unroll
+        for (int m = 16; m; m >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, m));
+        const float weight = exp2_approx(mine.x - (most == -INFINITY ? 0.0f : most));
+        float total = mine.y * weight;
+#pragma unroll
+        for (int m = 16; m; m >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, m);
+        float value[kOwn] = {};
+#pragma unroll 4
+        for (int j = 0; j < splits; ++j) {
+            const float w = __shfl_sync(0xFFFFFFFFu, weight, j);
+            float v[kOwn];
+            if constexpr (kOwn == 4)
+                *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(rows + (int64_t)j * kDim);
+            else
+                *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(rows + (int64_t)j * kDim);
+#pragma unroll
+            for (int e = 0; e < kOwn; ++e) value[e] = __fmaf_rn(v[e], w, value[e]);
+        }
+        const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+        uint32_t* out = reinterpret_cast<uint32_t*>(p.out + at * kDim + lane * kOwn);
+#pragma unroll
+        for (int e = 0; e < kOwn; e += 2) out[e / 2] = pack_bf16(value[e] * inverse, value[e + 1] * inverse);
+    }
+}
+
+// Many splits: one CTA per (token, head), a quarter of the splits per warp, four channels per lane
+// (head_dim 64: two splits side by side in a warp).
 template <int kDim>
 __global__ void __launch_bounds__(128) combine_kernel(const Params p, int rows_per_tile) {
     wait_for_launcher();
@@ -471,10 +515,17 @@ struct Plan {
     size_t workspace;
 };
 
+static size_t workspace_of(int64_t tokens, int64_t heads, int64_t head_dim, int64_t splits) {
+    return splits > 1 ? (size_t)tokens * heads * splits * (head_dim + 2) * sizeof(float) : 0;
+}
+
 // Up to 32 rows per key/value head: the kernel for few rows, whose 16-row tiles read the keys once
 // each; more: the tensor-core kernel with its 256-row tiles.  Splits of the keys: few rows, enough
-// CTAs for two on every SM, runs of 4 to 16 tiles; many rows, only where there are fewer CTAs than
-// SMs, runs of at least 8 tiles.
+// CTAs for two on every SM, runs of 4 to 16 tiles.  Many rows: one CTA per SM at most, runs of at
+// least 8 tiles, and no more than pays: a split takes its share of about 0.93 us per 64 keys off the
+// time and adds the writing and reading of its partial rows at about 0.7 TB/s, so that the square
+// root of their quotient is the best number (8 x 32 heads over 32768 keys: 465 -> 35 us with 37 splits;
+// 4 x 128 tokens over 2048 keys: 46.5 us without, 57.8 with 3).
 static Plan make_plan(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t head_dim,
                       int64_t max_query, int64_t max_kv) {
     Plan plan;
@@ -485,17 +536,22 @@ static Plan make_plan(int64_t tokens, int64_t sequences, int64_t heads, int64_t 
     if (tiles * kv_heads > 65535) tiles = 65535 / kv_heads;
     plan.row_tiles = (int)tiles;
     const int64_t all = (max_kv + kKeys - 1) / kKeys, lists = sequences * kv_heads * tiles;
-    int64_t chunk;
+    int64_t chunk, splits;
     if (plan.wide) {
-        chunk = lists >= sms ? all : (all * lists + sms - 1) / sms;
+        const double whole = 0.93e-6 * (double)all, each = (double)(tokens * heads * (head_dim + 2) * 4) / 0.7e12;
+        const int64_t most = (sms + lists - 1) / lists, best = (int64_t)sqrt(whole / each);
+        const int64_t wanted = best < 1 || most < 2 ? 1 : best < most ? best : most;
+        chunk = (all + wanted - 1) / wanted;
         chunk = ((chunk < 8 ? 8 : chunk) + 1) / 2 * 2;  // whole 128-key tiles
+        splits = (all + chunk - 1) / chunk;
     } else {
         chunk = (all * lists + 2 * sms - 1) / (2 * sms);
         chunk = chunk < 4 ? 4 : chunk > 16 ? 16 : chunk;
+        splits = (all + chunk - 1) / chunk;
     }
     plan.chunk = (int)chunk;
-    plan.splits = (int)((all + chunk - 1) / chunk);
-    plan.workspace = plan.splits > 1 ? (size_t)tokens * heads * plan.splits * (head_dim + 2) * sizeof(float) : 0;
+    plan.splits = (int)splits;
+    plan.workspace = workspace_of(tokens, heads, head_dim, splits);
     return plan;
 }
 
@@ -524,9 +580,15 @@ int launch(const Params& p, const Plan& plan, const CUtensorMap& k_map, const CU
     }
     if (plan.splits == 1) return UE5M3_OK;
     int64_t blocks = max_query * p.heads;
-    if (blocks > 65535) blocks = 65535;
-    error = launch_after(combine_kernel<kDim>, dim3((unsigned)blocks, p.sequences), 128, 0, stream, true, p,
-                         plan.wide ? kWideRows : kRows);
+    const int tile_rows = plan.wide ? kWideRows : kRows;
+    if (plan.splits <= 16) {
+        blocks = (blocks + 7) / 8;
+        if (blocks > 65535) blocks = 65535;
+        error = launch_after(combine_few_kernel<kDim>, dim3((unsigned)blocks, p.sequences), 256, 0, stream, true, p, tile_rows);
+    } else {
+        if (blocks > 65535) blocks = 65535;
+        error = launch_after(combine_kernel<kDim>, dim3((unsigned)blocks, p.sequences), 128, 0, stream, true, p, tile_rows);
+    }
     return record_cuda_error(error);
 }
 

@@ -554,12 +554,24 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                                              __uint_as_float(x[8 * e + 2 * k + 1]) * inverse);
                         to[e] = make_uint4(w[0], w[1], w[2], w[3]);
                     }
-                } else if (present) {
-                    float4* to = reinterpret_cast<float4*>(p.partial + (out_at * p.splits + blockIdx.x) * kDim + 32 * i);
+                } else if (splits > 1) {
+                    // a thread has a row, a store wants neighbouring pieces: through this tile's part of Q, which
+                    // is read no more
+                    unsigned char* turn = smem + Shared::kQ + t * kTileBytes + (warp % 4) * 4096;
+                    __syncwarp();
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        to[e] = make_float4(__uint_as_float(x[4 * e]), __uint_as_float(x[4 * e + 1]),
-                                            __uint_as_float(x[4 * e + 2]), __uint_as_float(x[4 * e + 3]));
+                        *reinterpret_cast<uint4*>(turn + lane * 128 + ((e ^ (lane & 7)) << 4)) =
+                            make_uint4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
+                    __syncwarp();
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int from = e * 4 + lane / 8, piece = lane % 8;
+                        const int64_t row_at = __shfl_sync(0xFFFFFFFFu, present ? out_at : -1, from);
+                        if (row_at >= 0)
+                            *reinterpret_cast<uint4*>(p.partial + (row_at * p.splits + blockIdx.x) * kDim + 32 * i + 4 * piece) =
+                                *reinterpret_cast<const uint4*>(turn + from * 128 + ((piece ^ (from & 7)) << 4));
+                    }
                 }
             }
             if (splits > 1 && present) {
