@@ -502,6 +502,17 @@ def test_sample_tails_without_weight(vocabulary):
         check_sample(logits, uniforms, **settings)
 
 
+@pytest.mark.parametrize("vocabulary", [3000, 40000])
+@pytest.mark.parametrize("top_k,top_p", [(0, 0.5), (0, 0.999), (700, 0.9), (2500, 0.9), (2500, 1.0)])
+def test_sample_subnormal_logits_and_temperature(vocabulary, top_k, top_p):
+    # all logits within one of the first bins, most of them without weight
+    generator = torch.Generator().manual_seed(vocabulary + top_k)
+    steps = torch.randint(0, 400, (2, vocabulary), generator=generator)
+    logits = (steps.double() * -2.0 ** -149).float()
+    assert logits.unique().numel() == 400
+    check_sample(logits, torch.tensor([0.3, 0.97]), temperature=2.0 ** -148, top_k=top_k, top_p=top_p)
+
+
 def test_sample_strided_rows():
     from ue5m3_fp4 import serving
 

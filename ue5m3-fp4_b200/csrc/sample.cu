@@ -311,10 +311,11 @@ __device__ Found first_step(cg::cluster_group& cluster, Shared& s, const float* 
     return scan_bins<kWeighted>(cluster, s, buffer, need, share);
 }
 
-// In the first step's bins: weights of zero, which are not counted, lie in the last one only.
+// Whether the first step counted an element that is not masked.  Weights of zero lie in its last bin,
+// save at temperatures so small that the bins' scale is held back.
 template <bool kWeighted>
-__device__ __forceinline__ bool counted(const Row& row, float v, uint32_t bin) {
-    return !kWeighted || bin < kBins - 1 || weight_of(row, v) != 0;
+__device__ __forceinline__ bool counted(const Row& row, float v) {
+    return !kWeighted || weight_of(row, v) != 0;
 }
 
 // This CTA's elements that `look`, a glance at the logit, and `take` name (the caller has counted them:
@@ -370,7 +371,7 @@ __device__ uint64_t search(cg::cluster_group& cluster, Shared& s, const float* d
     uint64_t low = floor, high = ~0ull;
     if (found.inside <= kCandidates) {
         gather(s, data, count, base, [&](float v) { return first_bin(row, v) == found.bin; },
-               [&](float v, uint64_t rank) { return rank >= floor && counted<kWeighted>(row, v, found.bin); });
+               [&](float v, uint64_t rank) { return rank >= floor && counted<kWeighted>(row, v); });
     } else {
         if (threadIdx.x == 0) {
             s.low = ~0ull;
@@ -636,7 +637,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
     }
     if (few) {
         gather(s, data, count, first, [&](float v) { return first_bin(row, v) <= found.bin; },
-               [&](float v, uint64_t) { return row_total == 0 || counted<true>(row, v, first_bin(row, v)); });
+               [&](float v, uint64_t) { return row_total == 0 || counted<true>(row, v); });
         cluster.sync();
         if (rank_in_cluster == 0)
             finish_few(cluster, s, p, row, row_index, row_total ? 0 : top_k, top_p, least, row_total);
