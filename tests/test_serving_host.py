@@ -44,13 +44,24 @@ def test_decode_factor_follows_the_quantizer():
     assert decode_factor(0.11, 448.0) == float(1.0 / (torch.tensor(2688.0) / amax))
 
 
+def test_packed_linear_state_holds_the_tensor_scale():
+    saved = PackedFP4Linear(packed(), torch.zeros(8))
+    saved.tensor_amax, saved.scale_target = 0.3, 256.0
+    loaded = PackedFP4Linear(packed(), torch.ones(8))
+    loaded.load_state_dict(saved.state_dict())
+    assert (loaded.tensor_amax, loaded.scale_target) == (0.3, 256.0) and not loaded.bias.any()
+    without = {name: value for name, value in saved.state_dict().items() if name != "_extra_state"}
+    with pytest.raises(RuntimeError, match="_extra_state"):
+        loaded.load_state_dict(without)
+
+
 def test_packed_linear_takes_frozen_weights_only():
     with pytest.raises(TypeError):
         PackedFP4Linear(torch.zeros(4, 4))
     with pytest.raises(ValueError, match="bias"):
         PackedFP4Linear(packed(), torch.zeros(3))
     layer = PackedFP4Linear(packed(), torch.zeros(8))
-    assert set(layer.state_dict()) == {"codes", "scales", "bias"}
+    assert set(layer.state_dict()) == {"codes", "scales", "bias", "_extra_state"}
     with pytest.raises(ValueError, match="input width"):
         layer(torch.ones(1, 31))
     model = torch.nn.Sequential(UE5M3Linear(64, 64, module_name="a"), torch.nn.Linear(64, 64))

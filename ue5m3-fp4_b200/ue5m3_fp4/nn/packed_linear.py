@@ -17,7 +17,7 @@ from ue5m3_fp4.packed import PackedFP4Tensor
 
 class PackedFP4Linear(torch.nn.Module):
     """``x @ W.T + bias`` with a packed weight; no gradients.  Reads 0.5 byte per weight element and
-    one byte per block; the cost grows with every 32 rows of ``x``."""
+    one byte per block; the cost grows with every 32 rows of bf16 ``x`` and every 8 of fp32."""
 
     def __init__(self, weight: PackedFP4Tensor, bias: Tensor | None = None) -> None:
         super().__init__()
@@ -39,6 +39,16 @@ class PackedFP4Linear(torch.nn.Module):
         if not isinstance(module, UE5M3Linear):
             raise TypeError("from_frozen expects a UE5M3Linear")
         return cls(module.packed_weight(), module.bias)
+
+    def get_extra_state(self) -> Tensor:
+        """The tensor scale: codes and block scales mean nothing without it."""
+
+        return torch.tensor([self.tensor_amax, self.scale_target], dtype=torch.float64)
+
+    def set_extra_state(self, state: Tensor) -> None:
+        if not isinstance(state, Tensor) or tuple(state.shape) != (2,):
+            raise ValueError("the state of a packed linear holds its tensor amax and its scale target")
+        self.tensor_amax, self.scale_target = (float(value) for value in state.tolist())
 
     def forward(self, inputs: Tensor) -> Tensor:
         from ue5m3_fp4.serving import packed_matvec
