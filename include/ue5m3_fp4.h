@@ -368,8 +368,9 @@ int ue5m3_gemm_fp4_fallback_ws(const uint8_t *a_codes, const uint8_t *a_sf_raw, 
  * [rows, ceil(cols/2)] and UE5M3 scale bytes [rows, ceil(cols/block)] (two_d == 0) or
  * [ceil(rows/block), ceil(cols/block)], as ue5m3_quantize writes them.  dec is the tensor-scale
  * decode factor (formats.py:408).  fp32 sums in an order fixed by the sizes; out is rounded once.
- * ldx / ldo: row strides of x / out in elements.  Any sizes; code rows on 16-byte boundaries
- * (ceil(cols/2) % 16 == 0) are read with wide loads.  The cost grows with tokens / 32.
+ * ldx / ldo: row strides of x / out in elements.  Up to 2^24 tokens, 2^30 rows and 2^22
+ * cols; widths that are a multiple of 128 (codes on a 16-byte, scales on an 8-byte boundary) are read
+ * with wide copies.  The cost grows with every 32 bf16 tokens and every 8 fp32 ones.
  */
 int ue5m3_packed_matvec(const void *x, int x_dtype, int64_t tokens, int64_t ldx,
                         const uint8_t *codes, const uint8_t *scales, int64_t rows, int64_t cols,

@@ -86,8 +86,9 @@ def packed_matvec(
     ``scales`` as ``quantize_packed`` and ``PackedFP4Tensor`` hold them) for a few rows of bf16 or
     fp32 activations, which are not quantized.  Sums are fp32; the result is rounded once, to
     ``out_dtype`` (default: that of ``x``).  Any ``rows`` and ``cols``; the last axis of ``x`` must be
-    contiguous.  The cost grows with every 32 rows of bf16 ``x`` (8 rows are read at the cost of one):
-    for whole prompts use the GEMM."""
+    contiguous.  The cost grows with every 32 rows of bf16 ``x`` and every 8 of fp32 (8 rows are read at
+    the cost of one): for whole prompts use the GEMM.  At most 2^24 rows of ``x``, 2^30 ``rows`` and
+    2^22 ``cols``."""
 
     _require_cuda(x, "x")
     _no_gradient(x, bias)
@@ -253,7 +254,9 @@ def paged_attention(
     need = _workspace_bytes(tokens, sequences, heads, kv_heads, head_dim, max_query_length, max_kv_length)
     # from the current stream's pool, for this call alone: calls and captured graphs share nothing
     workspace = q.new_empty(need // 2) if need else None
-    _call(_native.load().ue5m3_paged_attention, "ue5m3_paged_attention", 2 if need else 1, index, q.data_ptr(),
+    # kernels: attention, the rows of split sequences, new keys ahead of the kernel for many rows
+    launches = 1 + (need > 0) + (k_pointer is not None and max_query_length * (heads // kv_heads) > 32)
+    _call(_native.load().ue5m3_paged_attention, "ue5m3_paged_attention", launches, index, q.data_ptr(),
           *_strides("q", q), tokens, heads, ctypes.byref(cache), kv_lengths.data_ptr(), query_starts.data_ptr(),
           max_query_length, max_kv_length, scale, k_pointer, *k_strides, v_pointer, *v_strides, out.data_ptr(),
           zero_tail, None if workspace is None else workspace.data_ptr(), need, b200.gemm_status(q.device).data_ptr())
