@@ -21,6 +21,11 @@
 // hundred, a peaked nucleus), these are gathered and the rest happens among them in one CTA.
 // Otherwise the elements of the bin that holds the threshold are ranked against one another, or the
 // search goes on inside it with bins of the 64-bit rank (many equal logits).
+//
+// Measured (fp32): one row of 131072, top-k and top-p: 13.3 us, the steps of eight CTAs that wait
+// for one another at four cluster barriers; 64 rows of 131072 with top-p alone: 111 us, against 5 us for the bytes and
+// 6.5 us for the exponentials at the rate of the fp64 pipe: two CTAs fit on an SM, so the 512 take
+// almost two turns, and within a turn the passes over a slice wait for shared memory and atomics.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
