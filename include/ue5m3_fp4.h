@@ -370,12 +370,16 @@ int ue5m3_gemm_fp4_fallback_ws(const uint8_t *a_codes, const uint8_t *a_sf_raw, 
  * decode factor (formats.py:408).  fp32 sums in an order fixed by the sizes; out is rounded once.
  * ldx / ldo: row strides of x / out in elements.  Up to 2^24 tokens, 2^30 rows and 2^22
  * cols; widths that are a multiple of 128 (codes on a 16-byte, scales on an 8-byte boundary) are read
- * with wide copies.  The cost grows with every 32 bf16 tokens and every 8 fp32 ones.
+ * with wide copies.  More than 8 tokens take a workspace (16-byte aligned, contents free) of
+ * ue5m3_packed_matvec_workspace_bytes bytes, 0 up to 8, in use until the call's kernels are done; the
+ * weight is then read once for every 64 bf16 or 32 fp32 tokens.
  */
 int ue5m3_packed_matvec(const void *x, int x_dtype, int64_t tokens, int64_t ldx,
                         const uint8_t *codes, const uint8_t *scales, int64_t rows, int64_t cols,
                         int block, int two_d, float dec, const void *bias, int bias_dtype,
-                        void *out, int out_dtype, int64_t ldo, void *stream);
+                        void *out, int out_dtype, int64_t ldo, void *workspace,
+                        size_t workspace_bytes, void *stream);
+size_t ue5m3_packed_matvec_workspace_bytes(int x_dtype, int64_t tokens, int64_t cols);
 
 /*
  * A paged key/value cache (host struct of device pointers): bf16 pages [pages][page_size][kv_heads]

@@ -57,8 +57,9 @@ def check_matvec(x, codes, scales, rows, cols, block, two_d, *, bias=None, out_d
     if bias is not None:
         expect, size = expect + bias.double(), size + bias.double().abs()
     # 128 products per tensor-core sum in eight steps of at most 2^-21 of the sum of magnitudes each,
-    # then one fp32 addition per further chunk and warp, factor and bias
-    additions = math.ceil(cols / 2048) + 20
+    # then one fp32 addition per further chunk and warp (16 warps share the axis up to eight tokens, at
+    # least two above), factor and bias
+    additions = math.ceil(cols / (2048 if flat.shape[0] <= 8 else 256)) + 20
     tolerance = size * (8 * 2.0 ** -21 + additions * 2.0 ** -24)
     tolerance = tolerance + expect.abs() * (2.0 ** -8 if got.dtype is torch.bfloat16 else 2.0 ** -24) + 1e-38
     error = (got.cpu().double().reshape(-1, rows) - expect).abs()
@@ -76,6 +77,70 @@ def test_matvec_matches_the_definition(tokens, rows, cols, block, two_d, dtype):
     codes, scales = packed_weight(rows, cols, block, two_d, seed=cols)
     bias = torch.randn(rows, generator=g).to(DTYPES[dtype]) if rows % 2 else None
     check_matvec(x, codes, scales, rows, cols, block, two_d, bias=bias)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("block,two_d", [(16, True), (32, False)])
+@pytest.mark.parametrize("tokens,rows,cols", [(9, 128, 128), (12, 1, 33), (16, 129, 256), (33, 257, 1152), (32, 1000, 1003),
+                                              (65, 64, 2560), (130, 40, 4224), (100, 300, 77), (40, 515, 20096)])
+def test_matvec_of_many_tokens(tokens, rows, cols, block, two_d, dtype):
+    """Token tiles, blocks of 128 rows, and reduction axes shared by one to eight CTAs."""
+
+    g = torch.Generator().manual_seed(tokens + cols)
+    wide = torch.randn(tokens, cols + 5, generator=g).to(DTYPES[dtype])
+    codes, scales = packed_weight(rows, cols, block, two_d, seed=cols)
+    bias = torch.randn(rows, generator=g) if rows % 2 else None
+    for x in (wide[:, :cols].contiguous(), wide[:, 1:cols + 1]):  # rows on 16-byte boundaries, and not
+        got = check_matvec(x, codes, scales, rows, cols, block, two_d, bias=bias)
+        assert torch.equal(got, check_matvec(x, codes, scales, rows, cols, block, two_d, bias=bias))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_matvec_of_many_tokens_keeps_rows_apart(dtype):
+    """A row's infinities, NaN and magnitudes are its own; the others are as they are without them."""
+
+    from ue5m3_fp4 import serving
+
+    rows, cols = 150, 700
+    codes, scales = packed_weight(rows, cols, 16, False, seed=6)
+    x = torch.randn(45, cols, generator=torch.Generator().manual_seed(8)).to(DTYPES[dtype])
+    kw = dict(rows=rows, cols=cols, block_size=16, two_dimensional=False, tensor_amax=1.0)
+    plain = serving.packed_matvec(x.cuda(), codes.cuda(), scales.cuda(), **kw)
+    mixed = x.clone()
+    mixed[3, 17], mixed[9], mixed[20, 699], mixed[44] = math.inf, x[9] * 2.0 ** 90, math.nan, x[44] * 2.0 ** -90
+    got = serving.packed_matvec(mixed.cuda(), codes.cuda(), scales.cuda(), **kw)
+    same = [t for t in range(45) if t not in (3, 9, 20, 44)]
+    assert torch.equal(got[same], plain[same])
+    assert not bool(got[3].isfinite().any()) and bool(got[20].isnan().all())
+    assert torch.equal(got[9], plain[9] * 2.0 ** 90) and torch.equal(got[44], plain[44] * 2.0 ** -90)
+
+
+def test_matvec_of_many_tokens_in_two_graphs_and_on_two_streams():
+    from ue5m3_fp4 import serving
+
+    rows, cols = 300, 2048
+    codes, scales = (t.cuda() for t in packed_weight(rows, cols, 32, False, seed=7))
+    kw = dict(rows=rows, cols=cols, block_size=32, two_dimensional=False, tensor_amax=1.0)
+    inputs = [torch.randn(tokens, cols, device="cuda", dtype=torch.bfloat16) for tokens in (20, 60)]
+    expect = [serving.packed_matvec(x, codes, scales, **kw) for x in inputs]
+    graphs, outs = [], []
+    for x in inputs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(serving.packed_matvec(x, codes, scales, **kw))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for turn in range(3):
+        for out in outs:
+            out.zero_()
+        torch.cuda.synchronize()
+        eager = []
+        for graph, stream, x in zip(graphs, streams, reversed(inputs)):
+            with torch.cuda.stream(stream):
+                graph.replay()
+                eager.append(serving.packed_matvec(x, codes, scales, **kw))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, expect))
+        assert all(torch.equal(a, b) for a, b in zip(eager, reversed(expect)))
 
 
 def test_matvec_takes_every_scale_byte_and_code():

@@ -126,7 +126,8 @@ def test_library_refuses_bad_arguments():
 
     def matvec(**over):
         a = dict(x=fake, x_dtype=0, tokens=1, ldx=64, codes=fake, scales=fake, rows=8, cols=64, block=16, two_d=0, dec=1.0,
-                 bias=None, bias_dtype=0, out=fake, out_dtype=0, ldo=8) | over
+                 bias=None, bias_dtype=0, out=fake, out_dtype=0, ldo=8, workspace=None,
+                 workspace_bytes=0) | over
         return lib.ue5m3_packed_matvec(*a.values(), None)
 
     assert matvec(x=None) == matvec(codes=None) == matvec(scales=None) == matvec(out=None) == 1
@@ -134,6 +135,12 @@ def test_library_refuses_bad_arguments():
     assert matvec(block=8) == 2
     assert matvec(x=odd) == matvec(out=odd) == matvec(bias=odd) == 4
     assert matvec(cols=1 << 23, ldx=1 << 23) == 8
+    # more than eight tokens take a workspace
+    need = lib.ue5m3_packed_matvec_workspace_bytes(0, 9, 64)
+    assert need > 0 and lib.ue5m3_packed_matvec_workspace_bytes(0, 8, 64) == 0
+    assert lib.ue5m3_packed_matvec_workspace_bytes(1, 9, 64) > need
+    assert matvec(tokens=9) == matvec(tokens=9, workspace=fake, workspace_bytes=need - 1) == 7
+    assert matvec(tokens=9, workspace=fake + 8, workspace_bytes=need) == 4
 
     def attention(cache_over=None, **over):
         c = dict(k_pages=fake, v_pages=fake, k_page_stride=1024, k_slot_stride=64, k_head_stride=64, v_page_stride=1024,

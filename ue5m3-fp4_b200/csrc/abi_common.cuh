@@ -17,6 +17,11 @@ int check_launch();
 int record_cuda_error(cudaError_t error);
 void record_error_text(const char* text);
 
+// Programmatic launches: the next kernel of a call starts while this one ends, and waits for it
+// where it first reads what this one writes.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_launcher() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // Dynamic shared memory above 48 KiB has to be asked for once per kernel and device.
 template <auto kKernel>
 cudaError_t allow_shared(int bytes) {

@@ -34,6 +34,7 @@ namespace matvec {
 
 constexpr int kWarps = 16;
 constexpr int kThreads = kWarps * 32;
+constexpr int kFewTokens = 8;          // up to here a CTA converts the activations itself
 constexpr int kChunk = 128;          // reduction elements of one warp step: 64 bytes of a row's codes
 constexpr int kPartialFloats = 23552;  // 92 KiB of partial sums per CTA
 constexpr int kRing = 3;             // tiles of codes and scales in shared memory, 36 KiB each at two chunks per warp
@@ -124,6 +125,41 @@ __device__ __forceinline__ Raw<kFp32> load_raw(const Params& p, int token, bool 
                 raw.words[i] = in ? __ldg(reinterpret_cast<const uint32_t*>(row) + i) : 0;
             else
                 raw.words[i / 2] |= (in ? (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(row) + i) : 0u) << (16 * (i & 1));
+        }
+    }
+    return raw;
+}
+
+// The same by a whole warp, for activations whose rows do not start on 16-byte boundaries, as those of
+// an odd width: tokens token0 ... token0 + here - 1 (eight at most) side by side, 32 elements at a time,
+// through `mine` (kStageWords of shared memory).
+template <bool kFp32>
+__device__ __forceinline__ Raw<kFp32> load_staged(const Params& p, int token0, int here, int chunk, uint32_t* mine) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (j < here)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int k = chunk * kChunk + q * 32 + lane;
+                const int64_t at = (int64_t)(token0 + j) * p.ldx + k;
+                uint32_t word = 0;
+                if (k < p.k)
+                    word = kFp32 ? __ldg(reinterpret_cast<const uint32_t*>(p.x) + at)
+                                 : (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(p.x) + at);
+                mine[j * 144 + q * 36 + lane] = word;
+            }
+    __syncwarp();
+    Raw<kFp32> raw;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint4 w = g < here ? *reinterpret_cast<const uint4*>(mine + g * 144 + c * 36 + 4 * i) : make_uint4(0, 0, 0, 0);
+        if constexpr (kFp32) {
+            raw.words[4 * i] = w.x, raw.words[4 * i + 1] = w.y, raw.words[4 * i + 2] = w.z, raw.words[4 * i + 3] = w.w;
+        } else {
+            raw.words[2 * i] = w.x | w.y << 16;
+            raw.words[2 * i + 1] = w.z | w.w << 16;
         }
     }
     return raw;
@@ -232,8 +268,41 @@ __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
     return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
 }
 
-// kTiles: tiles of 8 tokens that a CTA computes at a time; kDepth: chunks that a warp keeps in registers.
-template <bool kFp32, int kTiles, int kDepth, bool kVector, int kBlock>
+// The scales of a lane's two rows (g and g + 8 of a 16-row tile) in one chunk, as fp16 pairs: [row][half]
+template <int kBlock>
+__device__ __forceinline__ void scale_pairs(const Piece (&piece)[2], uint32_t (&scale)[2][2]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        scale[h][0] = scale_half2(kBlock == 16 ? piece[h].scales & 0xFFu : piece[h].scales);
+        scale[h][1] = kBlock == 16 ? scale_half2(piece[h].scales >> 8) : scale[h][0];
+    }
+}
+
+// step j of the chunk's four: eight elements of each of the two rows
+template <int kBlock>
+__device__ __forceinline__ void decode(const Piece (&piece)[2], const uint32_t (&scale)[2][2], int j, uint32_t (&a)[2][4]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        e2m1x8_to_half2(word_of(piece[h].codes, j), a[h]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[h][i] = mul_half2(a[h][i], scale[h][j / 2]);
+    }
+}
+
+__device__ __forceinline__ void store(const Params& p, int token, int64_t row, float value) {
+    value *= p.factor;
+    if (p.bias)
+        value += p.bias_fp32 ? reinterpret_cast<const float*>(p.bias)[row]
+                             : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.bias)[row]);
+    const int64_t at = token * p.ldo + row;
+    if (p.out_fp32)
+        reinterpret_cast<float*>(p.out)[at] = value;
+    else
+        reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(value);
+}
+
+// Up to eight tokens.  kDepth: chunks that a warp keeps in registers.
+template <bool kFp32, int kDepth, bool kVector, int kBlock>
 __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params p) {
     extern __shared__ uint4 ring[];  // kVector: [slot]{codes [chunk][row half][thread], scales [warp][chunk][row]}
     constexpr int kSlot = slot_pieces(kDepth);
@@ -250,258 +319,196 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
     const int last_row = (int)((int64_t)p.rows * (group + 1) / groups);
     const int block_rows = p.rows_per_block;
     const int stride = (int)p.code_stride, scale_stride = (int)p.scale_stride;
-    constexpr int kTokens = kTiles * 8;
-    for (int token0 = 0; token0 < p.tokens; token0 += kTokens) {
-        const int tokens = min(kTokens, p.tokens - token0);
-        for (int row0 = first_row; row0 < last_row; row0 += block_rows) {
-            const int row_count = min(block_rows, last_row - row0);
-            const uint8_t* codes = p.codes + row0 * p.code_stride;
-            const int scale_row0 = row0 >> p.row_shift;
-            const uint8_t* scales = p.scales + scale_row0 * p.scale_stride;
-            // rows from which 3 bytes back and 19 bytes further on are still inside the weight
-            const bool inner = row0 * p.code_stride >= 3 && (int64_t)(p.rows - row0 - row_count) * p.code_stride >= 20;
-            // Pieces of the tiles to come.  Wide rows: codes and scales wait in a ring in shared memory,
-            // kRing - 1 tiles ahead: the codes in the slots of the lane that decodes them, the scale bytes
-            // of a row's chunk side by side.  A row or chunk behind the end is not copied: what its slot
-            // holds is finite, and meets zeros or is not stored.  Other rows: in registers, one tile ahead.
-            Piece next[kDepth][2];
-            auto load = [&](int pass, int tile) {
+    const int tokens = p.tokens;
+    for (int row0 = first_row; row0 < last_row; row0 += block_rows) {
+        const int row_count = min(block_rows, last_row - row0);
+        const uint8_t* codes = p.codes + row0 * p.code_stride;
+        const int scale_row0 = row0 >> p.row_shift;
+        const uint8_t* scales = p.scales + scale_row0 * p.scale_stride;
+        // rows from which 3 bytes back and 19 bytes further on are still inside the weight
+        const bool inner = row0 * p.code_stride >= 3 && (int64_t)(p.rows - row0 - row_count) * p.code_stride >= 20;
+        // Pieces of the tiles to come.  Wide rows: codes and scales wait in a ring in shared memory,
+        // kRing - 1 tiles ahead: the codes in the slots of the lane that decodes them, the scale bytes
+        // of a row's chunk side by side.  A row or chunk behind the end is not copied: what its slot
+        // holds is finite, and meets zeros or is not stored.  Other rows: in registers, one tile ahead.
+        Piece next[kDepth][2];
+        auto load = [&](int pass, int tile) {
+#pragma unroll
+            for (int d = 0; d < kDepth; ++d) {
+                // a chunk behind the end is read as the row's last bytes
+                const int byte = min((first_chunk + (pass * kDepth + d) * kWarps + warp) * (kChunk / 2) + 16 * c, stride - 1);
+                const int block = byte * 2 >> kBlockShift;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int row = min(tile + g + 8 * h, row_count - 1);
+                    const uint32_t code = row * stride + byte;
+                    const uint32_t scale = ((row0 + row >> p.row_shift) - scale_row0) * scale_stride;
+                    const uint32_t last = scale + scale_stride - 1;
+                    if (inner)
+                        next[d][h] = load_piece<Loads::kWords, kBlock>(codes, scales, code, scale + block, last, 0);
+                    else
+                        next[d][h] = load_piece<Loads::kBytes, kBlock>(codes, scales, code, scale + block, last, stride - byte);
+                }
+            }
+        };
+        // the (pass, tile) that is copied next, and where this lane's first row of it lies
+        int ahead_pass = 0, ahead_tile = 0;
+        const uint8_t *ahead_codes = nullptr, *ahead_scales = nullptr;
+        auto locate = [&]() {
+            const int chunk = first_chunk + ahead_pass * kDepth * kWarps + warp;
+            ahead_codes = codes + (int64_t)(ahead_tile + g) * stride + chunk * (kChunk / 2) + 16 * c;
+            ahead_scales = scales + chunk * (kChunk / kBlock);
+        };
+        auto copy_ahead = [&](int slot) {
+            if (ahead_pass < passes) {
+                uint4* to = ring + slot * kSlot + threadIdx.x;
+                uint8_t* scales_to = reinterpret_cast<uint8_t*>(ring + slot * kSlot + kDepth * 2 * kThreads) + warp * kDepth * 128;
+                const int row = ahead_tile + g + 8 * c;  // lanes 0 and 1 of a row bring the scales of it and the one 8 on
+                const int scale_row = (row0 + row >> p.row_shift) - scale_row0;
 #pragma unroll
                 for (int d = 0; d < kDepth; ++d) {
-                    // a chunk behind the end is read as the row's last bytes
-                    const int byte = min((first_chunk + (pass * kDepth + d) * kWarps + warp) * (kChunk / 2) + 16 * c, stride - 1);
-                    const int block = byte * 2 >> kBlockShift;
+                    if (first_chunk + (ahead_pass * kDepth + d) * kWarps + warp >= chunks) continue;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int row = min(tile + g + 8 * h, row_count - 1);
-                        const uint32_t code = row * stride + byte;
-                        const uint32_t scale = ((row0 + row >> p.row_shift) - scale_row0) * scale_stride;
-                        const uint32_t last = scale + scale_stride - 1;
-                        if (inner)
-                            next[d][h] = load_piece<Loads::kWords, kBlock>(codes, scales, code, scale + block, last, 0);
-                        else
-                            next[d][h] = load_piece<Loads::kBytes, kBlock>(codes, scales, code, scale + block, last, stride - byte);
-                    }
+                    for (int h = 0; h < 2; ++h)
+                        if (ahead_tile + g + 8 * h < row_count)
+                            copy_async<16>(to + (d * 2 + h) * kThreads, ahead_codes + h * 8 * stride + d * kWarps * (kChunk / 2));
+                    if (c < 2 && row < row_count)
+                        copy_async<kChunk / kBlock>(scales_to + d * 128 + (g + 8 * c) * (kChunk / kBlock),
+                                                    ahead_scales + scale_row * scale_stride + d * kWarps * (kChunk / kBlock));
                 }
-            };
-            // the (pass, tile) that is copied next, and where this lane's first row of it lies
-            int ahead_pass = 0, ahead_tile = 0;
-            const uint8_t *ahead_codes = nullptr, *ahead_scales = nullptr;
-            auto locate = [&]() {
-                const int chunk = first_chunk + ahead_pass * kDepth * kWarps + warp;
-                ahead_codes = codes + (int64_t)(ahead_tile + g) * stride + chunk * (kChunk / 2) + 16 * c;
-                ahead_scales = scales + chunk * (kChunk / kBlock);
-            };
-            auto copy_ahead = [&](int slot) {
-                if (ahead_pass < passes) {
-                    uint4* to = ring + slot * kSlot + threadIdx.x;
-                    uint8_t* scales_to = reinterpret_cast<uint8_t*>(ring + slot * kSlot + kDepth * 2 * kThreads) + warp * kDepth * 128;
-                    const int row = ahead_tile + g + 8 * c;  // lanes 0 and 1 of a row bring the scales of it and the one 8 on
-                    const int scale_row = (row0 + row >> p.row_shift) - scale_row0;
-#pragma unroll
-                    for (int d = 0; d < kDepth; ++d) {
-                        if (first_chunk + (ahead_pass * kDepth + d) * kWarps + warp >= chunks) continue;
-#pragma unroll
-                        for (int h = 0; h < 2; ++h)
-                            if (ahead_tile + g + 8 * h < row_count)
-                                copy_async<16>(to + (d * 2 + h) * kThreads, ahead_codes + h * 8 * stride + d * kWarps * (kChunk / 2));
-                        if (c < 2 && row < row_count)
-                            copy_async<kChunk / kBlock>(scales_to + d * 128 + (g + 8 * c) * (kChunk / kBlock),
-                                                        ahead_scales + scale_row * scale_stride + d * kWarps * (kChunk / kBlock));
-                    }
-                    ahead_tile += 16;
-                    ahead_codes += 16 * stride;
-                    if (ahead_tile >= row_count) {
-                        ahead_tile = 0, ++ahead_pass;
-                        locate();
-                    }
+                ahead_tile += 16;
+                ahead_codes += 16 * stride;
+                if (ahead_tile >= row_count) {
+                    ahead_tile = 0, ++ahead_pass;
+                    locate();
                 }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-            };
-            // Activations whose rows do not start on 16-byte boundaries, as those of an odd width: read by the
-            // whole warp side by side, 32 elements of a token at a time, and taken from shared memory.
-            auto load_staged = [&](int t, int chunk) {
-                uint32_t* mine = reinterpret_cast<uint32_t*>(ring) + warp * kStageWords;
-                const int here = chunk < chunks ? min(8, tokens - 8 * t) : 0;
-                __syncwarp();
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (j < here)
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            const int k = chunk * kChunk + q * 32 + lane;
-                            const int64_t at = (int64_t)(token0 + 8 * t + j) * p.ldx + k;
-                            uint32_t word = 0;
-                            if (k < p.k)
-                                word = kFp32 ? __ldg(reinterpret_cast<const uint32_t*>(p.x) + at)
-                                             : (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(p.x) + at);
-                            mine[j * 144 + q * 36 + lane] = word;
-                        }
-                __syncwarp();
-                Raw<kFp32> raw;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint4 w = g < here ? *reinterpret_cast<const uint4*>(mine + g * 144 + c * 36 + 4 * i) : make_uint4(0, 0, 0, 0);
-                    if constexpr (kFp32) {
-                        raw.words[4 * i] = w.x, raw.words[4 * i + 1] = w.y, raw.words[4 * i + 2] = w.z, raw.words[4 * i + 3] = w.w;
-                    } else {
-                        raw.words[2 * i] = w.x | w.y << 16;
-                        raw.words[2 * i + 1] = w.z | w.w << 16;
-                    }
-                }
-                return raw;
-            };
-            int slot_now = 0;
-            if constexpr (kVector) {
-                locate();
-#pragma unroll
-                for (int i = 0; i < kRing - 1; ++i) copy_ahead(i);
-            } else {
-                load(0, 0);
             }
-            for (int pass = 0; pass < passes; ++pass) {
-                uint32_t b[kDepth][kTiles][kParts][16];
-                float undo[kDepth][kTiles][2];
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        int slot_now = 0;
+        if constexpr (kVector) {
+            locate();
 #pragma unroll
-                for (int d = 0; d < kDepth; ++d)
+            for (int i = 0; i < kRing - 1; ++i) copy_ahead(i);
+        } else {
+            load(0, 0);
+        }
+        for (int pass = 0; pass < passes; ++pass) {
+            uint32_t b[kDepth][kParts][16];
+            float undo[kDepth][2];
 #pragma unroll
-                    for (int t = 0; t < kTiles; ++t) {
-                        const int token = 8 * t + g, chunk = first_chunk + (pass * kDepth + d) * kWarps + warp;
-                        float mine;
-                        make_fragments<kFp32>(kVector ? load_raw<kFp32>(p, token0 + token, token < tokens && chunk < chunks, chunk)
-                                                      : load_staged(t, chunk),
-                                              b[d][t], mine);
-                        undo[d][t][0] = __shfl_sync(0xFFFFFFFFu, mine, 8 * c);
-                        undo[d][t][1] = __shfl_sync(0xFFFFFFFFu, mine, 8 * c + 4);
-                    }
-                float* slot = partial + (warp * tokens + 2 * c) * block_rows + g;
+            for (int d = 0; d < kDepth; ++d) {
+                const int chunk = first_chunk + (pass * kDepth + d) * kWarps + warp;
+                float mine;
+                make_fragments<kFp32>(
+                    kVector ? load_raw<kFp32>(p, g, g < tokens && chunk < chunks, chunk)
+                            : load_staged<kFp32>(p, 0, chunk < chunks ? tokens : 0, chunk, reinterpret_cast<uint32_t*>(ring) + warp * kStageWords),
+                    b[d], mine);
+                undo[d][0] = __shfl_sync(0xFFFFFFFFu, mine, 8 * c);
+                undo[d][1] = __shfl_sync(0xFFFFFFFFu, mine, 8 * c + 4);
+            }
+            float* slot = partial + (warp * tokens + 2 * c) * block_rows + g;
 #pragma unroll 2
-                for (int tile = 0; tile < row_count; tile += 16, slot += 16) {
-                    Piece now[kDepth][2];
-                    if constexpr (kVector) {
-                        __syncwarp();  // the slot that is filled now has been read
-                        copy_ahead(slot_now == 0 ? kRing - 1 : slot_now - 1);
-                        asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
-                        __syncwarp();  // scales come from other lanes
-                        const uint4* from = ring + slot_now * kSlot + threadIdx.x;
-                        const uint8_t* scales_from =
-                            reinterpret_cast<const uint8_t*>(ring + slot_now * kSlot + kDepth * 2 * kThreads) + warp * kDepth * 128;
+            for (int tile = 0; tile < row_count; tile += 16, slot += 16) {
+                Piece now[kDepth][2];
+                if constexpr (kVector) {
+                    __syncwarp();  // the slot that is filled now has been read
+                    copy_ahead(slot_now == 0 ? kRing - 1 : slot_now - 1);
+                    asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
+                    __syncwarp();  // scales come from other lanes
+                    const uint4* from = ring + slot_now * kSlot + threadIdx.x;
+                    const uint8_t* scales_from =
+                        reinterpret_cast<const uint8_t*>(ring + slot_now * kSlot + kDepth * 2 * kThreads) + warp * kDepth * 128;
 #pragma unroll
-                        for (int d = 0; d < kDepth; ++d)
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                now[d][h].codes = from[(d * 2 + h) * kThreads];
-                                const uint8_t* at = scales_from + d * 128 + (g + 8 * h) * (kChunk / kBlock) + c * (32 / kBlock);
-                                now[d][h].scales = kBlock == 16 ? *reinterpret_cast<const uint16_t*>(at) : *at;
-                            }
-                        slot_now = slot_now == kRing - 1 ? 0 : slot_now + 1;
-                    } else {
-#pragma unroll
-                        for (int d = 0; d < kDepth; ++d) now[d][0] = next[d][0], now[d][1] = next[d][1];
-                        if (tile + 16 < row_count)
-                            load(pass, tile + 16);
-                        else if (pass + 1 < passes)
-                            load(pass + 1, 0);
-                    }
-                    float total[kTiles][4];
-#pragma unroll
-                    for (int d = 0; d < kDepth; ++d) {
-                        float sum[kTiles][kParts][4] = {};
-                        uint32_t scale[2][2];
+                    for (int d = 0; d < kDepth; ++d)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            scale[h][0] = scale_half2(kBlock == 16 ? now[d][h].scales & 0xFFu : now[d][h].scales);
-                            scale[h][1] = kBlock == 16 ? scale_half2(now[d][h].scales >> 8) : scale[h][0];
+                            now[d][h].codes = from[(d * 2 + h) * kThreads];
+                            const uint8_t* at = scales_from + d * 128 + (g + 8 * h) * (kChunk / kBlock) + c * (32 / kBlock);
+                            now[d][h].scales = kBlock == 16 ? *reinterpret_cast<const uint16_t*>(at) : *at;
                         }
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            uint32_t a[2][4];
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                e2m1x8_to_half2(word_of(now[d][h].codes, j), a[h]);
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) a[h][i] = mul_half2(a[h][i], scale[h][j / 2]);
-                            }
-#pragma unroll
-                            for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-                                for (int part = 0; part < kParts; ++part) {
-                                    const uint32_t(&x)[16] = b[d][t][part];
-                                    mma_f16(sum[t][part], a[0][0], a[1][0], a[0][1], a[1][1], x[4 * j], x[4 * j + 1]);
-                                    mma_f16(sum[t][part], a[0][2], a[1][2], a[0][3], a[1][3], x[4 * j + 2], x[4 * j + 3]);
-                                }
-                        }
-#pragma unroll
-                        for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                float whole = sum[t][0][i];
-                                if constexpr (kFp32)
-                                    whole = __fmaf_rn(sum[t][2][i], 0x1p-22f, __fmaf_rn(sum[t][1][i], 0x1p-11f, whole));
-                                total[t][i] = d == 0 ? whole * undo[d][t][i & 1] : __fmaf_rn(whole, undo[d][t][i & 1], total[t][i]);
-                            }
-                    }
-#pragma unroll
-                    for (int t = 0; t < kTiles; ++t)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i)
-                            if (8 * t + 2 * c + i < tokens) {
-                                float* at = slot + (8 * t + i) * block_rows;
-                                if (pass > 0) {
-                                    total[t][i] += at[0];
-                                    total[t][i + 2] += at[8];
-                                }
-                                at[0] = total[t][i];
-                                at[8] = total[t][i + 2];
-                            }
-                }
-            }
-            __syncthreads();
-            if (p.split > 1) {
-                // the sums of this CTA's warps, in the place of its first warp's; then those of the cluster
-                for (int i = threadIdx.x; i < row_count * tokens; i += kThreads) {
-                    const int token = i / row_count, r = i - token * row_count;
-                    float value = 0.0f;
-#pragma unroll
-                    for (int w = 0; w < kWarps; ++w) value += partial[(w * tokens + token) * block_rows + r];
-                    partial[token * block_rows + r] = value;
-                }
-                cooperative_groups::this_cluster().sync();
-            }
-            for (int i = share * kThreads + threadIdx.x; i < row_count * tokens; i += p.split * kThreads) {
-                const int token = i / row_count, r = i - token * row_count;
-                float value = 0.0f;
-                if (p.split > 1) {
-                    for (int q = 0; q < p.split; ++q)
-                        value += cooperative_groups::this_cluster().map_shared_rank(partial, q)[token * block_rows + r];
+                    slot_now = slot_now == kRing - 1 ? 0 : slot_now + 1;
                 } else {
 #pragma unroll
-                    for (int w = 0; w < kWarps; ++w) value += partial[(w * tokens + token) * block_rows + r];
+                    for (int d = 0; d < kDepth; ++d) now[d][0] = next[d][0], now[d][1] = next[d][1];
+                    if (tile + 16 < row_count)
+                        load(pass, tile + 16);
+                    else if (pass + 1 < passes)
+                        load(pass + 1, 0);
                 }
-                value *= p.factor;
-                const int64_t n = row0 + r;
-                if (p.bias)
-                    value += p.bias_fp32 ? reinterpret_cast<const float*>(p.bias)[n]
-                                         : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.bias)[n]);
-                const int64_t at = (int64_t)(token0 + token) * p.ldo + n;
-                if (p.out_fp32)
-                    reinterpret_cast<float*>(p.out)[at] = value;
-                else
-                    reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(value);
+                float total[4];
+#pragma unroll
+                for (int d = 0; d < kDepth; ++d) {
+                    float sum[kParts][4] = {};
+                    uint32_t scale[2][2];
+                    scale_pairs<kBlock>(now[d], scale);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t a[2][4];
+                        decode<kBlock>(now[d], scale, j, a);
+#pragma unroll
+                        for (int part = 0; part < kParts; ++part) {
+                            const uint32_t(&x)[16] = b[d][part];
+                            mma_f16(sum[part], a[0][0], a[1][0], a[0][1], a[1][1], x[4 * j], x[4 * j + 1]);
+                            mma_f16(sum[part], a[0][2], a[1][2], a[0][3], a[1][3], x[4 * j + 2], x[4 * j + 3]);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float whole = sum[0][i];
+                        if constexpr (kFp32)
+                            whole = __fmaf_rn(sum[2][i], 0x1p-22f, __fmaf_rn(sum[1][i], 0x1p-11f, whole));
+                        total[i] = d == 0 ? whole * undo[d][i & 1] : __fmaf_rn(whole, undo[d][i & 1], total[i]);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (2 * c + i < tokens) {
+                        float* at = slot + i * block_rows;
+                        if (pass > 0) {
+                            total[i] += at[0];
+                            total[i + 2] += at[8];
+                        }
+                        at[0] = total[i];
+                        at[8] = total[i + 2];
+                    }
             }
-            if (p.split > 1)
-                cooperative_groups::this_cluster().sync();  // the others have read this CTA's sums
-            else
-                __syncthreads();
         }
+        __syncthreads();
+        if (p.split > 1) {
+            // the sums of this CTA's warps, in the place of its first warp's; then those of the cluster
+            for (int i = threadIdx.x; i < row_count * tokens; i += kThreads) {
+                const int token = i / row_count, r = i - token * row_count;
+                float value = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) value += partial[(w * tokens + token) * block_rows + r];
+                partial[token * block_rows + r] = value;
+            }
+            cooperative_groups::this_cluster().sync();
+        }
+        for (int i = share * kThreads + threadIdx.x; i < row_count * tokens; i += p.split * kThreads) {
+            const int token = i / row_count, r = i - token * row_count;
+            float value = 0.0f;
+            if (p.split > 1) {
+                for (int q = 0; q < p.split; ++q)
+                    value += cooperative_groups::this_cluster().map_shared_rank(partial, q)[token * block_rows + r];
+            } else {
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) value += partial[(w * tokens + token) * block_rows + r];
+            }
+            store(p, token, row0 + r, value);
+        }
+        if (p.split > 1)
+            cooperative_groups::this_cluster().sync();  // the others have read this CTA's sums
+        else
+            __syncthreads();
     }
 }
 
-template <bool kFp32, int kTiles, int kDepth, bool kVector, int kBlock>
-int launch(Params p, cudaStream_t stream) {
-    const int used = p.tokens < kTiles * 8 ? p.tokens : kTiles * 8;
+template <bool kFp32, int kDepth, bool kVector, int kBlock>
+int launch_few(Params p, cudaStream_t stream) {
     constexpr size_t kRingBytes = (kVector ? kRing * slot_pieces(kDepth) : kStagePieces) * sizeof(uint4);
-    constexpr auto kKernel = packed_matvec_kernel<kFp32, kTiles, kDepth, kVector, kBlock>;
+    constexpr auto kKernel = packed_matvec_kernel<kFp32, kDepth, kVector, kBlock>;
     cudaError_t error = allow_shared<kKernel>((int)kRingBytes + kPartialFloats * 4);
     if (error != cudaSuccess) return record_cuda_error(error);
     // Few rows and a long reduction axis: with the rows spread over all SMs, every one of them would convert
@@ -516,11 +523,11 @@ int launch(Params p, cudaStream_t stream) {
     }
     if (grid > p.rows) grid = p.rows;
     const int own = (p.rows + grid - 1) / grid;
-    int block = kPartialFloats / (kWarps * used) / 16 * 16;
+    int block = kPartialFloats / (kWarps * p.tokens) / 16 * 16;
     const int need = (own + 15) / 16 * 16;
     if (block > need) block = need;
     p.rows_per_block = block;
-    const size_t bytes = kRingBytes + (size_t)kWarps * used * block * sizeof(float);
+    const size_t bytes = kRingBytes + (size_t)kWarps * p.tokens * block * sizeof(float);
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(grid * p.split);
     config.blockDim = dim3(kThreads);
@@ -536,22 +543,282 @@ int launch(Params p, cudaStream_t stream) {
     return record_cuda_error(cudaLaunchKernelEx(&config, kKernel, p));
 }
 
+// ---- more than eight tokens ---------------------------------------------------------------------
+
+constexpr int kManyWarps = 8;     // four times 32 rows, for each of two halves of the CTA's chunks
+constexpr int kManyThreads = kManyWarps * 32;
+constexpr int kManyRows = 128;
+constexpr int kManyPad = kManyRows + 4;  // rows of a token's sums: the lanes of a fragment meet no bank twice
+constexpr int kManyRing = 3;                // chunks on their way per half, one of them in use
+constexpr int kManySlot = 2 * 2 * 32 + 16;  // 16-byte pieces: 32 rows' codes of a chunk, and their scales
+// ... and of a chunk's activations: fragments, and the factors behind them
+__host__ __device__ constexpr int many_stage(int tiles, int parts) { return tiles * (parts * 128 + 2); }
+
+// The activations as the product reads them: [chunk][tile of 8 tokens][part][step][lane] 16 bytes, and
+// the factors that undo the chunks' powers of two: [chunk][tile][token].  One warp per chunk and tile.
+template <bool kFp32>
+__global__ void __launch_bounds__(kManyThreads) prepare_kernel(const Params p, uint4* fragments, float* undo, int chunks, int tiles) {
+    constexpr int kParts = kFp32 ? 3 : 1;
+    __shared__ uint4 stage[kManyWarps * kStageWords / 4];
+    launch_dependents();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int64_t unit = (int64_t)blockIdx.x * kManyWarps + warp;
+    const int chunk = (int)(unit / tiles), tile = (int)(unit % tiles);
+    if (chunk >= chunks) return;
+    const int here = min(8, p.tokens - 8 * tile);
+    uint32_t b[kParts][16];
+    float mine;
+    make_fragments<kFp32>(p.vector_x ? load_raw<kFp32>(p, 8 * tile + g, g < here, chunk)
+                                     : load_staged<kFp32>(p, 8 * tile, here, chunk, reinterpret_cast<uint32_t*>(stage) + warp * kStageWords),
+                          b, mine);
+    uint4* to = fragments + unit * (kParts * 128) + lane;
+#pragma unroll
+    for (int part = 0; part < kParts; ++part)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            to[part * 128 + j * 32] = make_uint4(b[part][4 * j], b[part][4 * j + 1], b[part][4 * j + 2], b[part][4 * j + 3]);
+    if (c == 0) undo[unit * 8 + g] = mine;
+}
+
+template <bool kFp32, int kTiles, bool kVector, int kBlock>
+__global__ void __launch_bounds__(kManyThreads, kFp32 || kTiles > 4 ? 1 : 2)
+    packed_matmul_kernel(const Params p, const uint4* fragments, const float* undo, int chunks, int tiles) {
+    constexpr int kParts = kFp32 ? 3 : 1, kBlockShift = kBlock == 16 ? 4 : 5;
+    constexpr int kStage = many_stage(kTiles, kParts);
+    // activations [half][slot], then, kVector, codes and scales [warp][slot]; afterwards the sums [half][token][row]
+    extern __shared__ uint4 ring[];
+    float* partial = reinterpret_cast<float*>(ring);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int row_blocks = (p.rows + kManyRows - 1) / kManyRows;
+    const int share = blockIdx.x % p.split, place = blockIdx.x / p.split;
+    const int block_row = place % row_blocks * kManyRows, tile0 = place / row_blocks * kTiles;
+    const int here = min(kTiles, tiles - tile0);
+    const int row0 = block_row + warp % 4 * 32, half = warp / 4;
+    const int first = (int)((int64_t)chunks * share / p.split) + half, last = (int)((int64_t)chunks * (share + 1) / p.split);
+    const int count = last > first ? (last - first + 1) / 2 : 0;
+    const bool active = row0 < p.rows;
+    const int stride = (int)p.code_stride, scale_stride = (int)p.scale_stride;
+    const uint8_t* codes = p.codes + row0 * p.code_stride;
+    const int scale_row0 = row0 >> p.row_shift;
+    const uint8_t* scales = p.scales + scale_row0 * p.scale_stride;
+    const int row_count = min(32, p.rows - row0);
+
+    // codes and scales of the chunks to come: as in the kernel for few tokens, with the scales of a row per lane
+    uint4* slots = ring + 2 * kManyRing * kStage + warp * kManyRing * kManySlot;
+    auto copy_codes = [&](int i) {
+        if (i < count && active) {
+            const int chunk = first + 2 * i;
+            uint4* to = slots + i % kManyRing * kManySlot;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int row = 8 * q + g;
+                if (row < row_count) copy_async<16>(to + q * 32 + lane, codes + row * stride + chunk * (kChunk / 2) + 16 * c);
+            }
+            if (lane < row_count)
+                copy_async<kChunk / kBlock>(reinterpret_cast<uint8_t*>(to + 128) + lane * 8,
+                                            scales + ((row0 + lane >> p.row_shift) - scale_row0) * scale_stride + chunk * (kChunk / kBlock));
+        }
+    };
+    // the chunks' activations, by the four warps that use them
+    uint4* stages = ring + half * kManyRing * kStage;
+    auto copy_activations = [&](int i) {
+        if (i < count) {
+            const int64_t unit = (int64_t)(first + 2 * i) * tiles + tile0;
+            uint4* to = stages + i % kManyRing * kStage;
+            const uint4* from = fragments + unit * (kParts * 128);
+            for (int at = threadIdx.x & 127; at < here * kParts * 128; at += 128)
+                copy_async<16>(to + at, reinterpret_cast<const uint8_t*>(from + at));
+            if ((threadIdx.x & 127) < here * 2)
+                copy_async<16>(to + kTiles * kParts * 128 + (threadIdx.x & 127),
+                               reinterpret_cast<const uint8_t*>(undo + unit * 8 + (threadIdx.x & 127) * 4));
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    const bool inner = row0 * p.code_stride >= 3 && (int64_t)(p.rows - row0 - row_count) * p.code_stride >= 20;
+    Piece next[2][2];
+    auto load = [&](int i) {
+        const int byte = min((first + 2 * i) * (kChunk / 2) + 16 * c, stride - 1), block = byte * 2 >> kBlockShift;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int row = min(8 * q + g, row_count - 1);
+            const uint32_t code = row * stride + byte, scale = ((row0 + row >> p.row_shift) - scale_row0) * scale_stride;
+            next[q / 2][q % 2] =
+                inner ? load_piece<Loads::kWords, kBlock>(codes, scales, code, scale + block, scale + scale_stride - 1, 0)
+                      : load_piece<Loads::kBytes, kBlock>(codes, scales, code, scale + block, scale + scale_stride - 1, stride - byte);
+        }
+    };
+    if constexpr (kVector) {
+#pragma unroll
+        for (int i = 0; i < kManyRing - 1; ++i) copy_codes(i);
+    } else {
+        if (count > 0 && active) load(0);
+    }
+    wait_for_launcher();  // the activations are prepared
+#pragma unroll
+    for (int i = 0; i < kManyRing - 1; ++i) copy_activations(i);
+
+    float total[2][kTiles][4] = {};
+    for (int i = 0; i < count; ++i) {
+        // this thread's copies for chunk i are there; behind the barrier all are, and the slot before is free
+        asm volatile("cp.async.wait_group %0;" ::"n"(kManyRing - 2) : "memory");
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+        if constexpr (kVector) copy_codes(i + kManyRing - 1);
+        copy_activations(i + kManyRing - 1);
+        if (!active) continue;
+        Piece now[2][2];
+        if constexpr (kVector) {
+            const uint4* from = slots + i % kManyRing * kManySlot;
+            const uint8_t* scales_from = reinterpret_cast<const uint8_t*>(from + 128) + g * 8 + c * (32 / kBlock);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                now[q / 2][q % 2].codes = from[q * 32 + lane];
+                const uint8_t* at = scales_from + q * 64;
+                now[q / 2][q % 2].scales = kBlock == 16 ? *reinterpret_cast<const uint16_t*>(at) : *at;
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) now[q / 2][q % 2] = next[q / 2][q % 2];
+            if (i + 1 < count) load(i + 1);
+        }
+        const uint4* from = stages + i % kManyRing * kStage + lane;
+        const float2* undo_from = reinterpret_cast<const float2*>(from - lane + kTiles * kParts * 128) + c;
+        uint32_t scale[2][2][2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) scale_pairs<kBlock>(now[r], scale[r]);
+        float sum[2][kTiles][kParts][4] = {};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t a[2][2][4];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) decode<kBlock>(now[r], scale[r], j, a[r]);
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) {
+                if (t % 2 == 0 && t >= here) break;  // a tile behind the last one: sums that are not stored
+#pragma unroll
+                for (int part = 0; part < kParts; ++part) {
+                    const uint4 x = from[(t * kParts + part) * 128 + j * 32];
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        mma_f16(sum[r][t][part], a[r][0][0], a[r][1][0], a[r][0][1], a[r][1][1], x.x, x.y);
+                        mma_f16(sum[r][t][part], a[r][0][2], a[r][1][2], a[r][0][3], a[r][1][3], x.z, x.w);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) {
+            if (t % 2 == 0 && t >= here) break;
+            const float2 back = undo_from[t * 4];
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float whole = sum[r][t][0][e];
+                    if constexpr (kFp32)
+                        whole = __fmaf_rn(sum[r][t][kParts - 1][e], 0x1p-22f, __fmaf_rn(sum[r][t][kParts / 2][e], 0x1p-11f, whole));
+                    total[r][t][e] = __fmaf_rn(whole, e & 1 ? back.y : back.x, total[r][t][e]);
+                }
+        }
+    }
+
+    __syncthreads();  // the ring's memory takes the sums
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                partial[(half * kTiles * 8 + 8 * t + 2 * c + (e & 1)) * kManyPad + warp % 4 * 32 + 16 * r + g + 8 * (e >> 1)] = total[r][t][e];
+    __syncthreads();
+    const int tokens = min(kTiles * 8, p.tokens - tile0 * 8);
+    constexpr int kOther = kTiles * 8 * kManyPad;  // the second half's sums
+    if (p.split > 1) {
+        for (int i = threadIdx.x; i < kManyRows * tokens; i += kManyThreads) {
+            float* at = partial + i / kManyRows * kManyPad + i % kManyRows;
+            *at += at[kOther];
+        }
+        cooperative_groups::this_cluster().sync();
+    }
+    for (int i = share * kManyThreads + threadIdx.x; i < kManyRows * tokens; i += p.split * kManyThreads) {
+        const int token = i / kManyRows, row = i % kManyRows, at = token * kManyPad + row;
+        if (block_row + row >= p.rows) continue;
+        float value = 0.0f;
+        if (p.split > 1) {
+            for (int q = 0; q < p.split; ++q) value += cooperative_groups::this_cluster().map_shared_rank(partial, q)[at];
+        } else {
+            value = partial[at] + partial[at + kOther];
+        }
+        store(p, tile0 * 8 + token, block_row + row, value);
+    }
+    if (p.split > 1) cooperative_groups::this_cluster().sync();  // the others have read this CTA's sums
+}
+
+// bytes of the prepared activations: fragments, and the factors behind them
+size_t workspace_of(bool fp32, int64_t tokens, int64_t cols) {
+    if (tokens <= kFewTokens) return 0;
+    return (size_t)((cols + kChunk - 1) / kChunk) * ((tokens + 7) / 8) * ((fp32 ? 3 : 1) * 2048 + 32);
+}
+
+template <bool kFp32, int kTiles, bool kVector, int kBlock>
+int launch_many(Params p, void* workspace, cudaStream_t stream) {
+    constexpr auto kKernel = packed_matmul_kernel<kFp32, kTiles, kVector, kBlock>;
+    constexpr int kSums = 2 * kTiles * 8 * kManyPad * 4,
+                  kRingBytes = (2 * many_stage(kTiles, kFp32 ? 3 : 1) + (kVector ? kManyWarps * kManySlot : 0)) * kManyRing * 16;
+    constexpr int kBytes = kSums > kRingBytes ? kSums : kRingBytes;
+    cudaError_t error = allow_shared<kKernel>(kBytes);
+    if (error != cudaSuccess) return record_cuda_error(error);
+    const int chunks = (p.k + kChunk - 1) / kChunk, tiles = (p.tokens + 7) / 8;
+    const int64_t places = (int64_t)((p.rows + kManyRows - 1) / kManyRows) * ((tiles + kTiles - 1) / kTiles);
+    const int64_t units = (int64_t)chunks * tiles;
+    if (places > 0x7FFFFFFF / 8 || units > (int64_t)0x7FFFFFFF * kManyWarps) {
+        record_error_text("more rows times tokens than one launch covers");
+        return UE5M3_ERR_TOO_LARGE;
+    }
+    uint4* fragments = reinterpret_cast<uint4*>(workspace);
+    float* undo = reinterpret_cast<float*>(fragments + units * (kFp32 ? 384 : 128));
+    prepare_kernel<kFp32><<<(unsigned)((units + kManyWarps - 1) / kManyWarps), kManyThreads, 0, stream>>>(p, fragments, undo, chunks, tiles);
+    const int status = check_launch();
+    if (status != UE5M3_OK) return status;
+    // Fewer blocks of rows than SMs have room for: clusters share the reduction axis.
+    const int64_t room = sm_count() * (kFp32 || kTiles > 4 ? 1 : 2) / places;
+    p.split = room < 1 ? 1 : room > 8 ? 8 : (int)room;
+    if (p.split > (chunks + 3) / 4) p.split = (chunks + 3) / 4;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)(places * p.split));
+    config.blockDim = dim3(kManyThreads);
+    config.dynamicSmemBytes = kBytes;
+    config.stream = stream;
+    cudaLaunchAttribute attributes[2];
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = p.split;
+    attributes[1].val.clusterDim.y = 1;
+    attributes[1].val.clusterDim.z = 1;
+    config.attrs = attributes;
+    config.numAttrs = p.split > 1 ? 2 : 1;
+    return record_cuda_error(cudaLaunchKernelEx(&config, kKernel, p, (const uint4*)fragments, (const float*)undo, chunks, tiles));
+}
+
 template <bool kVector, int kBlock>
-int dispatch(const Params& p, bool fp32, cudaStream_t s) {
-    constexpr int kDepth = kVector ? 2 : 1;
-    if (fp32) return launch<true, 1, 1, kVector, kBlock>(p, s);
-    if (p.tokens <= 8) return launch<false, 1, kDepth, kVector, kBlock>(p, s);
-    if (p.tokens <= 16) return launch<false, 2, 1, kVector, kBlock>(p, s);
-    return launch<false, 4, 1, kVector, kBlock>(p, s);
+int dispatch(const Params& p, bool fp32, void* workspace, cudaStream_t s) {
+    if (p.tokens <= kFewTokens)
+        return fp32 ? launch_few<true, 1, kVector, kBlock>(p, s) : launch_few<false, kVector ? 2 : 1, kVector, kBlock>(p, s);
+    if (fp32) return launch_many<true, 4, kVector, kBlock>(p, workspace, s);
+    return p.tokens <= 32 ? launch_many<false, 4, kVector, kBlock>(p, workspace, s) : launch_many<false, 8, kVector, kBlock>(p, workspace, s);
 }
 
 }  // namespace matvec
 }  // namespace ue5m3
 
+extern "C" size_t ue5m3_packed_matvec_workspace_bytes(int x_dtype, int64_t tokens, int64_t cols) {
+    return tokens > 0 && cols > 0 ? ue5m3::matvec::workspace_of(x_dtype == UE5M3_DTYPE_FP32, tokens, cols) : 0;
+}
+
 extern "C" int ue5m3_packed_matvec(const void* x, int x_dtype, int64_t tokens, int64_t ldx, const uint8_t* codes,
                                    const uint8_t* scales, int64_t rows, int64_t cols, int block, int two_d, float dec,
                                    const void* bias, int bias_dtype, void* out, int out_dtype, int64_t ldo,
-                                   void* stream) {
+                                   void* workspace, size_t workspace_bytes, void* stream) {
     using namespace ue5m3;
     if (!x || !codes || !scales || !out || tokens <= 0 || rows <= 0 || cols <= 0 || ldx < cols || ldo < rows)
         return UE5M3_ERR_INVALID_ARGUMENT;
@@ -566,6 +833,9 @@ extern "C" int ue5m3_packed_matvec(const void* x, int x_dtype, int64_t tokens, i
     if ((uintptr_t)x % element || (uintptr_t)out % (out_dtype == UE5M3_DTYPE_FP32 ? 4 : 2) ||
         (bias && (uintptr_t)bias % (bias_dtype == UE5M3_DTYPE_FP32 ? 4 : 2)))
         return UE5M3_ERR_ALIGNMENT;
+    const size_t need = matvec::workspace_of(fp32, tokens, cols);
+    if (need > 0 && (!workspace || workspace_bytes < need)) return UE5M3_ERR_SCRATCH;
+    if (need > 0 && (uintptr_t)workspace % 16) return UE5M3_ERR_ALIGNMENT;
     matvec::Params p;
     p.x = x;
     p.ldx = ldx;
@@ -587,6 +857,6 @@ extern "C" int ue5m3_packed_matvec(const void* x, int x_dtype, int64_t tokens, i
     p.out_fp32 = out_dtype == UE5M3_DTYPE_FP32;
     p.factor = 16.0f * dec;
     cudaStream_t s = (cudaStream_t)stream;
-    if (block == 16) return vector ? matvec::dispatch<true, 16>(p, fp32, s) : matvec::dispatch<false, 16>(p, fp32, s);
-    return vector ? matvec::dispatch<true, 32>(p, fp32, s) : matvec::dispatch<false, 32>(p, fp32, s);
+    if (block == 16) return vector ? matvec::dispatch<true, 16>(p, fp32, workspace, s) : matvec::dispatch<false, 16>(p, fp32, workspace, s);
+    return vector ? matvec::dispatch<true, 32>(p, fp32, workspace, s) : matvec::dispatch<false, 32>(p, fp32, workspace, s);
 }

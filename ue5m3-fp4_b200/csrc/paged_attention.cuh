@@ -115,11 +115,6 @@ __device__ __forceinline__ bool odd_piece(const uint4& v) {
     return odd_pair(v.x) || odd_pair(v.y) || odd_pair(v.z) || odd_pair(v.w);
 }
 
-// Programmatic launches: the next kernel of a call starts while this one ends, and waits for it
-// where it first reads what this one writes.
-__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_launcher() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 template <typename... Arguments>
 cudaError_t launch_after(void (*kernel)(Arguments...), dim3 grid, unsigned threads, size_t shared, cudaStream_t stream,
                          bool early, Arguments... arguments) {

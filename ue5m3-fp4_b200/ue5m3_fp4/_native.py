@@ -117,7 +117,10 @@ def load() -> ctypes.CDLL:
     lib.ue5m3_test_e2m1_cvt.restype = i32
     lib.ue5m3_test_e2m1_cvt.argtypes = [ctypes.c_uint32, ctypes.c_uint64, p, p, p]
     lib.ue5m3_packed_matvec.restype = i32
-    lib.ue5m3_packed_matvec.argtypes = [p, i32, i64, i64, p, p, i64, i64, i32, i32, f32, p, i32, p, i32, i64, p]
+    lib.ue5m3_packed_matvec.argtypes = [p, i32, i64, i64, p, p, i64, i64, i32, i32, f32, p, i32, p, i32, i64, p, ctypes.c_size_t,
+                                        p]
+    lib.ue5m3_packed_matvec_workspace_bytes.restype = ctypes.c_size_t
+    lib.ue5m3_packed_matvec_workspace_bytes.argtypes = [i32, i64, i64]
     lib.ue5m3_paged_attention_workspace_bytes.restype = sz
     lib.ue5m3_paged_attention_workspace_bytes.argtypes = [i64] * 7
     lib.ue5m3_paged_attention.restype = i32

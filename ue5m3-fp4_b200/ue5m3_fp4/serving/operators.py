@@ -124,9 +124,13 @@ def packed_matvec(
             ldx = cols
         if (step != 1 and cols > 1) or ldx < cols:
             raise ValueError("the last axis of x must be contiguous and its rows must not overlap")
-        _call(_native.load().ue5m3_packed_matvec, "ue5m3_packed_matvec", 1, index, flat.data_ptr(), x_code, tokens, ldx,
+        # more than eight rows: prepared once, in memory of the current stream's pool for this call alone
+        library = _native.load()
+        need = library.ue5m3_packed_matvec_workspace_bytes(x_code, tokens, cols) if tokens > 8 else 0
+        workspace = x.new_empty(need, dtype=torch.uint8) if need else None
+        _call(library.ue5m3_packed_matvec, "ue5m3_packed_matvec", 2 if need else 1, index, flat.data_ptr(), x_code, tokens, ldx,
               codes.data_ptr(), scales.data_ptr(), rows, cols, block_size, two_dimensional, factor, bias_pointer,
-              bias_code, out.data_ptr(), out_code, rows)
+              bias_code, out.data_ptr(), out_code, rows, None if workspace is None else workspace.data_ptr(), need)
     return out if x.ndim == 2 else out.view(*x.shape[:-1], rows)
 
 
