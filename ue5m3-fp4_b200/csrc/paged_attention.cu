@@ -525,9 +525,10 @@ static size_t workspace_of(int64_t tokens, int64_t heads, int64_t head_dim, int6
 }
 
 // Up to 32 rows per key/value head: the kernel for few rows, whose 16-row tiles read the keys once
-// each; more: the tensor-core kernel with its 256-row tiles.  Splits of the keys: few rows, enough
-// CTAs for two on every SM, runs of 4 to 16 tiles.  Many rows: one CTA per SM at most, runs of at
-// least 8 tiles, and no more than pays: a split takes its share of about 0.93 us per 64 keys off the
+// each (32 rows, 16 sequences of 4096 keys: 44 us against 70; one of 32768: 26 against 34); more: the
+// tensor-core kernel with its 256-row tiles (64 rows, the same: 71 us against 76, 35 against 42).
+// Splits of the keys: few rows, enough CTAs for two on every SM, runs of 4 to 16 tiles.  Many rows:
+// one CTA per SM at most, runs of at least 8 tiles, and no more than pays: a split takes its share of about 0.93 us per 64 keys off the
 // time and adds the writing and reading of its partial rows at about 0.7 TB/s, so that the square
 // root of their quotient is the best number (8 x 32 heads over 32768 keys: 465 -> 35 us with 37 splits;
 // 4 x 128 tokens over 2048 keys: 46.5 us without, 57.8 with 3).
