@@ -17,15 +17,18 @@
 // distributed shared memory by every CTA for itself (one cluster barrier per step).  The first
 // step's bins are linear in (max - l) / T, which spreads real logits (bins of the integer order
 // would put a fifth of a row into one of them); what lies in the last, open bin is counted in
-// registers.  Where the first step leaves at most 1024 elements that can be kept (top-k of a few
+// registers.  Where the first step leaves at most 256 elements that can be kept (top-k of a few
 // hundred, a peaked nucleus), these are gathered and the rest happens among them in one CTA.
 // Otherwise the elements of the bin that holds the threshold are ranked against one another, or the
 // search goes on inside it with bins of the 64-bit rank (many equal logits).
 //
-// Measured (fp32): one row of 131072, top-k and top-p: 13.3 us, the steps of eight CTAs that wait
-// for one another at four cluster barriers; 64 rows of 131072 with top-p alone: 111 us, against 5 us for the bytes and
-// 6.5 us for the exponentials at the rate of the fp64 pipe: two CTAs fit on an SM, so the 512 take
-// almost two turns, and within a turn the passes over a slice wait for shared memory and atomics.
+// Measured (fp32): one row of 131072, top-k and top-p: 12.9 us, the steps of eight CTAs that wait
+// for one another at four cluster barriers; top-p alone 27 us; 64 rows of 131072 with top-p alone:
+// 84 us, against 5 us for the bytes and 6.5 us for the exponentials at the rate of the fp64 pipe: two
+// CTAs fit on an SM, so the 512 take almost two turns, each with 15000 cycles of weights and their
+// atomics (32 logits a thread) and as much again in steps that wait.  Weights of the nucleus alone in
+// the last step, bins summed once per CTA before the others read them, and ranking by all threads of
+// the cluster took it there from 111.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -43,6 +46,7 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = kThreads;          // one bin per thread in the scan over bins
 constexpr int kCandidates = 1024;        // elements that are ranked against one another
+constexpr int kFew = 256;                // ... in one CTA, to the end (64 rows of 32000, top-k 400: 59 us; 512: 77)
 constexpr int kMaxCluster = 8;
 constexpr int64_t kMaxVocabulary = 1 << 18;
 constexpr float kBinsPerUnit = 32.0f;    // first step: bins of (max - l) / T, the last one open
@@ -68,7 +72,9 @@ struct Params {
 
 struct alignas(16) Shared {
     double power[8];             // 2^(j / 8)
-    uint32_t hist[2][4][kBins];  // [buffer][count, weight bits 0..14, 15..29, 30..44]
+    uint32_t hist[4][kBins];  // [count, weight bits 0..16, 17..33, 34..44]: 2^15 summands fit
+    uint64_t bin_weight[2][kBins];  // a step's bins of this CTA for the others, which may still read those of the
+    uint32_t bin_number[2][kBins];  // step before
     uint64_t mine[kCandidates];  // this CTA's candidates
     uint64_t all[kCandidates];
     uint64_t weight[kCandidates];
@@ -210,9 +216,9 @@ __device__ __forceinline__ uint64_t warp_running(uint64_t v) {
 }
 
 __device__ __forceinline__ void add_weight(uint32_t (*hist)[kBins], uint32_t bin, uint64_t w) {
-    atomicAdd(&hist[1][bin], (uint32_t)(w & 0x7FFF));
-    atomicAdd(&hist[2][bin], (uint32_t)(w >> 15 & 0x7FFF));
-    atomicAdd(&hist[3][bin], (uint32_t)(w >> 30));
+    atomicAdd(&hist[1][bin], (uint32_t)(w & 0x1FFFF));
+    atomicAdd(&hist[2][bin], (uint32_t)(w >> 17 & 0x1FFFF));
+    if (w >> 34) atomicAdd(&hist[3][bin], (uint32_t)(w >> 34));  // within a factor of 1000 of the largest
 }
 
 // Where a histogram's running mass reaches `need`.
@@ -230,22 +236,26 @@ struct Found {
 template <bool kWeighted>
 __device__ Found scan_bins(cg::cluster_group& cluster, Shared& s, int& buffer, uint64_t& need, float share) {
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    __syncthreads();
+    s.bin_number[buffer][t] = s.hist[0][t];
+    if (kWeighted) s.bin_weight[buffer][t] = (uint64_t)s.hist[1][t] + ((uint64_t)s.hist[2][t] << 17) + ((uint64_t)s.hist[3][t] << 34);
     cluster.sync();
     const int ctas = cluster.num_blocks();
-    uint32_t parts[kMaxCluster][4];
+    uint64_t weights[kMaxCluster];
+    uint32_t numbers_of[kMaxCluster];
     for_each_cta([&](int r) {
         const Shared* other = cluster.map_shared_rank(&s, r < ctas ? r : 0);
-#pragma unroll
-        for (int i = 0; i < (kWeighted ? 4 : 1); ++i) parts[r][i] = other->hist[buffer][i][t];
+        numbers_of[r] = other->bin_number[buffer][t];
+        if (kWeighted) weights[r] = other->bin_weight[buffer][t];
     });
     uint64_t mass = 0;
     uint32_t number = 0;
     for_each_cta([&](int r) {
         if (r >= ctas) return;
-        number += parts[r][0];
-        if (kWeighted) mass += (uint64_t)parts[r][1] + ((uint64_t)parts[r][2] << 15) + ((uint64_t)parts[r][3] << 30);
+        number += numbers_of[r];
+        if (kWeighted) mass += weights[r];
     });
-    buffer ^= 1;  // the next step writes the other one, which nobody reads any more
+    buffer ^= 1;
     if (!kWeighted) mass = number;
     uint64_t running = warp_running(mass), numbers = kWeighted ? warp_running(number) : 0;
     if (lane == 31) {
@@ -279,8 +289,8 @@ __device__ Found scan_bins(cg::cluster_group& cluster, Shared& s, int& buffer, u
     return found;
 }
 
-__device__ __forceinline__ void clear_bins(Shared& s, int buffer) {
-    for (int i = 0; i < 4; ++i) s.hist[buffer][i][threadIdx.x] = 0;
+__device__ __forceinline__ void clear_bins(Shared& s) {
+    for (int i = 0; i < 4; ++i) s.hist[i][threadIdx.x] = 0;
     __syncthreads();
 }
 
@@ -288,8 +298,8 @@ __device__ __forceinline__ void clear_bins(Shared& s, int buffer) {
 template <bool kWeighted>
 __device__ Found first_step(cg::cluster_group& cluster, Shared& s, const float* data, int count, uint32_t base, const Row& row,
                             uint64_t floor, uint64_t& need, float share, int& buffer) {
-    clear_bins(s, buffer);
-    uint32_t(*hist)[kBins] = s.hist[buffer];
+    clear_bins(s);
+    uint32_t(*hist)[kBins] = s.hist;
     uint64_t last_number = 0, last_weight = 0;
     for_each_four(data, count, [&](const float(&v)[4], int i) {
 #pragma unroll
@@ -368,6 +378,13 @@ __device__ int collect(cg::cluster_group& cluster, Shared& s, const Row& row) {
     return candidates;
 }
 
+// How many neighbouring threads share a candidate: a power of two, so that all have one if there are enough.
+__device__ __forceinline__ int lanes_of(int candidates, int threads) {
+    int lanes = 1;
+    while (lanes < 32 && 2 * lanes * candidates <= threads) lanes *= 2;
+    return lanes;
+}
+
 // A threshold search whose first step left too many elements: the rank of the last one that is kept.
 template <bool kWeighted>
 __device__ uint64_t search(cg::cluster_group& cluster, Shared& s, const float* data, int count, uint32_t base, const Row& row,
@@ -404,8 +421,8 @@ __device__ uint64_t search(cg::cluster_group& cluster, Shared& s, const float* d
         while (true) {
             int shift = 0;
             while ((high - low) >> shift >= kBins) ++shift;
-            clear_bins(s, buffer);
-            uint32_t(*hist)[kBins] = s.hist[buffer];
+            clear_bins(s);
+            uint32_t(*hist)[kBins] = s.hist;
             for_each(data, count, [&](float v, int i) {
                 const uint64_t rank = rank_of(key_of(v), base + i);
                 if (rank < low || rank > high) return;
@@ -429,12 +446,18 @@ __device__ uint64_t search(cg::cluster_group& cluster, Shared& s, const float* d
     }
     cluster.sync();
     const int candidates = collect<kWeighted>(cluster, s, row);
-    for (int i = threadIdx.x; i < candidates; i += kThreads) {
-        const uint64_t rank = s.all[i];
-        uint64_t before = above;
-        for (int j = 0; j < candidates; ++j)
-            if (s.all[j] > rank) before += s.weight[j];
-        if (before < need && before + s.weight[i] >= need) s.found = rank;
+    // the element with which the running mass reaches `need`: the candidates are shared by all threads of the cluster
+    const int ctas = cluster.num_blocks(), threads = ctas * kThreads, me = cluster.block_rank() * kThreads + threadIdx.x;
+    const int lanes = lanes_of(candidates, threads), lane = me & (lanes - 1);
+    for (int base = 0; base < candidates; base += threads / lanes) {
+        const int i = base + me / lanes;
+        const uint64_t rank = i < candidates ? s.all[i] : 0;
+        uint64_t sum = 0;
+        for (int j = lane; j < candidates; j += lanes) sum += s.all[j] > rank ? s.weight[j] : 0;
+        for (int d = lanes >> 1; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+        const uint64_t before = above + sum;
+        if (i < candidates && lane == 0 && before < need && before + s.weight[i] >= need)
+            for (int r = 0; r < ctas; ++r) cluster.map_shared_rank(&s, r)->found = rank;
     }
     cluster.sync();  // found is written, and nobody still reads this CTA's candidates
     const uint64_t rank = s.found;
@@ -453,67 +476,58 @@ __device__ __forceinline__ float logprob_of(const Row& row, float v, uint64_t to
 
 // The rest of a row whose candidates are few, in one CTA: ranked, cut by top-k, top-p (of row_total,
 // or, where that is 0, of what top-k keeps) and min-p, and summed in vocabulary order.  Quadratic in
-// the number of candidates, each thread with its own.
+// the number of candidates, each for one to 32 neighbouring threads.
 __device__ void finish_few(cg::cluster_group& cluster, Shared& s, const Params& p, const Row& row, int row_index, int top_k,
                            float top_p, double least, uint64_t row_total) {
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    const int t = threadIdx.x, warp = t >> 5;
     const int candidates = collect<true>(cluster, s, row);
-    constexpr int kOwn = kCandidates / kThreads;
-    uint64_t rank[kOwn], weight[kOwn], before[kOwn];
+    const int lanes = lanes_of(candidates, kThreads), lane = t & (lanes - 1), i = t / lanes;
+    const bool present = i < candidates;
+    const uint64_t rank = present ? s.all[i] : 0;
+    uint64_t weight = present ? s.weight[i] : 0;
+    auto group_sum = [&](auto v) {
+        for (int d = lanes >> 1; d; d >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, d);
+        return v;
+    };
     auto total_of_kept = [&]() {
-        uint64_t sum = 0;
-#pragma unroll
-        for (int o = 0; o < kOwn; ++o) sum += weight[o];
-        sum = warp_total(sum);
+        uint64_t sum = warp_total(lane == 0 ? weight : 0);
         __syncthreads();
-        if (lane == 0) s.warp_sum[warp] = sum;
+        if ((t & 31) == 0) s.warp_sum[warp] = sum;
         __syncthreads();
         sum = 0;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) sum += s.warp_sum[w];
         return sum;
     };
-#pragma unroll
-    for (int o = 0; o < kOwn; ++o) {
-        const int i = t + o * kThreads;
-        rank[o] = weight[o] = before[o] = 0;
-        if (i >= candidates) continue;
-        rank[o] = s.all[i];
-        weight[o] = s.weight[i];
-        int place = 0;
-        for (int j = 0; j < candidates; ++j)
-            if (s.all[j] > rank[o]) {
+    int place = 0;
+    uint64_t before = 0;
+    if (present)
+        for (int j = lane; j < candidates; j += lanes)
+            if (s.all[j] > rank) {
                 ++place;
-                before[o] += s.weight[j];
+                before += s.weight[j];
             }
-        if (top_k > 0 && place >= top_k) weight[o] = 0;
-    }
+    place = group_sum(place);
+    before = group_sum(before);
+    if (top_k > 0 && place >= top_k) weight = 0;
     if (top_p < 1.0f) {
         const uint64_t total = row_total ? row_total : total_of_kept();
-        const uint64_t need = top_p > 0.0f ? share_of(top_p, total, true) : 1;
-#pragma unroll
-        for (int o = 0; o < kOwn; ++o)
-            if (before[o] >= need) weight[o] = 0;
+        if (before >= (top_p > 0.0f ? share_of(top_p, total, true) : 1)) weight = 0;
     }
-#pragma unroll
-    for (int o = 0; o < kOwn; ++o)
-        if ((double)weight[o] < least && value_of((uint32_t)(rank[o] >> 32)) != row.top) weight[o] = 0;
+    const float value = value_of((uint32_t)(rank >> 32));
+    if ((double)weight < least && value != row.top) weight = 0;
     const uint64_t total = total_of_kept();  // between its barriers everyone has read s.weight
     const uint64_t border = border_of(p.uniforms[row_index], total);
-#pragma unroll
-    for (int o = 0; o < kOwn; ++o)
-        if (t + o * kThreads < candidates) s.weight[t + o * kThreads] = weight[o];
+    if (present && lane == 0) s.weight[i] = weight;
     __syncthreads();
-#pragma unroll
-    for (int o = 0; o < kOwn; ++o) {
-        if (weight[o] == 0) continue;
-        uint64_t running = 0;
-        for (int j = 0; j < candidates; ++j)
-            if ((uint32_t)s.all[j] > (uint32_t)rank[o]) running += s.weight[j];  // a lower index has the larger complement
-        if (running <= border && running + weight[o] > border) {
-            p.tokens[row_index] = (long long)(0xFFFFFFFFu - (uint32_t)rank[o]);
-            p.logprobs[row_index] = logprob_of(row, value_of((uint32_t)(rank[o] >> 32)), total);
-        }
+    uint64_t running = 0;
+    if (weight != 0)  // the same for all threads of a candidate
+        for (int j = lane; j < candidates; j += lanes)
+            if ((uint32_t)s.all[j] > (uint32_t)rank) running += s.weight[j];  // a lower index has the larger complement
+    running = group_sum(running);
+    if (weight != 0 && lane == 0 && running <= border && running + weight > border) {
+        p.tokens[row_index] = (long long)(0xFFFFFFFFu - (uint32_t)rank);
+        p.logprobs[row_index] = logprob_of(row, value, total);
     }
 }
 
@@ -625,14 +639,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
         uint64_t need = top_k;
         found = first_step<false>(cluster, s, data, count, first, row, 0, need, 0.0f, buffer);
         if (found.total > need) {
-            few = found.through <= kCandidates;
+            few = found.through <= kFew;
             if (!few) threshold = search<false>(cluster, s, data, count, first, row, 0, need, found, buffer);
         }
     }
     if (!few && top_p < 1.0f) {
         uint64_t need = 1;
         found = first_step<true>(cluster, s, data, count, first, row, threshold, need, top_p, buffer);
-        few = threshold == 0 && found.through <= kCandidates;
+        few = threshold == 0 && found.through <= kFew;
         if (few)
             row_total = found.total;
         else {
@@ -650,36 +664,44 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
         return;
     }
 
-    // the kept weight of every warp's run of the slice
-    auto kept_weight = [&](int i) -> uint64_t {
-        const float v = data[i];
-        const bool kept = v != -INFINITY && rank_of(key_of(v), (uint32_t)(first + i)) >= threshold;
-        const uint64_t w = weight_of(row, v);
-        return kept && (v == row.top || (double)w >= least) ? w : 0;
+    // Every thread has neighbouring elements, at most 64, and takes them in an order of its own, so that a
+    // warp's reads meet few banks twice.  Which are kept is known before any weight is computed: in a
+    // nucleus, few.
+    const int own = max((count + kThreads - 1) / kThreads, 1), from = min(t * own, count), to = min(from + own, count);
+    auto kept = [&](float v, int i) {
+        return v != -INFINITY && rank_of(key_of(v), (uint32_t)(first + i)) >= threshold;
     };
-    const int run = (count + kThreads - 1) / kThreads * 32;
-    const int from = min(warp * run, count), to = min(from + run, count);
-    auto sum_runs = [&]() {
-        uint64_t sum = 0;
-#pragma unroll 4
-        for (int i = from + lane; i < to; i += 32) sum += kept_weight(i);
-        return warp_total(sum);
+    auto kept_weight = [&](float v) -> uint64_t {
+        const uint64_t w = weight_of(row, v);
+        return v == row.top || (double)w >= least ? w : 0;
+    };
+    auto sum_own = [&]() {
+        uint64_t mask = 0, sum = 0;
+        for (int e = 0, at = lane % own; e < own; ++e, at = at + 1 < own ? at + 1 : 0) {
+            const int i = from + at;
+            if (i < to && kept(data[i], i)) mask |= (uint64_t)1 << at;
+        }
+        while (mask) {
+            const int at = __ffsll((long long)mask) - 1;
+            mask &= mask - 1;
+            sum += kept_weight(data[from + at]);
+        }
+        return sum;
     };
     // What this CTA keeps: the bins above the one with top-p's threshold and, of that one, the
     // candidates down to it; where there is no such step, or min-p cuts too, the sum over its slice.
     const bool from_bins = in_bins && !(least > 0.0);
     uint64_t sum = 0;
     if (from_bins) {
-        const uint32_t(*hist)[kBins] = s.hist[buffer ^ 1];
-        if (t < (int)found.bin) sum = (uint64_t)hist[1][t] + ((uint64_t)hist[2][t] << 15) + ((uint64_t)hist[3][t] << 30);
+        if (t < (int)found.bin) sum = s.bin_weight[buffer ^ 1][t];
         for (int i = t; i < (int)s.count; i += kThreads)
             if (s.mine[i] >= threshold) sum += weight_of(row, value_of((uint32_t)(s.mine[i] >> 32)));
-        sum = warp_total(sum);
     } else {
-        sum = sum_runs();
+        sum = sum_own();
     }
+    const uint64_t warp_sum = warp_total(sum);
     __syncthreads();
-    if (lane == 0) s.warp_sum[warp] = sum;
+    if (lane == 0) s.warp_sum[warp] = warp_sum;
     __syncthreads();
     if (t == 0) {
         uint64_t all = 0;
@@ -694,26 +716,30 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
         if (r < rank_in_cluster) before += sums[r];
     });
     const uint64_t border = border_of(p.uniforms[row_index], total);
-    if (from_bins && before <= border && before + s.cta_sum > border) {  // the token is in this CTA's slice
-        sum = sum_runs();
-        __syncthreads();
-        if (lane == 0) s.warp_sum[warp] = sum;
-        __syncthreads();
-    }
-    const bool here = before <= border && before + s.cta_sum > border;
-    for (int w = 0; w < warp; ++w) before += s.warp_sum[w];
-    if (here && before <= border && before + s.warp_sum[warp] > border) {
-        // this warp's run holds the token
-        for (int i0 = from; i0 < to; i0 += 32) {
-            const int i = i0 + lane;
-            const uint64_t w = i < to ? kept_weight(i) : 0;
-            const uint64_t running = warp_running(w);
-            if (w != 0 && before + running > border && before + running - w <= border) {
-                p.tokens[row_index] = first + i;
-                p.logprobs[row_index] = logprob_of(row, data[i], total);
+    if (before <= border && before + s.cta_sum > border) {  // the token is in this CTA's slice
+        if (from_bins) {
+            sum = sum_own();
+            const uint64_t sum_of_warp = warp_total(sum);
+            __syncthreads();
+            if (lane == 0) s.warp_sum[warp] = sum_of_warp;
+            __syncthreads();
+        }
+        for (int w = 0; w < warp; ++w) before += s.warp_sum[w];
+        if (before <= border && before + s.warp_sum[warp] > border) {  // ... in this warp's elements
+            const uint64_t running = before + warp_running(sum);
+            const uint32_t owner = __ballot_sync(0xFFFFFFFFu, running - sum <= border && running > border);
+            const int start = __shfl_sync(0xFFFFFFFFu, from, __ffs(owner) - 1), stop = __shfl_sync(0xFFFFFFFFu, to, __ffs(owner) - 1);
+            before = __shfl_sync(0xFFFFFFFFu, running - sum, __ffs(owner) - 1);
+            for (int i0 = start; i0 < stop; i0 += 32) {
+                const int i = i0 + lane;
+                const uint64_t w = i < stop && kept(data[i], i) ? kept_weight(data[i]) : 0;
+                const uint64_t through = before + warp_running(w);
+                if (w != 0 && through > border && through - w <= border) {
+                    p.tokens[row_index] = first + i;
+                    p.logprobs[row_index] = logprob_of(row, data[i], total);
+                }
+                before = __shfl_sync(0xFFFFFFFFu, through, 31);
             }
-            before += __shfl_sync(0xFFFFFFFFu, running, 31);
-            if (before > border) break;
         }
     }
     cluster.sync();  // nobody leaves while its sums may still be read
