@@ -38,7 +38,6 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
-#include <type_traits>
 
 #include "abi_common.cuh"
 
@@ -49,7 +48,7 @@ constexpr int kWarps = 16;
 constexpr int kThreads = kWarps * 32;
 constexpr int kFewTokens = 8;          // up to here a CTA converts the activations itself
 constexpr int kChunk = 128;          // reduction elements of one warp step: 64 bytes of a row's codes
-constexpr int kPartialFloats = 23552;  // 92 KiB of partial sums per CTA
+constexpr int kPartialFloats = 20480;  // 80 KiB of partial sums per CTA
 constexpr int kRing = 3;             // tiles of codes and scales in shared memory, 36 KiB each at two chunks per warp
 
 // one chunk of eight tokens, 36 words for every 32 elements: the lanes' reads meet no bank twice
@@ -59,6 +58,9 @@ constexpr int kStagePieces = kWarps * kStageWords / 4;
 // 16-byte pieces of a ring slot: the codes of 16 rows and `depth` chunks per warp, and their scales
 // (16 rows x 8 bytes, half of it used for blocks of 32)
 __host__ __device__ constexpr int slot_pieces(int depth) { return depth * 2 * kThreads + kWarps * depth * 8; }
+// ... and of a warp's part of it where rows start anywhere: for 16 rows the aligned pieces that hold their
+// bytes of one chunk, nine of 8 bytes of codes and three of 4 of scales
+constexpr int kPieceSlot = 16 * (9 * 8 + 3 * 4) / 16;
 
 struct Params {
     const void* x;
@@ -236,39 +238,6 @@ struct Piece {
     uint32_t scales;  // byte 0: elements 0..15 of the 32, byte 1: elements 16..31 (B = 32: byte 0 for all)
 };
 
-// Rows that do not start on 16-byte boundaries.
-enum class Loads {
-    kWords,  // any rows: aligned words, shifted into place; reads up to 19 bytes behind a row's end
-    kBytes   // byte by byte: the first row and the last ones of the weight
-};
-
-// The codes at `code` bytes and the scales at `scale` bytes (that of the lane's first element; the
-// row's last one is `last_scale`); `left`: the row's bytes from `code` on.
-template <Loads kLoads, int kBlock>
-__device__ __forceinline__ Piece load_piece(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
-                                            uint32_t code, uint32_t scale, uint32_t last_scale, int left) {
-    Piece piece;
-    const uint8_t* source = codes + code;
-    uint32_t w[4];
-    if constexpr (kLoads == Loads::kWords) {
-        const uint32_t off = (uint32_t)((uintptr_t)source & 3);
-        const uint32_t* words = reinterpret_cast<const uint32_t*>(source - off);
-        uint32_t v[5];
-#pragma unroll
-        for (int i = 0; i < 5; ++i) v[i] = __ldg(words + i);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(v[i], v[i + 1], 8 * off);
-    } else {
-        w[0] = w[1] = w[2] = w[3] = 0;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) w[i / 4] |= (uint32_t)__ldg(source + min(i, left - 1)) << (8 * (i % 4));
-    }
-    piece.codes = make_uint4(w[0], w[1], w[2], w[3]);
-    piece.scales = __ldg(scales + scale);
-    if (kBlock == 16) piece.scales |= (uint32_t)__ldg(scales + min(scale + 1, last_scale)) << 8;
-    return piece;
-}
-
 // kBytes aligned bytes, of which the first `there` exist; the others become zero
 template <int kBytes>
 __device__ __forceinline__ void copy_part_async(void* to, const uint8_t* from, int there) {
@@ -284,6 +253,57 @@ __device__ __forceinline__ void copy_async(void* to, const uint8_t* from) {
         asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(address), "l"(from) : "memory");
     else
         asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(address), "l"(from), "n"(kBytes) : "memory");
+}
+
+// Rows that start anywhere.  Of an array of `bytes` bytes the aligned pieces that hold `count` rows' bytes from
+// `column` on, a multiple of kSize: kPieces a row, neighbouring lanes side by side.  `row`, the first of
+// the rows, and the others after it stand for row >> shift of the array.  What lies behind the array
+// becomes zero.
+template <int kSize, int kPieces>
+__device__ __forceinline__ void copy_pieces(void* to, const uint8_t* array, int64_t bytes, int row_bytes, int shift, int row, int count,
+                                            int column) {
+    const int lane = threadIdx.x & 31;
+    const int64_t start = (row >> shift) * (int64_t)row_bytes;
+    const uint32_t off = (uint32_t)((uintptr_t)array + start) & (kSize - 1);
+    const uint8_t* base = array + start - off;  // below the array for its first row if it does not start on a piece
+    const int64_t left = bytes - start + off;   // from base on
+    const bool inner = start >= off && left > (int64_t)count * row_bytes + column + kSize * kPieces;
+    uint8_t* target = reinterpret_cast<uint8_t*>(to) + lane * kSize;
+    int r = lane / kPieces, piece = lane % kPieces;
+    for (int at = lane; at < count * kPieces; at += 32, target += 32 * kSize) {
+        const uint32_t from = (((row + r >> shift) - (row >> shift)) * row_bytes + off & ~(kSize - 1u)) + column + kSize * piece;
+        if (inner)
+            copy_async<kSize>(target, base + from);
+        else if (base + from < array)
+            for (uint32_t e = 0; e < kSize; ++e) target[e] = e >= off && e < left ? base[e] : 0;
+        else
+            copy_part_async<kSize>(target, from < left ? base + from : base + kSize, from < left ? (int)min(left - from, (int64_t)kSize) : 0);
+        r += 32 / kPieces, piece += 32 % kPieces;
+        if (piece >= kPieces) piece -= kPieces, ++r;
+    }
+}
+
+// ... of the weight, for one chunk: nine pieces of 8 bytes of a row's codes, three of 4 of its scales
+template <int kBlock>
+__device__ __forceinline__ void copy_row_pieces(const Params& p, uint4* codes_to, uint4* scales_to, int row, int count, int chunk) {
+    copy_pieces<8, 9>(codes_to, p.codes, p.rows * p.code_stride, (int)p.code_stride, 0, row, count, chunk * (kChunk / 2));
+    copy_pieces<4, 3>(scales_to, p.scales, ((int64_t)(p.rows - 1 >> p.row_shift) + 1) * p.scale_stride, (int)p.scale_stride, p.row_shift,
+                      row, count, chunk * (kChunk / kBlock));
+}
+
+// a lane's share of row `row` + r from there: the words shifted into place
+template <int kBlock>
+__device__ __forceinline__ Piece piece_of_row(const Params& p, const uint4* codes_from, const uint4* scales_from, int row, int r, int chunk) {
+    const int c = threadIdx.x & 3;
+    const uint32_t in_piece = (uint32_t)((uintptr_t)p.codes + (row + r) * p.code_stride) & 7, off = 8 * (in_piece & 3);
+    const uint32_t* at = reinterpret_cast<const uint32_t*>(codes_from) + r * 18 + (in_piece >> 2) + 4 * c;
+    const uint32_t scale_off = (uint32_t)((uintptr_t)p.scales + (row + r >> p.row_shift) * p.scale_stride + chunk * (kChunk / kBlock)) & 3;
+    const uint8_t* scale_at = reinterpret_cast<const uint8_t*>(scales_from) + r * 12 + scale_off + c * (32 / kBlock);
+    Piece piece;
+    piece.codes = make_uint4(__funnelshift_r(at[0], at[1], off), __funnelshift_r(at[1], at[2], off),
+                             __funnelshift_r(at[2], at[3], off), __funnelshift_r(at[3], at[4], off));
+    piece.scales = kBlock == 16 ? scale_at[0] | (uint32_t)scale_at[1] << 8 : scale_at[0];
+    return piece;
 }
 
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
@@ -326,12 +346,12 @@ __device__ __forceinline__ void store(const Params& p, int token, int64_t row, f
 // Up to eight tokens.  kDepth: chunks that a warp keeps in registers.
 template <bool kFp32, int kDepth, bool kVector, int kBlock>
 __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params p) {
-    extern __shared__ uint4 ring[];  // kVector: [slot]{codes [chunk][row half][thread], scales [warp][chunk][row]}
-    constexpr int kSlot = slot_pieces(kDepth);
-    // kVector: the ring; otherwise one chunk of eight tokens' activations per warp, on its way to the lanes
-    float* partial = reinterpret_cast<float*>(ring + (kVector ? kRing * kSlot : kStagePieces));  // [warp][token][row of the block]
+    // the ring: kVector: [slot]{codes [chunk][row half][thread], scales [warp][chunk][row]}, otherwise [slot][warp];
+    // there one chunk of eight tokens' activations per warp as well, on its way to the lanes
+    extern __shared__ uint4 ring[];
+    constexpr int kSlot = kVector ? slot_pieces(kDepth) : kWarps * kPieceSlot;
+    float* partial = reinterpret_cast<float*>(ring + kRing * kSlot + (kVector ? 0 : kStagePieces));  // [warp][token][row of the block]
     constexpr int kParts = kFp32 ? 3 : 1;
-    constexpr int kBlockShift = kBlock == 16 ? 4 : 5;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int share = blockIdx.x % p.split, group = blockIdx.x / p.split, groups = gridDim.x / p.split;
     const int all_chunks = (p.k + kChunk - 1) / kChunk;
@@ -347,32 +367,10 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
         const uint8_t* codes = p.codes + row0 * p.code_stride;
         const int scale_row0 = row0 >> p.row_shift;
         const uint8_t* scales = p.scales + scale_row0 * p.scale_stride;
-        // rows from which 3 bytes back and 19 bytes further on are still inside the weight
-        const bool inner = row0 * p.code_stride >= 3 && (int64_t)(p.rows - row0 - row_count) * p.code_stride >= 20;
-        // Pieces of the tiles to come.  Wide rows: codes and scales wait in a ring in shared memory,
-        // kRing - 1 tiles ahead: the codes in the slots of the lane that decodes them, the scale bytes
-        // of a row's chunk side by side.  A row or chunk behind the end is not copied: what its slot
-        // holds is finite, and meets zeros or is not stored.  Other rows: in registers, one tile ahead.
-        Piece next[kDepth][2];
-        auto load = [&](int pass, int tile) {
-#pragma unroll
-            for (int d = 0; d < kDepth; ++d) {
-                // a chunk behind the end is read as the row's last bytes
-                const int byte = min((first_chunk + (pass * kDepth + d) * kWarps + warp) * (kChunk / 2) + 16 * c, stride - 1);
-                const int block = byte * 2 >> kBlockShift;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int row = min(tile + g + 8 * h, row_count - 1);
-                    const uint32_t code = row * stride + byte;
-                    const uint32_t scale = ((row0 + row >> p.row_shift) - scale_row0) * scale_stride;
-                    const uint32_t last = scale + scale_stride - 1;
-                    if (inner)
-                        next[d][h] = load_piece<Loads::kWords, kBlock>(codes, scales, code, scale + block, last, 0);
-                    else
-                        next[d][h] = load_piece<Loads::kBytes, kBlock>(codes, scales, code, scale + block, last, stride - byte);
-                }
-            }
-        };
+        // Codes and scales of the tiles to come wait in a ring in shared memory, kRing - 1 tiles ahead.  Wide
+        // rows: the codes in the slots of the lane that decodes them, the scale bytes of a row's chunk side
+        // by side; others: the aligned pieces that hold them.  A row or chunk behind the end is not copied:
+        // what its slot holds is finite, and meets zeros or is not stored.
         // the (pass, tile) that is copied next, and where this lane's first row of it lies
         int ahead_pass = 0, ahead_tile = 0;
         const uint8_t *ahead_codes = nullptr, *ahead_scales = nullptr;
@@ -382,7 +380,14 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
             ahead_scales = scales + chunk * (kChunk / kBlock);
         };
         auto copy_ahead = [&](int slot) {
-            if (ahead_pass < passes) {
+            if (!kVector && ahead_pass < passes) {
+                const int chunk = first_chunk + ahead_pass * kWarps + warp;
+                uint4* to = ring + slot * kSlot + warp * kPieceSlot;
+                if (chunk < chunks)
+                    copy_row_pieces<kBlock>(p, to, to + 16 * 9 / 2, row0 + ahead_tile, min(16, row_count - ahead_tile), chunk);
+                ahead_tile += 16;
+                if (ahead_tile >= row_count) ahead_tile = 0, ++ahead_pass;
+            } else if (ahead_pass < passes) {
                 uint4* to = ring + slot * kSlot + threadIdx.x;
                 uint8_t* scales_to = reinterpret_cast<uint8_t*>(ring + slot * kSlot + kDepth * 2 * kThreads) + warp * kDepth * 128;
                 const int row = ahead_tile + g + 8 * c;  // lanes 0 and 1 of a row bring the scales of it and the one 8 on
@@ -408,13 +413,9 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
         int slot_now = 0;
-        if constexpr (kVector) {
-            locate();
+        if (kVector) locate();
 #pragma unroll
-            for (int i = 0; i < kRing - 1; ++i) copy_ahead(i);
-        } else {
-            load(0, 0);
-        }
+        for (int i = 0; i < kRing - 1; ++i) copy_ahead(i);
         for (int pass = 0; pass < passes; ++pass) {
             uint32_t b[kDepth][kParts][16];
             float undo[kDepth][2];
@@ -424,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
                 float mine;
                 make_fragments<kFp32>(
                     kVector ? load_raw<kFp32>(p, g, g < tokens && chunk < chunks, chunk)
-                            : load_staged<kFp32>(p, 0, chunk < chunks ? tokens : 0, chunk, reinterpret_cast<uint32_t*>(ring) + warp * kStageWords),
+                            : load_staged<kFp32>(p, 0, chunk < chunks ? tokens : 0, chunk, reinterpret_cast<uint32_t*>(ring + kRing * kSlot) + warp * kStageWords),
                     b[d], mine);
                 undo[d][0] = __shfl_sync(0xFFFFFFFFu, mine, 8 * c);
                 undo[d][1] = __shfl_sync(0xFFFFFFFFu, mine, 8 * c + 4);
@@ -433,11 +434,11 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
 #pragma unroll 2
             for (int tile = 0; tile < row_count; tile += 16, slot += 16) {
                 Piece now[kDepth][2];
+                __syncwarp();  // the slot that is filled now has been read
+                copy_ahead(slot_now == 0 ? kRing - 1 : slot_now - 1);
+                asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
+                __syncwarp();  // scales, and all of other rows, come from other lanes
                 if constexpr (kVector) {
-                    __syncwarp();  // the slot that is filled now has been read
-                    copy_ahead(slot_now == 0 ? kRing - 1 : slot_now - 1);
-                    asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
-                    __syncwarp();  // scales come from other lanes
                     const uint4* from = ring + slot_now * kSlot + threadIdx.x;
                     const uint8_t* scales_from =
                         reinterpret_cast<const uint8_t*>(ring + slot_now * kSlot + kDepth * 2 * kThreads) + warp * kDepth * 128;
@@ -449,15 +450,13 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
                             const uint8_t* at = scales_from + d * 128 + (g + 8 * h) * (kChunk / kBlock) + c * (32 / kBlock);
                             now[d][h].scales = kBlock == 16 ? *reinterpret_cast<const uint16_t*>(at) : *at;
                         }
-                    slot_now = slot_now == kRing - 1 ? 0 : slot_now + 1;
                 } else {
+                    const uint4* from = ring + slot_now * kSlot + warp * kPieceSlot;
 #pragma unroll
-                    for (int d = 0; d < kDepth; ++d) now[d][0] = next[d][0], now[d][1] = next[d][1];
-                    if (tile + 16 < row_count)
-                        load(pass, tile + 16);
-                    else if (pass + 1 < passes)
-                        load(pass + 1, 0);
+                    for (int h = 0; h < 2; ++h)
+                        now[0][h] = piece_of_row<kBlock>(p, from, from + 16 * 9 / 2, row0 + tile, g + 8 * h, first_chunk + pass * kWarps + warp);
                 }
+                slot_now = slot_now == kRing - 1 ? 0 : slot_now + 1;
                 float total[4];
 #pragma unroll
                 for (int d = 0; d < kDepth; ++d) {
@@ -529,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
 
 template <bool kFp32, int kDepth, bool kVector, int kBlock>
 int launch_few(Params p, cudaStream_t stream) {
-    constexpr size_t kRingBytes = (kVector ? kRing * slot_pieces(kDepth) : kStagePieces) * sizeof(uint4);
+    constexpr size_t kRingBytes = (kVector ? kRing * slot_pieces(kDepth) : kRing * kWarps * kPieceSlot + kStagePieces) * sizeof(uint4);
     constexpr auto kKernel = packed_matvec_kernel<kFp32, kDepth, kVector, kBlock>;
     cudaError_t error = allow_shared<kKernel>((int)kRingBytes + kPartialFloats * 4);
     if (error != cudaSuccess) return record_cuda_error(error);
@@ -633,39 +632,12 @@ __global__ void __launch_bounds__(kManyThreads, kFp32 || kTiles > 4 ? 1 : 2)
     // codes and scales of the chunks to come: wide rows as in the kernel for few tokens, with the scales of
     // a row per lane; others word by word
     uint4* slots = ring + 2 * kManyRing * kStage + warp * kManyRing * kSlot;
-    // Of an array of `bytes` bytes the aligned pieces that hold the rows' bytes from `column` on, a multiple of
-    // their size: kPieces a row, neighbouring lanes side by side.  What lies behind the array becomes zero.
-    auto copy_pieces = [&](auto size, auto pieces, void* to, const uint8_t* array, int64_t bytes, int row_bytes, int shift, int column) {
-        constexpr int kSize = decltype(size)::value, kPieces = decltype(pieces)::value;
-        const int64_t start = (row0 >> shift) * (int64_t)row_bytes;
-        const uint32_t off = (uint32_t)((uintptr_t)array + start) & (kSize - 1);
-        const uint8_t* base = array + start - off;  // below the array for its first row if it does not start on a piece
-        const int64_t left = bytes - start + off;   // from base on
-        const bool inner = start >= off && left > (int64_t)32 * row_bytes + column + kSize * kPieces;
-        uint8_t* target = reinterpret_cast<uint8_t*>(to) + lane * kSize;
-        int row = lane / kPieces, piece = lane % kPieces;
-        for (int at = lane; at < row_count * kPieces; at += 32, target += 32 * kSize) {
-            const uint32_t from = (((row0 + row >> shift) - (row0 >> shift)) * row_bytes + off & ~(kSize - 1u)) + column + kSize * piece;
-            if (inner)
-                copy_async<kSize>(target, base + from);
-            else if (base + from < array)
-                for (uint32_t e = 0; e < kSize; ++e) target[e] = e >= off && e < left ? base[e] : 0;
-            else
-                copy_part_async<kSize>(target, from < left ? base + from : base + kSize, from < left ? (int)min(left - from, (int64_t)kSize) : 0);
-            row += 32 / kPieces, piece += 32 % kPieces;
-            if (piece >= kPieces) piece -= kPieces, ++row;
-        }
-    };
     auto copy_codes = [&](int i) {
         if (i < count && active) {
             const int chunk = first + 2 * i;
             uint4* to = slots + i % kManyRing * kSlot;
             if constexpr (!kVector) {
-                copy_pieces(std::integral_constant<int, 8>(), std::integral_constant<int, 9>(), to, p.codes, p.rows * p.code_stride, stride,
-                            0, chunk * (kChunk / 2));
-                copy_pieces(std::integral_constant<int, 4>(), std::integral_constant<int, 3>(), to + 32 * 9 / 2, p.scales,
-                            ((int64_t)(p.rows - 1 >> p.row_shift) + 1) * p.scale_stride, scale_stride, p.row_shift,
-                            chunk * (kChunk / kBlock));
+                copy_row_pieces<kBlock>(p, to, to + 32 * 9 / 2, row0, row_count, chunk);
             } else {
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
@@ -718,20 +690,10 @@ __global__ void __launch_bounds__(kManyThreads, kFp32 || kTiles > 4 ? 1 : 2)
                 now[q / 2][q % 2].scales = kBlock == 16 ? *reinterpret_cast<const uint16_t*>(at) : *at;
             }
         } else {
-            const uint32_t* words = reinterpret_cast<const uint32_t*>(slots + i % kManyRing * kSlot);
-            const int chunk = first + 2 * i;
+            const uint4* slot = slots + i % kManyRing * kSlot;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int row = 8 * q + g;
-                const uint32_t in_piece = (uint32_t)((uintptr_t)p.codes + (row0 + row) * p.code_stride) & 7, off = in_piece & 3;
-                const uint32_t* at = words + row * 18 + (in_piece >> 2) + 4 * c;
-                now[q / 2][q % 2].codes = make_uint4(__funnelshift_r(at[0], at[1], 8 * off), __funnelshift_r(at[1], at[2], 8 * off),
-                                                     __funnelshift_r(at[2], at[3], 8 * off), __funnelshift_r(at[3], at[4], 8 * off));
-                const uint32_t scale_off =
-                    (uint32_t)((uintptr_t)p.scales + (row0 + row >> p.row_shift) * p.scale_stride + chunk * (kChunk / kBlock)) & 3;
-                const uint8_t* scale_at = reinterpret_cast<const uint8_t*>(words + 32 * 18 + row * 3) + scale_off + c * (32 / kBlock);
-                now[q / 2][q % 2].scales = kBlock == 16 ? scale_at[0] | (uint32_t)scale_at[1] << 8 : scale_at[0];
-            }
+            for (int q = 0; q < 4; ++q)
+                now[q / 2][q % 2] = piece_of_row<kBlock>(p, slot, slot + 32 * 9 / 2, row0, 8 * q + g, first + 2 * i);
         }
         const uint4* from = stages + i % kManyRing * kStage + lane;
         const float2* undo_from = reinterpret_cast<const float2*>(from - lane + kTiles * kParts * 128) + c;
