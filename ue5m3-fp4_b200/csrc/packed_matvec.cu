@@ -58,9 +58,10 @@ constexpr int kStagePieces = kWarps * kStageWords / 4;
 // 16-byte pieces of a ring slot: the codes of 16 rows and `depth` chunks per warp, and their scales
 // (16 rows x 8 bytes, half of it used for blocks of 32)
 __host__ __device__ constexpr int slot_pieces(int depth) { return depth * 2 * kThreads + kWarps * depth * 8; }
-// ... and of a warp's part of it where rows start anywhere: for 16 rows the aligned pieces that hold their
-// bytes of one chunk, nine of 8 bytes of codes and three of 4 of scales
-constexpr int kPieceSlot = 16 * (9 * 8 + 3 * 4) / 16;
+// ... and of one where rows start anywhere: for 16 rows the aligned pieces that hold their bytes of the 16
+// warps' chunks, codes and scales
+constexpr int kRowPieces = kWarps * kChunk / 2 / 16 + 1, kRowScalePieces = kWarps * kChunk / 16 / 16 + 1;
+constexpr int kRowSlot = 16 * (kRowPieces + kRowScalePieces);
 
 struct Params {
     const void* x;
@@ -283,6 +284,20 @@ __device__ __forceinline__ void copy_pieces(void* to, const uint8_t* array, int6
     }
 }
 
+// The aligned pieces of 16 bytes that hold `wanted` of an array's bytes from `at` on, by one warp.
+__device__ __forceinline__ void copy_run(uint4* to, const uint8_t* array, int64_t bytes, int64_t at, int wanted) {
+    const int lane = threadIdx.x & 31, off = (int)((uintptr_t)(array + at) & 15);
+    for (int piece = lane; piece * 16 < off + wanted; piece += 32) {
+        const int64_t from = at - off + 16 * piece, left = bytes - from;
+        if (from < 0)  // the first piece of an array that does not start on one
+            for (int e = 0; e < 16; ++e) reinterpret_cast<uint8_t*>(to + piece)[e] = from + e >= 0 && e < left ? array[from + e] : 0;
+        else if (left >= 16)
+            copy_async<16>(to + piece, array + from);
+        else
+            copy_part_async<16>(to + piece, left > 0 ? array + from : array + at - off + 16, left > 0 ? (int)left : 0);
+    }
+}
+
 // ... of the weight, for one chunk: nine pieces of 8 bytes of a row's codes, three of 4 of its scales
 template <int kBlock>
 __device__ __forceinline__ void copy_row_pieces(const Params& p, uint4* codes_to, uint4* scales_to, int row, int count, int chunk) {
@@ -346,10 +361,10 @@ __device__ __forceinline__ void store(const Params& p, int token, int64_t row, f
 // Up to eight tokens.  kDepth: chunks that a warp keeps in registers.
 template <bool kFp32, int kDepth, bool kVector, int kBlock>
 __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params p) {
-    // the ring: kVector: [slot]{codes [chunk][row half][thread], scales [warp][chunk][row]}, otherwise [slot][warp];
+    // the ring: kVector: [slot]{codes [chunk][row half][thread], scales [warp][chunk][row]}, otherwise [slot]{codes [row], scales [row]};
     // there one chunk of eight tokens' activations per warp as well, on its way to the lanes
     extern __shared__ uint4 ring[];
-    constexpr int kSlot = kVector ? slot_pieces(kDepth) : kWarps * kPieceSlot;
+    constexpr int kSlot = kVector ? slot_pieces(kDepth) : kRowSlot;
     float* partial = reinterpret_cast<float*>(ring + kRing * kSlot + (kVector ? 0 : kStagePieces));  // [warp][token][row of the block]
     constexpr int kParts = kFp32 ? 3 : 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -369,7 +384,8 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
         const uint8_t* scales = p.scales + scale_row0 * p.scale_stride;
         // Codes and scales of the tiles to come wait in a ring in shared memory, kRing - 1 tiles ahead.  Wide
         // rows: the codes in the slots of the lane that decodes them, the scale bytes of a row's chunk side
-        // by side; others: the aligned pieces that hold them.  A row or chunk behind the end is not copied:
+        // by side; others: a row of the tile per warp, its bytes of all warps' chunks in one run, for which the
+        // CTA's warps wait for one another at every tile.  A row or chunk behind the end is not copied:
         // what its slot holds is finite, and meets zeros or is not stored.
         // the (pass, tile) that is copied next, and where this lane's first row of it lies
         int ahead_pass = 0, ahead_tile = 0;
@@ -381,10 +397,16 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
         };
         auto copy_ahead = [&](int slot) {
             if (!kVector && ahead_pass < passes) {
-                const int chunk = first_chunk + ahead_pass * kWarps + warp;
-                uint4* to = ring + slot * kSlot + warp * kPieceSlot;
-                if (chunk < chunks)
-                    copy_row_pieces<kBlock>(p, to, to + 16 * 9 / 2, row0 + ahead_tile, min(16, row_count - ahead_tile), chunk);
+                const int chunk = first_chunk + ahead_pass * kWarps, here = min(kWarps, chunks - chunk);
+                uint4* to = ring + slot * kSlot;
+                const int64_t row = row0 + ahead_tile + warp;
+                if (ahead_tile + warp < row_count) {
+                    copy_run(to + warp * kRowPieces, p.codes, p.rows * p.code_stride, row * p.code_stride + chunk * (kChunk / 2),
+                             here * (kChunk / 2));
+                    copy_run(to + 16 * kRowPieces + warp * kRowScalePieces, p.scales,
+                             ((int64_t)(p.rows - 1 >> p.row_shift) + 1) * p.scale_stride,
+                             (row >> p.row_shift) * p.scale_stride + chunk * (kChunk / kBlock), here * (kChunk / kBlock));
+                }
                 ahead_tile += 16;
                 if (ahead_tile >= row_count) ahead_tile = 0, ++ahead_pass;
             } else if (ahead_pass < passes) {
@@ -434,11 +456,11 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
 #pragma unroll 2
             for (int tile = 0; tile < row_count; tile += 16, slot += 16) {
                 Piece now[kDepth][2];
-                __syncwarp();  // the slot that is filled now has been read
-                copy_ahead(slot_now == 0 ? kRing - 1 : slot_now - 1);
-                asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
-                __syncwarp();  // scales, and all of other rows, come from other lanes
                 if constexpr (kVector) {
+                    __syncwarp();  // the slot that is filled now has been read
+                    copy_ahead(slot_now == 0 ? kRing - 1 : slot_now - 1);
+                    asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
+                    __syncwarp();  // scales come from other lanes
                     const uint4* from = ring + slot_now * kSlot + threadIdx.x;
                     const uint8_t* scales_from =
                         reinterpret_cast<const uint8_t*>(ring + slot_now * kSlot + kDepth * 2 * kThreads) + warp * kDepth * 128;
@@ -451,10 +473,26 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
                             now[d][h].scales = kBlock == 16 ? *reinterpret_cast<const uint16_t*>(at) : *at;
                         }
                 } else {
-                    const uint4* from = ring + slot_now * kSlot + warp * kPieceSlot;
+                    asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
+                    __syncthreads();  // all copies of this tile are there, and the slot before has been read
+                    copy_ahead(slot_now == 0 ? kRing - 1 : slot_now - 1);
+                    const uint4* from = ring + slot_now * kSlot;
+                    const int chunk = first_chunk + pass * kWarps;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        now[0][h] = piece_of_row<kBlock>(p, from, from + 16 * 9 / 2, row0 + tile, g + 8 * h, first_chunk + pass * kWarps + warp);
+                    for (int h = 0; h < 2; ++h) {
+                        const int r = g + 8 * h;
+                        const int64_t row = row0 + tile + r;
+                        const uint32_t off = (uint32_t)((uintptr_t)p.codes + row * p.code_stride) & 15;
+                        const uint32_t* at = reinterpret_cast<const uint32_t*>(from + r * kRowPieces) + (off >> 2) + warp * 16 + 4 * c;
+                        const uint32_t scale_off =
+                            (uint32_t)((uintptr_t)p.scales + (row >> p.row_shift) * p.scale_stride + chunk * (kChunk / kBlock)) & 15;
+                        const uint8_t* scale_at = reinterpret_cast<const uint8_t*>(from + 16 * kRowPieces + r * kRowScalePieces) + scale_off +
+                                                  warp * (kChunk / kBlock) + c * (32 / kBlock);
+                        const uint32_t turn = 8 * (off & 3);
+                        now[0][h].codes = make_uint4(__funnelshift_r(at[0], at[1], turn), __funnelshift_r(at[1], at[2], turn),
+                                                     __funnelshift_r(at[2], at[3], turn), __funnelshift_r(at[3], at[4], turn));
+                        now[0][h].scales = kBlock == 16 ? scale_at[0] | (uint32_t)scale_at[1] << 8 : scale_at[0];
+                    }
                 }
                 slot_now = slot_now == kRing - 1 ? 0 : slot_now + 1;
                 float total[4];
@@ -528,7 +566,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
 
 template <bool kFp32, int kDepth, bool kVector, int kBlock>
 int launch_few(Params p, cudaStream_t stream) {
-    constexpr size_t kRingBytes = (kVector ? kRing * slot_pieces(kDepth) : kRing * kWarps * kPieceSlot + kStagePieces) * sizeof(uint4);
+    constexpr size_t kRingBytes = (kVector ? kRing * slot_pieces(kDepth) : kRing * kRowSlot + kStagePieces) * sizeof(uint4);
     constexpr auto kKernel = packed_matvec_kernel<kFp32, kDepth, kVector, kBlock>;
     cudaError_t error = allow_shared<kKernel>((int)kRingBytes + kPartialFloats * 4);
     if (error != cudaSuccess) return record_cuda_error(error);
