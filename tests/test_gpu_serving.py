@@ -43,11 +43,12 @@ def packed_weight(rows: int, cols: int, block: int, two_d: bool, seed: int, low:
     return codes, scales
 
 
-def check_matvec(x, codes, scales, rows, cols, block, two_d, *, bias=None, out_dtype=None, amax=0.37, target=448.0):
+def check_matvec(x, codes, scales, rows, cols, block, two_d, *, bias=None, out_dtype=None, amax=0.37, target=448.0,
+                 placed=None):
     from ue5m3_fp4 import serving
     from ue5m3_fp4.serving.operators import decode_factor
 
-    got = serving.packed_matvec(x.cuda(), codes.cuda(), scales.cuda(), rows=rows, cols=cols, block_size=block,
+    got = serving.packed_matvec(x.cuda(), *(placed or (codes.cuda(), scales.cuda())), rows=rows, cols=cols, block_size=block,
                                 two_dimensional=two_d, tensor_amax=amax, scale_target=target,
                                 bias=None if bias is None else bias.cuda(), out_dtype=out_dtype)
     assert got.shape == (*x.shape[:-1], rows) and got.dtype is (out_dtype or x.dtype)
@@ -93,6 +94,24 @@ def test_matvec_of_many_tokens(tokens, rows, cols, block, two_d, dtype):
     for x in (wide[:, :cols].contiguous(), wide[:, 1:cols + 1]):  # rows on 16-byte boundaries, and not
         got = check_matvec(x, codes, scales, rows, cols, block, two_d, bias=bias)
         assert torch.equal(got, check_matvec(x, codes, scales, rows, cols, block, two_d, bias=bias))
+
+
+@pytest.mark.parametrize("block,two_d", [(16, False), (16, True), (32, False), (32, True)])
+@pytest.mark.parametrize("tokens", [1, 8, 20, 70])
+def test_matvec_of_weights_that_start_anywhere(tokens, block, two_d):
+    """The first and last bytes of codes and scales, at every place in the aligned pieces they are read by."""
+
+    for shift in (0, 1, 5, 15):
+        for rows, cols in ((1, 1), (2, 3), (17, 9), (40, 33), (33, 130), (5, 2049)):
+            codes, scales = packed_weight(rows, cols, block, two_d, seed=shift + cols)
+            placed = []
+            for part in (codes, scales):
+                buffer = torch.full((part.numel() + 48,), 0xFF, dtype=torch.uint8, device="cuda")
+                view = buffer[shift:shift + part.numel()].view(part.shape)
+                view.copy_(part)
+                placed.append(view)
+            x = torch.randn(tokens, cols, generator=torch.Generator().manual_seed(cols)).to(torch.bfloat16)
+            check_matvec(x, codes, scales, rows, cols, block, two_d, placed=placed)
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
