@@ -20,8 +20,8 @@
 // 16-row tile are not loaded, so that all SMs read the same number of bytes), every one of its
 // warps w the 128-element chunks w, w + 16, ... of the reduction axis.  A warp keeps the activations
 // of its chunks in registers (as mma fragments) while it walks over the CTA's rows; the sums of
-// the 16 warps meet in shared memory once per block of rows.  Measured: 1 x 21504 x 4096: 15.3 us,
-// 2.9 TB/s of 6.5; 8 x 4096 x 21504: 20.1 us, 2.3 TB/s; 1 x 512 x 4096: 4.7 us.  The walk itself reads
+// the 16 warps meet in shared memory once per block of rows.  Measured: 1 x 21504 x 4096: 15.6 us,
+// 2.8 TB/s of 6.5; 8 x 4096 x 21504: 20.5 us, 2.3 TB/s; 1 x 512 x 4096: 4.8 us.  The walk itself reads
 // at about three quarters of the memory's rate; the rest is the launch, the loading and conversion of
 // the activations (some 5000 cycles in which no weight is decoded) and the sums at the end.  Rows that
 // start anywhere come as aligned pieces and are shifted into place: 1 x 21504 x 4095: 29 us (word by
@@ -389,6 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
         // by side; others: a row of the tile per warp, its bytes of all warps' chunks in one run, for which the
         // CTA's warps wait for one another at every tile.  A row or chunk behind the end is not copied:
         // what its slot holds is finite, and meets zeros or is not stored.
+
         // the (pass, tile) that is copied next, and where this lane's first row of it lies
         int ahead_pass = 0, ahead_tile = 0;
         const uint8_t *ahead_codes = nullptr, *ahead_scales = nullptr;

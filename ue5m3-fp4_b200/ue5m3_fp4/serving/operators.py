@@ -60,6 +60,11 @@ def decode_factor(tensor_amax: float, scale_target: float) -> float:
 
 
 @functools.lru_cache(maxsize=4096)
+def _matvec_workspace_bytes(*sizes: int) -> int:
+    return _native.load().ue5m3_packed_matvec_workspace_bytes(*sizes)
+
+
+@functools.lru_cache(maxsize=4096)
 def _checked_factor(tensor_amax: float, scale_target: float) -> float:
     if not 0 <= tensor_amax < float("inf"):
         raise ValueError("tensor_amax must be finite and not negative")
@@ -126,7 +131,7 @@ def packed_matvec(
             raise ValueError("the last axis of x must be contiguous and its rows must not overlap")
         # more than eight rows: prepared once, in memory of the current stream's pool for this call alone
         library = _native.load()
-        need = library.ue5m3_packed_matvec_workspace_bytes(x_code, tokens, cols) if tokens > 8 else 0
+        need = _matvec_workspace_bytes(x_code, tokens, cols) if tokens > 8 else 0
         workspace = x.new_empty(need, dtype=torch.uint8) if need else None
         _call(library.ue5m3_packed_matvec, "ue5m3_packed_matvec", 2 if need else 1, index, flat.data_ptr(), x_code, tokens, ldx,
               codes.data_ptr(), scales.data_ptr(), rows, cols, block_size, two_dimensional, factor, bias_pointer,
