@@ -38,9 +38,9 @@ cudaError_t allow_shared(int bytes) {
 // once per kernel, device and size.
 template <auto kKernel>
 int resident_clusters(int size, int threads, int shared) {
-    static int known[64][5] = {};
+    static int known[64][9] = {};
     int device = 0;
-    if (cudaGetDevice(&device) != cudaSuccess || device >= 64 || size > 4) return 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device >= 64 || size > 8) return 0;
     if (known[device][size] == 0) {
         cudaLaunchConfig_t config = {};
         config.gridDim = dim3(size);
