@@ -1,0 +1,80 @@
+"""The token-by-token operators where inputs, sizes and callers are unusual: activations of very different
+size side by side, weights of many rows, settings that are not numbers, graphs and streams side by side.
+
+Tolerances count roundings, as in test_gpu_serving.py, whose plain implementations in 64 bits are used here.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from test_gpu_serving import DTYPES, check_matvec, packed_weight
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- packed matrix-vector products ----------------------------------------------------------------
+
+
+def without_columns(codes: torch.Tensor, columns) -> torch.Tensor:
+    """The weight with zeros in these columns."""
+
+    codes = codes.clone()
+    for column in columns:
+        codes[:, column // 2] &= 0x0F if column % 2 else 0xF0
+    return codes
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("spread", [30, 33, 40, 60, 100])
+@pytest.mark.parametrize("tokens,rows,cols,block,two_d", [(1, 40, 384, 16, False), (8, 33, 1003, 32, False), (3, 150, 4096, 16, True),
+                                                          (9, 130, 384, 32, True), (20, 40, 1003, 16, False), (45, 257, 640, 16, True),
+                                                          (70, 20, 300, 32, False)])
+def test_matvec_keeps_small_activations_beside_large_ones(tokens, rows, cols, block, two_d, dtype, spread):
+    """Elements 2^spread times their neighbours that meet zeros of the weight: what is left is the
+    neighbours' sum, to the same tolerance as without them.  Rows without such elements come out bit for
+    bit as in a batch that has none."""
+
+    from ue5m3_fp4 import serving
+
+    g = torch.Generator().manual_seed(spread + cols)
+    codes, scales = packed_weight(rows, cols, block, two_d, seed=cols)
+    large = [5, 130, 131, cols - 1]
+    codes = without_columns(codes, large)
+    x = torch.randn(tokens, cols, generator=g, dtype=torch.float64)
+    plain = x.clone().to(DTYPES[dtype])
+    touched = list(range(0, tokens, 3))
+    for t in touched:
+        x[t, large] *= 2.0 ** (spread if t % 2 else 0)
+        if t % 2 == 0:  # ... or the neighbours are small: same ratio
+            x[t] *= 2.0 ** -spread
+            x[t, large] *= 2.0 ** spread
+    x = x.to(DTYPES[dtype])
+    got = check_matvec(x, codes, scales, rows, cols, block, two_d, out_dtype=torch.float32, amax=448.0 * 6)
+    kw = dict(rows=rows, cols=cols, block_size=block, two_dimensional=two_d, tensor_amax=448.0 * 6, out_dtype=torch.float32)
+    without = serving.packed_matvec(plain.cuda(), codes.cuda(), scales.cuda(), **kw)
+    others = [t for t in range(tokens) if t not in touched]
+    assert torch.equal(got[others], without[others])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("tokens", [2, 12])
+def test_matvec_of_all_exponents_in_one_chunk(tokens, dtype):
+    """Elements from the type's smallest to 2^100 in one row, zeros among them; the weight is zero from 2^-60 up
+    in its first half of rows, from 2^40 in the others, so that every size is the largest one somewhere."""
+
+    rows, cols = 64, 256
+    codes, scales = packed_weight(rows, cols, 16, False, seed=3)
+    exponents = torch.linspace(-140, 100, cols).round()
+    g = torch.Generator().manual_seed(4)
+    x = (1 + torch.rand(tokens, cols, generator=g, dtype=torch.float64)) * torch.exp2(exponents.double())
+    x[:, ::17] = 0
+    x = (x * torch.where(torch.rand(tokens, cols, generator=g) < 0.5, -1.0, 1.0)).to(DTYPES[dtype])
+    codes[:32] = without_columns(codes[:32], [j for j in range(cols) if exponents[j] >= -60])
+    codes[32:] = without_columns(codes[32:], [j for j in range(cols) if exponents[j] >= 40])
+    check_matvec(x, codes, scales, rows, cols, 16, False, out_dtype=torch.float32, amax=448.0 * 6)
+    x[:, 0], x[0, 255] = 1.0, math.inf  # beside an infinity, in a row of its own
+    check_matvec(x[1:], codes, scales, rows, cols, 16, False, out_dtype=torch.float32, amax=448.0 * 6)

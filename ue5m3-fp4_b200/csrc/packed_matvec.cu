@@ -6,12 +6,14 @@
 // Arithmetic.  p * s has at most six significant bits and lies between 2^-18 and 2^19, so
 // p * (s / 16) is EXACT in fp16 for every code and every scale byte.  x does not fit fp16 as it
 // is: 128 consecutive elements of a row share a power of two that brings their largest one to
-// [2^14, 2^15).  A bf16 element that is no smaller than 2^-32 of that largest one is then exact in
-// fp16; below that it is off by at most 2^-40 of the largest one.  An fp32 element is cut into
-// three fp16 parts (11 bits each) with a product of its own each.  Tensor cores
-// (mma.m16n8k16, weights as the 16-row operand, activations as the 8 columns) sum 128 products in
-// fp32; the power of two is multiplied back when that sum joins the fp32 total.  The order of all
-// sums is fixed by the sizes: the same call gives the same bits.
+// [2^14, 2^15).  A bf16 element whose exponent is no more than 31 below that of the largest one is then
+// exact in fp16, and an fp32 element down to 37 in three fp16 parts (11 bits each) with a product of
+// its own each.  Tensor cores (mma.m16n8k16, weights as the 16-row operand, activations as the 8
+// columns) sum 128 products in fp32; the power of two is multiplied back when that sum joins the fp32
+// total.  The order of all sums is fixed by the sizes: the same call gives the same bits.
+// Where a row's 128 elements span more than that (a wide column), they count as zeros there and enter in a
+// second product of their own: as they are, in bf16 (fp32: three bf16 parts), with the same weights, which
+// bf16 holds as exactly as fp16.  Doing so for every chunk would double the work of decoding.
 //
 // What bounds it: reading the codes, 0.5 byte per weight element, plus the scales.  Decoding costs
 // one cvt.rn.f16x2.e2m1x2 and one packed multiply per two weights.
@@ -84,6 +86,14 @@ struct Params {
     int bias_fp32, out_fp32;
     float factor;          // 16 * dec
 };
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 
 // eight codes -> four fp16 pairs, exactly
 __device__ __forceinline__ void e2m1x8_to_half2(uint32_t word, uint32_t (&d)[4]) {
@@ -184,24 +194,58 @@ __device__ __forceinline__ Raw<kFp32> load_staged(const Params& p, int token0, i
     return raw;
 }
 
-// One chunk's activations as mma B fragments (fp32: three, of 11 bits each, the second to be multiplied
-// by 2^-11, the third by 2^-22), and the factor that undoes the chunk's power of two.  Lane (g, c) =
-// (lane / 4, lane % 4) brings column g and elements 32 c ... 32 c + 31; step j of the chunk's eight mma
-// takes its elements 4 j ... 4 j + 3.
+// The largest magnitude among the 128 elements of a lane's token, and the smallest of this lane's that are
+// not zero, less one unit: as the bits of an fp32.  Three operations for two bf16 elements, two for an fp32 one.
 template <bool kFp32>
-__device__ __forceinline__ void make_fragments(const Raw<kFp32>& raw, uint32_t (&b)[kFp32 ? 3 : 1][16], float& undo) {
-    uint32_t top = 0;  // the largest magnitude's bits, as those of an fp32; a NaN's are larger than all numbers'
+__device__ __forceinline__ void range_of(const Raw<kFp32>& raw, uint32_t& top, uint32_t& least) {
+    least = 0xFFFFFFFFu;
     if constexpr (kFp32) {
+        float most = 0.0f;  // a NaN does not count
 #pragma unroll
-        for (int i = 0; i < 32; ++i) top = max(top, raw.words[i] & 0x7FFFFFFFu);
+        for (int i = 0; i < 32; i += 2) {
+            const float a = fabsf(__uint_as_float(raw.words[i])), b = fabsf(__uint_as_float(raw.words[i + 1]));
+            asm("max.f32 %0, %0, %1, %2;" : "+f"(most) : "f"(a), "f"(b));
+            // twice the magnitude: the sign leaves the word
+            least = __vimin3_u32(least, 2 * raw.words[i] - 1, 2 * raw.words[i + 1] - 1);
+        }
+        top = __float_as_uint(most);
+        least >>= 1;
     } else {
-        uint32_t two = 0;
+        uint32_t two = 0;  // a NaN's bits are larger than all numbers'
 #pragma unroll
-        for (int i = 0; i < 16; ++i) asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(two) : "r"(raw.words[i] & 0x7FFF7FFFu));
+        for (int i = 0; i < 16; i += 2) {
+            const uint32_t a = raw.words[i] & 0x7FFF7FFFu, b = raw.words[i + 1] & 0x7FFF7FFFu;
+            two = __vimax3_u16x2(two, a, b);
+            least = __viaddmin_u16x2(a, 0xFFFFFFFFu, least);
+            least = __viaddmin_u16x2(b, 0xFFFFFFFFu, least);
+        }
         top = max(two << 16, two & 0xFFFF0000u);
+        least = min(least << 16, least & 0xFFFF0000u);
     }
     top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
     top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+}
+
+// Whether one of the lane's elements does not fit next to its chunk's largest one: with exponents e and f it
+// becomes a multiple of 2^(e - f + 7) (fp32: 2^(e - f - 9)), the last part holds multiples of 2^-24 (2^-46).  Beside
+// an infinity or a NaN it does not matter.
+template <bool kFp32>
+__device__ __forceinline__ bool too_small(uint32_t top, uint32_t least) {
+    constexpr uint32_t kSpan = (kFp32 ? 37 : 31) << 23, kUnit = kFp32 ? 1 : 1 << 16;
+    const uint32_t exponent = top & 0x7F800000u;
+    return exponent > kSpan && exponent < 0x7F800000u && least < exponent - kSpan - kUnit;
+}
+
+// One chunk's activations as mma B fragments (fp32: three, of 11 bits each, the second to be multiplied
+// by 2^-11, the third by 2^-22), and the factor that undoes the chunk's power of two.  Lane (g, c) =
+// (lane / 4, lane % 4) brings column g and elements 32 c ... 32 c + 31; step j of the chunk's eight mma
+// takes its elements 4 j ... 4 j + 3.  A wide column's fragments are zero; returns whether one
+// of the eight columns is wide.
+template <bool kFp32>
+__device__ __forceinline__ bool make_fragments(const Raw<kFp32>& raw, uint32_t (&b)[kFp32 ? 3 : 1][16], float& undo) {
+    uint32_t top, least;
+    range_of<kFp32>(raw, top, least);
+    const uint32_t small = __ballot_sync(0xFFFFFFFFu, too_small<kFp32>(top, least));
     // 2^(14 - e) for a largest element in [2^e, 2^(e+1)), held to 2^126 so that its inverse is a
     // normal number; an infinity or a NaN among the elements stays one in fp16
     const int field = min(268 - (int)(top >> 23), 253);
@@ -231,6 +275,13 @@ __device__ __forceinline__ void make_fragments(const Raw<kFp32>& raw, uint32_t (
             b[0][i] = *reinterpret_cast<const uint32_t*>(&h);
         }
     }
+    if (small >> (threadIdx.x & 28) & 15) {  // seldom
+#pragma unroll
+        for (int part = 0; part < (kFp32 ? 3 : 1); ++part)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) b[part][i] = 0;
+    }
+    return small != 0;
 }
 
 // The 16 bytes of codes (32 elements) and the scale bytes of one row that a lane decodes in one
@@ -348,6 +399,88 @@ __device__ __forceinline__ void decode(const Piece (&piece)[2], const uint32_t (
     }
 }
 
+// Seldom: the wide columns among tokens token0 ... token0 + here - 1 (eight at most) in one chunk, times
+// `row_count` rows from row0 on, added to[token * stride + row].  By one warp; a lane adds to the places of tokens
+// 2 c and 2 c + 1 and rows g and g + 8 of every 16.  fp32 elements are cut off to 8 bits, not rounded: every rest
+// is exact, and 2^8 of it is below twice the element.
+template <bool kFp32, int kBlock>
+__device__ __forceinline__ void add_wide(const Params& p, int chunk, int token0, int here, int row0, int row_count, float* to, int stride) {
+    constexpr int kParts = kFp32 ? 3 : 1;
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const Raw<kFp32> raw = load_raw<kFp32>(p, token0 + g, g < here, chunk);
+    uint32_t top, least;
+    range_of<kFp32>(raw, top, least);
+    const uint32_t small = __ballot_sync(0xFFFFFFFFu, too_small<kFp32>(top, least));
+    if (small == 0) return;
+    const bool wide = small >> (lane & 28) & 15;
+    uint32_t b[kParts][16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        if constexpr (kFp32) {
+            uint32_t lo = wide ? raw.words[2 * i] : 0, hi = wide ? raw.words[2 * i + 1] : 0;
+#pragma unroll
+            for (int part = 0; part < 3; ++part) {
+                b[part][i] = lo >> 16 | (hi & 0xFFFF0000u);
+                lo = __float_as_uint((__uint_as_float(lo) - __uint_as_float(lo & 0xFFFF0000u)) * 256.0f);
+                hi = __float_as_uint((__uint_as_float(hi) - __uint_as_float(hi & 0xFFFF0000u)) * 256.0f);
+            }
+        } else {
+            b[0][i] = wide ? raw.words[i] : 0;
+        }
+    }
+#pragma unroll 1
+    for (int tile = 0; tile < row_count; tile += 16) {
+        Piece now[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int64_t row = row0 + min(tile + g + 8 * h, row_count - 1);
+            const uint8_t *codes = p.codes + row * p.code_stride, *scales = p.scales + (row >> p.row_shift) * p.scale_stride;
+            uint32_t words[4] = {};
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const int at = chunk * (kChunk / 2) + 16 * c + 4 * w + i;
+                    if (at < p.code_stride) words[w] |= (uint32_t)codes[at] << (8 * i);
+                }
+            now[h].codes = make_uint4(words[0], words[1], words[2], words[3]);
+            now[h].scales = 0;
+            for (int i = 0; i < 32 / kBlock; ++i) {
+                const int at = chunk * (kChunk / kBlock) + c * (32 / kBlock) + i;
+                if (at < p.scale_stride) now[h].scales |= (uint32_t)scales[at] << (8 * i);
+            }
+        }
+        uint32_t scale[2][2];
+        scale_pairs<kBlock>(now, scale);
+        float sum[kParts][4] = {};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t a[2][4];
+            decode<kBlock>(now, scale, j, a);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {  // six significant bits, 2^-22 ... 2^16: exact in bf16
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a[h][i]));
+                    a[h][i] = __float_as_uint(f.x) >> 16 | (__float_as_uint(f.y) & 0xFFFF0000u);
+                }
+#pragma unroll
+            for (int part = 0; part < kParts; ++part) {
+                mma_bf16(sum[part], a[0][0], a[1][0], a[0][1], a[1][1], b[part][4 * j], b[part][4 * j + 1]);
+                mma_bf16(sum[part], a[0][2], a[1][2], a[0][3], a[1][3], b[part][4 * j + 2], b[part][4 * j + 3]);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int token = 2 * c + (e & 1), row = tile + g + 8 * (e >> 1);
+            if (!(small >> (4 * token) & 15) || row >= row_count) continue;
+            float whole = sum[0][e];
+            if constexpr (kFp32) whole = __fmaf_rn(sum[2][e], 0x1p-16f, __fmaf_rn(sum[1][e], 0x1p-8f, whole));
+            to[token * stride + row] += whole;
+        }
+    }
+}
+
 __device__ __forceinline__ void store(const Params& p, int token, int64_t row, float value) {
     value *= p.factor;
     if (p.bias)
@@ -438,6 +571,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
         int slot_now = 0;
+        bool wide = false;  // whether one of this warp's chunks has a wide column
         if (kVector) locate();
 #pragma unroll
         for (int i = 0; i < kRing - 1; ++i) copy_ahead(i);
@@ -448,10 +582,11 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
             for (int d = 0; d < kDepth; ++d) {
                 const int chunk = first_chunk + (pass * kDepth + d) * kWarps + warp;
                 float mine;
-                make_fragments<kFp32>(
+                const bool any = make_fragments<kFp32>(
                     kVector ? load_raw<kFp32>(p, g, g < tokens && chunk < chunks, chunk)
                             : load_staged<kFp32>(p, 0, chunk < chunks ? tokens : 0, chunk, reinterpret_cast<uint32_t*>(ring + kRing * kSlot) + warp * kStageWords),
                     b[d], mine);
+                wide = wide || any;
                 undo[d][0] = __shfl_sync(0xFFFFFFFFu, mine, 8 * c);
                 undo[d][1] = __shfl_sync(0xFFFFFFFFu, mine, 8 * c + 4);
             }
@@ -536,6 +671,10 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
                     }
             }
         }
+        if (wide)
+#pragma unroll 1
+            for (int chunk = first_chunk + warp; chunk < chunks; chunk += kWarps)
+                add_wide<kFp32, kBlock>(p, chunk, 0, tokens, row0, row_count, partial + warp * tokens * block_rows, block_rows);
         __syncthreads();
         if (p.split > 1) {
             // the sums of this CTA's warps, in the place of its first warp's; then those of the cluster
@@ -619,34 +758,77 @@ __host__ __device__ constexpr int many_slot(bool vector) { return vector ? 2 * 2
 __host__ __device__ constexpr int many_stage(int tiles, int parts) { return tiles * (parts * 128 + 2); }
 
 // The activations as the product reads them: [chunk][tile of 8 tokens][part][step][lane] 16 bytes, and
-// the factors that undo the chunks' powers of two: [chunk][tile][token].  One warp per chunk and tile.
+// the factors that undo the chunks' powers of two: [chunk][tile][token].  One warp per chunk and tile; a byte
+// per CTA tells whether one of its columns is wide (up to four bytes of zeros behind the last).
 template <bool kFp32>
-__global__ void __launch_bounds__(kManyThreads) prepare_kernel(const Params p, uint4* fragments, float* undo, int chunks, int tiles) {
+__global__ void __launch_bounds__(kManyThreads) prepare_kernel(const Params p, uint4* fragments, float* undo, uint8_t* wide, int chunks, int tiles) {
     constexpr int kParts = kFp32 ? 3 : 1;
     __shared__ uint4 stage[kManyWarps * kStageWords / 4];
     launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int64_t unit = (int64_t)blockIdx.x * kManyWarps + warp;
     const int chunk = (int)(unit / tiles), tile = (int)(unit % tiles);
-    if (chunk >= chunks) return;
-    const int here = min(8, p.tokens - 8 * tile);
-    uint32_t b[kParts][16];
-    float mine;
-    make_fragments<kFp32>(p.vector_x ? load_raw<kFp32>(p, 8 * tile + g, g < here, chunk)
-                                     : load_staged<kFp32>(p, 8 * tile, here, chunk, reinterpret_cast<uint32_t*>(stage) + warp * kStageWords),
-                          b, mine);
-    uint4* to = fragments + unit * (kParts * 128) + lane;
+    bool any = false;
+    if (chunk < chunks) {
+        const int here = min(8, p.tokens - 8 * tile);
+        uint32_t b[kParts][16];
+        float mine;
+        any = make_fragments<kFp32>(p.vector_x ? load_raw<kFp32>(p, 8 * tile + g, g < here, chunk)
+                                               : load_staged<kFp32>(p, 8 * tile, here, chunk, reinterpret_cast<uint32_t*>(stage) + warp * kStageWords),
+                                    b, mine);
+        uint4* to = fragments + unit * (kParts * 128) + lane;
 #pragma unroll
-    for (int part = 0; part < kParts; ++part)
+        for (int part = 0; part < kParts; ++part)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            to[part * 128 + j * 32] = make_uint4(b[part][4 * j], b[part][4 * j + 1], b[part][4 * j + 2], b[part][4 * j + 3]);
-    if (c == 0) undo[unit * 8 + g] = mine;
+            for (int j = 0; j < 4; ++j)
+                to[part * 128 + j * 32] = make_uint4(b[part][4 * j], b[part][4 * j + 1], b[part][4 * j + 2], b[part][4 * j + 3]);
+        if (c == 0) undo[unit * 8 + g] = mine;
+    }
+    any = __syncthreads_or(any);
+    if (threadIdx.x < (blockIdx.x + 1 < gridDim.x ? 1 : 4)) wide[blockIdx.x + threadIdx.x] = any && threadIdx.x == 0;
+}
+
+// What a warp of the product owns: rows row0 ... of its CTA's block, every second chunk from `first` to before
+// `last`, tiles tile0 ... tile0 + here - 1.
+struct Share {
+    int block_row, own, row0, row_count, tile0, here, half, first, last;
+};
+
+template <int kTiles>
+__device__ __forceinline__ Share share_of(const Params& p, int chunks, int tiles, int block, int warp) {
+    Share s;
+    const int share = block % p.split, place = block / p.split;
+    // groups of tokens, as even as their number allows (72 x 4096 x 4096: 26.8 -> 22.1 us); those of a block of
+    // rows start side by side
+    const int groups = (tiles + kTiles - 1) / kTiles, each = (tiles + groups - 1) / groups;
+    const int row_block = place / groups;
+    s.tile0 = place % groups * each;
+    s.block_row = (int)((int64_t)p.rows * row_block / p.row_blocks);
+    s.own = (int)((int64_t)p.rows * (row_block + 1) / p.row_blocks) - s.block_row;  // kManyRows at most
+    s.here = min(each, tiles - s.tile0);
+    s.row0 = s.block_row + warp % 4 * 32;
+    s.half = warp / 4;
+    s.first = (int)((int64_t)chunks * share / p.split) + s.half;
+    s.last = (int)((int64_t)chunks * (share + 1) / p.split);
+    s.row_count = min(32, s.own - warp % 4 * 32);
+    return s;
+}
+
+// The block's and the thread's index, read again: what follows from them is computed again, not kept.
+__device__ __forceinline__ int block_index_again() {
+    int v;
+    asm volatile("mov.u32 %0, %%ctaid.x;" : "=r"(v));
+    return v;
+}
+__device__ __forceinline__ int thread_index_again() {
+    int v;
+    asm volatile("mov.u32 %0, %%tid.x;" : "=r"(v));
+    return v;
 }
 
 template <bool kFp32, int kTiles, bool kVector, int kBlock>
 __global__ void __launch_bounds__(kManyThreads, kFp32 || kTiles > 4 ? 1 : 2)
-    packed_matmul_kernel(const Params p, const uint4* fragments, const float* undo, int chunks, int tiles) {
+    packed_matmul_kernel(const Params p, const uint4* fragments, const float* undo, const uint8_t* wide, int chunks, int tiles) {
     constexpr int kParts = kFp32 ? 3 : 1;
     constexpr int kStage = many_stage(kTiles, kParts);
     // activations [half][slot], then, kVector, codes and scales [warp][slot]; afterwards the sums [half][token][row]
@@ -654,18 +836,10 @@ __global__ void __launch_bounds__(kManyThreads, kFp32 || kTiles > 4 ? 1 : 2)
     constexpr int kSlot = many_slot(kVector);
     float* partial = reinterpret_cast<float*>(ring);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int share = blockIdx.x % p.split, place = blockIdx.x / p.split;
-    // groups of tokens, as even as their number allows (72 x 4096 x 4096: 26.8 -> 22.1 us); those of a block of
-    // rows start side by side
-    const int groups = (tiles + kTiles - 1) / kTiles, each = (tiles + groups - 1) / groups;
-    const int row_block = place / groups, tile0 = place % groups * each;
-    const int block_row = (int)((int64_t)p.rows * row_block / p.row_blocks);
-    const int own = (int)((int64_t)p.rows * (row_block + 1) / p.row_blocks) - block_row;  // kManyRows at most
-    const int here = min(each, tiles - tile0);
-    const int row0 = block_row + warp % 4 * 32, half = warp / 4;
-    const int first = (int)((int64_t)chunks * share / p.split) + half, last = (int)((int64_t)chunks * (share + 1) / p.split);
-    const int count = last > first ? (last - first + 1) / 2 : 0;
-    const int row_count = min(32, own - warp % 4 * 32);
+    const Share mine = share_of<kTiles>(p, chunks, tiles, blockIdx.x, warp);
+    const int share = blockIdx.x % p.split, tile0 = mine.tile0, block_row = mine.block_row, own = mine.own, here = mine.here,
+              row0 = mine.row0, half = mine.half, first = mine.first, row_count = mine.row_count;
+    const int count = mine.last > first ? (mine.last - first + 1) / 2 : 0;
     const bool active = row_count > 0;
     const int stride = (int)p.code_stride, scale_stride = (int)p.scale_stride;
     const uint8_t* codes = p.codes + row0 * p.code_stride;
@@ -713,6 +887,10 @@ __global__ void __launch_bounds__(kManyThreads, kFp32 || kTiles > 4 ? 1 : 2)
     wait_for_launcher();  // the activations are prepared
 #pragma unroll
     for (int i = 0; i < kManyRing - 1; ++i) copy_activations(i);
+
+    // the preparation's first 128 bytes about wide columns, looked at in the end
+    const int prepared = (int)(((int64_t)chunks * tiles + kManyWarps - 1) / kManyWarps);
+    uint32_t any_wide = 4 * lane < prepared ? __ldcg(reinterpret_cast<const uint32_t*>(wide) + lane) : 0;
 
     float total[2][kTiles][4] = {};
     for (int i = 0; i < count; ++i) {
@@ -787,6 +965,20 @@ __global__ void __launch_bounds__(kManyThreads, kFp32 || kTiles > 4 ? 1 : 2)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 partial[(half * kTiles * 8 + 8 * t + 2 * c + (e & 1)) * kManyPad + warp % 4 * 32 + 16 * r + g + 8 * (e >> 1)] = total[r][t][e];
+    for (int i = 128 + 4 * lane; i < prepared; i += 128) any_wide |= __ldcg(reinterpret_cast<const uint32_t*>(wide + i));
+    if (__any_sync(0xFFFFFFFFu, any_wide != 0)) {
+        const Share again = share_of<kTiles>(p, chunks, tiles, block_index_again(), thread_index_again() >> 5);
+        if (again.row_count > 0)
+#pragma unroll 1
+            for (int chunk = again.first; chunk < again.last; chunk += 2)
+#pragma unroll 1
+                for (int t = 0; t < again.here; ++t) {
+                    const int tile = again.tile0 + t;
+                    if (__ldcg(wide + ((int64_t)chunk * tiles + tile) / kManyWarps) != 0)
+                        add_wide<kFp32, kBlock>(p, chunk, 8 * tile, min(8, p.tokens - 8 * tile), again.row0, again.row_count,
+                                                partial + (again.half * kTiles + t) * 8 * kManyPad + again.row0 - again.block_row, kManyPad);
+                }
+    }
     __syncthreads();
     const int tokens = min(here * 8, p.tokens - tile0 * 8);
     constexpr int kOther = kTiles * 8 * kManyPad;  // the second half's sums
@@ -811,10 +1003,11 @@ __global__ void __launch_bounds__(kManyThreads, kFp32 || kTiles > 4 ? 1 : 2)
     if (p.split > 1) cooperative_groups::this_cluster().sync();  // the others have read this CTA's sums
 }
 
-// bytes of the prepared activations: fragments, and the factors behind them
+// bytes of the prepared activations: fragments, factors and the bytes of wide columns
 size_t workspace_of(bool fp32, int64_t tokens, int64_t cols) {
     if (tokens <= kFewTokens) return 0;
-    return (size_t)((cols + kChunk - 1) / kChunk) * ((tokens + 7) / 8) * ((fp32 ? 3 : 1) * 2048 + 32);
+    const size_t units = (size_t)((cols + kChunk - 1) / kChunk) * ((tokens + 7) / 8);
+    return units * ((fp32 ? 3 : 1) * 2048 + 32) + (units + kManyWarps - 1) / kManyWarps + 4;
 }
 
 template <bool kFp32, int kTiles, bool kVector, int kBlock>
@@ -848,7 +1041,8 @@ int launch_many(Params p, void* workspace, cudaStream_t stream) {
     }
     uint4* fragments = reinterpret_cast<uint4*>(workspace);
     float* undo = reinterpret_cast<float*>(fragments + units * (kFp32 ? 384 : 128));
-    prepare_kernel<kFp32><<<(unsigned)((units + kManyWarps - 1) / kManyWarps), kManyThreads, 0, stream>>>(p, fragments, undo, chunks, tiles);
+    uint8_t* wide = reinterpret_cast<uint8_t*>(undo + units * 8);
+    prepare_kernel<kFp32><<<(unsigned)((units + kManyWarps - 1) / kManyWarps), kManyThreads, 0, stream>>>(p, fragments, undo, wide, chunks, tiles);
     const int status = check_launch();
     if (status != UE5M3_OK) return status;
     cudaLaunchConfig_t config = {};
@@ -865,7 +1059,7 @@ int launch_many(Params p, void* workspace, cudaStream_t stream) {
     attributes[1].val.clusterDim.z = 1;
     config.attrs = attributes;
     config.numAttrs = p.split > 1 ? 2 : 1;
-    return record_cuda_error(cudaLaunchKernelEx(&config, kKernel, p, (const uint4*)fragments, (const float*)undo, chunks, tiles));
+    return record_cuda_error(cudaLaunchKernelEx(&config, kKernel, p, (const uint4*)fragments, (const float*)undo, (const uint8_t*)wide, chunks, tiles));
 }
 
 template <bool kVector, int kBlock>
