@@ -431,7 +431,8 @@ int ue5m3_paged_attention(const void *q, int64_t q_token_stride, int64_t q_head_
  * running weight exceeds uniform * (weight of all kept).  temperature <= 0: the largest logit.
  * Minus infinity masks a token.  logprobs: log of the token's share of the kept weight.  A row with
  * a NaN, or without a logit above minus infinity, gives token -1 and NaN.  Each setting is a value,
- * or a device array with one value per row where its pointer is not NULL.  Exact sums of fp64
+ * or a device array with one value per row where its pointer is not NULL; a NaN temperature takes the
+ * largest logit, a NaN top_p or min_p cuts nothing, a NaN uniform counts as 0.  Exact sums of fp64
  * weights rounded to multiples of 2^-44: the same inputs give the same token.
  * vocabulary <= 2^18.
  */

@@ -11,7 +11,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_serving import DTYPES, check_matvec, packed_weight
+from test_gpu_serving import DTYPES, check_matvec, check_sample, packed_weight
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +78,34 @@ def test_matvec_of_all_exponents_in_one_chunk(tokens, dtype):
     check_matvec(x, codes, scales, rows, cols, 16, False, out_dtype=torch.float32, amax=448.0 * 6)
     x[:, 0], x[0, 255] = 1.0, math.inf  # beside an infinity, in a row of its own
     check_matvec(x[1:], codes, scales, rows, cols, 16, False, out_dtype=torch.float32, amax=448.0 * 6)
+
+
+# ---- sampling ---------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("vocabulary", [700, 9000, 131072])
+@pytest.mark.parametrize("top_p", [0.3, 0.9, 0.999, 1.0])
+@pytest.mark.parametrize("top_k", [0, 40, 600])
+def test_sample_settings_that_are_not_numbers(vocabulary, top_p, top_k):
+    """A NaN among the settings of the rows: every row gets a token, that of the setting that cuts nothing."""
+
+    from ue5m3_fp4 import serving
+
+    g = torch.Generator().manual_seed(vocabulary)
+    logits, uniforms = 0.5 * torch.randn(6, vocabulary, generator=g), torch.tensor([0.0, 0.2, 0.5, 0.8, 0.9999, math.nan])
+    plain = dict(temperature=torch.full((6,), 0.9), top_k=torch.full((6,), top_k, dtype=torch.int32), top_p=torch.full((6,), top_p),
+                 min_p=torch.zeros(6))
+    clean = uniforms.nan_to_num()
+    expect = check_sample(logits, clean, **plain)
+
+    def run(**over):
+        settings = {name: value.cuda() for name, value in {**plain, **over}.items()}
+        return serving.sample_tokens(logits.cuda(), uniforms.cuda(), **settings)
+
+    nan = torch.full((6,), math.nan)
+    got = run(min_p=nan)
+    assert torch.equal(got[0], expect[0]) and torch.equal(got[1], expect[1])
+    got = run(top_p=nan)
+    assert torch.equal(got[0], check_sample(logits, clean, **{**plain, "top_p": torch.ones(6)})[0])
+    got = run(temperature=nan)
+    assert torch.equal(got[0].cpu(), logits.argmax(1)) and not bool(got[1].any())

@@ -602,7 +602,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const Params p) {
     const float temperature = p.temperature_dev ? p.temperature_dev[row_index] : p.temperature;
     const int top_k = p.top_k_dev ? p.top_k_dev[row_index] : p.top_k;
     const float top_p = p.top_p_dev ? p.top_p_dev[row_index] : p.top_p;
-    const float min_p = p.min_p_dev ? p.min_p_dev[row_index] : p.min_p;
+    const float min_p = fmaxf(p.min_p_dev ? p.min_p_dev[row_index] : p.min_p, 0.0f);  // a NaN cuts nothing, everywhere
     if (top != top || top == -INFINITY) {
         if (rank_in_cluster == 0 && t == 0) {
             p.tokens[row_index] = -1;

@@ -300,7 +300,9 @@ def sample_tokens(
     ``top_p`` of theirs (1: all), of these the tokens with at least ``min_p`` of the largest weight.
     The token is the first kept one, in vocabulary order, whose running weight exceeds
     ``uniform * (weight of all kept)``.  temperature 0 takes the largest logit.  Each setting is a
-    number or a tensor with one per row (int32 for ``top_k``, fp32 otherwise).  Minus infinity masks a
+    number or a tensor with one per row (int32 for ``top_k``, fp32 otherwise; there a value outside its
+    range counts as the nearest in it, a NaN ``temperature`` as 0, a NaN ``top_p`` or ``min_p`` as none, and a NaN
+    in ``uniforms`` as 0).  Minus infinity masks a
     token; a row with a NaN, or with every token masked, gives token -1 and NaN.  Sums are exact: the
     same inputs give the same tokens, whatever the launch."""
 
