@@ -162,8 +162,14 @@ def _strides(name: str, tensor: Tensor) -> tuple[int, ...]:
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(*sizes: int) -> int:
-    return _native.load().ue5m3_paged_attention_workspace_bytes(*sizes)
+def _workspace_bytes(index: int, *sizes: int) -> int:
+    """Asked for once per device and sizes: into how many parts sequences are split depends on the device's SMs."""
+
+    function = _native.load().ue5m3_paged_attention_workspace_bytes
+    if index == torch._C._cuda_getDevice():
+        return function(*sizes)
+    with torch.cuda.device(index):
+        return function(*sizes)
 
 
 def paged_attention(
@@ -260,7 +266,7 @@ def paged_attention(
         k_pages.data_ptr(), v_pages.data_ptr(), *_strides("k_pages", k_pages), *_strides("v_pages", v_pages), pages,
         page_size, kv_heads, head_dim, page_table.data_ptr(), sequences, width,
         table_stride if sequences > 1 else width)
-    need = _workspace_bytes(tokens, sequences, heads, kv_heads, head_dim, max_query_length, max_kv_length)
+    need = _workspace_bytes(index, tokens, sequences, heads, kv_heads, head_dim, max_query_length, max_kv_length)
     # from the current stream's pool, for this call alone: calls and captured graphs share nothing
     workspace = q.new_empty(need // 2) if need else None
     # kernels: attention, the rows of split sequences, new keys ahead of the kernel for many rows
