@@ -9,7 +9,7 @@ import pytest
 import torch
 
 from ue5m3_fp4 import _native
-from ue5m3_fp4.serving import operators
+from ue5m3_fp4.serving import PagedKVCache, operators
 
 
 def test_attention_workspace_is_planned_on_the_operands_device(monkeypatch):
@@ -42,3 +42,30 @@ def test_attention_workspace_is_planned_on_the_operands_device(monkeypatch):
         assert asked == [0, 1, 0] and current[0] == 1
     finally:
         operators._workspace_bytes.cache_clear()
+
+
+def test_steps_without_all_their_tokens_are_refused():
+    """Fewer ids or query rows than the step has tokens: the last rows of some sequences would be read from
+    behind the tensors, and their keys would be missing from the cache."""
+
+    from ue5m3_fp4.integrations.torchtitan.shaped_stack import NemotronHShapedStack, ShapedConfig
+
+    cache = PagedKVCache(layers=1, pages=8, page_size=16, kv_heads=1, head_dim=64, sequences=2, max_length=64, device="cpu")
+    assert cache.step_tokens == 0
+    cache.begin_step([3, 2])
+    assert cache.step_tokens == 5
+    rows = torch.zeros(4, 1, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="5 tokens"):
+        cache.attend(0, rows, rows, rows)
+    model = NemotronHShapedStack(ShapedConfig(hidden_size=64, intermediate_size=64, mamba_inner=64, mamba_extra=16, attention_heads=1,
+                                              kv_heads=1, head_dim=64, vocab_size=10, num_hidden_layers=2,
+                                              hybrid_override_pattern="M*"), device="cpu")
+    for ids in (torch.zeros(4, dtype=torch.int64), torch.zeros(1, 5, dtype=torch.int64), torch.zeros(0, dtype=torch.int64)):
+        with pytest.raises(ValueError, match="5 tokens"):
+            model.serve(ids, cache)
+    with pytest.raises(RuntimeError, match="begin_step"):
+        model.serve(torch.zeros(5, dtype=torch.int64), model.make_cache(sequences=2, max_length=16))
+    # refused steps leave the cache as it was; padding behind the step's tokens is taken (and gets as far as the GPU)
+    assert cache.lengths == (3, 2)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        cache.attend(0, torch.zeros(7, 1, 64, dtype=torch.bfloat16), rows, rows)

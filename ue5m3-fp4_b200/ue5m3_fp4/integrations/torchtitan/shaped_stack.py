@@ -167,8 +167,12 @@ class NemotronHShapedStack(nn.Module):
         the logits [sequences, vocabulary] of each sequence's last one (those of a sequence without new
         tokens mean nothing).  The linears may be float, ``UE5M3Linear`` in inference or
         ``PackedFP4Linear``; may be captured into a CUDA graph and replayed after the next begin_step
-        with the same counts."""
+        with the same counts.  Ids behind the step's tokens are padding."""
 
+        if cache.step_tokens == 0:
+            raise RuntimeError("begin_step has not been called")
+        if input_ids.ndim != 1 or input_ids.numel() < cache.step_tokens:
+            raise ValueError(f"input_ids must be 1-d and hold the step's {cache.step_tokens} tokens")
         x = self.embed_tokens(input_ids)
         attention = 0
         for layer in self.layers:

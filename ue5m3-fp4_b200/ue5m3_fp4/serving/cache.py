@@ -45,6 +45,7 @@ class PagedKVCache:
         table, self.kv_lengths, self.query_starts, self.last_rows = self._words.split(counts)
         self.page_table = table.view(sequences, self._width)
         self.max_query_length = self.max_kv_length = 0
+        self.step_tokens = 0  # of all slots, in the step that was begun last
 
     @property
     def lengths(self) -> tuple[int, ...]:
@@ -76,7 +77,7 @@ class PagedKVCache:
         starts = [0]
         for count in new:
             starts.append(starts[-1] + count)
-        self.max_query_length, self.max_kv_length = max(new), max(lengths)
+        self.max_query_length, self.max_kv_length, self.step_tokens = max(new), max(lengths), starts[-1]
         words = [page for held in self._pages for page in held + [-1] * (self._width - len(held))]
         # the last row of a slot without new tokens is immaterial, but a row
         words += lengths + starts + [max(stop - 1, 0) for stop in starts[1:]]
@@ -96,10 +97,13 @@ class PagedKVCache:
 
     def attend(self, layer: int, q: Tensor, k: Tensor, v: Tensor, *, scale: float | None = None) -> Tensor:
         """Write the step's keys and values [tokens, kv_heads, head_dim] of one layer and attend with its
-        queries [tokens, heads, head_dim] (:func:`paged_attention`)."""
+        queries [tokens, heads, head_dim] (:func:`paged_attention`).  At least the tokens of the step, which come
+        first; rows behind them are padding."""
 
         if self.max_query_length == 0:
             raise RuntimeError("begin_step has not been called")
+        if q.shape[0] < self.step_tokens:
+            raise ValueError(f"the step has {self.step_tokens} tokens, q has rows for {q.shape[0]}")
         return paged_attention(q, self.k[layer], self.v[layer], self.page_table, self.kv_lengths, self.query_starts,
                                max_query_length=self.max_query_length, max_kv_length=self.max_kv_length, scale=scale,
                                new_k=k, new_v=v)
