@@ -109,3 +109,52 @@ def test_sample_settings_that_are_not_numbers(vocabulary, top_p, top_k):
     assert torch.equal(got[0], check_sample(logits, clean, **{**plain, "top_p": torch.ones(6)})[0])
     got = run(temperature=nan)
     assert torch.equal(got[0].cpu(), logits.argmax(1)) and not bool(got[1].any())
+
+
+# ---- packed linears ---------------------------------------------------------------------------------
+
+
+def frozen_linear(weight: torch.Tensor):
+    from ue5m3_fp4 import FP4InferenceScalingController
+    from ue5m3_fp4.nn import UE5M3Linear
+
+    model = torch.nn.Sequential(UE5M3Linear(weight.shape[1], weight.shape[0], bias=False, module_name="proj", device="cuda",
+                                            dtype=torch.bfloat16))
+    with torch.no_grad():
+        model[0].weight.copy_(weight)
+    controller = FP4InferenceScalingController(model.eval(), activation_mode="current_tensor", checkpoint_identity={"name": "none"})
+    controller.reset_after_checkpoint_load()
+    controller.calibrate_and_freeze_weights()
+    return model
+
+
+def test_packed_linears_take_the_weight_that_was_installed(tmp_path, monkeypatch):
+    """A layer whose forward operand came from a file packs and exports that weight, not its parameter; a
+    parameter written to afterwards counts again."""
+
+    from ue5m3_fp4.nn import pack_frozen_linears
+
+    monkeypatch.setenv("UE5M3_GEMM_PATH", "fp4")
+    g = torch.Generator().manual_seed(1)
+    own, other = ((0.02 * torch.randn(192, 256, generator=g)).clamp(-0.05, 0.05).to(torch.bfloat16).cuda() for _ in range(2))
+    own[0, 0] = other[0, 0] = 0.06  # the same amax: the file fits the layer
+    frozen_linear(other)[0].export_packed_weight(tmp_path / "other")
+    model = frozen_linear(own)
+    of_parameter = model[0].packed_weight()
+    model[0].load_packed_weight(tmp_path / "other")
+    expect = frozen_linear(other)[0].packed_weight()
+    assert not torch.equal(of_parameter.codes, expect.codes)
+    packed = model[0].packed_weight()
+    assert torch.equal(packed.codes, expect.codes) and torch.equal(packed.scales, expect.scales)
+    model[0].export_packed_weight(tmp_path / "again")
+    assert (tmp_path / "again").read_bytes() == (tmp_path / "other").read_bytes()
+    written = frozen_linear(own)
+    written[0].load_packed_weight(tmp_path / "other")
+    with torch.no_grad():
+        written[0].weight.mul_(1.0)
+    assert torch.equal(written[0].packed_weight().codes, of_parameter.codes)
+    pack_frozen_linears(model)
+    x = torch.randn(3, 256, device="cuda").to(torch.bfloat16)
+    reference = x.double() @ expect.dequantize().double().T
+    got = model(x).double()
+    assert bool(((got - reference).abs() <= 2.0 ** -8 * reference.abs() + 1e-5).all())

@@ -568,21 +568,28 @@ class UE5M3Linear(torch.nn.Module):
         return dict(self.__dict__.get("_scale_histograms") or {})
 
     def export_packed_weight(self, path) -> None:
-        """Write this layer's weight, quantized with its FROZEN amax, as a packed FP4 tensor file
-        (``ue5m3_fp4.packed.PackedFP4Tensor``): what a quantized-evaluation run needs of the
+        """Write this layer's weight, quantized with its FROZEN amax (:meth:`packed_weight`), as a packed FP4 tensor
+        file (``ue5m3_fp4.packed.PackedFP4Tensor``): what a quantized-evaluation run needs of the
         weight, at 0.5625 byte per element.  Requires the post-load lifecycle to have frozen the
         weight scale."""
 
         self.packed_weight().save(path)
 
     def packed_weight(self):
-        """This layer's weight, quantized with its FROZEN amax, as a ``PackedFP4Tensor``."""
+        """The weight that this layer's forward pass multiplies with, as a ``PackedFP4Tensor``: what
+        ``load_packed_weight`` has installed, if the parameter has not been written to since, otherwise the
+        parameter, quantized with its FROZEN amax."""
 
         from ue5m3_fp4.packed import PackedFP4Tensor
 
         frozen = self._inference["frozen_weights"].get("forward.w") if self._inference["active"] else None
         if frozen is None:
             raise RuntimeError("Weight amax has not been frozen after checkpoint load")
+        cached = self.__dict__.get("_packed_weight_cache")
+        if cached is not None and cached[2] is not None:
+            reference = self._reference_tensor(float(frozen), self.weight)
+            if cached[0] == self._packed_weight_key(self.weight, reference, _OperandPlan(self)):
+                return cached[2]
         return PackedFP4Tensor.quantize(
             self.weight.detach(), block_size=self.recipe.block_size, two_dimensional=self.recipe.two_dimensional_weights,
             tensor_amax=float(frozen), scale_target=self.recipe.scale_target_for("weight", self.module_name),
@@ -612,7 +619,7 @@ class UE5M3Linear(torch.nn.Module):
         if packed.tensor_amax != float(torch.tensor(float(frozen), dtype=torch.float32)):
             raise ValueError("packed weight was quantized with another tensor amax than the frozen one")
         reference = self._reference_tensor(float(frozen), self.weight)
-        self._remember_packed_frozen_weight(self.weight, reference, plan, packed.gemm_operand(shift_headroom=1))
+        self._remember_packed_frozen_weight(self.weight, reference, plan, packed.gemm_operand(shift_headroom=1), packed)
 
     def _packed_frozen_weight(self, weight: torch.Tensor, reference: torch.Tensor, plan):
         cached = self.__dict__.get("_packed_weight_cache")
@@ -620,8 +627,10 @@ class UE5M3Linear(torch.nn.Module):
             return cached[1]
         return None
 
-    def _remember_packed_frozen_weight(self, weight: torch.Tensor, reference: torch.Tensor, plan, operand) -> None:
-        self.__dict__["_packed_weight_cache"] = (self._packed_weight_key(weight, reference, plan), operand)
+    def _remember_packed_frozen_weight(self, weight: torch.Tensor, reference: torch.Tensor, plan, operand,
+                                       installed=None) -> None:
+        # installed: the packed tensor from which the operand was made, when it came from a file
+        self.__dict__["_packed_weight_cache"] = (self._packed_weight_key(weight, reference, plan), operand, installed)
 
     def _forward_reference(self, role: str, tensor: torch.Tensor) -> torch.Tensor:
         state = self._inference

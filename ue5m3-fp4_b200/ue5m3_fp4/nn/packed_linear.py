@@ -34,7 +34,8 @@ class PackedFP4Linear(torch.nn.Module):
 
     @classmethod
     def from_frozen(cls, module: UE5M3Linear) -> PackedFP4Linear:
-        """The packed form of a linear whose weight amax is frozen (``UE5M3Linear.packed_weight``)."""
+        """The packed form of a linear whose weight amax is frozen (``UE5M3Linear.packed_weight``): of the weight
+        that ``load_packed_weight`` has installed, if it has."""
 
         if not isinstance(module, UE5M3Linear):
             raise TypeError("from_frozen expects a UE5M3Linear")
