@@ -72,6 +72,13 @@ extern "C" {
 #define UE5M3_FAKE_DEQUANT 3 /* p*(s*dec)      formats.py:439,450                       */
 
 int ue5m3_abi_version(void);
+
+/*
+ * The library's own status words on the current device (device int[4], zero at the start), for callers
+ * that hand the same ones to every call that takes status_dev.  Allocates nothing, and may be called while
+ * a stream is being captured.
+ */
+int ue5m3_status_words(int **words);
 const char *ue5m3_status_string(int status);
 
 /* Last CUDA error text recorded by this thread's most recent failing call (host string). */

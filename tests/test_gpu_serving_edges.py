@@ -7,6 +7,9 @@ Tolerances count roundings, as in test_gpu_serving.py, whose plain implementatio
 from __future__ import annotations
 
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -158,3 +161,45 @@ def test_packed_linears_take_the_weight_that_was_installed(tmp_path, monkeypatch
     reference = x.double() @ expect.dequantize().double().T
     got = model(x).double()
     assert bool(((got - reference).abs() <= 2.0 ** -8 * reference.abs() + 1e-5).all())
+
+
+# ---- graphs -----------------------------------------------------------------------------------------
+
+
+FIRST_CALL = """
+import sys
+sys.path.insert(0, "ue5m3-fp4_b200")
+import torch
+from ue5m3_fp4 import serving
+from ue5m3_fp4.backends import b200
+
+pages = torch.randn(4, 16, 2, 64, device="cuda").to(torch.bfloat16)
+q = torch.randn(1, 4, 64, device="cuda").to(torch.bfloat16)
+table, kv, starts = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([[2, 0, 3]], [40], [0, 1]))
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = serving.paged_attention(q, pages, pages, table, kv, starts, max_query_length=1)
+words = b200.gemm_status(q.device)
+assert words.tolist() == [0, 0, 0, 0]
+expect = serving.paged_attention(q, pages, pages, table, kv, starts, max_query_length=1)
+assert bool(expect.isfinite().all())
+graph.replay()
+assert torch.equal(out, expect)
+words[0] = 1  # a recorded failure stays until it is cleared
+graph.replay()
+assert bool(out.isnan().all()) and words.tolist() == [1, 0, 0, 0]
+words.zero_()
+graph.replay()
+assert torch.equal(out, expect)
+print("done")
+"""
+
+
+def test_first_call_under_capture_leaves_the_status_words_to_all():
+    """A process whose first call of the library is captured: a failure recorded on the device is not cleared by the
+    graph's replays, and outputs are NaN until it is."""
+
+    root = Path(__file__).resolve().parent.parent
+    done = subprocess.run([sys.executable, "-c", FIRST_CALL], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and done.stdout.strip() == "done", done.stderr[-2000:]

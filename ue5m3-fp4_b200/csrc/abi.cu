@@ -36,7 +36,15 @@ int sm_count() {
     return counts[device];
 }
 
+// one set per device that the library is loaded on; zero from the start
+static __device__ int g_status_words[4];
+
 }  // namespace ue5m3
+
+extern "C" int ue5m3_status_words(int** words) {
+    if (!words) return UE5M3_ERR_INVALID_ARGUMENT;
+    return ue5m3::record_cuda_error(cudaGetSymbolAddress((void**)words, ue5m3::g_status_words));
+}
 
 extern "C" int ue5m3_abi_version(void) { return UE5M3_ABI_VERSION; }
 

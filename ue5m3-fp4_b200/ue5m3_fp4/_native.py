@@ -116,6 +116,8 @@ def load() -> ctypes.CDLL:
     lib.ue5m3_place_row_windows.argtypes = [p, p, p, i64, i32, p, p, p, i64, i32, i64, p]
     lib.ue5m3_test_e2m1_cvt.restype = i32
     lib.ue5m3_test_e2m1_cvt.argtypes = [ctypes.c_uint32, ctypes.c_uint64, p, p, p]
+    lib.ue5m3_status_words.restype = i32
+    lib.ue5m3_status_words.argtypes = [ctypes.POINTER(p)]
     lib.ue5m3_packed_matvec.restype = i32
     lib.ue5m3_packed_matvec.argtypes = [p, i32, i64, i64, p, p, i64, i64, i32, i32, f32, p, i32, p, i32, i64, p, ctypes.c_size_t,
                                         p]

@@ -8,6 +8,7 @@ falls back to another implementation.
 
 from __future__ import annotations
 
+import ctypes
 import math
 from dataclasses import dataclass
 
@@ -316,12 +317,24 @@ def _alpha_arguments(alpha, device: torch.device) -> tuple:
 _status_words: dict[torch.device, Tensor] = {}
 
 
+class _DeviceWords:
+    """int32 words at a device address, for ``torch.as_tensor``."""
+
+    def __init__(self, address: int, count: int) -> None:
+        self.__cuda_array_interface__ = {"shape": (count,), "typestr": "<i4", "data": (address, False), "version": 3}
+
+
 def gemm_status(device: torch.device) -> Tensor:
-    """Device int32[4] written by the GEMM when a bounded wait expires (all zero = healthy)."""
+    """Device int32[4] written by the GEMM when a bounded wait expires (all zero = healthy).  The library's own
+    memory: words that a call allocated while a graph is captured would lie in the graph's memory, and each
+    replay would clear them."""
 
     words = _status_words.get(device)
     if words is None:
-        words = torch.zeros(4, dtype=torch.int32, device=device)
+        address = ctypes.c_void_p()
+        with torch.cuda.device(device):
+            _native.check(_native.load().ue5m3_status_words(ctypes.byref(address)), "ue5m3_status_words", 0)
+            words = torch.as_tensor(_DeviceWords(address.value, 4), device=device)
         _status_words[device] = words
     return words
 
