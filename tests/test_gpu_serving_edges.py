@@ -14,7 +14,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from test_gpu_serving import DTYPES, check_matvec, check_sample, packed_weight
+from test_gpu_serving import DTYPES, check_matvec, check_sample, packed_weight, run_attention, unpack
 
 pytestmark = pytest.mark.gpu
 
@@ -35,7 +35,8 @@ def without_columns(codes: torch.Tensor, columns) -> torch.Tensor:
 @pytest.mark.parametrize("spread", [30, 33, 40, 60, 100])
 @pytest.mark.parametrize("tokens,rows,cols,block,two_d", [(1, 40, 384, 16, False), (8, 33, 1003, 32, False), (3, 150, 4096, 16, True),
                                                           (9, 130, 384, 32, True), (20, 40, 1003, 16, False), (45, 257, 640, 16, True),
-                                                          (70, 20, 300, 32, False)])
+                                                          (70, 20, 300, 32, False), (16, 21504, 256, 32, True),
+                                                          (8, 30011, 300, 16, False)])
 def test_matvec_keeps_small_activations_beside_large_ones(tokens, rows, cols, block, two_d, dtype, spread):
     """Elements 2^spread times their neighbours that meet zeros of the weight: what is left is the
     neighbours' sum, to the same tolerance as without them.  Rows without such elements come out bit for
@@ -83,6 +84,44 @@ def test_matvec_of_all_exponents_in_one_chunk(tokens, dtype):
     check_matvec(x[1:], codes, scales, rows, cols, 16, False, out_dtype=torch.float32, amax=448.0 * 6)
 
 
+@pytest.mark.parametrize("cols", [256, 255])
+@pytest.mark.parametrize("block,two_d", [(16, False), (32, True)])
+@pytest.mark.parametrize("tokens,rows,dtype", [(16, 21504, "bf16"), (60, 21504, "bf16"), (40, 9601, "bf16"), (16, 12001, "fp32"),
+                                               (8, 30011, "bf16"), (8, 30011, "fp32"), (1, 131072, "bf16")])
+def test_matvec_of_many_rows(tokens, rows, cols, block, two_d, dtype):
+    """Blocks of rows that start at any row, also inside a tile of scales, when they are spread over the SMs' last turn;
+    up to eight tokens, more rows to a CTA than one pass over its shared memory takes."""
+
+    g = torch.Generator().manual_seed(rows + cols)
+    x = torch.randn(tokens, cols, generator=g).to(DTYPES[dtype])
+    codes, scales = packed_weight(rows, cols, block, two_d, seed=cols)
+    bias = torch.randn(rows, generator=g) if rows % 2 else None
+    check_matvec(x, codes, scales, rows, cols, block, two_d, bias=bias)
+
+
+@pytest.mark.parametrize("cols", [4096, 4095])
+@pytest.mark.parametrize("tokens", [1, 9])
+def test_matvec_of_weights_beyond_32_bits(tokens, cols):
+    """Codes of more than 2^31 bytes: the last rows, against those rows alone."""
+
+    from ue5m3_fp4 import serving
+
+    rows, last = 1_060_000, 300
+    codes = torch.zeros(rows, (cols + 1) // 2, dtype=torch.uint8, device="cuda")
+    scales = torch.zeros(rows, (cols + 15) // 16, dtype=torch.uint8, device="cuda")
+    assert codes.numel() > 2 ** 31
+    some_codes, some_scales = packed_weight(last, cols, 16, False, seed=1)
+    codes[-last:], scales[-last:] = some_codes.cuda(), some_scales.cuda()
+    x = torch.randn(tokens, cols, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+    alone = check_matvec(x, some_codes, some_scales, last, cols, 16, False, out_dtype=torch.float32, amax=448.0 * 6)
+    got = serving.packed_matvec(x.cuda(), codes, scales, rows=rows, cols=cols, block_size=16, two_dimensional=False,
+                                tensor_amax=448.0 * 6, out_dtype=torch.float32)
+    assert not bool(got[:, :-last].any())
+    # the reduction axis is shared by other numbers of CTAs: the order of the fp32 sums may differ
+    size = x.double().abs() @ unpack(some_codes, some_scales, last, cols, 16, False).T.abs()
+    assert bool(((got[:, -last:] - alone).cpu().double().abs() <= size * (16 * 2.0 ** -21 + 60 * 2.0 ** -24)).all())
+
+
 # ---- sampling ---------------------------------------------------------------------------------------
 
 
@@ -112,6 +151,47 @@ def test_sample_settings_that_are_not_numbers(vocabulary, top_p, top_k):
     assert torch.equal(got[0], check_sample(logits, clean, **{**plain, "top_p": torch.ones(6)})[0])
     got = run(temperature=nan)
     assert torch.equal(got[0].cpu(), logits.argmax(1)) and not bool(got[1].any())
+
+
+def test_sample_rows_beyond_32_bits():
+    """Rows 2^30 elements apart: the third starts 2^31 elements behind the first."""
+
+    from ue5m3_fp4 import serving
+
+    vocabulary, apart = 5000, 2 ** 30
+    memory = torch.empty(2 * apart + vocabulary, dtype=torch.bfloat16, device="cuda")
+    logits = memory.as_strided((3, vocabulary), (apart, 1))
+    logits.copy_(3 * torch.randn(3, vocabulary, generator=torch.Generator().manual_seed(1)))
+    uniforms = torch.tensor([0.1, 0.6, 0.9], device="cuda")
+    got, expect = (serving.sample_tokens(rows, uniforms, top_p=0.9) for rows in (logits, logits.contiguous()))
+    assert torch.equal(got[0], expect[0]) and torch.equal(got[1], expect[1])
+
+
+# ---- attention over a paged cache -----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("lengths,queries", [([700, 90], [1, 1]), ([700, 130], [60, 100])])
+def test_attention_over_a_cache_beyond_32_bits(lengths, queries):
+    """Pages of more than 2^31 elements, used at their end and in the middle: bit for bit as in a small cache with the
+    same contents, the new keys and values included."""
+
+    from ue5m3_fp4 import serving
+
+    expect, q, (k, v, table, kv, starts) = run_attention(lengths, queries, page=64, kv_heads=4, group=4, dim=128, seed=2)
+    count = k.shape[0]
+    pages = 2 ** 31 // (64 * 4 * 128) + 1000
+    large_k, large_v = (torch.empty(pages, 64, 4, 128, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    place = torch.arange(count, device="cuda").to(torch.int32)
+    place = torch.where(place % 2 == 0, pages - 1 - place, pages // 2 + place)
+    large_k[place.long()], large_v[place.long()] = k, v
+    moved = torch.where(table >= 0, place[table.clamp(min=0).long()], table)
+    new_k, new_v = (torch.randn(sum(queries), 4, 128, device="cuda").to(torch.bfloat16) for _ in range(2))
+    for more in ({}, dict(new_k=new_k, new_v=new_v)):
+        small = serving.paged_attention(q, k, v, table, kv, starts, max_query_length=max(queries), **more)
+        got = serving.paged_attention(q, large_k, large_v, moved, kv, starts, max_query_length=max(queries), **more)
+        assert torch.equal(got, small)
+    bits = lambda t: t.view(torch.int16)  # noqa: E731
+    assert torch.equal(bits(large_k[place.long()]), bits(k)) and torch.equal(bits(large_v[place.long()]), bits(v))
 
 
 # ---- packed linears ---------------------------------------------------------------------------------
@@ -163,7 +243,48 @@ def test_packed_linears_take_the_weight_that_was_installed(tmp_path, monkeypatch
     assert bool(((got - reference).abs() <= 2.0 ** -8 * reference.abs() + 1e-5).all())
 
 
-# ---- graphs -----------------------------------------------------------------------------------------
+# ---- graphs and streams ------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("cases", [[([5000], [1], 1, 8, 128), ([3001], [2], 2, 3, 64)],
+                                   [([4000, 90], [1, 1], 2, 4, 64), ([3500], [40], 1, 8, 64)],
+                                   [([2600, 700], [33, 5], 1, 2, 128), ([5000], [300], 1, 1, 128)]])
+def test_split_attention_in_two_graphs_and_on_two_streams(cases):
+    """Sequences split over CTAs leave partial rows in a workspace: two captured calls with data and lengths of their
+    own, replayed side by side on two streams next to eager calls, share none."""
+
+    from ue5m3_fp4 import serving
+    from ue5m3_fp4.serving.operators import _workspace_bytes
+
+    calls = []
+    for i, (lengths, queries, kv_heads, group, dim) in enumerate(cases):
+        expect, q, (k, v, table, kv, starts) = run_attention(lengths, queries, page=32, kv_heads=kv_heads, group=group, dim=dim, seed=i)
+        longest = table.shape[1] * 32
+        assert _workspace_bytes(q.get_device(), sum(queries), len(lengths), kv_heads * group, kv_heads, dim, max(queries), longest) > 0
+        call = lambda q=q, k=k, v=v, table=table, kv=kv, starts=starts, n=max(queries): (  # noqa: E731
+            serving.paged_attention(q, k, v, table, kv, starts, max_query_length=n))
+        assert torch.equal(call(), expect)
+        calls.append((call, expect))
+    graphs = []
+    for call, _ in calls:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+        graphs.append((graph, out))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        for _, out in graphs:
+            out.zero_()
+        torch.cuda.synchronize()
+        eager = []
+        for (graph, _), stream, (call, _) in zip(graphs, streams, reversed(calls)):
+            with torch.cuda.stream(stream):
+                for _ in range(3):
+                    graph.replay()
+                    eager.append(call())
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, expect) for (_, out), (_, expect) in zip(graphs, calls))
+        assert all(torch.equal(out, calls[1][1]) for out in eager[:3]) and all(torch.equal(out, calls[0][1]) for out in eager[3:])
 
 
 FIRST_CALL = """
