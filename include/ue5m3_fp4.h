@@ -410,7 +410,7 @@ typedef struct ue5m3_paged_cache {
  * 0 ... L - n + i.  A token that sees no key gets zeros.  new_k, new_v (both or neither): the new
  * tokens' keys and values [tokens, kv_heads, head_dim], written into their pages first.  Rows
  * behind the last sequence are left as they are, or zeroed when zero_tail != 0.
- * scale is positive.  query_starts and kv_lengths are read on the device; max_query and max_kv are bounds from which
+ * scale is positive and at most 2^126.  query_starts and kv_lengths are read on the device; max_query and max_kv are bounds from which
  * the launch is sized (larger actual values are right, only slower).  A page that the table does
  * not name among the cache's is not touched: rows that need it come out as NaN (others that share
  * their tile may, too); the same where kv_lengths exceeds the table.

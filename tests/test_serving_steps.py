@@ -4,6 +4,7 @@ for, steps that do not match the cache.  No GPU is needed; nothing here launches
 from __future__ import annotations
 
 import contextlib
+import ctypes
 
 import pytest
 import torch
@@ -69,3 +70,21 @@ def test_steps_without_all_their_tokens_are_refused():
     assert cache.lengths == (3, 2)
     with pytest.raises(RuntimeError, match="CUDA tensor"):
         cache.attend(0, torch.zeros(7, 1, 64, dtype=torch.bfloat16), rows, rows)
+
+
+def test_expanded_pages_and_scales_out_of_range_are_refused():
+    """Pages that share memory would be written to by several keys at a time; a scale above 2^126 would be infinite
+    once log2(e) is in it."""
+
+    pages = torch.zeros(1, 16, 2, 64, dtype=torch.bfloat16)
+    assert operators._strides("k_pages", pages) == (2048, 128, 64)
+    assert operators._strides("k_pages", torch.zeros(5, 16, 1, 128, dtype=torch.bfloat16)[:, :, :, :64]) == (2048, 128, 64)
+    for bad in (pages.expand(4, 16, 2, 64), pages[:, :1].expand(1, 16, 2, 64), pages[:, :, :1].expand(1, 16, 2, 64)):
+        with pytest.raises(ValueError, match="expanded"):
+            operators._strides("k_pages", bad)
+    assert operators._strides("new_k", torch.zeros(3, 1, 64, dtype=torch.bfloat16).expand(3, 4, 64)) == (64, 0)
+    library, fake = _native.load(), 0x10000
+    cache = _native.PagedCache(fake, fake, 1024, 64, 64, 1024, 64, 64, 4, 16, 1, 64, fake, 1, 2, 2)
+    for scale in (2.0 ** 127, 3e38):
+        assert library.ue5m3_paged_attention(fake, 128, 64, 1, 2, ctypes.byref(cache), fake, fake, 1, 32, scale, None, 0, 0, None, 0, 0,
+                                             fake, 1, None, 0, None, None) == 1

@@ -624,7 +624,7 @@ extern "C" int ue5m3_paged_attention(const void* q, int64_t q_token_stride, int6
     using namespace ue5m3;
     using namespace ue5m3::paged;
     if (!q || !cache || !kv_lengths || !query_starts || !out || !cache->k_pages || !cache->v_pages ||
-        !cache->page_table || (new_k == nullptr) != (new_v == nullptr) || !(scale > 0.0f) || scale > 3e38f)
+        !cache->page_table || (new_k == nullptr) != (new_v == nullptr) || !(scale > 0.0f) || scale > 0x1p126f)
         return UE5M3_ERR_INVALID_ARGUMENT;
     const int64_t dim = cache->head_dim;
     if (!paged_sizes_ok(tokens, cache->sequences, heads, cache->kv_heads, dim, max_query, max_kv) || cache->pages <= 0 ||

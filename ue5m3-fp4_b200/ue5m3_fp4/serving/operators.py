@@ -149,6 +149,8 @@ def _strides(name: str, tensor: Tensor) -> tuple[int, ...]:
     strides = tensor.stride()
     if strides[-1] != 1:
         raise ValueError(f"{name} must have contiguous channels")
+    if tensor.ndim == 4 and any(stride == 0 and size > 1 for size, stride in zip(tensor.shape, strides)):
+        raise ValueError(f"{name} must not be expanded: every key and value has a place of its own")
     if 1 in tensor.shape[:-1]:
         strides = tuple(0 if size == 1 else stride for size, stride in zip(tensor.shape, strides))
         if tensor.ndim == 4:  # the tensor map of the pages takes no zero strides
@@ -236,8 +238,8 @@ def paged_attention(
         raise ValueError("max_query_length and max_kv_length must be positive")
     if scale is None:
         scale = head_dim ** -0.5
-    elif not 0 < scale < float("inf"):
-        raise ValueError("scale must be positive and finite")
+    elif not 0 < scale <= 2.0 ** 126:  # times log2(e), in fp32
+        raise ValueError("scale must be positive and no larger than 2^126")
     zero_tail = out is None
     if zero_tail:
         out = q.new_empty((tokens, heads, head_dim))
