@@ -13,7 +13,7 @@
 // total.  The order of all sums is fixed by the sizes: the same call gives the same bits.
 // Where a row's 128 elements span more than that (a wide column), they count as zeros there and enter in a
 // second product of their own: as they are, in bf16 (fp32: three bf16 parts), with the same weights, which
-// bf16 holds as exactly as fp16.  Doing so for every chunk would double the work of decoding.
+// bf16 holds as exactly as fp16.  (Every chunk this way: 19 operations in place of 8 to decode eight codes.)
 //
 // What bounds it: reading the codes, 0.5 byte per weight element, plus the scales.  Decoding costs
 // one cvt.rn.f16x2.e2m1x2 and one packed multiply per two weights.
@@ -22,20 +22,22 @@
 // 16-row tile are not loaded, so that all SMs read the same number of bytes), every one of its
 // warps w the 128-element chunks w, w + 16, ... of the reduction axis.  A warp keeps the activations
 // of its chunks in registers (as mma fragments) while it walks over the CTA's rows; the sums of
-// the 16 warps meet in shared memory once per block of rows.  Measured: 1 x 21504 x 4096: 15.6 us,
-// 2.8 TB/s of 6.5; 8 x 4096 x 21504: 20.5 us, 2.3 TB/s; 1 x 512 x 4096: 4.8 us.  The walk itself reads
-// at about three quarters of the memory's rate; the rest is the launch, the loading and conversion of
-// the activations (some 5000 cycles in which no weight is decoded) and the sums at the end.  Rows that
-// start anywhere come as aligned pieces and are shifted into place: 1 x 21504 x 4095: 29 us (word by
-// word into registers 51, pieces per warp and chunk 34).
+// the 16 warps meet in shared memory once per block of rows.  Measured: 1 x 21504 x 4096: 15.5 us,
+// 2.9 TB/s of 6.5 (fp32 22.3); 8 x 4096 x 21504: 20.6 us, 2.3 TB/s (fp32 36.3); 1 x 512 x 4096: 4.8 us.
+// Of its active cycles the first one issues in 55 % of the slots and keeps the ALU, which decodes, busy
+// for 42 %; launch, conversion of the activations (a look at their range costs 0.3 us of it) and
+// the sums at the end do not overlap with the walk.  Rows that start anywhere come as aligned pieces
+// and are shifted into place: 1 x 21504 x 4095: 29 us (word by word into registers 51, pieces per warp
+// and chunk 34).
 //
 // More tokens.  There every CTA would convert all activations for its few rows: a short kernel writes
 // them as fragments once (tokens x K x 2 bytes, three times that for fp32), and CTAs of 128 rows take
 // them through a ring in shared memory, next to codes and scales, four warps of 32 rows for each of
-// two halves of the chunks.  Measured: 64 x 18560 x 4096: 105 -> 39.8 us, 244 TFLOP/s, about one mma in
-// 16 cycles and quarter of an SM; 33 x 4096 x 4096: 31 -> 13.5; 60 x 2718 x 15245, whose rows start
-// anywhere: 258 -> 46; fp32, three products each, 40 x 2000 x 3001: 47.5 -> 17.5, 64 x 4096 x 4096: 30.
-// Bound by the products' issue from 32 tokens on, by decoding and the fragments' way from L2 below
+// two halves of the chunks.  Measured: 64 x 18560 x 4096: 105 -> 40.3 us, 242 TFLOP/s, an mma in 17.5 active
+// cycles of each quarter of an SM, the tensor pipe 47 % busy; 33 x 4096 x 4096: 31 -> 13.8; 60 x 2718 x 15245,
+// whose rows start anywhere: 258 -> 47; fp32, three products each, 40 x 2000 x 3001: 47.5 -> 17.5,
+// 64 x 4096 x 4096: 30.4; 2048 x 21504 x 4096, the weight decoded again for every 64 rows: 1444.  Bound by the
+// products' issue from 32 tokens on, by decoding and the fragments' way from L2 below
 // (16 x 21504 x 4096: 32 us).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -847,7 +849,7 @@ __global__ void __launch_bounds__(kManyThreads, kFp32 || kTiles > 4 ? 1 : 2)
     const uint8_t* scales = p.scales + scale_row0 * p.scale_stride;
 
     // codes and scales of the chunks to come: wide rows as in the kernel for few tokens, with the scales of
-    // a row per lane; others word by word
+    // a row per lane; others in aligned pieces of 8 and 4 bytes
     uint4* slots = ring + 2 * kManyRing * kStage + warp * kManyRing * kSlot;
     auto copy_codes = [&](int i) {
         if (i < count && active) {

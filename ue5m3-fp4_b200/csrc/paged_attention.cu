@@ -532,6 +532,8 @@ static size_t workspace_of(int64_t tokens, int64_t heads, int64_t head_dim, int6
 // time and adds the writing and reading of its partial rows at about 0.7 TB/s, so that the square
 // root of their quotient is the best number (8 x 32 heads over 32768 keys: 465 -> 35 us with 37 splits;
 // 4 x 128 tokens over 2048 keys: 46.5 us without, 57.8 with 3).
+// One plan serves the whole call and goes by its longest query and sequence: single tokens behind long
+// contexts are split as finely as they need only in a call without a prompt chunk.
 static Plan make_plan(int64_t tokens, int64_t sequences, int64_t heads, int64_t kv_heads, int64_t head_dim,
                       int64_t max_query, int64_t max_kv) {
     Plan plan;

@@ -18,12 +18,17 @@
 // TMEM, 2 and 3 the values of keys that not every row sees (cleared, or kept finite, before a product
 // meets them), 4..11 the softmax of the two tiles (TMEM lanes by warp % 4).
 //
-// Measured: 2048 tokens of 8192 keys, 32 heads over 4 key/value heads of 128: 235 us, 1024 TFLOP/s of
-// 1649.  Per 2 x 128 x 128 scores it takes 3500 cycles, of which the products are 2048: TMEM has room
-// for one S per tile beside the outputs, so a tile's products wait for its softmax and only the other
-// tile's hide it.  Scores by the issuing warp's additions to constant descriptors: 300 -> 243 us;
-// probabilities handed over in halves and keys' stages released by the warps that see the scores: 236.
-// Slower, each: 64 keys per step 306, a polynomial in place of some ex2, scores read from TMEM twice.
+// Measured: 2048 tokens of 8192 keys, 32 heads over 4 key/value heads of 128: 236 us, 1020 TFLOP/s of
+// 1649.  Per 2 x 128 x 128 scores an SM is active for 3800 cycles, in 2070 of which its tensor pipe is: with
+// head_dim 128 TMEM has room for one whole S per tile beside the outputs, so a tile's products wait for
+// its softmax and only the other tile's hide it (head_dim 64 leaves 128 columns unused).  Scores by the
+// issuing warp's additions to constant descriptors: 300 -> 243 us; probabilities handed over in halves and
+// keys' stages released by the warps that see the scores: 236.  Slower, each: 64 keys per step 306, a
+// polynomial in place of some ex2, scores read from TMEM twice.
+//
+// A probability is rounded to bf16 for its product, its row's sum takes it unrounded: with the output's
+// own rounding the relative error is 0.0023 where one rounding leaves 0.0017.  Summing the rounded ones
+// instead gives 0.0022 and takes 287 us in place of 236 (the softmax's registers no longer suffice).
 #include <math.h>
 
 #include "abi_common.cuh"

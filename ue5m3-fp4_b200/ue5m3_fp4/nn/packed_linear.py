@@ -17,7 +17,9 @@ from ue5m3_fp4.packed import PackedFP4Tensor
 
 class PackedFP4Linear(torch.nn.Module):
     """``x @ W.T + bias`` with a packed weight; no gradients.  Reads 0.5 byte per weight element and
-    one byte per block, once for up to 64 rows of bf16 ``x`` and 32 of fp32."""
+    one byte per block, once for every 64 rows of bf16 ``x`` and every 32 of fp32: made for the tokens of a decoding
+    step.  Whole prompts are right too, but read and decode the weight that often; where they
+    dominate, the frozen ``UE5M3Linear`` (whose GEMM quantizes its activations) is the faster form."""
 
     def __init__(self, weight: PackedFP4Tensor, bias: Tensor | None = None) -> None:
         super().__init__()

@@ -91,9 +91,9 @@ def packed_matvec(
     ``scales`` as ``quantize_packed`` and ``PackedFP4Tensor`` hold them) for a few rows of bf16 or
     fp32 activations, which are not quantized.  Sums are fp32; the result is rounded once, to
     ``out_dtype`` (default: that of ``x``).  Any ``rows`` and ``cols``; the last axis of ``x`` must be
-    contiguous.  Eight rows are read at the cost of one; the weight is read once for every 64 rows of bf16
-    ``x`` and every 32 of fp32, whose products grow with each: for whole prompts use the GEMM.  At most 2^24 rows of ``x``, 2^30 ``rows``
-    and 2^22 ``cols``."""
+    contiguous.  Eight rows are read at the cost of one; the weight is read and decoded once for every 64 rows
+    of bf16 ``x`` and every 32 of fp32, so that whole prompts run at no more than about 250 TFLOP/s.
+    At most 2^24 rows of ``x``, 2^30 ``rows`` and 2^22 ``cols``."""
 
     _require_cuda(x, "x")
     _no_gradient(x, bias)
