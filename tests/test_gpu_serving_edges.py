@@ -36,7 +36,8 @@ def without_columns(codes: torch.Tensor, columns) -> torch.Tensor:
 @pytest.mark.parametrize("tokens,rows,cols,block,two_d", [(1, 40, 384, 16, False), (8, 33, 1003, 32, False), (3, 150, 4096, 16, True),
                                                           (9, 130, 384, 32, True), (20, 40, 1003, 16, False), (45, 257, 640, 16, True),
                                                           (70, 20, 300, 32, False), (16, 21504, 256, 32, True),
-                                                          (8, 30011, 300, 16, False)])
+                                                          (8, 30011, 300, 16, False), (2, 20, 140000, 16, False),
+                                                          (30, 70, 9000, 32, False)])
 def test_matvec_keeps_small_activations_beside_large_ones(tokens, rows, cols, block, two_d, dtype, spread):
     """Elements 2^spread times their neighbours that meet zeros of the weight: what is left is the
     neighbours' sum, to the same tolerance as without them.  Rows without such elements come out bit for
@@ -46,7 +47,7 @@ def test_matvec_keeps_small_activations_beside_large_ones(tokens, rows, cols, bl
 
     g = torch.Generator().manual_seed(spread + cols)
     codes, scales = packed_weight(rows, cols, block, two_d, seed=cols)
-    large = [5, 130, 131, cols - 1]
+    large = [5, 130, 131, cols // 2, cols - 1]
     codes = without_columns(codes, large)
     x = torch.randn(tokens, cols, generator=g, dtype=torch.float64)
     plain = x.clone().to(DTYPES[dtype])
@@ -62,6 +63,22 @@ def test_matvec_keeps_small_activations_beside_large_ones(tokens, rows, cols, bl
     without = serving.packed_matvec(plain.cuda(), codes.cuda(), scales.cuda(), **kw)
     others = [t for t in range(tokens) if t not in touched]
     assert torch.equal(got[others], without[others])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("tokens,rows,cols,block,two_d", [(1, 150, 4096, 16, True), (8, 300, 8192, 32, False), (5, 90, 2049, 16, False),
+                                                          (64, 520, 4096, 16, True), (20, 129, 6000, 32, False)])
+def test_matvec_of_squared_relus(tokens, rows, cols, block, two_d, dtype):
+    """Activations as a squared-ReLU MLP makes them: half of them zero, a few very small, here and there alone in the
+    columns of the weight that are not zero."""
+
+    g = torch.Generator().manual_seed(cols)
+    x = torch.relu(torch.randn(tokens, cols, generator=g)).to(torch.bfloat16).square().to(DTYPES[dtype])
+    x[::2, 77::128] = 2.0 ** -40
+    codes, scales = packed_weight(rows, cols, block, two_d, seed=cols)
+    check_matvec(x, codes, scales, rows, cols, block, two_d)
+    codes[:rows // 2] = without_columns(codes[:rows // 2], [j for j in range(cols) if j % 128 != 77])
+    check_matvec(x, codes, scales, rows, cols, block, two_d, out_dtype=torch.float32, amax=448.0 * 6)
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])

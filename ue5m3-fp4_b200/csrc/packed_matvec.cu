@@ -12,8 +12,10 @@
 // columns) sum 128 products in fp32; the power of two is multiplied back when that sum joins the fp32
 // total.  The order of all sums is fixed by the sizes: the same call gives the same bits.
 // Where a row's 128 elements span more than that (a wide column), they count as zeros there and enter in a
-// second product of their own: as they are, in bf16 (fp32: three bf16 parts), with the same weights, which
-// bf16 holds as exactly as fp16.  (Every chunk this way: 19 operations in place of 8 to decode eight codes.)
+// second product of their own, after the others: as they are, in bf16 (fp32: three bf16 parts), with the same
+// weights, which bf16 holds as exactly as fp16.  (Every chunk this way: 19 operations in place of 8 to
+// decode eight codes.)  Of squared ReLUs of normal numbers one column in 360 is wide: 8 x 4096 x 21504 takes
+// 23.8 us with them, 21.5 without; 64 x 4096 x 21504 62.7 and 53.9; with nothing but wide columns 42 and 259.
 //
 // What bounds it: reading the codes, 0.5 byte per weight element, plus the scales.  Decoding costs
 // one cvt.rn.f16x2.e2m1x2 and one packed multiply per two weights.
@@ -33,12 +35,12 @@
 // More tokens.  There every CTA would convert all activations for its few rows: a short kernel writes
 // them as fragments once (tokens x K x 2 bytes, three times that for fp32), and CTAs of 128 rows take
 // them through a ring in shared memory, next to codes and scales, four warps of 32 rows for each of
-// two halves of the chunks.  Measured: 64 x 18560 x 4096: 105 -> 40.3 us, 242 TFLOP/s, an mma in 17.5 active
-// cycles of each quarter of an SM, the tensor pipe 47 % busy; 33 x 4096 x 4096: 31 -> 13.8; 60 x 2718 x 15245,
+// two halves of the chunks.  Measured: 64 x 18560 x 4096: 105 -> 41.1 us, 237 TFLOP/s, an mma in 17.5 active
+// cycles of each quarter of an SM, the tensor pipe 47 % busy; 33 x 4096 x 4096: 31 -> 13.7; 60 x 2718 x 15245,
 // whose rows start anywhere: 258 -> 47; fp32, three products each, 40 x 2000 x 3001: 47.5 -> 17.5,
-// 64 x 4096 x 4096: 30.4; 2048 x 21504 x 4096, the weight decoded again for every 64 rows: 1444.  Bound by the
+// 64 x 4096 x 4096: 30.5; 2048 x 21504 x 4096, the weight decoded again for every 64 rows: 1444.  Bound by the
 // products' issue from 32 tokens on, by decoding and the fragments' way from L2 below
-// (16 x 21504 x 4096: 32 us).
+// (16 x 21504 x 4096: 32.7 us).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -241,8 +243,8 @@ __device__ __forceinline__ bool too_small(uint32_t top, uint32_t least) {
 // One chunk's activations as mma B fragments (fp32: three, of 11 bits each, the second to be multiplied
 // by 2^-11, the third by 2^-22), and the factor that undoes the chunk's power of two.  Lane (g, c) =
 // (lane / 4, lane % 4) brings column g and elements 32 c ... 32 c + 31; step j of the chunk's eight mma
-// takes its elements 4 j ... 4 j + 3.  A wide column's fragments are zero; returns whether one
-// of the eight columns is wide.
+// takes its elements 4 j ... 4 j + 3.  A wide column's fragments are zero, its factor negative; returns
+// whether one of the eight columns is wide.
 template <bool kFp32>
 __device__ __forceinline__ bool make_fragments(const Raw<kFp32>& raw, uint32_t (&b)[kFp32 ? 3 : 1][16], float& undo) {
     uint32_t top, least;
@@ -278,6 +280,7 @@ __device__ __forceinline__ bool make_fragments(const Raw<kFp32>& raw, uint32_t (
         }
     }
     if (small >> (threadIdx.x & 28) & 15) {  // seldom
+        undo = -1.0f;
 #pragma unroll
         for (int part = 0; part < (kFp32 ? 3 : 1); ++part)
 #pragma unroll
@@ -401,21 +404,67 @@ __device__ __forceinline__ void decode(const Piece (&piece)[2], const uint32_t (
     }
 }
 
-// Seldom: the wide columns among tokens token0 ... token0 + here - 1 (eight at most) in one chunk, times
-// `row_count` rows from row0 on, added to[token * stride + row].  By one warp; a lane adds to the places of tokens
-// 2 c and 2 c + 1 and rows g and g + 8 of every 16.  fp32 elements are cut off to 8 bits, not rounded: every rest
-// is exact, and 2^8 of it is below twice the element.
-template <bool kFp32, int kBlock>
-__device__ __forceinline__ void add_wide(const Params& p, int chunk, int token0, int here, int row0, int row_count, float* to, int stride) {
-    constexpr int kParts = kFp32 ? 3 : 1;
-    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const Raw<kFp32> raw = load_raw<kFp32>(p, token0 + g, g < here, chunk);
+// The wide columns of one chunk, seldom needed.  What one warp reads for them: a chunk of eight tokens at most, and
+// its codes and scales for up to kRowTiles times 16 rows.
+template <bool kFp32, int kRowTiles>
+struct Wide {
+    Raw<kFp32> raw;
+    Piece pieces[kRowTiles][2];
+};
+
+// 32 codes from `at` on, which may lie anywhere; what is not in the array counts as zero
+__device__ __forceinline__ uint4 load_codes_anywhere(const uint8_t* at, const uint8_t* array, const uint8_t* end) {
+    const uint32_t off = (uint32_t)(uintptr_t)at & 3;
+    const uint8_t* aligned = at - off;
+    uint32_t w[5];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) {
+        const uint8_t* from = aligned + 4 * i;
+        w[i] = 0;
+        if (from >= array && from + 4 <= end) {
+            w[i] = __ldg(reinterpret_cast<const uint32_t*>(from));
+        } else {
+#pragma unroll 1
+            for (int e = 0; e < 4; ++e)
+                if (from + e >= array && from + e < end) w[i] |= (uint32_t)from[e] << (8 * e);
+        }
+    }
+    return make_uint4(__funnelshift_r(w[0], w[1], 8 * off), __funnelshift_r(w[1], w[2], 8 * off), __funnelshift_r(w[2], w[3], 8 * off),
+                      __funnelshift_r(w[3], w[4], 8 * off));
+}
+
+// ... of rows row0 ... row0 + row_count - 1, the last one again in the place of missing ones
+template <bool kFp32, bool kVector, int kBlock, int kRowTiles>
+__device__ __forceinline__ void load_pieces(const Params& p, Wide<kFp32, kRowTiles>& wide, int chunk, int row0, int row_count) {
+    const int g = (threadIdx.x & 31) >> 2, c = threadIdx.x & 3;
+#pragma unroll
+    for (int tile = 0; tile < kRowTiles; ++tile)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            Piece& piece = wide.pieces[tile][h];
+            const int64_t row = row0 + min(16 * tile + g + 8 * h, row_count - 1);
+            const uint8_t* codes = p.codes + row * p.code_stride + chunk * (kChunk / 2) + 16 * c;
+            const uint8_t* scales = p.scales + (row >> p.row_shift) * p.scale_stride;
+            const int at = chunk * (kChunk / kBlock) + c * (32 / kBlock);
+            if constexpr (kVector) {
+                piece.codes = __ldg(reinterpret_cast<const uint4*>(codes));
+                piece.scales = kBlock == 16 ? __ldg(reinterpret_cast<const uint16_t*>(scales + at)) : __ldg(scales + at);
+            } else {
+                piece.codes = load_codes_anywhere(codes, p.codes, p.codes + p.rows * p.code_stride);
+                piece.scales = at < p.scale_stride ? __ldg(scales + at) : 0;
+                if (kBlock == 16 && at + 1 < p.scale_stride) piece.scales |= (uint32_t)__ldg(scales + at + 1) << 8;
+            }
+        }
+}
+
+// The wide columns' fragments: bf16; fp32 elements are cut off to 8 bits, not rounded, so that every rest is exact
+// and 2^8 of it below twice the element.  Returns four bits for every token with a wide column.
+template <bool kFp32>
+__device__ __forceinline__ uint32_t make_wide_fragments(const Raw<kFp32>& raw, uint32_t (&b)[kFp32 ? 3 : 1][16]) {
     uint32_t top, least;
     range_of<kFp32>(raw, top, least);
     const uint32_t small = __ballot_sync(0xFFFFFFFFu, too_small<kFp32>(top, least));
-    if (small == 0) return;
-    const bool wide = small >> (lane & 28) & 15;
-    uint32_t b[kParts][16];
+    const bool wide = small >> (threadIdx.x & 28) & 15;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         if constexpr (kFp32) {
@@ -430,56 +479,42 @@ __device__ __forceinline__ void add_wide(const Params& p, int chunk, int token0,
             b[0][i] = wide ? raw.words[i] : 0;
         }
     }
-#pragma unroll 1
-    for (int tile = 0; tile < row_count; tile += 16) {
-        Piece now[2];
+    return small;
+}
+
+// ... times 16 rows, added to[token * stride + row]: a lane's tokens are 2 c and 2 c + 1, its rows g and g + 8
+template <bool kFp32, int kBlock>
+__device__ __forceinline__ void add_wide(const Piece (&now)[2], const uint32_t (&b)[kFp32 ? 3 : 1][16], uint32_t small, int row_count,
+                                         float* to, int stride) {
+    constexpr int kParts = kFp32 ? 3 : 1;
+    const int g = (threadIdx.x & 31) >> 2, c = threadIdx.x & 3;
+    uint32_t scale[2][2];
+    scale_pairs<kBlock>(now, scale);
+    float sum[kParts][4] = {};
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int64_t row = row0 + min(tile + g + 8 * h, row_count - 1);
-            const uint8_t *codes = p.codes + row * p.code_stride, *scales = p.scales + (row >> p.row_shift) * p.scale_stride;
-            uint32_t words[4] = {};
-#pragma unroll 1
-            for (int i = 0; i < 4; ++i)
+    for (int j = 0; j < 4; ++j) {
+        uint32_t a[2][4];
+        decode<kBlock>(now, scale, j, a);
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const int at = chunk * (kChunk / 2) + 16 * c + 4 * w + i;
-                    if (at < p.code_stride) words[w] |= (uint32_t)codes[at] << (8 * i);
-                }
-            now[h].codes = make_uint4(words[0], words[1], words[2], words[3]);
-            now[h].scales = 0;
-            for (int i = 0; i < 32 / kBlock; ++i) {
-                const int at = chunk * (kChunk / kBlock) + c * (32 / kBlock) + i;
-                if (at < p.scale_stride) now[h].scales |= (uint32_t)scales[at] << (8 * i);
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {  // six significant bits, 2^-22 ... 2^16: exact in bf16
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a[h][i]));
+                a[h][i] = __float_as_uint(f.x) >> 16 | (__float_as_uint(f.y) & 0xFFFF0000u);
             }
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) {
+            mma_bf16(sum[part], a[0][0], a[1][0], a[0][1], a[1][1], b[part][4 * j], b[part][4 * j + 1]);
+            mma_bf16(sum[part], a[0][2], a[1][2], a[0][3], a[1][3], b[part][4 * j + 2], b[part][4 * j + 3]);
         }
-        uint32_t scale[2][2];
-        scale_pairs<kBlock>(now, scale);
-        float sum[kParts][4] = {};
+    }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint32_t a[2][4];
-            decode<kBlock>(now, scale, j, a);
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {  // six significant bits, 2^-22 ... 2^16: exact in bf16
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a[h][i]));
-                    a[h][i] = __float_as_uint(f.x) >> 16 | (__float_as_uint(f.y) & 0xFFFF0000u);
-                }
-#pragma unroll
-            for (int part = 0; part < kParts; ++part) {
-                mma_bf16(sum[part], a[0][0], a[1][0], a[0][1], a[1][1], b[part][4 * j], b[part][4 * j + 1]);
-                mma_bf16(sum[part], a[0][2], a[1][2], a[0][3], a[1][3], b[part][4 * j + 2], b[part][4 * j + 3]);
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int token = 2 * c + (e & 1), row = tile + g + 8 * (e >> 1);
-            if (!(small >> (4 * token) & 15) || row >= row_count) continue;
-            float whole = sum[0][e];
-            if constexpr (kFp32) whole = __fmaf_rn(sum[2][e], 0x1p-16f, __fmaf_rn(sum[1][e], 0x1p-8f, whole));
-            to[token * stride + row] += whole;
-        }
+    for (int e = 0; e < 4; ++e) {
+        const int token = 2 * c + (e & 1), row = g + 8 * (e >> 1);
+        if (!(small >> (4 * token) & 15) || row >= row_count) continue;
+        float whole = sum[0][e];
+        if constexpr (kFp32) whole = __fmaf_rn(sum[kParts - 1][e], 0x1p-16f, __fmaf_rn(sum[kParts / 2][e], 0x1p-8f, whole));
+        to[token * stride + row] += whole;
     }
 }
 
@@ -573,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
         int slot_now = 0;
-        bool wide = false;  // whether one of this warp's chunks has a wide column
+        uint32_t wide = 0;  // bit i: this warp's i-th chunk has a wide column; bit 31: one of those from the 32nd on has
         if (kVector) locate();
 #pragma unroll
         for (int i = 0; i < kRing - 1; ++i) copy_ahead(i);
@@ -588,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
                     kVector ? load_raw<kFp32>(p, g, g < tokens && chunk < chunks, chunk)
                             : load_staged<kFp32>(p, 0, chunk < chunks ? tokens : 0, chunk, reinterpret_cast<uint32_t*>(ring + kRing * kSlot) + warp * kStageWords),
                     b[d], mine);
-                wide = wide || any;
+                wide |= any ? 1u << min(pass * kDepth + d, 31) : 0;
                 undo[d][0] = __shfl_sync(0xFFFFFFFFu, mine, 8 * c);
                 undo[d][1] = __shfl_sync(0xFFFFFFFFu, mine, 8 * c + 4);
             }
@@ -673,10 +708,29 @@ __global__ void __launch_bounds__(kThreads, 1) packed_matvec_kernel(const Params
                     }
             }
         }
-        if (wide)
+        // wide columns, seldom: chunk by chunk of this warp's that has some, 64 rows at a time
+        for (int turn = 0; wide; ++turn) {
+            if (turn < 31 && !(wide & 1)) {
+                wide >>= 1;
+                continue;
+            }
+            const int chunk = first_chunk + turn * kWarps + warp;
+            if (chunk >= chunks) break;
+            if (turn < 31) wide >>= 1;  // the last bit stands for all further ones
+            uint32_t b[kParts][16];
+            Wide<kFp32, 4> now;
+            load_pieces<kFp32, kVector, kBlock, 4>(p, now, chunk, row0, row_count);
+            const uint32_t small = make_wide_fragments<kFp32>(load_raw<kFp32>(p, g, g < tokens, chunk), b);
 #pragma unroll 1
-            for (int chunk = first_chunk + warp; chunk < chunks; chunk += kWarps)
-                add_wide<kFp32, kBlock>(p, chunk, 0, tokens, row0, row_count, partial + warp * tokens * block_rows, block_rows);
+            for (int r = 0; r < row_count; r += 64) {
+                if (r > 0) load_pieces<kFp32, kVector, kBlock, 4>(p, now, chunk, row0 + r, row_count - r);
+#pragma unroll
+                for (int tile = 0; tile < 4; ++tile)
+                    if (r + 16 * tile < row_count)
+                        add_wide<kFp32, kBlock>(now.pieces[tile], b, small, row_count - r - 16 * tile,
+                                                partial + warp * tokens * block_rows + r + 16 * tile, block_rows);
+            }
+        }
         __syncthreads();
         if (p.split > 1) {
             // the sums of this CTA's warps, in the place of its first warp's; then those of the cluster
@@ -760,8 +814,8 @@ __host__ __device__ constexpr int many_slot(bool vector) { return vector ? 2 * 2
 __host__ __device__ constexpr int many_stage(int tiles, int parts) { return tiles * (parts * 128 + 2); }
 
 // The activations as the product reads them: [chunk][tile of 8 tokens][part][step][lane] 16 bytes, and
-// the factors that undo the chunks' powers of two: [chunk][tile][token].  One warp per chunk and tile; a byte
-// per CTA tells whether one of its columns is wide (up to four bytes of zeros behind the last).
+// the factors that undo the chunks' powers of two: [chunk][tile][token], and a byte that tells whether a column is
+// wide: [chunk][tile].  One warp per chunk and tile.
 template <bool kFp32>
 __global__ void __launch_bounds__(kManyThreads) prepare_kernel(const Params p, uint4* fragments, float* undo, uint8_t* wide, int chunks, int tiles) {
     constexpr int kParts = kFp32 ? 3 : 1;
@@ -770,24 +824,22 @@ __global__ void __launch_bounds__(kManyThreads) prepare_kernel(const Params p, u
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int64_t unit = (int64_t)blockIdx.x * kManyWarps + warp;
     const int chunk = (int)(unit / tiles), tile = (int)(unit % tiles);
-    bool any = false;
-    if (chunk < chunks) {
-        const int here = min(8, p.tokens - 8 * tile);
-        uint32_t b[kParts][16];
-        float mine;
-        any = make_fragments<kFp32>(p.vector_x ? load_raw<kFp32>(p, 8 * tile + g, g < here, chunk)
-                                               : load_staged<kFp32>(p, 8 * tile, here, chunk, reinterpret_cast<uint32_t*>(stage) + warp * kStageWords),
-                                    b, mine);
-        uint4* to = fragments + unit * (kParts * 128) + lane;
+    if (chunk >= chunks) return;
+    const int here = min(8, p.tokens - 8 * tile);
+    uint32_t b[kParts][16];
+    float mine;
+    const bool any =
+        make_fragments<kFp32>(p.vector_x ? load_raw<kFp32>(p, 8 * tile + g, g < here, chunk)
+                                         : load_staged<kFp32>(p, 8 * tile, here, chunk, reinterpret_cast<uint32_t*>(stage) + warp * kStageWords),
+                              b, mine);
+    uint4* to = fragments + unit * (kParts * 128) + lane;
 #pragma unroll
-        for (int part = 0; part < kParts; ++part)
+    for (int part = 0; part < kParts; ++part)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                to[part * 128 + j * 32] = make_uint4(b[part][4 * j], b[part][4 * j + 1], b[part][4 * j + 2], b[part][4 * j + 3]);
-        if (c == 0) undo[unit * 8 + g] = mine;
-    }
-    any = __syncthreads_or(any);
-    if (threadIdx.x < (blockIdx.x + 1 < gridDim.x ? 1 : 4)) wide[blockIdx.x + threadIdx.x] = any && threadIdx.x == 0;
+        for (int j = 0; j < 4; ++j)
+            to[part * 128 + j * 32] = make_uint4(b[part][4 * j], b[part][4 * j + 1], b[part][4 * j + 2], b[part][4 * j + 3]);
+    if (c == 0) undo[unit * 8 + g] = mine;
+    if (lane == 0) wide[unit] = any;
 }
 
 // What a warp of the product owns: rows row0 ... of its CTA's block, every second chunk from `first` to before
@@ -890,10 +942,7 @@ __global__ void __launch_bounds__(kManyThreads, kFp32 || kTiles > 4 ? 1 : 2)
 #pragma unroll
     for (int i = 0; i < kManyRing - 1; ++i) copy_activations(i);
 
-    // the preparation's first 128 bytes about wide columns, looked at in the end
-    const int prepared = (int)(((int64_t)chunks * tiles + kManyWarps - 1) / kManyWarps);
-    uint32_t any_wide = 4 * lane < prepared ? __ldcg(reinterpret_cast<const uint32_t*>(wide) + lane) : 0;
-
+    uint32_t signs = 0;  // of the factors: that of a wide column is negative
     float total[2][kTiles][4] = {};
     for (int i = 0; i < count; ++i) {
         // this thread's copies for chunk i are there; behind the barrier all are, and the slot before is free
@@ -947,6 +996,7 @@ __global__ void __launch_bounds__(kManyThreads, kFp32 || kTiles > 4 ? 1 : 2)
         for (int t = 0; t < kTiles; ++t) {
             if (t % 2 == 0 && t >= here) break;
             const float2 back = undo_from[t * 4];
+            if (t < here) signs |= __float_as_uint(back.x) | __float_as_uint(back.y);
 #pragma unroll
             for (int r = 0; r < 2; ++r)
 #pragma unroll
@@ -967,19 +1017,48 @@ __global__ void __launch_bounds__(kManyThreads, kFp32 || kTiles > 4 ? 1 : 2)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 partial[(half * kTiles * 8 + 8 * t + 2 * c + (e & 1)) * kManyPad + warp % 4 * 32 + 16 * r + g + 8 * (e >> 1)] = total[r][t][e];
-    for (int i = 128 + 4 * lane; i < prepared; i += 128) any_wide |= __ldcg(reinterpret_cast<const uint32_t*>(wide + i));
-    if (__any_sync(0xFFFFFFFFu, any_wide != 0)) {
+    if (__any_sync(0xFFFFFFFFu, signs >> 31)) {
+        // wide columns, seldom: 32 of the half's chunks at a time, each lane looks at one; then one unit (chunk and tile)
+        // after the other, the next one's reads in flight
         const Share again = share_of<kTiles>(p, chunks, tiles, block_index_again(), thread_index_again() >> 5);
-        if (again.row_count > 0)
+        float* sums = partial + again.half * kTiles * 8 * kManyPad + again.row0 - again.block_row;
 #pragma unroll 1
-            for (int chunk = again.first; chunk < again.last; chunk += 2)
+        for (int base = again.first; base < again.last && again.row_count > 0; base += 64) {
+            const int mine = base + 2 * lane;
+            uint32_t bits = 0;  // of the tiles of this lane's chunk
+            if (mine < again.last)
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t)
+                    if (t < again.here && __ldcg(wide + (int64_t)mine * tiles + again.tile0 + t)) bits |= 1u << t;
+            auto next = [&]() {  // a unit that is left: lane * 8 + tile, or -1
+                const uint32_t left = __ballot_sync(0xFFFFFFFFu, bits != 0);
+                if (left == 0) return -1;
+                const int from = __ffs(left) - 1, t = __ffs(__shfl_sync(0xFFFFFFFFu, bits, from)) - 1;
+                if (lane == from) bits &= bits - 1;
+                return from * 8 + t;
+            };
+            Wide<kFp32, 2> now, then;
+            auto load = [&](Wide<kFp32, 2>& unit, int at) {
+                const int chunk = base + 2 * (at / 8), token = 8 * (again.tile0 + at % 8);
+                load_pieces<kFp32, kVector, kBlock, 2>(p, unit, chunk, again.row0, again.row_count);
+                unit.raw = load_raw<kFp32>(p, token + g, token + g < p.tokens, chunk);
+            };
+            int at = next();
+            if (at >= 0) load(now, at);
 #pragma unroll 1
-                for (int t = 0; t < again.here; ++t) {
-                    const int tile = again.tile0 + t;
-                    if (__ldcg(wide + ((int64_t)chunk * tiles + tile) / kManyWarps) != 0)
-                        add_wide<kFp32, kBlock>(p, chunk, 8 * tile, min(8, p.tokens - 8 * tile), again.row0, again.row_count,
-                                                partial + (again.half * kTiles + t) * 8 * kManyPad + again.row0 - again.block_row, kManyPad);
-                }
+            while (at >= 0) {
+                const int following = next();
+                if (following >= 0) load(then, following);
+                uint32_t b[kParts][16];
+                const uint32_t small = make_wide_fragments<kFp32>(now.raw, b);
+#pragma unroll
+                for (int tile = 0; tile < 2; ++tile)
+                    add_wide<kFp32, kBlock>(now.pieces[tile], b, small, again.row_count - 16 * tile,
+                                            sums + at % 8 * 8 * kManyPad + 16 * tile, kManyPad);
+                now = then;
+                at = following;
+            }
+        }
     }
     __syncthreads();
     const int tokens = min(here * 8, p.tokens - tile0 * 8);
@@ -1009,7 +1088,7 @@ __global__ void __launch_bounds__(kManyThreads, kFp32 || kTiles > 4 ? 1 : 2)
 size_t workspace_of(bool fp32, int64_t tokens, int64_t cols) {
     if (tokens <= kFewTokens) return 0;
     const size_t units = (size_t)((cols + kChunk - 1) / kChunk) * ((tokens + 7) / 8);
-    return units * ((fp32 ? 3 : 1) * 2048 + 32) + (units + kManyWarps - 1) / kManyWarps + 4;
+    return units * ((fp32 ? 3 : 1) * 2048 + 32 + 1);
 }
 
 template <bool kFp32, int kTiles, bool kVector, int kBlock>
