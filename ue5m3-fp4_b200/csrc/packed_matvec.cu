@@ -27,7 +27,7 @@
 // the 16 warps meet in shared memory once per block of rows.  Measured: 1 x 21504 x 4096: 15.5 us,
 // 2.9 TB/s of 6.5 (fp32 22.3); 8 x 4096 x 21504: 20.6 us, 2.3 TB/s (fp32 36.3); 1 x 512 x 4096: 4.8 us.
 // Of its active cycles the first one issues in 55 % of the slots and keeps the ALU, which decodes, busy
-// for 42 %; launch, conversion of the activations (a look at their range costs 0.3 us of it) and
+// for 41 %; launch, conversion of the activations (a look at their range costs 0.3 us of it) and
 // the sums at the end do not overlap with the walk.  Rows that start anywhere come as aligned pieces
 // and are shifted into place: 1 x 21504 x 4095: 29 us (word by word into registers 51, pieces per warp
 // and chunk 34).
@@ -35,8 +35,8 @@
 // More tokens.  There every CTA would convert all activations for its few rows: a short kernel writes
 // them as fragments once (tokens x K x 2 bytes, three times that for fp32), and CTAs of 128 rows take
 // them through a ring in shared memory, next to codes and scales, four warps of 32 rows for each of
-// two halves of the chunks.  Measured: 64 x 18560 x 4096: 105 -> 41.1 us, 237 TFLOP/s, an mma in 17.5 active
-// cycles of each quarter of an SM, the tensor pipe 47 % busy; 33 x 4096 x 4096: 31 -> 13.7; 60 x 2718 x 15245,
+// two halves of the chunks.  Measured: 64 x 18560 x 4096: 105 -> 41.1 us, 237 TFLOP/s, an mma in 17.8 active
+// cycles of each quarter of an SM, the tensor pipe 46 % busy; 33 x 4096 x 4096: 31 -> 13.7; 60 x 2718 x 15245,
 // whose rows start anywhere: 258 -> 47; fp32, three products each, 40 x 2000 x 3001: 47.5 -> 17.5,
 // 64 x 4096 x 4096: 30.5; 2048 x 21504 x 4096, the weight decoded again for every 64 rows: 1444.  Bound by the
 // products' issue from 32 tokens on, by decoding and the fragments' way from L2 below
